@@ -4,6 +4,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -783,6 +784,284 @@ void reencode_fnuz(at::Tensor& src, at::Tensor& dst) {
     raise_on(hfrk_reencode_fnuz(src.data_ptr(), dst.data_ptr(), (size_t)src.numel(), current_stream(src)), "reencode_fnuz");
 }
 
+// ---- rotary positions, the paged cache and attention over it -----------------------------------------------------------------------
+// Each operator's arguments are put into the C ABI's struct by a function that returns what is wrong with them, or nullptr.
+
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }  // (of one, a tensor may hold any)
+
+bool heads_16bit(const at::Tensor& t) {
+    return t.dim() == 3 && is_16bit(t.scalar_type()) && (t.size(2) <= 1 || t.stride(2) == 1);
+}
+
+bool repeats_itself(const at::Tensor& t) { return t.numel() > 0 && at::has_internal_overlap(t) == at::MemOverlap::Yes; }
+
+// Whether the memory from a tensor's first to its last element meets another's.
+bool meets(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    auto end = [](const at::Tensor& t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return static_cast<const uint8_t*>(t.data_ptr()) + (last + 1) * (int64_t)t.element_size();
+    };
+    return static_cast<const uint8_t*>(a.data_ptr()) < end(b) && static_cast<const uint8_t*>(b.data_ptr()) < end(a);
+}
+
+bool same_memory(const at::Tensor& a, const at::Tensor& b) {
+    return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && stride_of(a, 0) == stride_of(b, 0) && stride_of(a, 1) == stride_of(b, 1);
+}
+
+bool is_index(const at::Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+
+// A scale: one float, or one a key head.
+const char* scale_arg(const std::optional<at::Tensor>& scale, const at::Tensor& like, int64_t heads, bool fp8, const float** ptr, int* stride) {
+    *ptr = nullptr;
+    *stride = 0;
+    if (!scale.has_value()) return nullptr;
+    if (!fp8) return "key_scale and value_scale belong to a float8_e4m3fn cache";
+    if (scale->scalar_type() != at::kFloat || !scale->is_contiguous() || (scale->numel() != 1 && scale->numel() != heads) || scale->device() != like.device())
+        return "key_scale and value_scale must be float32 with 1 or kv_heads elements, on the tensors' device";
+    *ptr = scale->data_ptr<float>();
+    *stride = scale->numel() == 1 ? 0 : 1;
+    return nullptr;
+}
+
+const char* rotation_args(hfrk_append_args& a, const at::Tensor& like, int64_t tokens, const std::optional<at::Tensor>& positions,
+                          const std::optional<at::Tensor>& frequencies, double magnitude, bool interleaved) {
+    a.magnitude = (float)magnitude;
+    a.interleaved = interleaved ? 1 : 0;
+    if (positions.has_value() != frequencies.has_value()) return "positions and frequencies come together";
+    if (!frequencies.has_value()) return nullptr;
+    if (positions->dim() != 1 || positions->size(0) != tokens || !is_index(*positions) || !positions->is_contiguous() || positions->device() != like.device())
+        return "positions must be a contiguous int32 or int64 tensor with one element per token, on the tensors' device";
+    if (frequencies->dim() != 1 || !frequencies->is_contiguous() || frequencies->device() != like.device() || 2 * frequencies->numel() > like.size(2) ||
+        (frequencies->scalar_type() != at::kFloat && frequencies->scalar_type() != at::kDouble))
+        return "frequencies must be a contiguous float32 or float64 tensor of at most head_dim / 2 elements, on the tensors' device";
+    a.positions = positions->data_ptr();
+    a.positions_wide = positions->scalar_type() == at::kLong ? 1 : 0;
+    a.frequencies = frequencies->data_ptr();
+    a.frequencies_wide = frequencies->scalar_type() == at::kDouble ? 1 : 0;
+    a.rotated = 2 * (int)frequencies->numel();
+    return nullptr;
+}
+
+// `heads` to be rotated into `output`.
+const char* turned_args(hfrk_append_args& a, const at::Tensor& heads, const at::Tensor& output) {
+    if (!heads_16bit(heads)) return "heads to rotate must be a float16 or bfloat16 [tokens, heads, head_dim] tensor with unit stride along head_dim";
+    if (!heads_16bit(output) || output.sizes() != heads.sizes() || output.scalar_type() != heads.scalar_type() || output.device() != heads.device())
+        return "the rotated heads' output must have their shape, dtype and device and unit stride along head_dim";
+    if (repeats_itself(output) || (meets(heads, output) && !same_memory(heads, output))) return "the rotated heads' output must be the input itself or lie apart from it";
+    if (heads.size(0) >= (int64_t(1) << 31) || heads.size(1) > 65536 || heads.size(2) > 1024 || heads.size(2) < 1) return "at most 65536 heads of 1 to 1024 values";
+    a.query = heads.data_ptr();
+    a.query_token_stride = stride_of(heads, 0);
+    a.query_head_stride = stride_of(heads, 1);
+    a.query_output = output.data_ptr();
+    a.output_token_stride = stride_of(output, 0);
+    a.output_head_stride = stride_of(output, 1);
+    a.tokens = (int)heads.size(0);
+    a.heads = (int)heads.size(1);
+    a.head_dim = (int)heads.size(2);
+    a.dtype = heads.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16;
+    return nullptr;
+}
+
+const char* rotary_args(hfrk_append_args& a, const at::Tensor& x, const at::Tensor& positions, const at::Tensor& frequencies, double magnitude,
+                        bool interleaved, const at::Tensor& output) {
+    const char* why = turned_args(a, x, output);
+    return why ? why : rotation_args(a, x, x.size(0), positions, frequencies, magnitude, interleaved);
+}
+
+struct CacheArgs {
+    int64_t page, place, head;
+};
+
+const char* cache_arg(const at::Tensor& cache, const at::Tensor& like, int64_t kv_heads, int64_t head_dim, CacheArgs& s) {
+    if (cache.dim() != 4 || cache.size(2) != kv_heads || cache.size(3) != head_dim || (head_dim > 1 && cache.stride(3) != 1))
+        return "a cache must be [pages, page_size, kv_heads, head_dim] with unit stride along head_dim";
+    if (cache.scalar_type() != like.scalar_type() && cache.scalar_type() != at::kFloat8_e4m3fn) return "a cache must have the heads' dtype or float8_e4m3fn";
+    if (cache.device() != like.device()) return "the caches must be on the heads' device";
+    if (cache.size(0) >= (int64_t(1) << 31) || cache.size(1) >= (int64_t(1) << 31) || cache.size(1) < 1) return "a cache has less than 2^31 pages of 1 to 2^31 places";
+    s = {stride_of(cache, 0), stride_of(cache, 1), stride_of(cache, 2)};
+    return nullptr;
+}
+
+const char* caches_alike(const at::Tensor& key_cache, const at::Tensor& value_cache) {
+    if (value_cache.sizes() != key_cache.sizes() || value_cache.scalar_type() != key_cache.scalar_type()) return "key_cache and value_cache must have one shape and dtype";
+    return nullptr;
+}
+
+const char* append_args(hfrk_append_args& a, const at::Tensor& key, const at::Tensor& value, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                        const at::Tensor& slots, const std::optional<at::Tensor>& positions, const std::optional<at::Tensor>& frequencies, double magnitude,
+                        bool interleaved, const std::optional<at::Tensor>& query, const at::Tensor& query_output, const std::optional<at::Tensor>& key_scale,
+                        const std::optional<at::Tensor>& value_scale) {
+    if (!heads_16bit(key) || !heads_16bit(value) || key.sizes() != value.sizes() || key.scalar_type() != value.scalar_type() || key.device() != value.device())
+        return "key and value must be float16 or bfloat16 [tokens, kv_heads, head_dim] tensors of one shape, dtype and device, with unit stride along head_dim";
+    const int64_t tokens = key.size(0), kv_heads = key.size(1), head_dim = key.size(2);
+    if (tokens >= (int64_t(1) << 31) || kv_heads < 1 || kv_heads > 65536 || head_dim < 1 || head_dim > 1024) return "1 to 65536 key heads of 1 to 1024 values";
+    if (query.has_value()) {
+        if (const char* why = turned_args(a, *query, query_output)) return why;
+        if (query->size(0) != tokens || query->size(2) != head_dim || query->scalar_type() != key.scalar_type() || query->device() != key.device())
+            return "query must have as many tokens as key, its head_dim, dtype and device";
+        if (!same_memory(*query, query_output) && (meets(query_output, key) || meets(query_output, value))) return "query_output must lie apart from key and value";
+    }
+    CacheArgs k, v;
+    if (const char* why = cache_arg(key_cache, key, kv_heads, head_dim, k)) return why;
+    if (const char* why = cache_arg(value_cache, key, kv_heads, head_dim, v)) return why;
+    if (const char* why = caches_alike(key_cache, value_cache)) return why;
+    for (const at::Tensor* cache : {&key_cache, &value_cache}) {
+        if (repeats_itself(*cache) || meets(*cache, key) || meets(*cache, value) || (query.has_value() && (meets(*cache, *query) || meets(*cache, query_output))))
+            return "the caches must lie apart from the step's tensors and not overlap themselves";
+    }
+    if (key_cache.numel() > 0 && key_cache.data_ptr() == value_cache.data_ptr()) return "key_cache and value_cache must not be the same memory";
+    if (slots.dim() != 1 || slots.size(0) != tokens || !is_index(slots) || !slots.is_contiguous() || slots.device() != key.device())
+        return "slots must be a contiguous int32 or int64 tensor with one element per token, on the tensors' device";
+    if (const char* why = rotation_args(a, key, tokens, positions, frequencies, magnitude, interleaved)) return why;
+    const bool fp8 = key_cache.scalar_type() == at::kFloat8_e4m3fn;
+    if (const char* why = scale_arg(key_scale, key, kv_heads, fp8, &a.key_scale, &a.key_scale_stride)) return why;
+    if (const char* why = scale_arg(value_scale, key, kv_heads, fp8, &a.value_scale, &a.value_scale_stride)) return why;
+    a.key = key.data_ptr();
+    a.key_token_stride = stride_of(key, 0);
+    a.key_head_stride = stride_of(key, 1);
+    a.value = value.data_ptr();
+    a.value_token_stride = stride_of(value, 0);
+    a.value_head_stride = stride_of(value, 1);
+    a.key_cache = key_cache.data_ptr();
+    a.key_page_stride = k.page;
+    a.key_place_stride = k.place;
+    a.key_cache_head_stride = k.head;
+    a.value_cache = value_cache.data_ptr();
+    a.value_page_stride = v.page;
+    a.value_place_stride = v.place;
+    a.value_cache_head_stride = v.head;
+    a.slots = slots.data_ptr();
+    a.slots_wide = slots.scalar_type() == at::kLong ? 1 : 0;
+    a.tokens = (int)tokens;
+    a.kv_heads = (int)kv_heads;
+    a.head_dim = (int)head_dim;
+    a.pages = (int)key_cache.size(0);
+    a.page_size = (int)key_cache.size(1);
+    a.dtype = key.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16;
+    a.cache_dtype = fp8 ? HFRK_FP8_E4M3FN : a.dtype;
+    return nullptr;
+}
+
+const char* attention_args(hfrk_attention_args& a, const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                           const at::Tensor& page_table, const at::Tensor& lengths, const std::optional<at::Tensor>& starts,
+                           const std::optional<at::Tensor>& mask, double scale, const std::optional<at::Tensor>& key_scale,
+                           const std::optional<at::Tensor>& value_scale, const std::optional<at::Tensor>& out_scale, const at::Tensor& output) {
+    if (!heads_16bit(query)) return "query must be a float16 or bfloat16 [tokens, heads, head_dim] tensor with unit stride along head_dim";
+    const int64_t tokens = query.size(0), heads = query.size(1), head_dim = query.size(2);
+    if (key_cache.dim() != 4) return "a cache must be [pages, page_size, kv_heads, head_dim] with unit stride along head_dim";
+    const int64_t kv_heads = key_cache.size(2);
+    CacheArgs k, v;
+    if (const char* why = cache_arg(key_cache, query, kv_heads, head_dim, k)) return why;
+    if (const char* why = cache_arg(value_cache, query, kv_heads, head_dim, v)) return why;
+    if (const char* why = caches_alike(key_cache, value_cache)) return why;
+    if (kv_heads < 1 || heads < 1 || heads % kv_heads != 0) return "heads must be a multiple of kv_heads";
+    if (page_table.dim() != 2 || page_table.scalar_type() != at::kInt || (page_table.size(1) > 1 && page_table.stride(1) != 1) || page_table.device() != query.device())
+        return "page_table must be an int32 [seqs, columns] tensor with unit stride along its rows, on the query's device";
+    const int64_t seqs = page_table.size(0);
+    if (lengths.dim() != 1 || lengths.size(0) != seqs || lengths.scalar_type() != at::kInt || !lengths.is_contiguous() || lengths.device() != query.device())
+        return "lengths must be a contiguous int32 tensor with one element per sequence, on the query's device";
+    if (starts.has_value()) {
+        if (starts->dim() != 1 || starts->size(0) != seqs + 1 || starts->scalar_type() != at::kInt || !starts->is_contiguous() || starts->device() != query.device())
+            return "starts must be a contiguous int32 tensor with one element per sequence and one more, on the query's device";
+        a.starts = starts->data_ptr<int32_t>();
+    } else if (seqs > 0 ? tokens % seqs != 0 : tokens != 0) {
+        return "without starts every sequence has the same number of tokens";
+    }
+    if (mask.has_value()) {
+        if (mask->dim() != 2 || mask->size(0) != tokens || (mask->scalar_type() != at::kBool && mask->scalar_type() != at::kByte) ||
+            (mask->size(1) > 1 && mask->stride(1) != 1) || mask->device() != query.device() || mask->size(1) >= (int64_t(1) << 31))
+            return "mask must be a bool or uint8 [tokens, drafted] tensor with unit stride along its rows, on the query's device";
+        a.mask_columns = (int)mask->size(1);
+        a.mask_stride = stride_of(*mask, 0);
+        a.mask = mask->data_ptr();
+        static const uint8_t none = 0;
+        if (!a.mask) a.mask = &none;  // no columns: never read, and not a chain
+    }
+    const bool fp8 = key_cache.scalar_type() == at::kFloat8_e4m3fn;
+    if (const char* why = scale_arg(key_scale, query, kv_heads, fp8, &a.key_scale, &a.key_scale_stride)) return why;
+    if (const char* why = scale_arg(value_scale, query, kv_heads, fp8, &a.value_scale, &a.value_scale_stride)) return why;
+    if (out_scale.has_value()) {
+        if (out_scale->numel() != 1 || out_scale->scalar_type() != at::kFloat || out_scale->device() != query.device()) return "out_scale must be one float32 on the query's device";
+        a.out_scale = out_scale->data_ptr<float>();
+    }
+    if (output.dim() != 3 || output.sizes() != query.sizes() || (head_dim > 1 && output.stride(2) != 1) || output.device() != query.device() ||
+        output.scalar_type() != (out_scale.has_value() ? at::kFloat8_e4m3fn : query.scalar_type()))
+        return "output must have the query's shape, device and dtype (float8_e4m3fn with out_scale) and unit stride along head_dim";
+    if (repeats_itself(output) || meets(output, query) || meets(output, key_cache) || meets(output, value_cache)) return "output must lie apart from the query and the caches";
+    if (tokens >= (int64_t(1) << 31) || heads > 65536 || seqs > (1 << 20) || page_table.size(1) >= (int64_t(1) << 31)) return "too many tokens, heads or sequences";
+    a.query = query.data_ptr();
+    a.query_token_stride = stride_of(query, 0);
+    a.query_head_stride = stride_of(query, 1);
+    a.output = output.data_ptr();
+    a.output_token_stride = stride_of(output, 0);
+    a.output_head_stride = stride_of(output, 1);
+    a.key_cache = key_cache.data_ptr();
+    a.key_page_stride = k.page;
+    a.key_place_stride = k.place;
+    a.key_cache_head_stride = k.head;
+    a.value_cache = value_cache.data_ptr();
+    a.value_page_stride = v.page;
+    a.value_place_stride = v.place;
+    a.value_cache_head_stride = v.head;
+    a.page_table = page_table.data_ptr<int32_t>();
+    a.table_stride = stride_of(page_table, 0);
+    a.table_columns = (int)page_table.size(1);
+    a.lengths = lengths.data_ptr<int32_t>();
+    a.scale = (float)scale;
+    a.tokens = (int)tokens;
+    a.seqs = (int)seqs;
+    a.heads = (int)heads;
+    a.kv_heads = (int)kv_heads;
+    a.head_dim = (int)head_dim;
+    a.pages = (int)key_cache.size(0);
+    a.page_size = (int)key_cache.size(1);
+    a.dtype = query.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16;
+    a.cache_dtype = fp8 ? HFRK_FP8_E4M3FN : a.dtype;
+    return nullptr;
+}
+
+// The workspace is the call's own, from torch's allocator: calls on several streams, and captured graphs, do not share it.
+int run_attention(const hfrk_attention_args& a, const at::Tensor& query) {
+    const size_t bytes = hfrk_tree_attention_workspace_bytes(&a);
+    at::Tensor workspace;
+    if (bytes) workspace = at::empty({(int64_t)bytes}, query.options().dtype(at::kByte));
+    return hfrk_tree_attention(&a, bytes ? workspace.data_ptr() : nullptr, bytes, current_stream(query));
+}
+
+void rotary(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& frequencies, double magnitude, bool interleaved, at::Tensor& output) {
+    hfrk_append_args a = {};
+    const char* const why = rotary_args(a, x, positions, frequencies, magnitude, interleaved, output);
+    TORCH_CHECK(!why, why);
+    DeviceScope scope(x);
+    raise_on(hfrk_append_kv(&a, current_stream(x)), "rotary");
+}
+
+void append_kv(const at::Tensor& key, const at::Tensor& value, at::Tensor& key_cache, at::Tensor& value_cache, const at::Tensor& slots,
+               const std::optional<at::Tensor>& positions, const std::optional<at::Tensor>& frequencies, double magnitude, bool interleaved,
+               const std::optional<at::Tensor>& query, const std::optional<at::Tensor>& query_output, const std::optional<at::Tensor>& key_scale,
+               const std::optional<at::Tensor>& value_scale) {
+    TORCH_CHECK(query.has_value() == query_output.has_value(), "query and query_output come together");
+    hfrk_append_args a = {};
+    const char* const why = append_args(a, key, value, key_cache, value_cache, slots, positions, frequencies, magnitude, interleaved, query,
+                                        query_output.has_value() ? *query_output : key, key_scale, value_scale);
+    TORCH_CHECK(!why, why);
+    DeviceScope scope(key);
+    raise_on(hfrk_append_kv(&a, current_stream(key)), "append_kv");
+}
+
+void tree_attention(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& page_table,
+                    const at::Tensor& lengths, const std::optional<at::Tensor>& starts, const std::optional<at::Tensor>& mask, double scale,
+                    const std::optional<at::Tensor>& key_scale, const std::optional<at::Tensor>& value_scale, const std::optional<at::Tensor>& out_scale,
+                    at::Tensor& output) {
+    hfrk_attention_args a = {};
+    const char* const why = attention_args(a, query, key_cache, value_cache, page_table, lengths, starts, mask, scale, key_scale, value_scale, out_scale, output);
+    TORCH_CHECK(!why, why);
+    DeviceScope scope(query);
+    raise_on(run_attention(a, query), "tree_attention");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(_HFRK_C, ops) {
@@ -877,6 +1156,17 @@ TORCH_LIBRARY(_HFRK_C, ops) {
     ops.impl("swiglu_dynamic_new", c10::kCUDA, &swiglu_dynamic_new);
     for (const char* name : {"residual_rms_new", "residual_rms_dynamic_new", "swiglu_new", "swiglu_dynamic_new"})
         ops.impl(name, torch::dispatch(c10::DispatchKey::Autograd, torch::CppFunction::makeFallthrough()));
+
+    ops.def("rotary(Tensor x, Tensor positions, Tensor frequencies, float magnitude, bool interleaved, Tensor! output) -> ()");
+    ops.impl("rotary", c10::kCUDA, &rotary);
+    ops.def(
+        "append_kv(Tensor key, Tensor value, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots, Tensor? positions, Tensor? frequencies, "
+        "float magnitude, bool interleaved, Tensor? query, Tensor(c!)? query_output, Tensor? key_scale, Tensor? value_scale) -> ()");
+    ops.impl("append_kv", c10::kCUDA, &append_kv);
+    ops.def(
+        "tree_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor page_table, Tensor lengths, Tensor? starts, Tensor? mask, "
+        "float scale, Tensor? key_scale, Tensor? value_scale, Tensor? out_scale, Tensor(a!) output) -> ()");
+    ops.impl("tree_attention", c10::kCUDA, &tree_attention);
 
     ops.def("quantize_fp8(Tensor input, Tensor? scale_tensor, Tensor! output, Tensor! scales) -> ()");
     ops.impl("quantize_fp8", c10::kCUDA, &quantize_fp8);

@@ -1,0 +1,438 @@
+// Attention of a step's queries over a paged cache: the kernel.
+//
+//   o_i = sum_j 2^(c s_ij - m_i) v_j / sum_j 2^(c s_ij - m_i),  s_ij = q_i . k_j,  c = scale * key_scale * log2(e)
+//
+// over the cached tokens j that row i sees, m_i the largest c s_ij so far (one pass: when it grows, what has been summed is scaled down).
+// A row is one drafted token and one of the query heads that share a key head, so a group of heads reads its keys and values once.
+//
+// Each wave takes 32 cached tokens at a time and C blocks of 16 rows, straight from memory to registers and without LDS:
+//   S^T = K Q^T   keys are the A operand.  Row r of the two 16-row products is token 8 (r / 4) + 4 t + r % 4, so that a lane's eight scores are those
+//                 of eight tokens in a row, 8 g .. 8 g + 7 for lane group g = lane / 16, all of query row lane % 16
+//   O^T += V^T P  these eight are, rounded to 16 bits, already the B operand of the second product.  Its A operand is V^T: a lane has loaded
+//                 the same eight tokens' values of DP / 16 neighbouring columns, and turns that block within its own registers
+//   l += 1 P      the sum of the weights, as rounded, by one more product with ones
+// Scores, sums and statistics are fp32.  The weights are rounded to the cache's 16-bit type (half a step of 2^-8 or 2^-11 each, and the same
+// rounded weights make the sum, so that the rounding does not tilt the mean).
+//
+// The next tokens' keys are requested as soon as the scores have been made, their values as soon as the present ones are turned: a
+// wave has 16 KB (128 columns, 16 bits) in flight, and bytes bound the kernel up to about 64 rows.
+#pragma once
+
+#include "tree_attention.h"
+
+namespace hfrk {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+template <int DT>
+__device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
+    if constexpr (DT == HFRK_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ int pack2(float lo, float hi) {  // round to nearest even
+    if constexpr (DT == HFRK_BF16) return __builtin_bit_cast(int, __builtin_convertvector(v2f{lo, hi}, v2bf));
+    else return __builtin_bit_cast(int, __builtin_convertvector(v2f{lo, hi}, v2h));
+}
+
+// Two e4m3 values of a word's low or high half as 16-bit values; exact in both types.
+template <int DT, bool HIGH>
+__device__ __forceinline__ int widen2(int word) {
+    if constexpr (DT == HFRK_BF16) return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.f, HIGH));
+    else return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, HIGH));
+}
+
+// The largest of the four lanes that hold the same query row.
+__device__ __forceinline__ float row_max(float v) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+    const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+}
+
+// Eight values of a row of the result: divided by the sum of the weights, times the values' scale; a row that saw nothing is zero.
+template <int DT>
+__device__ __forceinline__ void store_row(const hfrk_attention_args& a, long token, int head, int d, const float (&o)[8], float total, float value_scale,
+                                          float inv_out_scale) {
+    const float by = total == 0.f ? 0.f : value_scale / total;
+    const long at = token * a.output_token_stride + head * a.output_head_stride + d;
+    if (a.out_scale) {
+        uint32_t w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            w[j] = cvt_pk_fp8(o[4 * j] * by * inv_out_scale, o[4 * j + 1] * by * inv_out_scale, 0u, false);
+            w[j] = cvt_pk_fp8(o[4 * j + 2] * by * inv_out_scale, o[4 * j + 3] * by * inv_out_scale, w[j], true);
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.output) + at) = make_uint2(w[0], w[1]);
+    } else {
+        *reinterpret_cast<v4i*>(static_cast<uint16_t*>(a.output) + at) =
+            v4i{pack2<DT>(o[0] * by, o[1] * by), pack2<DT>(o[2] * by, o[3] * by), pack2<DT>(o[4] * by, o[5] * by), pack2<DT>(o[6] * by, o[7] * by)};
+    }
+}
+
+// Of a pair of 16-bit values, those that are infinite or NaN: bit 15 of each half.  (Arithmetic on both halves at once, no conditions: as
+// conditions the rare path below took all scalar registers.)
+template <int DT>
+__device__ __forceinline__ uint32_t unbounded(uint32_t pair) {
+    constexpr uint32_t e = DT == HFRK_BF16 ? 0x7f807f80u : 0x7c007c00u;
+    return (((pair & e) ^ e) + 0x7fff7fffu & 0x80008000u) ^ 0x80008000u;
+}
+
+// Those bits as whole halves.
+__device__ __forceinline__ uint32_t halves(uint32_t bits) { return (bits << 1) - (bits >> 15); }
+
+// Of the unbounded ones, those that are NaN or of the wanted sign (sign: 0 plus, 0x80008000 minus), as the value one.
+template <int DT>
+__device__ __forceinline__ uint32_t counted(uint32_t pair, uint32_t bits, uint32_t sign) {
+    constexpr uint32_t f = DT == HFRK_BF16 ? 0x007f007fu : 0x03ff03ffu, one = DT == HFRK_BF16 ? 0x3f80u : 0x3c00u;
+    const uint32_t nan = (pair & f) + 0x7fff7fffu;
+    return (((nan | ~(pair ^ sign)) & bits) >> 15) * one;  // (`bits` has the halves' top bits only)
+}
+
+// One wave's operands of 32 cached tokens.
+template <int DP, bool FP8>
+struct CachedTile {
+    static constexpr int kKeyLoads = FP8 ? DP / 64 : DP / 32;   // 16-byte pieces of a key a lane holds
+    static constexpr int kValueWords = (FP8 ? DP / 16 : DP / 8) / 4;  // words of a value
+    v4i key[2][kKeyLoads];
+    uint32_t value[8][kValueWords];
+};
+
+template <int DT, bool FP8, int DP, int C>
+__global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1) attention_kernel(const AttentionArgs p) {
+    constexpr int kSteps = DP / 32;   // products of 32 columns in K Q^T
+    constexpr int kCols = DP / 16;    // V^T's 16-row blocks, and the neighbouring columns a lane loads
+    constexpr int kSize = FP8 ? 1 : 2;
+    constexpr int kPad = DP + 4;
+    typedef CachedTile<DP, FP8> Tile;
+    __shared__ __align__(16) float merged[kAttentionWaves][16][kPad];
+    __shared__ float statistics[kAttentionWaves][16][2];
+
+    const hfrk_attention_args& a = p.a;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int item = blockIdx.x / a.kv_heads, head = blockIdx.x - item * a.kv_heads;
+    const Part part = find_part(p, item);
+    if (!part.any) return;
+    const Sequence s = part.s;
+    const int row0 = part.block * p.rows, rows = s.count * p.group;
+    const int drafted = s.drafted;
+
+    // Lane group g has the columns kWindow g .. of keys and queries, read as whole 16-byte pieces one behind the other.  A head that ends inside
+    // a window: the window is moved to the head's end, and the query is zero in the columns that are not this group's.
+    constexpr int kWindow = DP / 4;
+    const int window = min(kWindow * g, a.head_dim - kWindow);
+    v4i query[C][kSteps];
+    int seen_to[C];      // chain: the last token this lane's row sees (-1: no row)
+    const uint8_t* sees[C];  // tree: its row of the mask
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int row = row0 + c * 16 + col, token = row / p.group, member = row - token * p.group;
+        const bool real = row < rows;
+        seen_to[c] = real ? drafted + token : -1;
+        sees[c] = static_cast<const uint8_t*>(a.mask) + (real ? (long)(s.first + token) * a.mask_stride : 0);
+        const uint16_t* const q = static_cast<const uint16_t*>(a.query) + (real ? (long)(s.first + token) * a.query_token_stride +
+                                                                                  (long)(head * p.group + member) * a.query_head_stride : 0);
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+            const int d = window + 8 * step;
+            query[c][step] = real && d >= kWindow * g ? *reinterpret_cast<const v4i*>(q + d) : v4i{0, 0, 0, 0};
+        }
+    }
+    const float scale = p.log2_scale * (FP8 && a.key_scale ? a.key_scale[head * a.key_scale_stride] : 1.f);
+
+    // where a lane reads: keys of two tokens, values of eight
+    const int key_token = 8 * (col >> 2) + (col & 3), value_token = 8 * g;
+    const int value_column = col * kCols < a.head_dim ? col * kCols : 0;  // (columns a head does not have are read elsewhere and not stored)
+    const uint8_t* const keys = static_cast<const uint8_t*>(a.key_cache) + ((long)head * a.key_cache_head_stride + window) * kSize;
+    const uint8_t* const values = static_cast<const uint8_t*>(a.value_cache) + ((long)head * a.value_cache_head_stride + value_column) * kSize;
+    const int32_t* const table = a.page_table + (long)part.b * a.table_stride;
+
+    struct Pages {
+        int key, value;
+    };
+    auto page_of = [&](int token) {
+        const uint32_t n = (uint32_t)token >> 3;
+        return (int)(p.page_magic ? __umulhi(n, p.page_magic) >> p.page_shift : n >> p.page_shift);
+    };
+    auto entry = [&](int token) {  // -1: no such page
+        const int at = page_of(token);
+        const int page = at < a.table_columns ? table[at] : -1;
+        return page >= 0 && page < a.pages ? page : -1;
+    };
+    auto pages_of = [&](int t0) { return Pages{entry(t0 + key_token), entry(t0 + value_token)}; };
+    auto load_keys = [&](Tile& tile, int t0, int page) {
+        const int token = t0 + key_token, in_page = token - page_of(token) * a.page_size;
+        const uint8_t* at = keys + ((long)max(page, 0) * a.key_page_stride + (long)in_page * a.key_place_stride) * kSize;
+#pragma unroll
+        for (int t = 0; t < 2; ++t, at += 4 * a.key_place_stride * kSize)
+#pragma unroll
+            for (int i = 0; i < Tile::kKeyLoads; ++i) tile.key[t][i] = *reinterpret_cast<const v4i*>(at + 16 * i);
+    };
+    auto load_values = [&](Tile& tile, int t0, int page) {
+        const int token = t0 + value_token, in_page = token - page_of(token) * a.page_size;
+        const uint8_t* at = values + ((long)max(page, 0) * a.value_page_stride + (long)in_page * a.value_place_stride) * kSize;
+#pragma unroll
+        for (int j = 0; j < 8; ++j, at += a.value_place_stride * kSize) {
+            if constexpr (Tile::kValueWords == 1) tile.value[j][0] = *reinterpret_cast<const uint32_t*>(at);
+            if constexpr (Tile::kValueWords == 2) *reinterpret_cast<uint2*>(tile.value[j]) = *reinterpret_cast<const uint2*>(at);
+            if constexpr (Tile::kValueWords >= 4) {
+#pragma unroll
+                for (int w = 0; w < Tile::kValueWords; w += 4) *reinterpret_cast<uint4*>(tile.value[j] + w) = *reinterpret_cast<const uint4*>(at + 4 * w);
+            }
+        }
+    };
+
+    v4f out[C][kCols], sum[C];
+    float top[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        top[c] = -INFINITY;
+        sum[c] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < kCols; ++f) out[c][f] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    constexpr int kOne = DT == HFRK_BF16 ? 0x3f803f80 : 0x3c003c00;
+    const v4i ones = {kOne, kOne, kOne, kOne};
+
+    // a chain's rows see nothing behind the block's last token
+    int end = min(part.to * kTileTokens, s.length);
+    if (!a.mask) end = min(end, drafted + (min(row0 + p.rows, rows) - 1) / p.group + 1);
+    int t0 = part.from * kTileTokens + wave * kWaveTokens;
+    Tile tile;
+    Pages now = {-1, -1}, next = {-1, -1};
+    if (t0 < end) {
+        now = pages_of(t0);
+        load_keys(tile, t0, now.key);
+        load_values(tile, t0, now.value);
+        if (t0 + kTileTokens < end) next = pages_of(t0 + kTileTokens);
+    }
+    for (; t0 < end; t0 += kTileTokens) {
+        const int t1 = t0 + kTileTokens;
+        const bool more = t1 < end;
+        Pages after = {-1, -1};
+        if (t1 + kTileTokens < end) after = pages_of(t1 + kTileTokens);
+
+        v4f score[C][2];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int step = 0; step < kSteps; ++step) {
+                    v4i k;
+                    if constexpr (FP8) {
+                        const int lo = tile.key[t][step / 2][2 * (step % 2)], hi = tile.key[t][step / 2][2 * (step % 2) + 1];
+                        k = v4i{widen2<DT, false>(lo), widen2<DT, true>(lo), widen2<DT, false>(hi), widen2<DT, true>(hi)};
+                    } else {
+                        k = tile.key[t][step];
+                    }
+                    acc = mfma16<DT>(k, query[c][step], acc);
+                }
+                score[c][t] = acc;
+            }
+        if (more) load_keys(tile, t1, next.key);
+
+        // Tokens that some row does not see: drafted ones, those behind the end, those without a page.
+        const bool lost = now.value < 0 || t0 + value_token + 7 >= s.length;
+        const bool some = t0 + kWaveTokens > drafted || __any(lost);
+        uint32_t here = 0xffu;  // of this lane's eight tokens, those that exist
+        uint32_t seen[C];  // and those that its row sees
+        if (some) {
+            const auto first_of_8 = [](int n) { return (1u << min(max(n, 0), 8)) - 1u; };
+            const int at = t0 + value_token - drafted;  // of the lane's first token among the drafted ones
+            const int known = min(s.count, a.mask_columns);
+            here = now.value < 0 ? 0u : first_of_8(s.length - (t0 + value_token));
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                if (a.mask) {
+                    uint32_t bits = 0;
+                    if (known > 0) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) bits |= min((uint32_t)sees[c][min(max(at + j, 0), known - 1)], 1u) << j;
+                    }
+                    seen[c] = ((bits & first_of_8(known - at)) | first_of_8(-at)) & here;
+                } else {
+                    seen[c] = first_of_8(seen_to[c] + 1 - (t0 + value_token)) & here;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!(seen[c] >> j & 1)) score[c][j / 4][j % 4] = -INFINITY;
+            }
+        }
+
+        v4i weight[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float most = score[c][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) most = fmaxf(most, score[c][j / 4][j % 4]);
+            most = row_max(most * scale);
+            if (__any(most > top[c])) {
+                const float grown = fmaxf(top[c], most);
+                const float shrink = top[c] == grown ? 1.f : __builtin_amdgcn_exp2f(top[c] - grown);
+                top[c] = grown;
+                sum[c] *= shrink;
+#pragma unroll
+                for (int f = 0; f < kCols; ++f) out[c][f] *= shrink;
+            }
+            const float base = top[c] == -INFINITY ? 0.f : top[c];
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(score[c][j / 4][j % 4], scale, -base));
+            weight[c] = v4i{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
+        }
+
+        // V^T: word q of column f holds tokens 2q and 2q + 1
+        v4i turned[kCols];
+#pragma unroll
+        for (int f = 0; f < kCols; f += 2)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t even, odd;
+                if constexpr (FP8) {
+                    even = f % 4 == 0 ? widen2<DT, false>(tile.value[2 * q][f / 4]) : widen2<DT, true>(tile.value[2 * q][f / 4]);
+                    odd = f % 4 == 0 ? widen2<DT, false>(tile.value[2 * q + 1][f / 4]) : widen2<DT, true>(tile.value[2 * q + 1][f / 4]);
+                } else {
+                    even = tile.value[2 * q][f / 2];
+                    odd = tile.value[2 * q + 1][f / 2];
+                }
+                turned[f][q] = (int)__builtin_amdgcn_perm(odd, even, 0x05040100u);
+                turned[f + 1][q] = (int)__builtin_amdgcn_perm(odd, even, 0x07060302u);
+            }
+        if (more) load_values(tile, t1, next.value);
+
+        if (some) {
+            // Weights of zero do not keep an infinity or a NaN out of the sums.  Memory behind the end and without a page is cleared; a drafted
+            // token's own infinities and NaN are taken out and reach the rows that see it by themselves: a product of marks with what is seen.
+            uint32_t keep[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) keep[q] = halves((here >> 2 * q & 1u) << 15 | (here >> (2 * q + 1) & 1u) << 31);
+            uint32_t bad = 0;
+#pragma unroll
+            for (int f = 0; f < kCols; ++f)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    turned[f][q] &= (int)keep[q];
+                    bad |= unbounded<DT>((uint32_t)turned[f][q]);
+                }
+            if (__any(bad != 0)) {
+                v4i sight[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        sight[c][q] = (int)(((seen[c] >> 2 * q & 1u) | (seen[c] >> (2 * q + 1) & 1u) << 16) * (uint32_t)(kOne & 0xffff));
+#pragma unroll
+                for (int f = 0; f < kCols; ++f) {
+                    __builtin_amdgcn_sched_barrier(0);  // one column at a time: all at once they take the registers of the usual path
+                    v4i plus, minus;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t pair = (uint32_t)turned[f][q], b = unbounded<DT>(pair);
+                        plus[q] = (int)counted<DT>(pair, b, 0u);
+                        minus[q] = (int)counted<DT>(pair, b, 0x80008000u);
+                        turned[f][q] = (int)(pair & ~halves(b));
+                    }
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const v4f none = {0.f, 0.f, 0.f, 0.f};
+                        const v4f up = mfma16<DT>(plus, sight[c], none), down = mfma16<DT>(minus, sight[c], none);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (up[r] > 0.f) out[c][f][r] += INFINITY;
+                            if (down[r] > 0.f) out[c][f][r] -= INFINITY;
+                        }
+                    }
+                }
+            }
+        }
+
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            sum[c] = mfma16<DT>(ones, weight[c], sum[c]);
+#pragma unroll
+            for (int f = 0; f < kCols; ++f) out[c][f] = mfma16<DT>(turned[f], weight[c], out[c][f]);
+        }
+        now = next;
+        next = after;
+    }
+
+    // The four waves' parts of a row: scaled to the largest of their largest scores and added, 16 rows at a time.
+    const float value_scale = FP8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f;
+    const float inv_out_scale = a.out_scale ? 1.f / a.out_scale[0] : 1.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if (row0 + c * 16 >= rows) break;  // (the same for the whole workgroup)
+        if (c > 0) __syncthreads();
+        if (g == 0) {
+            statistics[wave][col][0] = top[c];
+            statistics[wave][col][1] = sum[c][0];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int f = 0; f < kCols; f += 4)
+                *reinterpret_cast<v4f*>(&merged[wave][col][(4 * g + r) * kCols + f]) = v4f{out[c][f][r], out[c][f + 1][r], out[c][f + 2][r], out[c][f + 3][r]};
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * (DP / 8); i += kAttentionThreads) {
+            const int r = i / (DP / 8), d = 8 * (i - r * (DP / 8)), row = row0 + c * 16 + r;
+            if (row >= rows || d >= a.head_dim) continue;
+            float most = statistics[0][r][0];
+#pragma unroll
+            for (int w = 1; w < kAttentionWaves; ++w) most = fmaxf(most, statistics[w][r][0]);
+            float total = 0.f, o[8] = {};
+#pragma unroll
+            for (int w = 0; w < kAttentionWaves; ++w) {
+                const float part_top = statistics[w][r][0];
+                const float share = part_top == most ? 1.f : __builtin_amdgcn_exp2f(part_top - most);  // (equal: both may be -infinity)
+                total += share * statistics[w][r][1];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] += share * merged[w][r][d + j];
+            }
+            if (part.splits > 1) {
+                const long at = ((long)part.slot * a.kv_heads + head) * p.rows + c * 16 + r;
+                float* const to = p.partial + at * a.head_dim + d;
+                *reinterpret_cast<v4f*>(to) = v4f{o[0], o[1], o[2], o[3]};
+                *reinterpret_cast<v4f*>(to + 4) = v4f{o[4], o[5], o[6], o[7]};
+                if (d == 0) p.partial_ml[at] = make_float2(most, total);
+            } else {
+                const int token = row / p.group, member = row - token * p.group;
+                store_row<DT>(a, s.first + token, head * p.group + member, d, o, total, value_scale, inv_out_scale);
+            }
+        }
+    }
+    if (p.row_info && part.split == 0 && head == 0) {
+        for (int r = threadIdx.x; r < p.rows && row0 + r < rows; r += kAttentionThreads)
+            p.row_info[(long)s.first * p.group + row0 + r] = make_int4(part.slot - part.split, part.splits, r, 0);
+    }
+}
+
+template <int DP>
+int launch_attention(const AttentionArgs& p, int col_blocks, int grid, hipStream_t stream) {
+    const bool fp8 = p.a.cache_dtype == HFRK_FP8_E4M3FN;
+#define HFRK_ATTENTION(DT, FP8)                                                                                                             \
+    do {                                                                                                                                    \
+        if (col_blocks == 1) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 1>), dim3(grid), dim3(kAttentionThreads), 0, stream, p);      \
+        else if (col_blocks == 2) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(kAttentionThreads), 0, stream, p); \
+        else hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, DP == 256 ? 2 : 4>), dim3(grid), dim3(kAttentionThreads), 0, stream, p);      \
+    } while (0)
+    if (p.a.dtype == HFRK_BF16) {
+        if (fp8) HFRK_ATTENTION(HFRK_BF16, true);
+        else HFRK_ATTENTION(HFRK_BF16, false);
+    } else {
+        if (fp8) HFRK_ATTENTION(HFRK_F16, true);
+        else HFRK_ATTENTION(HFRK_F16, false);
+    }
+#undef HFRK_ATTENTION
+    HFRK_HIP_TRY(hipGetLastError());
+    return HFRK_SUCCESS;
+}
+
+}  // namespace hfrk

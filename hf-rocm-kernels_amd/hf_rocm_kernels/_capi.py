@@ -57,6 +57,45 @@ class TiledPlan(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int) for name in ("shape", "splits", "group_m")]
 
 
+def _pointers(*names):
+    return [(name, ctypes.c_void_p) for name in names]
+
+
+def _strides(*names):
+    return [(name, ctypes.c_int64) for name in names]
+
+
+def _ints(*names):
+    return [(name, ctypes.c_int) for name in names]
+
+
+class AppendArgs(ctypes.Structure):
+    """struct hfrk_append_args"""
+    _fields_ = [*_pointers("query"), *_strides("query_token_stride", "query_head_stride"),
+                *_pointers("query_output"), *_strides("output_token_stride", "output_head_stride"),
+                *_pointers("key"), *_strides("key_token_stride", "key_head_stride"),
+                *_pointers("value"), *_strides("value_token_stride", "value_head_stride"),
+                *_pointers("key_cache"), *_strides("key_page_stride", "key_place_stride", "key_cache_head_stride"),
+                *_pointers("value_cache"), *_strides("value_page_stride", "value_place_stride", "value_cache_head_stride"),
+                *_pointers("slots", "positions", "frequencies", "key_scale", "value_scale"),
+                *_ints("key_scale_stride", "value_scale_stride", "slots_wide", "positions_wide", "frequencies_wide"),
+                ("magnitude", ctypes.c_float),
+                *_ints("interleaved", "tokens", "heads", "kv_heads", "head_dim", "rotated", "pages", "page_size", "dtype", "cache_dtype")]
+
+
+class AttentionArgs(ctypes.Structure):
+    """struct hfrk_attention_args"""
+    _fields_ = [*_pointers("query"), *_strides("query_token_stride", "query_head_stride"),
+                *_pointers("output"), *_strides("output_token_stride", "output_head_stride"),
+                *_pointers("key_cache"), *_strides("key_page_stride", "key_place_stride", "key_cache_head_stride"),
+                *_pointers("value_cache"), *_strides("value_page_stride", "value_place_stride", "value_cache_head_stride"),
+                *_pointers("page_table"), *_strides("table_stride"), *_pointers("lengths", "starts", "mask"), *_strides("mask_stride"),
+                *_pointers("key_scale", "value_scale", "out_scale"), *_ints("key_scale_stride", "value_scale_stride"),
+                ("scale", ctypes.c_float),
+                *_ints("tokens", "seqs", "heads", "kv_heads", "head_dim", "pages", "page_size", "table_columns", "mask_columns", "dtype",
+                       "cache_dtype")]
+
+
 _i, _p, _f = ctypes.c_int, ctypes.c_void_p, ctypes.c_float
 
 # name -> (restype, argtypes); every symbol the header declares
@@ -100,6 +139,10 @@ SIGNATURES = {
     "hfrk_residual_rms_dynamic": (_i, [_p, _p, _p, _f, _p, _p, _p, _i, _i, _i, _i, _p]),
     "hfrk_swiglu_dynamic": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p]),
     "hfrk_quantize_fp8": (_i, [_p, _p, _p, _p, _i, _i, _i, _p]),
+    "hfrk_rotary": (_i, [_p, ctypes.c_int64, ctypes.c_int64, _p, ctypes.c_int64, ctypes.c_int64, _p, _i, _p, _i, _f] + [_i] * 6 + [_p]),
+    "hfrk_append_kv": (_i, [ctypes.POINTER(AppendArgs), _p]),
+    "hfrk_tree_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
+    "hfrk_tree_attention": (_i, [ctypes.POINTER(AttentionArgs), _p, ctypes.c_size_t, _p]),
     "hfrk_plan_table_load": (_i, [ctypes.c_char_p, _i, ctypes.POINTER(_i)]),
 }
 

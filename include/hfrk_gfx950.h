@@ -379,6 +379,97 @@ int hfrk_swiglu_dynamic(const void* gate_up, void* output, float* scales, void* 
 int hfrk_quantize_fp8(const void* input, const float* static_scale, void* output, float* scales, int rows, int cols,
                       int io_dtype, void* stream);
 
+/* Rotary positions.  Frequency j turns a pair of a head's first `rotated` values (an even number) by the angle position * frequency_j:
+ *   (x, y) -> magnitude * (x cos - y sin, y cos + x sin);   pairs (j, j + rotated/2), or (2j, 2j+1) where interleaved != 0
+ * The values behind them are copied.  The angle is formed in double, so far positions lose nothing.
+ *   x, output     16-bit (dtype) [tokens, heads, head_dim], unit stride in a head, strides between tokens and heads in elements; output may be x
+ *                 itself and must not overlap it otherwise
+ *   positions     [tokens] int32, or int64 with positions_wide != 0
+ *   frequencies   [rotated/2] radians per position, fp32, or fp64 with frequencies_wide != 0
+ * head_dim <= 1024.  Heads of whole 16 values on 16-byte boundaries take the vectorised kernel. */
+int hfrk_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* output, int64_t output_token_stride, int64_t output_head_stride,
+                const void* positions, int positions_wide, const void* frequencies, int frequencies_wide, float magnitude, int interleaved, int tokens,
+                int heads, int head_dim, int rotated, int dtype, void* stream);
+
+/* Appends a step's keys and values to a paged cache, the keys rotated on the way (rotated > 0, as in hfrk_rotary), and rotates the step's
+ * queries in the same launch (heads > 0).
+ *   key, value      16-bit (dtype) [tokens, kv_heads, head_dim], strides in elements
+ *   key_cache, value_cache   [pages, page_size, kv_heads, head_dim] of dtype, or e4m3fn (cache_dtype HFRK_FP8_E4M3FN), unit stride in a head and any
+ *                   strides (elements) between pages, a page's places and heads: tokens-major or heads-major pages
+ *   slots           [tokens] int32, or int64 with slots_wide != 0: token t goes to place slot % page_size of page slot / page_size; a slot that is
+ *                   negative or past the last page is not written (padding).  Slots that name one place twice leave either's values there
+ *   key_scale, value_scale   e4m3fn caches: e4m3fn(clamp(x / scale, +-448)), fp32 scales on the device, one (stride 0) or one a head (1); NULL: 1
+ *   query, query_output      as x and output of hfrk_rotary
+ * Nothing may overlap but query and query_output where they are the same. */
+typedef struct hfrk_append_args {
+    const void* query;
+    int64_t query_token_stride, query_head_stride;
+    void* query_output;
+    int64_t output_token_stride, output_head_stride;
+    const void* key;
+    int64_t key_token_stride, key_head_stride;
+    const void* value;
+    int64_t value_token_stride, value_head_stride;
+    void* key_cache;
+    int64_t key_page_stride, key_place_stride, key_cache_head_stride;
+    void* value_cache;
+    int64_t value_page_stride, value_place_stride, value_cache_head_stride;
+    const void* slots;
+    const void* positions;
+    const void* frequencies;
+    const float* key_scale;
+    const float* value_scale;
+    int key_scale_stride, value_scale_stride;
+    int slots_wide, positions_wide, frequencies_wide;
+    float magnitude;
+    int interleaved, tokens, heads, kv_heads, head_dim, rotated, pages, page_size, dtype, cache_dtype;
+} hfrk_append_args;
+
+int hfrk_append_kv(const hfrk_append_args* args, void* stream);
+
+/* Attention of a step's queries over a paged cache that holds the step's own keys and values too.
+ *   Sequence b has lengths[b] cached tokens; the last of them are its step's: rows starts[b] .. starts[b+1] of query.  Row i of a sequence (0 the first)
+ *   sees every token in front of the step's, and of the step's the j <= i (mask NULL: one token, or a chain), or the j with mask[row][j] != 0 (a tree).
+ *   output[row, head] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * key_scale * (q . k_j));  zero where a row sees nothing
+ *   query         16-bit (dtype) [tokens, heads, head_dim]; heads a multiple of kv_heads, query heads h * heads/kv_heads ... share key head h
+ *   output        [tokens, heads, head_dim] of dtype, or e4m3fn(clamp(result / out_scale[0], +-448)) where out_scale is not NULL.  Rows of no
+ *                 sequence are left as they are
+ *   key_cache, value_cache, key_scale, value_scale   as in hfrk_append_kv; the values are scale * e4m3fn
+ *   page_table    [seqs, table_columns] int32, rows table_stride elements apart: token t of a sequence is at place t % page_size of page
+ *                 page_table[b][t / page_size].  A token whose entry is no page, or lies behind the row's end, is seen by nobody and not read
+ *   lengths       [seqs] int32;  starts [seqs + 1] int32, not decreasing, or NULL: tokens / seqs rows each
+ *   mask          bytes [tokens, mask_columns], rows mask_stride bytes apart, or NULL
+ * Lengths, starts and tables are read on the device: a captured call may be replayed with others.  The number of parts that a sequence's tokens are
+ * split into follows from all lengths of the call, and with it the order of the sums; equal calls give equal bits.
+ * head_dim at least 16, a multiple of 8 up to 128, of 16 (e4m3fn caches: always) up to 256; page_size a multiple of 8; query, caches and 16-bit output on 16-byte
+ * boundaries with strides of whole 16-byte pieces; scale > 0; table_columns * page_size <= 2^30, tokens * heads <= 2^28.
+ * workspace: hfrk_tree_attention_workspace_bytes of it (0: none), 16-byte aligned, any contents, used by one call at a time. */
+typedef struct hfrk_attention_args {
+    const void* query;
+    int64_t query_token_stride, query_head_stride;
+    void* output;
+    int64_t output_token_stride, output_head_stride;
+    const void* key_cache;
+    int64_t key_page_stride, key_place_stride, key_cache_head_stride;
+    const void* value_cache;
+    int64_t value_page_stride, value_place_stride, value_cache_head_stride;
+    const int32_t* page_table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* starts;
+    const void* mask;
+    int64_t mask_stride;
+    const float* key_scale;
+    const float* value_scale;
+    const float* out_scale;
+    int key_scale_stride, value_scale_stride;
+    float scale;
+    int tokens, seqs, heads, kv_heads, head_dim, pages, page_size, table_columns, mask_columns, dtype, cache_dtype;
+} hfrk_attention_args;
+
+size_t hfrk_tree_attention_workspace_bytes(const hfrk_attention_args* args);
+int hfrk_tree_attention(const hfrk_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

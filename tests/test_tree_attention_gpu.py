@@ -1,0 +1,321 @@
+"""Attention over a paged cache against float64, at the sizes, masks and layouts where a kernel can go wrong."""
+import math
+
+import pytest
+import torch
+
+from hf_rocm_kernels import append_kv, rotary_frequencies, tree_attention
+from oracle import attention as oracle
+
+pytestmark = pytest.mark.gpu
+
+FP8 = torch.float8_e4m3fn
+
+
+class Step:
+    """A step's queries and the cache they read, on the CPU: pages in a random order, memory that nobody may read filled with NaN."""
+
+    def __init__(self, lengths, counts, heads, kv_heads, head_dim, page, dtype=torch.bfloat16, cache=None, layout="tokens", tree=None, seed=0, extra=0,
+                 uniform=False, loud=1.0):
+        g = self.g = torch.Generator().manual_seed(seed)
+        cache = cache or dtype
+        self.dtype, self.cache, self.lengths, self.counts = dtype, cache, lengths, counts
+        seqs, total = len(lengths), sum(counts)
+        need = [-(-n // page) for n in lengths]
+        columns = max(max(need), 1) + 1
+        order = torch.randperm(sum(need) + 3, generator=g).tolist()
+        pages = len(order)
+        self.table = torch.full((seqs, columns), -1, dtype=torch.int32)
+        for b, n in enumerate(need):
+            for i in range(n):
+                self.table[b, i] = order.pop()
+        shape = (pages, kv_heads, page, head_dim) if layout == "heads" else (pages, page, kv_heads, head_dim)
+        caches = [torch.full(shape, math.nan).to(cache) for _ in range(2)]
+        if layout == "heads":
+            caches = [c.transpose(1, 2) for c in caches]
+        for c in caches:
+            bytes_ = c.view(torch.uint8) if cache == FP8 else c
+            for b, n in enumerate(lengths):
+                for i in range(need[b]):
+                    rows = min(page, n - i * page)
+                    x = torch.randn(rows, kv_heads, head_dim, generator=g) * (60.0 if cache == FP8 else 1.0)
+                    x = x.clamp(-448, 448).to(cache)
+                    bytes_[int(self.table[b, i]), :rows] = x.view(torch.uint8) if cache == FP8 else x
+        self.key, self.value = caches
+        self.layout = layout
+        self.query = (torch.randn(total + extra, heads, head_dim, generator=g) * loud).to(dtype)
+        self.starts = None if uniform else torch.tensor([sum(counts[:b]) for b in range(seqs + 1)], dtype=torch.int32)
+        self.mask = None
+        if tree is not None:
+            width = max(counts) if tree == "full" else tree if isinstance(tree, int) else max(counts)
+            sees = torch.rand(total + extra, max(width, 1), generator=g) < 0.4
+            self.mask = sees[:, :width] if width else sees[:, :0]
+        self.key_scale = self.value_scale = None
+        if cache == FP8:
+            self.key_scale = torch.rand(kv_heads, generator=g) * 0.02 + 0.01
+            self.value_scale = torch.tensor([0.0173])
+        self.scale = 1.0 / math.sqrt(head_dim)
+
+    def args(self):
+        def up(t):
+            return None if t is None else t.cuda()
+        # (.cuda() keeps a transposed view's strides)
+        return dict(query=up(self.query), key_cache=up(self.key), value_cache=up(self.value), page_table=up(self.table),
+                    lengths=torch.tensor(self.lengths, dtype=torch.int32, device="cuda"), starts=up(self.starts), mask=up(self.mask),
+                    key_scale=up(self.key_scale), value_scale=up(self.value_scale))
+
+    def check(self, got, out_scale=None, lengths=None):
+        found = oracle.attention(self.query, self.key, self.value, self.table, torch.tensor(lengths or self.lengths), self.starts, self.mask, self.scale,
+                                 self.key_scale, self.value_scale)
+        want = found[0]
+        got = got.cpu().double() * (1.0 if out_scale is None else out_scale)
+        rows = sum(self.counts)
+        tol = oracle.attention_tolerance(found, self.dtype, max(max(self.lengths), 1), None if out_scale is None else FP8, out_scale or 1.0)[:rows]
+        want, got = want[:rows], got[:rows]
+        if out_scale is not None:
+            want = want.clamp(-448 * out_scale, 448 * out_scale)
+        fine = torch.isfinite(want)
+        assert torch.equal(fine, torch.isfinite(got)), "infinities or NaN in other places"
+        assert torch.equal(torch.isnan(want), torch.isnan(got)) and torch.equal(want[~fine & ~torch.isnan(want)], got[~fine & ~torch.isnan(got)])
+        off = (got - want).abs()[fine]
+        worst = float((off / tol[fine]).max()) if off.numel() else 0.0
+        assert worst <= 1.0, worst
+
+
+TYPES = [(torch.bfloat16, None), (torch.float16, None), (torch.bfloat16, FP8), (torch.float16, FP8)]
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("head_dim", [16, 64, 80, 96, 128, 144, 256])
+def test_one_token_of_each_length(dtype, cache, head_dim):
+    """Lengths around every boundary: a lane's eight tokens, a wave's 32, a workgroup's 128, a page's end, a split."""
+    lengths = [1, 7, 8, 9, 31, 32, 33, 64, 127, 128, 129, 200, 257, 0, 16, 500]
+    step = Step(lengths, [1] * len(lengths), 8, 2, head_dim, 24, dtype, cache, uniform=True, seed=head_dim)
+    step.check(tree_attention(**step.args()))
+
+
+@pytest.mark.parametrize("head_dim", [40, 72, 104])
+def test_heads_that_end_inside_a_window(head_dim):
+    step = Step([100, 33], [1, 1], 6, 3, head_dim, 16, torch.float16, uniform=True, layout="heads")
+    step.check(tree_attention(**step.args()))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 4), (32, 8), (5, 1), (35, 5), (14, 2), (16, 1), (48, 2)])
+@pytest.mark.parametrize("page,layout", [(8, "tokens"), (16, "heads"), (40, "tokens"), (1000, "heads")])
+def test_head_groups_and_pages(heads, kv_heads, page, layout):
+    step = Step([130, 77, 300], [1, 1, 1], heads, kv_heads, 64, page, torch.bfloat16, layout=layout, seed=heads)
+    step.check(tree_attention(**step.args()))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("counts", [[3, 1, 5], [9, 16, 1, 0, 7], [27, 40], [70, 1, 0, 33]])
+@pytest.mark.parametrize("tree", [False, True])
+def test_chains_and_trees(dtype, cache, head_dim, counts, tree):
+    """Blocks of 16, 32 and 64 rows, the last of a sequence ragged; sequences with no token, masks with empty rows, rows of nobody behind the last."""
+    lengths = [n + 37 * (i + 1) for i, n in enumerate(counts)]
+    lengths[0] = counts[0]  # nothing in front of the step: rows that see nothing
+    step = Step(lengths, counts, 8, 2, head_dim, 16, dtype, cache, tree="full" if tree else None, seed=sum(counts), extra=2)
+    if tree:
+        step.mask[1] = False
+    out = torch.full(step.query.shape, 7.0, dtype=dtype, device="cuda")
+    got = tree_attention(**step.args(), output=out)
+    assert got.data_ptr() == out.data_ptr()
+    step.check(got)
+    assert (got[sum(counts):] == 7.0).all()
+
+
+@pytest.mark.parametrize("seqs,most", [(70, 1), (130, 3), (3, 1)])
+def test_many_sequences(seqs, most):
+    """More sequences than a wave has lanes; some empty, one much longer than the others."""
+    g = torch.Generator().manual_seed(seqs)
+    counts = torch.randint(0, most + 1, (seqs,), generator=g).tolist()
+    lengths = [0 if n == 0 and i % 2 else n + int(torch.randint(0, 40, (1,), generator=g)) for i, n in enumerate(counts)]
+    counts[seqs // 2], lengths[seqs // 2] = most, 1500
+    step = Step(lengths, counts, 4, 2, 64, 16, torch.float16, seed=seqs)
+    step.check(tree_attention(**step.args()))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("counts,length", [([1], 5000), ([20], 3000), ([6, 1], 2500)])
+def test_long_caches_split_between_workgroups(dtype, cache, counts, length):
+    lengths = [length - 700 * i for i in range(len(counts))]
+    step = Step(lengths, counts, 4, 1, 128, 32, dtype, cache, seed=length, loud=3.0)
+    first = tree_attention(**step.args())
+    step.check(first)
+    again = tree_attention(**step.args())
+    assert torch.equal(first, again)  # equal calls, equal bits
+
+
+@pytest.mark.parametrize("dtype,cache", [(torch.bfloat16, None), (torch.float16, FP8)])
+def test_output_in_fp8(dtype, cache):
+    step = Step([300, 20, 0], [2, 5, 1], 8, 2, 128, 16, dtype, cache, seed=4)
+    for s in (0.004, 0.0002):  # the second saturates
+        got = tree_attention(**step.args(), out_scale=torch.tensor([s], device="cuda"))
+        assert got.dtype == FP8
+        step.check(got.float(), out_scale=float(torch.tensor(s)))
+
+
+def test_a_step_longer_than_its_cache_and_pages_that_are_missing():
+    step = Step([3, 90, 60, 50], [6, 2, 2, 4], 4, 2, 64, 16, seed=2)
+    step.table[1, 2] = -1          # a hole
+    step.table[2, :] = 10 ** 6     # no page of it exists: zeros
+    step.table[3, 0] = -2147483648
+    step.lengths[3] = 10 ** 9      # longer than its row of the table
+    step.lengths[1] = 89
+    args = step.args()
+    got = tree_attention(**args)
+    step.check(got)
+    assert (got[8:10] == 0).all()
+
+
+@pytest.mark.parametrize("width", [0, 2])
+def test_masks_with_fewer_columns_than_the_step(width):
+    step = Step([40, 6], [5, 6], 4, 2, 64, 16, tree=width, seed=6)
+    step.check(tree_attention(**step.args()))
+    step.mask = (step.mask * 255).to(torch.uint8)  # bytes, any but zero
+    step.check(tree_attention(**step.args()))
+
+
+@pytest.mark.parametrize("dtype,cache,what", [(d, None, w) for d in (torch.bfloat16, torch.float16) for w in (math.nan, math.inf, -math.inf)] +
+                         [(torch.bfloat16, FP8, math.nan)])  # (e4m3fn has no infinities)
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_infinities_and_nan_of_drafted_tokens_reach_only_those_who_see_them(dtype, cache, what, head_dim):
+    for counts in ([5, 1], [20, 3], [40]):
+        step = Step([n + 30 for n in counts], counts, 4, 2, head_dim, 8, dtype, cache, tree="full", seed=9)
+        token = step.lengths[0] - counts[0] + 2  # the third drafted token
+        page, place = int(step.table[0, token // 8]), token % 8
+        if cache == FP8:
+            step.value.view(torch.uint8)[page, place, 1, 3] = 0x7f
+        else:
+            step.value[page, place, 1, 3] = what
+        for i in range(counts[0]):
+            step.mask[i, 2] = i % 2 == 0
+        step.check(tree_attention(**step.args()))
+        # a key that nobody sees
+        step.mask[:counts[0], 2] = False
+        step.key.view(torch.uint8)[page, place] = 0x7f
+        if cache is None:
+            step.key[page, place] = what
+        step.check(tree_attention(**step.args()))
+
+
+def test_a_weight_that_underflows_and_scores_far_apart():
+    step = Step([200], [3], 4, 2, 64, 16, torch.float16, seed=3, loud=60.0)
+    step.check(tree_attention(**step.args()))
+
+
+def test_strides():
+    """A projection's slice as the query, keys and values of a page in one tensor, a table and a mask cut from wider ones."""
+    step = Step([100, 45], [4, 3], 8, 2, 64, 16, tree="full", seed=12)
+    args = step.args()
+    want = tree_attention(**args)
+    step.check(want)
+    rows = torch.zeros(7, 13, 64, dtype=torch.bfloat16, device="cuda")
+    rows[:, 2:10] = args["query"]
+    both = torch.stack((args["key_cache"], args["value_cache"]), dim=1)
+    table = torch.full((2, 50), -7, dtype=torch.int32, device="cuda")
+    table[:, 3:3 + step.table.shape[1]] = args["page_table"]
+    mask = torch.ones(7, 30, dtype=torch.bool, device="cuda")
+    mask[:, 5:5 + step.mask.shape[1]] = args["mask"]
+    wide = torch.zeros(7, 20, 64, dtype=torch.bfloat16, device="cuda")
+    got = tree_attention(rows[:, 2:10], both[:, 0], both[:, 1], table[:, 3:3 + step.table.shape[1]], args["lengths"], args["starts"],
+                         mask[:, 5:5 + step.mask.shape[1]], output=wide[:, 4:12])
+    assert torch.equal(got, want) and not wide[:, :4].any() and not wide[:, 12:].any()
+    by_heads = args["query"].transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(tree_attention(**{**args, "query": by_heads}), want)
+
+
+def test_offsets_past_32_bits():
+    memory = torch.zeros(2, 3, 1 << 30, dtype=torch.bfloat16, device="cuda")
+    far = [memory[i].view(-1).as_strided((3, 16, 2, 64), (1 << 30, 128, 64, 1)) for i in range(2)]
+    step = Step([40], [2], 4, 2, 64, 16, seed=1)
+    args = step.args()
+    used = step.table[0, :3].tolist()
+    for c, name in zip(far, ("key_cache", "value_cache")):
+        for i, p in enumerate(used):
+            c[i] = args[name][p]
+    table = torch.tensor([[0, 1, 2]], dtype=torch.int32, device="cuda")
+    got = tree_attention(**{**args, "key_cache": far[0], "value_cache": far[1], "page_table": table})
+    assert torch.equal(got, tree_attention(**args))
+
+
+def test_nothing_to_do():
+    step = Step([5], [1], 4, 2, 64, 16, uniform=True)
+    args = step.args()
+    none = tree_attention(**{**args, "query": args["query"][:0]})
+    assert none.shape == (0, 4, 64)
+    no_seqs = {**args, "query": args["query"][:0], "page_table": args["page_table"][:0], "lengths": args["lengths"][:0]}
+    assert tree_attention(**no_seqs).shape == (0, 4, 64)
+
+
+def test_two_streams_at_once():
+    steps = [Step([4000], [1], 8, 2, 128, 16, seed=s) for s in (1, 2)]
+    args = [s.args() for s in steps]
+    want = [tree_attention(**a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(tree_attention(**args[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
+def test_graphs_replayed_with_other_lengths():
+    """A captured step follows what the lengths, the table and the cache hold at its replay; two graphs have workspaces of their own."""
+    step = Step([3000, 900], [2, 2], 8, 2, 128, 16, seed=5)
+    args = step.args()
+    tree_attention(**args)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(tree_attention(**args))
+        graphs.append(graph)
+    for lengths in ([3000, 900], [10, 2500], [2, 2], [1700, 3]):
+        args["lengths"].copy_(torch.tensor([min(lengths[0], 3000), min(lengths[1], 900)]))
+        want = tree_attention(**args)
+        for out in outs:
+            out.fill_(math.nan)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out in outs)
+
+
+@pytest.mark.parametrize("cache", [None, FP8])
+def test_a_run_of_steps(cache):
+    """Prompts, then drafted trees, then single tokens through append and attention, as they are used; the cache the oracle reads is what the
+    append has written."""
+    g = torch.Generator().manual_seed(11)
+    heads, kv_heads, head_dim, page, seqs = 8, 2, 64, 16, 2
+    pages = 20
+    caches = [torch.full((pages, page, kv_heads, head_dim), math.nan).to(cache or torch.bfloat16).cuda() for _ in range(2)]
+    table = torch.randperm(pages, generator=g)[:seqs * 6].view(seqs, 6).int()
+    scales = [torch.tensor([0.02], device="cuda"), torch.tensor([0.015], device="cuda")] if cache else [None, None]
+    frequencies, magnitude = rotary_frequencies(head_dim, 500000.0, {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32})
+    held = [0, 0]
+    for counts, tree in (([40, 23], False), ([5, 7], True), ([1, 1], False), ([3, 0], False)):
+        total = sum(counts)
+        rows = torch.randn(total, heads + 2 * kv_heads, head_dim, generator=g).to(torch.bfloat16).cuda()
+        lengths = [h + n for h, n in zip(held, counts)]
+        at = [(b, t) for b in range(seqs) for t in range(held[b], lengths[b])]
+        slots = torch.tensor([int(table[b, t // page]) * page + t % page for b, t in at], device="cuda")
+        positions = torch.tensor([t for _, t in at], device="cuda")
+        query = append_kv(rows[:, heads:heads + kv_heads], rows[:, heads + kv_heads:], *caches, slots, positions, frequencies, magnitude=magnitude,
+                          query=rows[:, :heads], key_scale=scales[0], value_scale=scales[1])
+        mask = (torch.rand(total, max(counts), generator=g) < 0.5) if tree else None
+        starts = torch.tensor([0, counts[0], total], dtype=torch.int32)
+        got = tree_attention(query, *caches, table.cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"), starts.cuda(),
+                             None if mask is None else mask.cuda(), key_scale=scales[0], value_scale=scales[1])
+        found = oracle.attention(query.cpu(), caches[0].cpu(), caches[1].cpu(), table, torch.tensor(lengths), starts, mask, head_dim ** -0.5,
+                                 *[None if s is None else s.cpu() for s in scales])
+        assert ((got.cpu().double() - found[0]).abs() <= oracle.attention_tolerance(found, torch.bfloat16, max(lengths))).all()
+        held = lengths
