@@ -10,6 +10,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <cmath>
+
 #include "hfrk_gfx950.h"
 
 namespace {
@@ -1062,6 +1064,47 @@ void tree_attention(const at::Tensor& query, const at::Tensor& key_cache, const 
     raise_on(run_attention(a, query), "tree_attention");
 }
 
+// The same as their wrappers usually call them, allocation and checks in one native operator: a rotation of one token 7.8 -> 5.4 us a call, an append
+// of 32 tokens 12.0 -> 6.4.  What is none of the calls above is answered with no tensor, nothing launched: the wrapper then says what is wrong.
+at::Tensor rotary_new(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& frequencies, double magnitude, bool interleaved) {
+    if (!x.is_cuda()) return {};
+    DeviceScope scope(x);
+    at::Tensor output = at::empty(x.sizes(), x.options());
+    hfrk_append_args a = {};
+    if (rotary_args(a, x, positions, frequencies, magnitude, interleaved, output)) return {};
+    return hfrk_append_kv(&a, current_stream(x)) == HFRK_SUCCESS ? output : at::Tensor();
+}
+
+// (done, the rotated queries: none without a query)
+std::tuple<bool, at::Tensor> append_kv_new(const at::Tensor& key, const at::Tensor& value, at::Tensor& key_cache, at::Tensor& value_cache,
+                                           const at::Tensor& slots, const std::optional<at::Tensor>& positions, const std::optional<at::Tensor>& frequencies,
+                                           double magnitude, bool interleaved, const std::optional<at::Tensor>& query,
+                                           const std::optional<at::Tensor>& key_scale, const std::optional<at::Tensor>& value_scale) {
+    if (!key.is_cuda() || (query.has_value() && !frequencies.has_value())) return {false, at::Tensor()};
+    DeviceScope scope(key);
+    at::Tensor output = query.has_value() ? at::empty(query->sizes(), query->options()) : at::Tensor();
+    hfrk_append_args a = {};
+    if (append_args(a, key, value, key_cache, value_cache, slots, positions, frequencies, magnitude, interleaved, query, query.has_value() ? output : key,
+                    key_scale, value_scale) ||
+        hfrk_append_kv(&a, current_stream(key)) != HFRK_SUCCESS)
+        return {false, at::Tensor()};
+    return {true, output};
+}
+
+at::Tensor tree_attention_new(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& page_table,
+                              const at::Tensor& lengths, const std::optional<at::Tensor>& starts, const std::optional<at::Tensor>& mask,
+                              std::optional<double> scale, const std::optional<at::Tensor>& key_scale, const std::optional<at::Tensor>& value_scale,
+                              const std::optional<at::Tensor>& out_scale) {
+    if (!query.is_cuda() || query.dim() != 3 || query.size(2) < 1) return {};
+    DeviceScope scope(query);
+    at::Tensor output = at::empty(query.sizes(), out_scale.has_value() ? query.options().dtype(at::kFloat8_e4m3fn) : query.options());
+    hfrk_attention_args a = {};
+    if (attention_args(a, query, key_cache, value_cache, page_table, lengths, starts, mask, scale.has_value() ? *scale : 1.0 / std::sqrt((double)query.size(2)),
+                       key_scale, value_scale, out_scale, output))
+        return {};
+    return run_attention(a, query) == HFRK_SUCCESS ? output : at::Tensor();
+}
+
 }  // namespace
 
 TORCH_LIBRARY(_HFRK_C, ops) {
@@ -1167,6 +1210,19 @@ TORCH_LIBRARY(_HFRK_C, ops) {
         "tree_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor page_table, Tensor lengths, Tensor? starts, Tensor? mask, "
         "float scale, Tensor? key_scale, Tensor? value_scale, Tensor? out_scale, Tensor(a!) output) -> ()");
     ops.impl("tree_attention", c10::kCUDA, &tree_attention);
+
+    ops.def("rotary_new(Tensor x, Tensor positions, Tensor frequencies, float magnitude, bool interleaved) -> Tensor");
+    ops.impl("rotary_new", c10::kCUDA, &rotary_new);
+    ops.def(
+        "append_kv_new(Tensor key, Tensor value, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots, Tensor? positions, Tensor? frequencies, "
+        "float magnitude, bool interleaved, Tensor? query, Tensor? key_scale, Tensor? value_scale) -> (bool, Tensor)");
+    ops.impl("append_kv_new", c10::kCUDA, &append_kv_new);
+    ops.def(
+        "tree_attention_new(Tensor query, Tensor key_cache, Tensor value_cache, Tensor page_table, Tensor lengths, Tensor? starts, Tensor? mask, "
+        "float? scale, Tensor? key_scale, Tensor? value_scale, Tensor? out_scale) -> Tensor");
+    ops.impl("tree_attention_new", c10::kCUDA, &tree_attention_new);
+    for (const char* name : {"rotary_new", "append_kv_new", "tree_attention_new"})
+        ops.impl(name, torch::dispatch(c10::DispatchKey::Autograd, torch::CppFunction::makeFallthrough()));
 
     ops.def("quantize_fp8(Tensor input, Tensor? scale_tensor, Tensor! output, Tensor! scales) -> ()");
     ops.impl("quantize_fp8", c10::kCUDA, &quantize_fp8);

@@ -21,7 +21,7 @@ _RETURNS_STATUS = ("skinny_gemm_tb", "skinny_gemm_scaled", "skinny_gemm_fused", 
                    # a result of their own, _OTHER_RESULT; the wrappers keep fake calls away from these (utils/dispatch.py), a caller of
                    # torch.ops need not
                    "fp8_linear", "skinny_gemm_new", "skinny_gemm_into", "llama_mlp", "residual_rms_new", "residual_rms_dynamic_new", "swiglu_new",
-                   "swiglu_dynamic_new")
+                   "swiglu_dynamic_new", "rotary_new", "append_kv_new", "tree_attention_new")
 
 
 def _nothing(*args, **kwargs) -> None:
@@ -57,6 +57,18 @@ def _swiglu_dynamic_new(gate_up):
     return _swiglu_new(gate_up), gate_up.new_empty((gate_up.shape[0],), dtype=torch.float32)
 
 
+def _rotary_new(x, positions, frequencies, magnitude, interleaved):
+    return x.new_empty(x.shape)
+
+
+def _append_kv_new(key, value, key_cache, value_cache, slots, positions, frequencies, magnitude, interleaved, query, key_scale, value_scale):
+    return True, None if query is None else query.new_empty(query.shape)
+
+
+def _tree_attention_new(query, key_cache, value_cache, page_table, lengths, starts, mask, scale, key_scale, value_scale, out_scale):
+    return query.new_empty(query.shape, dtype=query.dtype if out_scale is None else torch.float8_e4m3fn)
+
+
 def _unless_mixed(answer, refusal):
     """A whole-call operator also lands here when one tensor among device tensors is a meta tensor, which the wrapper's look at its first
     argument does not show: that is no call of the operator's, and the general way refuses it."""
@@ -71,7 +83,9 @@ def _unless_mixed(answer, refusal):
 _OTHER_RESULT = {"fp8_linear": _unless_mixed(_fp8_linear, None), "skinny_gemm_new": _unless_mixed(_skinny_gemm_new, None),
                  "skinny_gemm_into": _unless_mixed(lambda A, B, scale, D: True, False), "llama_mlp": _unless_mixed(lambda *args, **kwargs: True, False),
                  "residual_rms_new": _unless_mixed(_residual_rms_new, None), "residual_rms_dynamic_new": _unless_mixed(_residual_rms_dynamic_new, (None, None)),
-                 "swiglu_new": _unless_mixed(_swiglu_new, None), "swiglu_dynamic_new": _unless_mixed(_swiglu_dynamic_new, (None, None))}
+                 "swiglu_new": _unless_mixed(_swiglu_new, None), "swiglu_dynamic_new": _unless_mixed(_swiglu_dynamic_new, (None, None)),
+                 "rotary_new": _unless_mixed(_rotary_new, None), "append_kv_new": _unless_mixed(_append_kv_new, (False, None)),
+                 "tree_attention_new": _unless_mixed(_tree_attention_new, None)}
 
 
 def register() -> None:

@@ -3,8 +3,11 @@ from typing import Optional
 import torch
 from torch import Tensor
 
+from ...utils.dispatch import runs_now
 from ..rotary.wrapped import heads_checks, rotation_checks
 from .binding import _append_kv
+
+_append_kv_new = torch.ops._HFRK_C.append_kv_new.default
 
 
 def cache_checks(key_cache: Tensor, value_cache: Tensor, kv_heads: int, head_dim: int, dtype: torch.dtype, device: torch.device) -> None:
@@ -86,6 +89,11 @@ def append_kv(
     Outputs:
         - the rotated queries, None without a query
     """
+    if query_output is None and runs_now(key):
+        done, output = _append_kv_new(key, value, key_cache, value_cache, slots, positions, frequencies, magnitude, interleaved, query, key_scale,
+                                      value_scale)  # one native operator; not done: what is wrong, say the checks
+        if done:
+            return output
     if query is not None and query_output is None:
         query_output = torch.empty(size=query.shape, dtype=query.dtype, device=query.device)
     append_kv_checks(key, value, key_cache, value_cache, slots, positions, frequencies, query, query_output, key_scale, value_scale)

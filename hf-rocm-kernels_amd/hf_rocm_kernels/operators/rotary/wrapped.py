@@ -3,8 +3,10 @@ from typing import Optional
 import torch
 from torch import Tensor
 
+from ...utils.dispatch import runs_now
 from .binding import _rotary
 
+_rotary_new = torch.ops._HFRK_C.rotary_new.default
 _IO_DTYPES = (torch.bfloat16, torch.float16)
 MAX_HEAD_DIM = 1024
 
@@ -57,6 +59,10 @@ def rotary(
     Angles are formed in 64 bits, the rotation in 32, rounded once.  Inference only: the result carries no gradient.
     """
     if output is None:
+        if runs_now(x):
+            output = _rotary_new(x, positions, frequencies, magnitude, interleaved)  # one native operator; None: what is wrong, say the checks
+            if output is not None:
+                return output
         output = torch.empty(size=x.shape, dtype=x.dtype, device=x.device)
     rotary_checks(x, positions, frequencies, output)
     _rotary(x, positions, frequencies, magnitude, interleaved, output)

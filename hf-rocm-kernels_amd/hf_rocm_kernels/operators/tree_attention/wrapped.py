@@ -4,10 +4,12 @@ from typing import Optional
 import torch
 from torch import Tensor
 
+from ...utils.dispatch import runs_now
 from ..append_kv.wrapped import cache_checks, scale_checks
 from ..rotary.wrapped import heads_checks
 from .binding import _tree_attention
 
+_tree_attention_new = torch.ops._HFRK_C.tree_attention_new.default
 MAX_HEAD_DIM = 256
 
 
@@ -90,6 +92,10 @@ def tree_attention(
     Lengths, starts and page_table stay on the device: no call waits for them, and a captured call may be replayed with others.  The result does not depend
     on other streams' calls (each has a workspace of its own), but how a sequence's tokens are split, and with it the last bits, depends on all lengths.
     """
+    if output is None and runs_now(query):
+        output = _tree_attention_new(query, key_cache, value_cache, page_table, lengths, starts, mask, scale, key_scale, value_scale, out_scale)
+        if output is not None:  # one native operator; None: what is wrong, say the checks
+            return output
     if scale is None:
         scale = 1.0 / math.sqrt(query.size(-1))
     if output is None:

@@ -261,3 +261,24 @@ def test_torch_forms_agree_with_the_oracle(interleaved):
 def test_package_lists_its_operators():
     for name in ("rotary", "rotary_frequencies", "append_kv", "tree_attention"):
         assert name in hf_rocm_kernels.__all__ and callable(getattr(hf_rocm_kernels, name))
+
+
+def test_whole_call_operators_take_no_meta_tensor_among_others():
+    """One meta tensor among tensors with data: no result that nobody computed; on meta tensors alone, shapes."""
+    ops = torch.ops._HFRK_C
+
+    def tensors(device, other=None, at=None):
+        def make(i, *shape, dtype=BF16):
+            return torch.empty(*shape, dtype=dtype, device=other if i == at else device)
+        return (make(0, 4, 4, 64), make(1, 4, 2, 64), make(2, 5, 16, 2, 64), make(3, 4, dtype=torch.long), make(4, 32, dtype=torch.float64),
+                make(5, 2, 3, dtype=torch.int32), make(6, 2, dtype=torch.int32))
+
+    turn = lambda q, k, c, p, f, table, n: ops.rotary_new(q, p, f, 1.0, False)
+    append = lambda q, k, c, p, f, table, n: ops.append_kv_new(k, k, c, c, p, p, f, 1.0, False, q, None, None)
+    attend = lambda q, k, c, p, f, table, n: ops.tree_attention_new(q, c, c, table, n, None, None, None, None, None, None)
+    alone = tensors("meta")
+    assert turn(*alone).shape == (4, 4, 64) and append(*alone)[0] and append(*alone)[1].shape == (4, 4, 64) and attend(*alone).shape == (4, 4, 64)
+    for at, call in ((3, turn), (4, turn), (2, attend), (5, attend), (6, attend)):
+        assert call(*tensors("cpu", "meta", at)) is None
+    for at in (1, 2, 3, 4):
+        assert append(*tensors("cpu", "meta", at)) == (False, None)

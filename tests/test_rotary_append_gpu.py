@@ -198,3 +198,42 @@ def test_append_on_another_stream_and_in_a_graph():
         want = step(eager)
         torch.cuda.synchronize()
         assert torch.equal(turned, want) and all(torch.equal(a, b) for a, b in zip(caches, eager))
+
+
+def test_whole_calls_and_general_ones_give_the_same_bits(monkeypatch):
+    from hf_rocm_kernels.operators.append_kv import wrapped as append_wrapped
+    from hf_rocm_kernels.operators.rotary import wrapped as rotary_wrapped
+    g = torch.Generator().manual_seed(2)
+    rows = torch.randn(7, 12, 64, generator=g).to(torch.float16).cuda()
+    positions, frequencies = torch.arange(7, device="cuda"), rotary_frequencies(64)[0]
+
+    def calls():
+        caches = [torch.zeros(2, 16, 2, 64, dtype=torch.float16, device="cuda") for _ in range(4)]
+        with_query = append_kv(rows[:, 8:10], rows[:, 10:], *caches[:2], positions, positions, frequencies, query=rows[:, :8])
+        assert append_kv(rows[:, 8:10], rows[:, 10:], *caches[2:], positions) is None
+        return [rotary(rows, positions, frequencies), with_query, *caches]
+
+    got = calls()
+    monkeypatch.setattr(rotary_wrapped, "_rotary_new", lambda *args: None)
+    monkeypatch.setattr(append_wrapped, "_append_kv_new", lambda *args: (False, None))
+    assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+
+
+def test_refused_on_the_device():
+    """What the checks in front do not see: results that overlap their inputs, and devices."""
+    rows = torch.zeros(3, 6, 64, dtype=torch.bfloat16, device="cuda")
+    positions, frequencies = torch.zeros(3, dtype=torch.long, device="cuda"), torch.ones(32, device="cuda")
+    with pytest.raises(RuntimeError, match="apart"):
+        rotary(rows[:, :4], positions, frequencies, output=rows[:, 1:5])
+    with pytest.raises(RuntimeError, match="apart"):
+        rotary(rows, positions, frequencies, output=rows[:, :1].expand(3, 6, 64))
+    with pytest.raises(AssertionError, match="positions.device"):
+        rotary(rows, positions.cpu(), frequencies)
+    cache = torch.zeros(3, 8, 2, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="same memory"):
+        append_kv(rows[:, 2:4], rows[:, 4:], cache, cache, positions)
+    with pytest.raises(RuntimeError, match="apart"):
+        append_kv(cache[:, 0], rows[:, 4:], cache, torch.zeros_like(cache), positions)
+    with pytest.raises(RuntimeError, match="query_output"):
+        append_kv(rows[:, 2:4], rows[:, 4:], cache, torch.zeros_like(cache), positions, positions, frequencies, query=rows[:, :2].clone(),
+                  query_output=rows[:, 3:5])

@@ -319,3 +319,26 @@ def test_a_run_of_steps(cache):
                                  *[None if s is None else s.cpu() for s in scales])
         assert ((got.cpu().double() - found[0]).abs() <= oracle.attention_tolerance(found, torch.bfloat16, max(lengths))).all()
         held = lengths
+
+
+def test_refused_on_the_device():
+    step = Step([40], [2], 4, 2, 64, 16)
+    args = step.args()
+    with pytest.raises(RuntimeError, match="apart"):
+        tree_attention(**args, output=args["query"])
+    with pytest.raises(RuntimeError, match="aligned"):
+        odd = torch.zeros(2 * 4 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(2, 4, 64)
+        tree_attention(**{**args, "query": odd})
+    with pytest.raises(AssertionError, match="lengths"):
+        tree_attention(**{**args, "lengths": args["lengths"].cpu()})
+
+
+def test_whole_calls_and_general_ones_give_the_same_bits(monkeypatch):
+    from hf_rocm_kernels.operators.tree_attention import wrapped
+    step = Step([1000, 45], [4, 3], 8, 2, 64, 16, tree="full", seed=12)
+    args = step.args()
+    scale = torch.tensor([0.01], device="cuda")
+    calls = lambda: [tree_attention(**args), tree_attention(**args, scale=0.3), tree_attention(**args, out_scale=scale).view(torch.uint8)]
+    got = calls()
+    monkeypatch.setattr(wrapped, "_tree_attention_new", lambda *args: None)
+    assert all(torch.equal(a, b) for a, b in zip(got, calls()))
