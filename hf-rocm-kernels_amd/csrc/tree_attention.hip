@@ -6,6 +6,9 @@ namespace hfrk {
 extern template int launch_attention<64>(const AttentionArgs& p, int col_blocks, int grid, hipStream_t stream);
 extern template int launch_attention<128>(const AttentionArgs& p, int col_blocks, int grid, hipStream_t stream);
 extern template int launch_attention<256>(const AttentionArgs& p, int col_blocks, int grid, hipStream_t stream);
+extern template int launch_attention_shared<64>(const AttentionArgs& p, int grid, hipStream_t stream);
+extern template int launch_attention_shared<128>(const AttentionArgs& p, int grid, hipStream_t stream);
+extern template int launch_attention_shared<256>(const AttentionArgs& p, int grid, hipStream_t stream);
 
 // One wave per row of the result whose tokens were split: a lane has eight columns, lane groups take the splits in turn.  The order of
 // the sums is fixed, so equal calls give equal bits.
@@ -80,7 +83,8 @@ static int check(const hfrk_attention_args& a) {
 
 // Rows of a block, the work list's bounds and the workspace, from what the host knows: sizes, not lengths.
 struct Decomposition {
-    int col_blocks, work, grid, slots;
+    bool shared;
+    int rows, work, grid, slots;
     size_t partial, ml, info;  // bytes
 };
 
@@ -88,9 +92,10 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     Decomposition d = {};
     const int group = a.heads / a.kv_heads;
     const long per = (a.tokens + a.seqs - 1) / a.seqs * (long)group;  // rows of a sequence, on average
-    d.col_blocks = per <= 16 ? 1 : per <= 32 || a.head_dim > 128 ? 2 : 4;
-    d.work = d.col_blocks == 4 ? 512 : 1024;
-    const int rows = 16 * d.col_blocks;
+    d.shared = per > 32;
+    d.rows = per <= 16 ? 16 : per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 || a.head_dim > 128 ? 128 : 256;
+    d.work = d.shared ? 512 : 1024;
+    const int rows = d.rows;
     const long blocks = (long)a.tokens * group / rows + a.seqs;
     const long tiles = ((long)a.table_columns * a.page_size + kTileTokens - 1) / kTileTokens;
     // sequences' splits are rounded up: one more than their share of the work each, and of those that are split at most twice their share
@@ -134,7 +139,7 @@ extern "C" int hfrk_tree_attention(const hfrk_attention_args* args, void* worksp
     }
     p.log2_scale = a.scale * 1.4426950408889634f;
     p.group = a.heads / a.kv_heads;
-    p.rows = 16 * d.col_blocks;
+    p.rows = d.rows;
     p.work = d.work;
     p.slots = d.slots;
     // n / m for n < 2^28, m = page_size / 8: with 2^(l-1) < m <= 2^l, ceil(2^(28+l) / m) is exact enough and has at most 29 bits
@@ -148,8 +153,14 @@ extern "C" int hfrk_tree_attention(const hfrk_attention_args* args, void* worksp
         p.page_shift = l - 1;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int launched = a.head_dim <= 64 ? launch_attention<64>(p, d.col_blocks, d.grid, s)
-                         : a.head_dim <= 128 ? launch_attention<128>(p, d.col_blocks, d.grid, s) : launch_attention<256>(p, d.col_blocks, d.grid, s);
+    int launched;
+    if (d.shared) {
+        launched = a.head_dim <= 64 ? launch_attention_shared<64>(p, d.grid, s)
+                   : a.head_dim <= 128 ? launch_attention_shared<128>(p, d.grid, s) : launch_attention_shared<256>(p, d.grid, s);
+    } else {
+        launched = a.head_dim <= 64 ? launch_attention<64>(p, d.rows / 16, d.grid, s)
+                   : a.head_dim <= 128 ? launch_attention<128>(p, d.rows / 16, d.grid, s) : launch_attention<256>(p, d.rows / 16, d.grid, s);
+    }
     if (launched != HFRK_SUCCESS || d.slots == 0) return launched;
     const long waves = (long)a.tokens * a.heads;
     const dim3 grid((unsigned)((waves + kAttentionWaves - 1) / kAttentionWaves));

@@ -2,7 +2,8 @@
 //
 //   o_i = sum_j 2^(c s_ij - m_i) v_j / sum_j 2^(c s_ij - m_i),  s_ij = q_i . k_j,  c = scale * key_scale * log2(e)
 //
-// over the cached tokens j that row i sees, m_i the largest c s_ij so far (one pass: when it grows, what has been summed is scaled down).
+// over the cached tokens j that row i sees, m_i the largest c s_ij so far or less by at most 8 (one pass: when it follows, what has been summed is
+// scaled down).
 // A row is one drafted token and one of the query heads that share a key head, so a group of heads reads its keys and values once.
 //
 // Each wave takes 32 cached tokens at a time and C blocks of 16 rows, straight from memory to registers and without LDS:
@@ -21,6 +22,8 @@
 #include "tree_attention.h"
 
 namespace hfrk {
+
+constexpr float kHeadroom = 8.f;  // weights may grow to 2^8 before a row's scale follows
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -273,9 +276,10 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
             float most = score[c][0][0];
 #pragma unroll
             for (int j = 1; j < 8; ++j) most = fmaxf(most, score[c][j / 4][j % 4]);
-            most = row_max(most * scale);
-            if (__any(most > top[c])) {
-                const float grown = fmaxf(top[c], most);
+            most *= scale;
+            // a row's scale follows its largest score when a lane has found one 2^8 above it, not with every step
+            if (__any(most > top[c] + kHeadroom)) {
+                const float grown = fmaxf(top[c], row_max(most));
                 const float shrink = top[c] == grown ? 1.f : __builtin_amdgcn_exp2f(top[c] - grown);
                 top[c] = grown;
                 sum[c] *= shrink;
@@ -420,8 +424,7 @@ int launch_attention(const AttentionArgs& p, int col_blocks, int grid, hipStream
 #define HFRK_ATTENTION(DT, FP8)                                                                                                             \
     do {                                                                                                                                    \
         if (col_blocks == 1) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 1>), dim3(grid), dim3(kAttentionThreads), 0, stream, p);      \
-        else if (col_blocks == 2) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(kAttentionThreads), 0, stream, p); \
-        else hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, DP == 256 ? 2 : 4>), dim3(grid), dim3(kAttentionThreads), 0, stream, p);      \
+        else hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(kAttentionThreads), 0, stream, p);                      \
     } while (0)
     if (p.a.dtype == HFRK_BF16) {
         if (fp8) HFRK_ATTENTION(HFRK_BF16, true);
