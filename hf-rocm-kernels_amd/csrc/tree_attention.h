@@ -19,6 +19,7 @@ struct AttentionArgs {
     int slots;                // partial results the workspace holds, per key head
     uint32_t page_magic;      // (t / 8) / (page_size / 8) as a multiplication: n * magic >> (32 + page_shift), or n >> page_shift where magic is 0
     int page_shift;
+    uint32_t key_page_bytes, key_place_bytes, value_page_bytes, value_place_bytes;  // strides, where 32 bits hold them (`narrow`)
     float* partial;           // [slots * kv_heads][rows][head_dim], divided by nothing
     float2* partial_ml;       // [slots * kv_heads][rows]: largest score (in log2 units) and sum
     int4* row_info;           // [tokens * group]: first slot, splits, row in its block
@@ -94,7 +95,7 @@ __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
         }
     }
     const long share = (total * p.a.kv_heads + p.work - 1) / p.work;
-    const int chunk = share < 1 ? 1 : (int)share;
+    const int chunk = __builtin_amdgcn_readfirstlane(share < 1 ? 1 : (int)share);
     int items = 0, slots = 0;
     for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
         int blocks, tiles;
@@ -106,20 +107,21 @@ __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
         const uint64_t found = __ballot(n > 0 && item >= items_to - n && item < items_to);
         if (found) {
             const int who = __ffsll((unsigned long long)found) - 1;
-            const int at = item - (__shfl(items_to, who) - __shfl(n, who));
+            const auto of = [who](int v) { return __builtin_amdgcn_readlane(v, who); };  // (into scalar registers: the same for the whole workgroup)
+            const int at = item - (of(items_to) - of(n));
             part.b = b0 + who;
-            part.splits = __shfl(splits, who);
-            part.block = at / part.splits;
+            part.splits = of(splits);
+            part.block = (uint32_t)at / (uint32_t)part.splits;
             part.split = at - part.block * part.splits;
-            part.slot = __shfl(slots_to, who) - __shfl(held, who) + at;
+            part.slot = of(slots_to) - of(held) + at;
             part.from = part.split * chunk;
-            part.to = min(part.from + chunk, __shfl(tiles, who));
-            part.s = {__shfl(s.first, who), __shfl(s.count, who), __shfl(s.length, who), __shfl(s.drafted, who)};
+            part.to = min(part.from + chunk, of(tiles));
+            part.s = {of(s.first), of(s.count), of(s.length), of(s.drafted)};
             part.any = true;
             return part;
         }
-        items = __shfl(items_to, p.a.seqs > 1 ? kWave - 1 : 0);
-        slots = __shfl(slots_to, p.a.seqs > 1 ? kWave - 1 : 0);
+        items = __builtin_amdgcn_readlane(items_to, p.a.seqs > 1 ? kWave - 1 : 0);
+        slots = __builtin_amdgcn_readlane(slots_to, p.a.seqs > 1 ? kWave - 1 : 0);
     }
     return part;
 }

@@ -88,12 +88,19 @@ struct Decomposition {
     size_t partial, ml, info;  // bytes
 };
 
+// Whether 32 bits hold a cache's strides and offsets in a page in bytes, as the kernels with LDS take them.
+static bool narrow(int64_t page, int64_t place, int page_size, int size) {
+    return page >= 0 && place >= 0 && page * size < (1LL << 32) && place * size * page_size < (1LL << 31);
+}
+
 static Decomposition decompose(const hfrk_attention_args& a) {
     Decomposition d = {};
     const int group = a.heads / a.kv_heads;
     const long per = (a.tokens + a.seqs - 1) / a.seqs * (long)group;  // rows of a sequence, on average
-    d.shared = per > 32;
-    d.rows = per <= 16 ? 16 : per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 || a.head_dim > 128 ? 128 : 256;
+    const int size = a.cache_dtype == HFRK_FP8_E4M3FN ? 1 : 2;
+    d.shared = per > 32 && narrow(a.key_page_stride, a.key_place_stride, a.page_size, size) &&
+               narrow(a.value_page_stride, a.value_place_stride, a.page_size, size);
+    d.rows = per <= 16 ? 16 : per <= 32 || !d.shared ? 32 : per <= 64 ? 64 : per <= 128 || a.head_dim > 128 ? 128 : 256;
     d.work = d.shared ? 512 : 1024;
     const int rows = d.rows;
     const long blocks = (long)a.tokens * group / rows + a.seqs;
@@ -142,6 +149,11 @@ extern "C" int hfrk_tree_attention(const hfrk_attention_args* args, void* worksp
     p.rows = d.rows;
     p.work = d.work;
     p.slots = d.slots;
+    const uint32_t size = a.cache_dtype == HFRK_FP8_E4M3FN ? 1 : 2;
+    p.key_page_bytes = (uint32_t)a.key_page_stride * size;
+    p.key_place_bytes = (uint32_t)a.key_place_stride * size;
+    p.value_page_bytes = (uint32_t)a.value_page_stride * size;
+    p.value_place_bytes = (uint32_t)a.value_place_stride * size;
     // n / m for n < 2^28, m = page_size / 8: with 2^(l-1) < m <= 2^l, ceil(2^(28+l) / m) is exact enough and has at most 29 bits
     const uint32_t m = (uint32_t)a.page_size / 8;
     int l = 0;

@@ -98,6 +98,93 @@ __device__ __forceinline__ uint32_t counted(uint32_t pair, uint32_t bits, uint32
     return (((nan | ~(pair ^ sign)) & bits) >> 15) * one;  // (`bits` has the halves' top bits only)
 }
 
+// Of the eight cached tokens from `first` on, those that a lane's C rows see: bit j token first + j.  page: they have one; seen_to: the last token a
+// row of a chain sees; sees: a row of the mask.
+template <int C>
+__device__ __forceinline__ void sight(const hfrk_attention_args& a, const Sequence& s, int first, bool page, const int (&seen_to)[C],
+                                      const uint8_t* const (&sees)[C], uint32_t (&seen)[C]) {
+    const auto first_of_8 = [](int n) { return (1u << min(max(n, 0), 8)) - 1u; };
+    const int at = first - s.drafted;  // of the first token among the drafted ones
+    const int known = min(s.count, a.mask_columns);
+    const uint32_t here = page ? first_of_8(s.length - first) : 0u;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if (a.mask) {
+            uint32_t bits = 0;
+            if (known > 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) bits |= min((uint32_t)sees[c][min(max(at + j, 0), known - 1)], 1u) << j;
+            }
+            seen[c] = ((bits & first_of_8(known - at)) | first_of_8(-at)) & here;
+        } else {
+            seen[c] = first_of_8(seen_to[c] + 1 - first) & here;
+        }
+    }
+}
+
+// Infinities and NaN among drafted tokens' values: which of a lane's sums one of either sign has reached (a NaN counts as both), a bit for each.
+template <int DT, int DP, int C>
+struct Marks {
+    static constexpr int kCols = DP / 16, kWords = (4 * kCols + 31) / 32;
+    uint32_t rise[C][kWords] = {}, fall[C][kWords] = {};
+
+    // `values`: in LDS, the lane's part of the operand of V^T's first 16-row block, the others 1 KB apart.  One block at a time, in a loop: unrolled, this
+    // rare path takes the registers of the usual one.
+    __device__ __forceinline__ void note(const uint32_t (&seen)[C], const v4i* values) {
+        constexpr uint32_t one = DT == HFRK_BF16 ? 0x3f80u : 0x3c00u;
+#pragma unroll 1
+        for (int f = 0; f < kCols; ++f) {
+            const v4i v = values[f * kWave];
+            v4i plus, minus;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t bits = unbounded<DT>((uint32_t)v[q]);
+                plus[q] = (int)counted<DT>((uint32_t)v[q], bits, 0u);
+                minus[q] = (int)counted<DT>((uint32_t)v[q], bits, 0x80008000u);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                v4i sights;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sights[q] = (int)(((seen[c] >> 2 * q & 1u) | (seen[c] >> (2 * q + 1) & 1u) << 16) * one);
+                const v4f none = {0.f, 0.f, 0.f, 0.f};
+                const v4f up = mfma16<DT>(plus, sights, none), down = mfma16<DT>(minus, sights, none);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {  // (a word holds 32 / kCols runs r of kCols bits)
+                    rise[c][r * kCols / 32] |= (up[r] > 0.f ? 1u : 0u) << (r * kCols % 32 + f);
+                    fall[c][r * kCols / 32] |= (down[r] > 0.f ? 1u : 0u) << (r * kCols % 32 + f);
+                }
+            }
+        }
+    }
+
+    // The same values without them.
+    static __device__ __forceinline__ v4i cleaned(v4i v) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] &= (int)~halves(unbounded<DT>((uint32_t)v[q]));
+        return v;
+    }
+
+    __device__ __forceinline__ void apply(v4f (&out)[C][kCols]) const {
+        uint32_t any = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) any |= rise[c][w] | fall[c][w];
+        if (!__any(any != 0)) return;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int f = 0; f < kCols; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int bit = r * kCols + f;
+                    if (rise[c][bit / 32] >> bit % 32 & 1) out[c][f][r] += INFINITY;
+                    if (fall[c][bit / 32] >> bit % 32 & 1) out[c][f][r] -= INFINITY;
+                }
+    }
+};
+
 // One wave's operands of 32 cached tokens.
 template <int DP, bool FP8>
 struct CachedTile {
@@ -203,6 +290,7 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
     constexpr int kOne = DT == HFRK_BF16 ? 0x3f803f80 : 0x3c003c00;
     const v4i ones = {kOne, kOne, kOne, kOne};
 
+    Marks<DT, DP, C> marks;
     // a chain's rows see nothing behind the block's last token
     int end = min(part.to * kTileTokens, s.length);
     if (!a.mask) end = min(end, drafted + (min(row0 + p.rows, rows) - 1) / p.group + 1);
@@ -245,25 +333,11 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
         // Tokens that some row does not see: drafted ones, those behind the end, those without a page.
         const bool lost = now.value < 0 || t0 + value_token + 7 >= s.length;
         const bool some = t0 + kWaveTokens > drafted || __any(lost);
-        uint32_t here = 0xffu;  // of this lane's eight tokens, those that exist
-        uint32_t seen[C];  // and those that its row sees
+        uint32_t seen[C];
         if (some) {
-            const auto first_of_8 = [](int n) { return (1u << min(max(n, 0), 8)) - 1u; };
-            const int at = t0 + value_token - drafted;  // of the lane's first token among the drafted ones
-            const int known = min(s.count, a.mask_columns);
-            here = now.value < 0 ? 0u : first_of_8(s.length - (t0 + value_token));
+            sight<C>(a, s, t0 + value_token, now.value >= 0, seen_to, sees, seen);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                if (a.mask) {
-                    uint32_t bits = 0;
-                    if (known > 0) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) bits |= min((uint32_t)sees[c][min(max(at + j, 0), known - 1)], 1u) << j;
-                    }
-                    seen[c] = ((bits & first_of_8(known - at)) | first_of_8(-at)) & here;
-                } else {
-                    seen[c] = first_of_8(seen_to[c] + 1 - (t0 + value_token)) & here;
-                }
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (!(seen[c] >> j & 1)) score[c][j / 4][j % 4] = -INFINITY;
@@ -314,47 +388,25 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
 
         if (some) {
             // Weights of zero do not keep an infinity or a NaN out of the sums.  Memory behind the end and without a page is cleared; a drafted
-            // token's own infinities and NaN are taken out and reach the rows that see it by themselves: a product of marks with what is seen.
-            uint32_t keep[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) keep[q] = halves((here >> 2 * q & 1u) << 15 | (here >> (2 * q + 1) & 1u) << 31);
+            // token's own are noted for the rows that see it, and taken out.
+            const int left = now.value < 0 ? 0 : min(max(s.length - (t0 + value_token), 0), 8);
             uint32_t bad = 0;
 #pragma unroll
-            for (int f = 0; f < kCols; ++f)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    turned[f][q] &= (int)keep[q];
-                    bad |= unbounded<DT>((uint32_t)turned[f][q]);
-                }
-            if (__any(bad != 0)) {
-                v4i sight[C];
-#pragma unroll
-                for (int c = 0; c < C; ++c)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        sight[c][q] = (int)(((seen[c] >> 2 * q & 1u) | (seen[c] >> (2 * q + 1) & 1u) << 16) * (uint32_t)(kOne & 0xffff));
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t keep = left >= 2 * q + 2 ? 0xffffffffu : left == 2 * q + 1 ? 0xffffu : 0u;
 #pragma unroll
                 for (int f = 0; f < kCols; ++f) {
-                    __builtin_amdgcn_sched_barrier(0);  // one column at a time: all at once they take the registers of the usual path
-                    v4i plus, minus;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t pair = (uint32_t)turned[f][q], b = unbounded<DT>(pair);
-                        plus[q] = (int)counted<DT>(pair, b, 0u);
-                        minus[q] = (int)counted<DT>(pair, b, 0x80008000u);
-                        turned[f][q] = (int)(pair & ~halves(b));
-                    }
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const v4f none = {0.f, 0.f, 0.f, 0.f};
-                        const v4f up = mfma16<DT>(plus, sight[c], none), down = mfma16<DT>(minus, sight[c], none);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            if (up[r] > 0.f) out[c][f][r] += INFINITY;
-                            if (down[r] > 0.f) out[c][f][r] -= INFINITY;
-                        }
-                    }
+                    turned[f][q] &= (int)keep;
+                    bad |= unbounded<DT>((uint32_t)turned[f][q]);
                 }
+            }
+            if (__any(bad != 0)) {
+                v4i* const parked = reinterpret_cast<v4i*>(&merged[wave][0][0]) + lane;  // (the wave's own part of LDS, not in use before the end)
+#pragma unroll
+                for (int f = 0; f < kCols; ++f) parked[f * kWave] = turned[f];
+                marks.note(seen, parked);
+#pragma unroll
+                for (int f = 0; f < kCols; ++f) turned[f] = Marks<DT, DP, C>::cleaned(parked[f * kWave]);
             }
         }
 
@@ -367,6 +419,8 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
         now = next;
         next = after;
     }
+
+    marks.apply(out);
 
     // The four waves' parts of a row: scaled to the largest of their largest scores and added, 16 rows at a time.
     const float value_scale = FP8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f;

@@ -76,27 +76,33 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
     const int32_t* const table = a.page_table + (long)part.b * a.table_stride;
     const uint8_t* const keys = static_cast<const uint8_t*>(a.key_cache) + (long)head * a.key_cache_head_stride * kSize;
     const uint8_t* const values = static_cast<const uint8_t*>(a.value_cache) + (long)head * a.value_cache_head_stride * kSize;
+    // Where the wave's tokens lie: the page's number is asked for a tile ahead of its use, and always, so that no wait for it takes in the requests of
+    // keys and values behind it.
     struct Place {
-        int entry, in_page;
+        int asked, at, in_page;
     };
-    auto place_of = [&](int token) {  // token: of the wave, a multiple of two at least
+    auto place_of = [&](int token) {  // the same token for the whole wave
         const uint32_t n = (uint32_t)token >> 3;
         const int at = (int)(p.page_magic ? __umulhi(n, p.page_magic) >> p.page_shift : n >> p.page_shift);
-        return Place{at < a.table_columns ? table[at] : -1, token - at * a.page_size};
+        return Place{table[min(at, a.table_columns - 1)], at, token - at * a.page_size};
     };
-    auto exists_page = [&](int entry) { return entry >= 0 && entry < a.pages; };
+    auto page_of = [&](const Place& place) {  // -1: none
+        const int page = __builtin_amdgcn_readfirstlane(place.asked);
+        return place.at < a.table_columns && page >= 0 && page < a.pages ? page : -1;
+    };
     typedef typename std::conditional<FP8, uint2, v4i>::type KeyPiece;
     KeyPiece key[kKeyUnits];
     uint32_t value[kValueUnits][2][kValueWords];
     Place key_place[kKeyUnits], value_place[kValueUnits];
-    bool value_here[kValueUnits];
+    int key_page[kKeyUnits], value_page[kValueUnits];  // of the tile that is to be requested
+    bool value_here[kValueUnits];                      // of the one that has been
     constexpr int kTokensAWave = kWave / kChunks > 0 ? kWave / kChunks : 1;  // key tokens a wave stages at a time
     static_assert(kWave % kChunks == 0 && kTokensAWave <= 8, "a wave's key pieces are of whole tokens within eight");
     const int key_chunk = lane % kChunks, key_row = lane / kChunks;
     const bool key_column = 8 * key_chunk < a.head_dim;
-    const long key_lane = ((long)key_row * a.key_place_stride + (key_column ? 8 * key_chunk : 0)) * kSize;
+    const uint32_t key_lane = key_row * p.key_place_bytes + (key_column ? 8 * key_chunk : 0) * kSize;
     const bool value_column = col * kCols < a.head_dim;
-    const long value_lane = ((long)(2 * g) * a.value_place_stride + (value_column ? col * kCols : 0)) * kSize;
+    const uint32_t value_lane = 2 * g * p.value_place_bytes + (value_column ? col * kCols : 0) * kSize;
     auto key_token = [&](int j) { return (wave * kWave + kThreads * j) / kChunks; };
     auto value_token = [&](int j) { return 8 * (wave + RW * TW * j); };
     auto find_places = [&](int t0) {
@@ -105,21 +111,25 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
 #pragma unroll
         for (int j = 0; j < kValueUnits; ++j) value_place[j] = place_of(t0 + value_token(j));
     };
-    auto request = [&](int t0) {
+    auto settle = [&]() {
+#pragma unroll
+        for (int j = 0; j < kKeyUnits; ++j) key_page[j] = page_of(key_place[j]);
+#pragma unroll
+        for (int j = 0; j < kValueUnits; ++j) value_page[j] = page_of(value_place[j]);
+    };
+    auto request = [&]() {
 #pragma unroll
         for (int j = 0; j < kKeyUnits; ++j) {
-            const int entry = __builtin_amdgcn_readfirstlane(key_place[j].entry);
-            const long at = (exists_page(entry) ? entry : 0) * a.key_page_stride + (long)key_place[j].in_page * a.key_place_stride;
-            key[j] = *reinterpret_cast<const KeyPiece*>(keys + at * kSize + key_lane);
+            const uint8_t* const page = keys + (uint64_t)(uint32_t)max(key_page[j], 0) * p.key_page_bytes;
+            key[j] = *reinterpret_cast<const KeyPiece*>(page + (key_place[j].in_page * p.key_place_bytes + key_lane));
         }
 #pragma unroll
         for (int j = 0; j < kValueUnits; ++j) {
-            const int entry = __builtin_amdgcn_readfirstlane(value_place[j].entry);
-            value_here[j] = exists_page(entry);
-            const long at = (value_here[j] ? entry : 0) * a.value_page_stride + (long)value_place[j].in_page * a.value_place_stride;
-            const uint8_t* from = values + at * kSize + value_lane;
+            value_here[j] = value_page[j] >= 0;
+            const uint8_t* const page = values + (uint64_t)(uint32_t)max(value_page[j], 0) * p.value_page_bytes;
 #pragma unroll
-            for (int t = 0; t < 2; ++t, from += a.value_place_stride * kSize) {
+            for (int t = 0; t < 2; ++t) {
+                const uint8_t* const from = page + ((value_place[j].in_page + t) * p.value_place_bytes + value_lane);
                 if constexpr (kValueWords == 1) value[j][t][0] = *reinterpret_cast<const uint32_t*>(from);
                 if constexpr (kValueWords == 2) *reinterpret_cast<uint2*>(value[j][t]) = *reinterpret_cast<const uint2*>(from);
                 if constexpr (kValueWords >= 4) {
@@ -163,13 +173,19 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
                 const uint32_t x = __builtin_amdgcn_perm(odd, even, 0x05040100u) & keep, y = __builtin_amdgcn_perm(odd, even, 0x07060302u) & keep;
                 *reinterpret_cast<uint32_t*>(to + f * 1024) = x;
                 *reinterpret_cast<uint32_t*>(to + (f + 1) * 1024) = y;
-                bad |= unbounded<DT>(x) | unbounded<DT>(y);
+                if (t0 + kSharedTokens > drafted) bad |= unbounded<DT>(x) | unbounded<DT>(y);
             }
             if (lane == 0) exists[buffer][token / 8] = value_here[j];
         }
-        const bool some = __any(bad != 0) && t0 + kSharedTokens > drafted;
+        const bool some = __any(bad != 0);
         if (lane == 0) unsafe[buffer][wave] = some;
     };
+
+    constexpr int kAhead = 4;                   // blocks of values a wave has requested from LDS
+    constexpr int kSwizzles = DP == 64 ? 2 : 4;
+    int key_offset[kSwizzles];  // where a lane reads a block of keys, by its step
+#pragma unroll
+    for (int i = 0; i < kSwizzles; ++i) key_offset[i] = (g * 16 + (col ^ swizzle(i, g))) * 16;
 
     v4f out[C][kCols], sum[C];
     float top[C];
@@ -183,29 +199,51 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
     constexpr int kOne = DT == HFRK_BF16 ? 0x3f803f80 : 0x3c003c00;
     const v4i ones = {kOne, kOne, kOne, kOne};
 
+    const auto what_is_seen = [&](int first, bool page, uint32_t (&seen)[C]) { sight<C>(a, s, first, page, seen_to, sees, seen); };
+    Marks<DT, DP, C> marks;
     int end = min(part.to * kTileTokens, s.length);
     if (!a.mask) end = min(end, drafted + (min(block0 + p.rows, rows) - 1) / p.group + 1);
     int t0 = part.from * kTileTokens;
     if (t0 < end) {
         find_places(t0);
-        request(t0);
-        if (t0 + kSharedTokens < end) find_places(t0 + kSharedTokens);
+        settle();
+        request();
+        find_places(t0 + kSharedTokens);
+        settle();
         put(0, t0);
-        if (t0 + kSharedTokens < end) request(t0 + kSharedTokens);
+        if (t0 + kSharedTokens < end) request();
     }
+    // The queries are here before the loop: waited for within it, a wait would take in the next tile's requests as well.
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) asm volatile("" : "+v"(query[c][step]));
     lds_barrier();
     int buffer = 0;
     for (; t0 < end; t0 += kSharedTokens, buffer ^= 1) {
         const int t1 = t0 + kSharedTokens, t2 = t1 + kSharedTokens;
-        if (t2 < end) find_places(t2);
+        find_places(t2);
         const uint8_t* const k_from = tiles[buffer][0];
         const uint8_t* const v_from = tiles[buffer][1];
-        bool poisoned = false;
         if (t1 > drafted) {
             int any = 0;
 #pragma unroll
             for (int w = 0; w < RW * TW; ++w) any |= unsafe[buffer][w];
-            poisoned = __builtin_amdgcn_readfirstlane(any) != 0;
+            if (__builtin_amdgcn_readfirstlane(any) != 0) {
+                // Rare: weights of zero do not keep an infinity or a NaN out of the sums.  They are noted for the rows that see their token, and taken out of
+                // the tile.
+                for (int half = token_wave; half < 2; half += TW) {
+                    uint32_t seen[C];
+                    what_is_seen(t0 + 32 * half + 8 * g, exists[buffer][4 * half + g] != 0, seen);
+                    marks.note(seen, reinterpret_cast<const v4i*>(v_from) + half * kCols * 64 + lane);
+                }
+                lds_barrier();
+                for (int i = threadIdx.x; i < kHalfBytes / 16; i += kThreads) {
+                    v4i* const x = reinterpret_cast<v4i*>(tiles[buffer][1]) + i;
+                    *x = Marks<DT, DP, C>::cleaned(*x);
+                }
+                lds_barrier();
+            }
         }
 #pragma unroll 1
         for (int half = token_wave; half < 2; half += TW) {
@@ -213,38 +251,35 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
             if (h0 >= end) break;
             v4f score[C][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                v4f acc[C];
+            for (int c = 0; c < C; ++c) score[c][0] = score[c][1] = v4f{0.f, 0.f, 0.f, 0.f};
+            const uint8_t* k_half[kSwizzles];
 #pragma unroll
-                for (int c = 0; c < C; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < kSwizzles; ++i) k_half[i] = k_from + half * (2 * kSteps * 1024) + key_offset[i];
+            v4i k[2][kSteps];
 #pragma unroll
-                for (int step = 0; step < kSteps; ++step) {
-                    const v4i k = *reinterpret_cast<const v4i*>(k_from + (((2 * half + t) * kSteps + step) * 64 + g * 16 + (col ^ swizzle(step, g))) * 16);
+            for (int step = 0; step < kSteps; ++step)
 #pragma unroll
-                    for (int c = 0; c < C; ++c) acc[c] = mfma16<DT>(k, query[c][step], acc[c]);
-                }
+                for (int t = 0; t < 2; ++t) k[t][step] = *reinterpret_cast<const v4i*>(k_half[step % kSwizzles] + (t * kSteps + step) * 1024);
+            __builtin_amdgcn_sched_barrier(0);  // all requests in front of the products, which otherwise wait for each by itself
 #pragma unroll
-                for (int c = 0; c < C; ++c) score[c][t] = acc[c];
-            }
+            for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int c = 0; c < C; ++c) score[c][t] = mfma16<DT>(k[t][step], query[c][step], score[c][t]);
+
+            // the first values are on their way while the weights are made
+            const uint8_t* const v_half = v_from + half * (kCols * 1024) + lane * 16;
+            v4i turned[kAhead];
+#pragma unroll
+            for (int f = 0; f < kAhead; ++f) turned[f] = *reinterpret_cast<const v4i*>(v_half + f * 1024);
 
             const bool here_page = exists[buffer][4 * half + g] != 0;
-            uint32_t seen[C];
             if (h0 + 32 > drafted || __any(!here_page || mine + 8 > s.length)) {
-                const auto first_of_8 = [](int n) { return (1u << min(max(n, 0), 8)) - 1u; };
-                const int at = mine - drafted, known = min(s.count, a.mask_columns);
-                const uint32_t here = here_page ? first_of_8(s.length - mine) : 0u;
+                uint32_t seen[C];
+                what_is_seen(mine, here_page, seen);
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    if (a.mask) {
-                        uint32_t bits = 0;
-                        if (known > 0) {
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) bits |= min((uint32_t)sees[c][min(max(at + j, 0), known - 1)], 1u) << j;
-                        }
-                        seen[c] = ((bits & first_of_8(known - at)) | first_of_8(-at)) & here;
-                    } else {
-                        seen[c] = first_of_8(seen_to[c] + 1 - mine) & here;
-                    }
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (!(seen[c] >> j & 1)) score[c][j / 4][j % 4] = -INFINITY;
@@ -283,50 +318,16 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
                 weight[c] = v4i{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
                 sum[c] = mfma16<DT>(ones, weight[c], sum[c]);
             }
-            const uint8_t* const v_half = v_from + (half * kCols * 64 + lane) * 16;
-            if (!poisoned) {
 #pragma unroll
-                for (int f = 0; f < kCols; ++f) {
-                    const v4i v = *reinterpret_cast<const v4i*>(v_half + f * 1024);
+            for (int f = 0; f < kCols; ++f) {
 #pragma unroll
-                    for (int c = 0; c < C; ++c) out[c][f] = mfma16<DT>(v, weight[c], out[c][f]);
-                }
-            } else {  // (t1 > drafted: `seen` is not set for a half that lies in front of the drafted tokens, where all is seen)
-                v4i sight[C];
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const uint32_t bits = h0 + 32 > drafted ? seen[c] : 0xffu;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) sight[c][q] = (int)(((bits >> 2 * q & 1u) | (bits >> (2 * q + 1) & 1u) << 16) * (uint32_t)(kOne & 0xffff));
-                }
-#pragma unroll
-                for (int f = 0; f < kCols; ++f) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    v4i v = *reinterpret_cast<const v4i*>(v_half + f * 1024);
-                    v4i plus, minus;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t pair = (uint32_t)v[q], b = unbounded<DT>(pair);
-                        plus[q] = (int)counted<DT>(pair, b, 0u);
-                        minus[q] = (int)counted<DT>(pair, b, 0x80008000u);
-                        v[q] = (int)(pair & ~halves(b));
-                    }
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const v4f none = {0.f, 0.f, 0.f, 0.f};
-                        const v4f up = mfma16<DT>(plus, sight[c], none), down = mfma16<DT>(minus, sight[c], none);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            if (up[r] > 0.f) out[c][f][r] += INFINITY;
-                            if (down[r] > 0.f) out[c][f][r] -= INFINITY;
-                        }
-                        out[c][f] = mfma16<DT>(v, weight[c], out[c][f]);
-                    }
-                }
+                for (int c = 0; c < C; ++c) out[c][f] = mfma16<DT>(turned[f % kAhead], weight[c], out[c][f]);
+                if (f + kAhead < kCols) turned[f % kAhead] = *reinterpret_cast<const v4i*>(v_half + (f + kAhead) * 1024);
             }
         }
+        settle();
         if (t1 < end) put(buffer ^ 1, t1);
-        if (t2 < end) request(t2);
+        if (t2 < end) request();
         lds_barrier();
     }
 
@@ -334,6 +335,8 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
         for (int r = threadIdx.x; r < p.rows && block0 + r < rows; r += kThreads)
             p.row_info[(long)s.first * p.group + block0 + r] = make_int4(part.slot, part.splits, r, 0);
     }
+
+    marks.apply(out);
 
     // ---- the token groups' parts of a row, then the result: a lane has DP / 4 neighbouring columns of its rows
     if constexpr (TW > 1) {
