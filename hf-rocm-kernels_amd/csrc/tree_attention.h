@@ -130,7 +130,7 @@ __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
 template <int DP>
 int launch_attention(const AttentionArgs& p, int col_blocks, int grid, hipStream_t stream);
 
-// The same for many rows, which share keys and values in LDS (tree_attention_shared.h): 64, 128 or (up to 128 columns) 256 rows a block.
+// The same for many rows, which share keys and values in LDS (tree_attention_shared.h): 128 or (up to 128 columns) 256 rows a block.
 template <int DP>
 int launch_attention_shared(const AttentionArgs& p, int grid, hipStream_t stream);
 

@@ -100,7 +100,7 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     const int size = a.cache_dtype == HFRK_FP8_E4M3FN ? 1 : 2;
     d.shared = per > 32 && narrow(a.key_page_stride, a.key_place_stride, a.page_size, size) &&
                narrow(a.value_page_stride, a.value_place_stride, a.page_size, size);
-    d.rows = per <= 16 ? 16 : per <= 32 || !d.shared ? 32 : per <= 64 ? 64 : per <= 128 || a.head_dim > 128 ? 128 : 256;
+    d.rows = per <= 16 ? 16 : per <= 32 || !d.shared ? 32 : per <= 128 || a.head_dim > 128 ? 128 : 256;
     d.work = d.shared ? 512 : 1024;
     const int rows = d.rows;
     const long blocks = (long)a.tokens * group / rows + a.seqs;

@@ -1,12 +1,13 @@
 // Attention of many rows a key head over a paged cache: keys and values through LDS, for drafted trees and chains.
 //
 // The mathematics and the operands' order are those of tree_attention_kernel.h.  There every wave has its own tokens and holds them in registers; here
-// RW waves share them, each with C blocks of 16 rows, and TW groups of such waves take the tile's 32-token halves in turn.  Products and
-// exponentials bound it: for 32 tokens and 16 rows of 128 columns 17 products of 16 cycles, and for a lane's eight scores about 50 vector instructions,
-// eight of them exponentials of 16 cycles; two waves a SIMD overlap the one with the other.
+// eight waves of C blocks of 16 rows share them.  Products and exponentials bound it: for 32 tokens and 16 rows of 128 columns 17 products of 16
+// cycles, and for a lane's eight scores about 40 vector instructions, eight of them exponentials of 16 cycles.  Waves i and i + 4 share a SIMD: in one
+// phase the first four have their products while the others have their exponentials, in the next the other way round, with a barrier between.
+// (All in step, the same work took the sum of the two: 400 us instead of TODO for trees of 64 tokens over 16 caches of 16384.)
 //
-// A tile is 64 tokens.  While one is computed on, the next is in flight to registers, 16 bytes a piece; behind the products it is written to the other
-// buffer, in the order in which lanes read it as matrix operands (fp8 converted, values turned in pairs of tokens), once for all waves:
+// A tile is 64 tokens.  While one is computed on, the next is in flight to registers, 16 bytes a piece; in a phase of exponentials it is written to
+// the other buffer, in the order in which lanes read it as matrix operands (fp8 converted, values turned in pairs of tokens), once for all waves:
 //   keys    block (16 tokens, 32 columns): lane (token row i, column group g) at 16 * (16 g + (i ^ swizzle)); the swizzle spreads the pieces of one token,
 //           which neighbouring threads write, over the banks
 //   values  block (32 tokens, 16 columns kCols i + f): lane (i, token group g) at 16 * (16 g + i), a pair of tokens a word
@@ -27,30 +28,29 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <int DT, bool FP8, int DP, int C, int RW, int TW>
-__global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const AttentionArgs p) {
-    constexpr int kThreads = 64 * RW * TW;
+constexpr int kSharedWaves = 8;
+
+template <int DT, bool FP8, int DP, int C>
+__global__ void __launch_bounds__(64 * kSharedWaves) attention_shared_kernel(const AttentionArgs p) {
+    constexpr int kThreads = 64 * kSharedWaves;
     constexpr int kSteps = DP / 32, kCols = DP / 16, kSize = FP8 ? 1 : 2;
     constexpr int kChunks = DP / 8;                                   // pieces of eight columns of a token
     constexpr int kKeyUnits = kSharedTokens * kChunks / kThreads;     // of keys a thread stages
-    constexpr int kValueUnits = kSharedTokens / 2 * 16 / kThreads;    // of values: two tokens, kCols columns
+    constexpr int kValueUnits = kSharedTokens / 2 * 16 / kThreads;    // of values: two tokens, kCols columns each
     constexpr int kValueWords = kCols * kSize / 4;
     constexpr int kHalfBytes = kSharedTokens * DP * 2;                // keys, or values, of a tile
     static_assert(kThreads * kKeyUnits == kSharedTokens * kChunks && kThreads * kValueUnits == kSharedTokens * 8, "whole units a thread");
-    static_assert(64 * RW * C * DP <= 4 * kHalfBytes || TW == 1, "the merge reuses the tiles");
     __shared__ __align__(16) uint8_t tiles[2][2][kHalfBytes];         // [buffer][keys, values]
     __shared__ int exists[2][kSharedTokens / 8];                      // whether eight tokens have a page
-    __shared__ int unsafe[2][RW * TW];                                // whether a wave has staged an infinity or a NaN among drafted tokens' values
-    __shared__ float statistics[RW][C * 16][2];
+    __shared__ int unsafe[2][kSharedWaves];                                // whether a wave has staged an infinity or a NaN among drafted tokens' values
 
     const hfrk_attention_args& a = p.a;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int row_wave = wave % RW, token_wave = wave / RW;
     const int item = blockIdx.x / a.kv_heads, head = blockIdx.x - item * a.kv_heads;
     const Part part = find_part(p, item);
     if (!part.any) return;
     const Sequence s = part.s;
-    const int block0 = part.block * p.rows, row0 = block0 + row_wave * 16 * C, rows = s.count * p.group;
+    const int block0 = part.block * p.rows, row0 = block0 + wave * 16 * C, rows = s.count * p.group;
     const int drafted = s.drafted;
 
     v4i query[C][kSteps];
@@ -92,96 +92,86 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
     };
     typedef typename std::conditional<FP8, uint2, v4i>::type KeyPiece;
     KeyPiece key[kKeyUnits];
-    uint32_t value[kValueUnits][2][kValueWords];
-    Place key_place[kKeyUnits], value_place[kValueUnits];
-    int key_page[kKeyUnits], value_page[kValueUnits];  // of the tile that is to be requested
-    bool value_here[kValueUnits];                      // of the one that has been
-    constexpr int kTokensAWave = kWave / kChunks > 0 ? kWave / kChunks : 1;  // key tokens a wave stages at a time
-    static_assert(kWave % kChunks == 0 && kTokensAWave <= 8, "a wave's key pieces are of whole tokens within eight");
+    uint32_t value[2][kValueWords];
+    Place place;
+    int page;        // of the tile that is to be requested, -1: none
+    bool page_here;  // whether the one that has been requested has one
+    constexpr int kKeyTokens = 8 / kKeyUnits;  // tokens whose keys a wave stages at a time
+    static_assert(kKeyTokens * kChunks == kWave && kValueUnits == 1, "a wave stages eight tokens");
+    const int token8 = 8 * wave;               // the wave's tokens in the tile
     const int key_chunk = lane % kChunks, key_row = lane / kChunks;
     const bool key_column = 8 * key_chunk < a.head_dim;
     const uint32_t key_lane = key_row * p.key_place_bytes + (key_column ? 8 * key_chunk : 0) * kSize;
     const bool value_column = col * kCols < a.head_dim;
     const uint32_t value_lane = 2 * g * p.value_place_bytes + (value_column ? col * kCols : 0) * kSize;
-    auto key_token = [&](int j) { return (wave * kWave + kThreads * j) / kChunks; };
-    auto value_token = [&](int j) { return 8 * (wave + RW * TW * j); };
-    auto find_places = [&](int t0) {
-#pragma unroll
-        for (int j = 0; j < kKeyUnits; ++j) key_place[j] = place_of(t0 + key_token(j));
-#pragma unroll
-        for (int j = 0; j < kValueUnits; ++j) value_place[j] = place_of(t0 + value_token(j));
-    };
-    auto settle = [&]() {
-#pragma unroll
-        for (int j = 0; j < kKeyUnits; ++j) key_page[j] = page_of(key_place[j]);
-#pragma unroll
-        for (int j = 0; j < kValueUnits; ++j) value_page[j] = page_of(value_place[j]);
-    };
+    auto find_place = [&](int t0) { place = place_of(t0 + token8); };
+    auto settle = [&]() { page = page_of(place); };
     auto request = [&]() {
+        page_here = page >= 0;
+        const uint64_t number = (uint32_t)max(page, 0);
+        const uint8_t* const k_page = keys + (number * p.key_page_bytes + place.in_page * p.key_place_bytes);
+        const uint8_t* const v_page = values + (number * p.value_page_bytes + place.in_page * p.value_place_bytes);
 #pragma unroll
-        for (int j = 0; j < kKeyUnits; ++j) {
-            const uint8_t* const page = keys + (uint64_t)(uint32_t)max(key_page[j], 0) * p.key_page_bytes;
-            key[j] = *reinterpret_cast<const KeyPiece*>(page + (key_place[j].in_page * p.key_place_bytes + key_lane));
-        }
+        for (int j = 0; j < kKeyUnits; ++j) key[j] = *reinterpret_cast<const KeyPiece*>(k_page + j * kKeyTokens * p.key_place_bytes + key_lane);
 #pragma unroll
-        for (int j = 0; j < kValueUnits; ++j) {
-            value_here[j] = value_page[j] >= 0;
-            const uint8_t* const page = values + (uint64_t)(uint32_t)max(value_page[j], 0) * p.value_page_bytes;
+        for (int t = 0; t < 2; ++t) {
+            const uint8_t* const from = v_page + t * p.value_place_bytes + value_lane;
+            if constexpr (kValueWords == 1) value[t][0] = *reinterpret_cast<const uint32_t*>(from);
+            if constexpr (kValueWords == 2) *reinterpret_cast<uint2*>(value[t]) = *reinterpret_cast<const uint2*>(from);
+            if constexpr (kValueWords >= 4) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint8_t* const from = page + ((value_place[j].in_page + t) * p.value_place_bytes + value_lane);
-                if constexpr (kValueWords == 1) value[j][t][0] = *reinterpret_cast<const uint32_t*>(from);
-                if constexpr (kValueWords == 2) *reinterpret_cast<uint2*>(value[j][t]) = *reinterpret_cast<const uint2*>(from);
-                if constexpr (kValueWords >= 4) {
-#pragma unroll
-                    for (int w = 0; w < kValueWords; w += 4) *reinterpret_cast<uint4*>(value[j][t] + w) = *reinterpret_cast<const uint4*>(from + 4 * w);
-                }
+                for (int w = 0; w < kValueWords; w += 4) *reinterpret_cast<uint4*>(value[t] + w) = *reinterpret_cast<const uint4*>(from + 4 * w);
             }
         }
     };
     auto swizzle = [](int step, int group) { return 4 * group + (DP == 64 ? 2 * step : step % 4); };
     auto put = [&](int buffer, int t0) {
         uint8_t* const k_to = tiles[buffer][0];
-        uint8_t* const v_to = tiles[buffer][1];
 #pragma unroll
         for (int j = 0; j < kKeyUnits; ++j) {
-            const int token = key_token(j) + key_row, w = token % 32;
-            const int t16 = token / 32 * 2 + w / 4 % 2, i = 4 * (w / 8) + w % 4, step = key_chunk / 4, group = key_chunk % 4;
+            const int w = token8 % 32 + j * kKeyTokens + key_row;  // (of 32: rows of two 16-token blocks)
+            const int t16 = token8 / 32 * 2 + w / 4 % 2, i = 4 * (w / 8) + w % 4, step = key_chunk / 4, group = key_chunk % 4;
             v4i x;
             if constexpr (FP8) x = v4i{widen2<DT, false>(key[j].x), widen2<DT, true>(key[j].x), widen2<DT, false>(key[j].y), widen2<DT, true>(key[j].y)};
             else x = key[j];
             if (!key_column) x = v4i{0, 0, 0, 0};
             *reinterpret_cast<v4i*>(k_to + ((t16 * kSteps + step) * 64 + group * 16 + (i ^ swizzle(step, group))) * 16) = x;
         }
-        uint32_t bad = 0;
-#pragma unroll
-        for (int j = 0; j < kValueUnits; ++j) {
-            const int token = value_token(j);
-            const int left = s.length - (t0 + token + 2 * g);
-            const uint32_t keep = value_here[j] ? (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u) : 0u;
-            uint8_t* const to = v_to + (token / 32 * kCols * 64 + token % 32 / 8 * 16 + col) * 16 + g * 4;
-#pragma unroll
-            for (int f = 0; f < kCols; f += 2) {
-                uint32_t even, odd;
-                if constexpr (FP8) {
-                    even = f % 4 == 0 ? widen2<DT, false>(value[j][0][f / 4]) : widen2<DT, true>(value[j][0][f / 4]);
-                    odd = f % 4 == 0 ? widen2<DT, false>(value[j][1][f / 4]) : widen2<DT, true>(value[j][1][f / 4]);
-                } else {
-                    even = value[j][0][f / 2];
-                    odd = value[j][1][f / 2];
-                }
-                const uint32_t x = __builtin_amdgcn_perm(odd, even, 0x05040100u) & keep, y = __builtin_amdgcn_perm(odd, even, 0x07060302u) & keep;
-                *reinterpret_cast<uint32_t*>(to + f * 1024) = x;
-                *reinterpret_cast<uint32_t*>(to + (f + 1) * 1024) = y;
-                if (t0 + kSharedTokens > drafted) bad |= unbounded<DT>(x) | unbounded<DT>(y);
-            }
-            if (lane == 0) exists[buffer][token / 8] = value_here[j];
+        uint32_t keep = 0xffffffffu;  // tokens behind the end and without a page are cleared
+        if (!page_here || t0 + kSharedTokens > s.length) {
+            const int left = page_here ? s.length - (t0 + token8 + 2 * g) : 0;
+            keep = (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
         }
-        const bool some = __any(bad != 0);
-        if (lane == 0) unsafe[buffer][wave] = some;
+        uint8_t* const v_to = tiles[buffer][1] + (token8 / 32 * kCols * 64 + token8 % 32 / 8 * 16 + col) * 16 + g * 4;
+        uint32_t pairs[kCols];
+#pragma unroll
+        for (int f = 0; f < kCols; f += 2) {
+            uint32_t even, odd;
+            if constexpr (FP8) {
+                even = f % 4 == 0 ? widen2<DT, false>(value[0][f / 4]) : widen2<DT, true>(value[0][f / 4]);
+                odd = f % 4 == 0 ? widen2<DT, false>(value[1][f / 4]) : widen2<DT, true>(value[1][f / 4]);
+            } else {
+                even = value[0][f / 2];
+                odd = value[1][f / 2];
+            }
+            pairs[f] = __builtin_amdgcn_perm(odd, even, 0x05040100u) & keep;
+            pairs[f + 1] = __builtin_amdgcn_perm(odd, even, 0x07060302u) & keep;
+            *reinterpret_cast<uint32_t*>(v_to + f * 1024) = pairs[f];
+            *reinterpret_cast<uint32_t*>(v_to + (f + 1) * 1024) = pairs[f + 1];
+        }
+        bool some = false;
+        if (t0 + kSharedTokens > drafted) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int f = 0; f < kCols; ++f) bad |= unbounded<DT>(pairs[f]);
+            some = __any(bad != 0);
+        }
+        if (lane == 0) {
+            exists[buffer][wave] = page_here;
+            unsafe[buffer][wave] = some;
+        }
     };
 
-    constexpr int kAhead = 4;                   // blocks of values a wave has requested from LDS
     constexpr int kSwizzles = DP == 64 ? 2 : 4;
     int key_offset[kSwizzles];  // where a lane reads a block of keys, by its step
 #pragma unroll
@@ -199,171 +189,150 @@ __global__ void __launch_bounds__(64 * RW * TW) attention_shared_kernel(const At
     constexpr int kOne = DT == HFRK_BF16 ? 0x3f803f80 : 0x3c003c00;
     const v4i ones = {kOne, kOne, kOne, kOne};
 
-    const auto what_is_seen = [&](int first, bool page, uint32_t (&seen)[C]) { sight<C>(a, s, first, page, seen_to, sees, seen); };
     Marks<DT, DP, C> marks;
     int end = min(part.to * kTileTokens, s.length);
     if (!a.mask) end = min(end, drafted + (min(block0 + p.rows, rows) - 1) / p.group + 1);
-    int t0 = part.from * kTileTokens;
-    if (t0 < end) {
-        find_places(t0);
+    const int begin = part.from * kTileTokens;
+    const int steps = begin < end ? (end - begin + 31) / 32 : 0, tiles_here = (steps + 1) / 2;
+    if (steps > 0) {
+        find_place(begin);
         settle();
         request();
-        find_places(t0 + kSharedTokens);
+        find_place(begin + kSharedTokens);
         settle();
-        put(0, t0);
-        if (t0 + kSharedTokens < end) request();
+        put(0, begin);
+        if (tiles_here > 1) request();
+        find_place(begin + 2 * kSharedTokens);
     }
     // The queries are here before the loop: waited for within it, a wait would take in the next tile's requests as well.
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int step = 0; step < kSteps; ++step) asm volatile("" : "+v"(query[c][step]));
-    lds_barrier();
-    int buffer = 0;
-    for (; t0 < end; t0 += kSharedTokens, buffer ^= 1) {
-        const int t1 = t0 + kSharedTokens, t2 = t1 + kSharedTokens;
-        find_places(t2);
-        const uint8_t* const k_from = tiles[buffer][0];
-        const uint8_t* const v_from = tiles[buffer][1];
-        if (t1 > drafted) {
-            int any = 0;
-#pragma unroll
-            for (int w = 0; w < RW * TW; ++w) any |= unsafe[buffer][w];
-            if (__builtin_amdgcn_readfirstlane(any) != 0) {
-                // Rare: weights of zero do not keep an infinity or a NaN out of the sums.  They are noted for the rows that see their token, and taken out of
-                // the tile.
-                for (int half = token_wave; half < 2; half += TW) {
-                    uint32_t seen[C];
-                    what_is_seen(t0 + 32 * half + 8 * g, exists[buffer][4 * half + g] != 0, seen);
-                    marks.note(seen, reinterpret_cast<const v4i*>(v_from) + half * kCols * 64 + lane);
-                }
-                lds_barrier();
-                for (int i = threadIdx.x; i < kHalfBytes / 16; i += kThreads) {
-                    v4i* const x = reinterpret_cast<v4i*>(tiles[buffer][1]) + i;
-                    *x = Marks<DT, DP, C>::cleaned(*x);
-                }
-                lds_barrier();
-            }
-        }
-#pragma unroll 1
-        for (int half = token_wave; half < 2; half += TW) {
-            const int h0 = t0 + 32 * half, mine = h0 + 8 * g;
-            if (h0 >= end) break;
-            v4f score[C][2];
-#pragma unroll
-            for (int c = 0; c < C; ++c) score[c][0] = score[c][1] = v4f{0.f, 0.f, 0.f, 0.f};
-            const uint8_t* k_half[kSwizzles];
-#pragma unroll
-            for (int i = 0; i < kSwizzles; ++i) k_half[i] = k_from + half * (2 * kSteps * 1024) + key_offset[i];
-            v4i k[2][kSteps];
-#pragma unroll
-            for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) k[t][step] = *reinterpret_cast<const v4i*>(k_half[step % kSwizzles] + (t * kSteps + step) * 1024);
-            __builtin_amdgcn_sched_barrier(0);  // all requests in front of the products, which otherwise wait for each by itself
-#pragma unroll
-            for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int c = 0; c < C; ++c) score[c][t] = mfma16<DT>(k[t][step], query[c][step], score[c][t]);
-
-            // the first values are on their way while the weights are made
-            const uint8_t* const v_half = v_from + half * (kCols * 1024) + lane * 16;
-            v4i turned[kAhead];
-#pragma unroll
-            for (int f = 0; f < kAhead; ++f) turned[f] = *reinterpret_cast<const v4i*>(v_half + f * 1024);
-
-            const bool here_page = exists[buffer][4 * half + g] != 0;
-            if (h0 + 32 > drafted || __any(!here_page || mine + 8 > s.length)) {
-                uint32_t seen[C];
-                what_is_seen(mine, here_page, seen);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (!(seen[c] >> j & 1)) score[c][j / 4][j % 4] = -INFINITY;
-                }
-            }
-
-            // A row's scale follows its largest score when a lane has found one 2^8 above it, not with every step.
-            float most[C];
-            bool grows = false;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                most[c] = score[c][0][0];
-#pragma unroll
-                for (int j = 1; j < 8; ++j) most[c] = fmaxf(most[c], score[c][j / 4][j % 4]);
-                most[c] *= scale;
-                grows |= most[c] > top[c] + kHeadroom;
-            }
-            if (__any(grows)) {
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const float grown = fmaxf(top[c], row_max(most[c]));
-                    const float shrink = top[c] == grown ? 1.f : __builtin_amdgcn_exp2f(top[c] - grown);
-                    top[c] = grown;
-                    sum[c] *= shrink;
-#pragma unroll
-                    for (int f = 0; f < kCols; ++f) out[c][f] *= shrink;
-                }
-            }
-            v4i weight[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const float base = top[c] == -INFINITY ? 0.f : top[c];
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(score[c][j / 4][j % 4], scale, -base));
-                weight[c] = v4i{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
-                sum[c] = mfma16<DT>(ones, weight[c], sum[c]);
-            }
-#pragma unroll
-            for (int f = 0; f < kCols; ++f) {
-#pragma unroll
-                for (int c = 0; c < C; ++c) out[c][f] = mfma16<DT>(turned[f % kAhead], weight[c], out[c][f]);
-                if (f + kAhead < kCols) turned[f % kAhead] = *reinterpret_cast<const v4i*>(v_half + (f + kAhead) * 1024);
-            }
-        }
-        settle();
-        if (t1 < end) put(buffer ^ 1, t1);
-        if (t2 < end) request();
-        lds_barrier();
-    }
-
     if (p.row_info && part.split == 0 && head == 0) {
         for (int r = threadIdx.x; r < p.rows && block0 + r < rows; r += kThreads)
             p.row_info[(long)s.first * p.group + block0 + r] = make_int4(part.slot, part.splits, r, 0);
     }
 
-    marks.apply(out);
-
-    // ---- the token groups' parts of a row, then the result: a lane has DP / 4 neighbouring columns of its rows
-    if constexpr (TW > 1) {
-        v4f* const parts = reinterpret_cast<v4f*>(&tiles[0][0][0]);
-        if (token_wave == 1) {
+    const auto load_keys = [&](int i, v4i (&k)[2][kSteps]) {
+        const uint8_t* const from = tiles[i >> 1 & 1][0] + (i & 1) * (2 * kSteps * 1024);
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) k[t][step] = *reinterpret_cast<const v4i*>(from + key_offset[step % kSwizzles] + (t * kSteps + step) * 1024);
+    };
+    const auto score_keys = [&](const v4i (&k)[2][kSteps], v4f (&score)[C][2]) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) score[c][0] = score[c][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int c = 0; c < C; ++c) score[c][t] = mfma16<DT>(k[t][step], query[c][step], score[c][t]);
+    };
+    constexpr int kAhead = kCols < 8 ? kCols : 8;  // blocks of values read in front of the exponentials: all, up to 128 columns
+    v4f score[C][2];
+    lds_barrier();
+    {
+        v4i k[2][kSteps];
+        load_keys(0, k);
+        score_keys(k, score);
+    }
+    for (int i = 0; i < steps; ++i) {
+        const int buffer = i >> 1 & 1, half = i & 1, h0 = begin + 32 * i, mine = h0 + 8 * g;
+        const bool here_page = exists[buffer][4 * half + g] != 0;
+        const uint8_t* const v_half = tiles[buffer][1] + half * (kCols * 1024) + lane * 16;
+        v4i turned[kAhead];
+#pragma unroll
+        for (int f = 0; f < kAhead; ++f) turned[f] = *reinterpret_cast<const v4i*>(v_half + f * 1024);
+        bool unclean = false;
+        if (h0 + 32 > drafted || __any(!here_page || mine + 8 > s.length)) {
+            uint32_t seen[C];
+            sight<C>(a, s, mine, here_page, seen_to, sees, seen);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                if (g == 0) {
-                    statistics[row_wave][c * 16 + col][0] = top[c];
-                    statistics[row_wave][c * 16 + col][1] = sum[c][0];
-                }
 #pragma unroll
-                for (int f = 0; f < kCols; ++f) parts[((row_wave * C + c) * kCols + f) * 64 + lane] = out[c][f];
+                for (int j = 0; j < 8; ++j)
+                    if (!(seen[c] >> j & 1)) score[c][j / 4][j % 4] = -INFINITY;
+            }
+            // Rare: weights of zero do not keep an infinity or a NaN out of the sums.  They are noted for the rows that see their token, and taken out.
+            int any = 0;
+#pragma unroll
+            for (int w = 0; w < kSharedWaves; ++w) any |= unsafe[buffer][w];
+            unclean = __builtin_amdgcn_readfirstlane(any) != 0;
+            if (unclean) {
+                marks.note(seen, reinterpret_cast<const v4i*>(v_half));
+#pragma unroll
+                for (int f = 0; f < kAhead; ++f) turned[f] = Marks<DT, DP, C>::cleaned(turned[f]);
             }
         }
-        lds_barrier();
-        if (token_wave == 1) return;
+        // A row's scale follows its largest score when a lane has found one 2^8 above it, not with every step.
+        float most[C];
+        bool grows = false;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const float other = statistics[row_wave][c * 16 + col][0], most = fmaxf(top[c], other);
-            const float mine = top[c] == most ? 1.f : __builtin_amdgcn_exp2f(top[c] - most), its = other == most ? 1.f : __builtin_amdgcn_exp2f(other - most);
-            sum[c][0] = mine * sum[c][0] + its * statistics[row_wave][c * 16 + col][1];
-            top[c] = most;
+            most[c] = score[c][0][0];
 #pragma unroll
-            for (int f = 0; f < kCols; ++f) out[c][f] = mine * out[c][f] + its * parts[((row_wave * C + c) * kCols + f) * 64 + lane];
+            for (int j = 1; j < 8; ++j) most[c] = fmaxf(most[c], score[c][j / 4][j % 4]);
+            most[c] *= scale;
+            grows |= most[c] > top[c] + kHeadroom;
+        }
+        if (__any(grows)) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float grown = fmaxf(top[c], row_max(most[c]));
+                const float shrink = top[c] == grown ? 1.f : __builtin_amdgcn_exp2f(top[c] - grown);
+                top[c] = grown;
+                sum[c] *= shrink;
+#pragma unroll
+                for (int f = 0; f < kCols; ++f) out[c][f] *= shrink;
+            }
+        }
+        // The next step's keys: from the second half of a tile on they are in the next one, which all have written by now.  (All have read this one's
+        // values too: behind the barrier its buffer is free, but where some blocks are read later.)
+        if (half == 1) lds_barrier();
+        v4i k[2][kSteps], weight[C];
+        v4f score_next[C][2];
+        load_keys(i + 1, k);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const float base = top[c] == -INFINITY ? 0.f : top[c];
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(score[c][j / 4][j % 4], scale, -base));
+            weight[c] = v4i{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
+        }
+        score_keys(k, score_next);
+#pragma unroll
+        for (int c = 0; c < C; ++c) sum[c] = mfma16<DT>(ones, weight[c], sum[c]);
+#pragma unroll
+        for (int f = 0; f < kCols; ++f) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) out[c][f] = mfma16<DT>(turned[f % kAhead], weight[c], out[c][f]);
+            if (f + kAhead < kCols) {
+                turned[f % kAhead] = *reinterpret_cast<const v4i*>(v_half + (f + kAhead) * 1024);
+                if (unclean) turned[f % kAhead] = Marks<DT, DP, C>::cleaned(turned[f % kAhead]);
+            }
+        }
+        if (half == 0) {
+            const int next = i / 2 + 1;
+            settle();
+            if (next < tiles_here) put(next & 1, h0 + kSharedTokens);
+            if (next + 1 < tiles_here) request();
+            find_place(h0 + 3 * kSharedTokens);
+        } else if constexpr (kAhead < kCols) {
+            lds_barrier();
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            score[c][0] = score_next[c][0];
+            score[c][1] = score_next[c][1];
         }
     }
+    marks.apply(out);
+
+    // a lane has DP / 4 neighbouring columns of its rows
     const float value_scale = FP8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f;
     const float inv_out_scale = a.out_scale ? 1.f / a.out_scale[0] : 1.f;
 #pragma unroll
@@ -396,9 +365,8 @@ int launch_attention_shared(const AttentionArgs& p, int grid, hipStream_t stream
     const bool fp8 = p.a.cache_dtype == HFRK_FP8_E4M3FN;
 #define HFRK_SHARED(DT, FP8)                                                                                                              \
     do {                                                                                                                                  \
-        if (p.rows == 64) hipLaunchKernelGGL((attention_shared_kernel<DT, FP8, DP, 1, 4, 2>), dim3(grid), dim3(512), 0, stream, p);        \
-        else if (p.rows == 128) hipLaunchKernelGGL((attention_shared_kernel<DT, FP8, DP, DP == 256 ? 1 : 2, DP == 256 ? 8 : 4, DP == 256 ? 1 : 2>), dim3(grid), dim3(512), 0, stream, p); \
-        else if constexpr (DP < 256) hipLaunchKernelGGL((attention_shared_kernel<DT, FP8, DP, 2, 8, 1>), dim3(grid), dim3(512), 0, stream, p); \
+        if (p.rows == 128) hipLaunchKernelGGL((attention_shared_kernel<DT, FP8, DP, 1>), dim3(grid), dim3(64 * kSharedWaves), 0, stream, p); \
+        else if constexpr (DP < 256) hipLaunchKernelGGL((attention_shared_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(64 * kSharedWaves), 0, stream, p); \
     } while (0)
     if (p.a.dtype == HFRK_BF16) {
         if (fp8) HFRK_SHARED(HFRK_BF16, true);
