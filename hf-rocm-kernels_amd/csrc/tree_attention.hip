@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(kAttentionThreads) attention_join_kernel(const
     float total = 0.f, o[8] = {};
     for (int s = lane / width; s < splits; s += kWave / width) {
         const float2 ml = p.partial_ml[at + s * step];
-        const float share = ml.x == most ? 1.f : __builtin_amdgcn_exp2f(ml.x - most);
+        const float share = __builtin_amdgcn_exp2f(ml.x - most);
         total += share * ml.y;
         if (d < a.head_dim) {
             const v4f* const from = reinterpret_cast<const v4f*>(p.partial + (at + s * step) * a.head_dim + d);

@@ -23,7 +23,8 @@
 
 namespace hfrk {
 
-constexpr float kHeadroom = 8.f;  // weights may grow to 2^8 before a row's scale follows
+constexpr float kHeadroom = 8.f;    // weights may grow to 2^8 before a row's scale follows
+constexpr float kNothing = -1e38f;  // the scale of a row that has seen nothing; finite, so that nothing has to be told apart
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -98,28 +99,49 @@ __device__ __forceinline__ uint32_t counted(uint32_t pair, uint32_t bits, uint32
     return (((nan | ~(pair ^ sign)) & bits) >> 15) * one;  // (`bits` has the halves' top bits only)
 }
 
-// Of the eight cached tokens from `first` on, those that a lane's C rows see: bit j token first + j.  page: they have one; seen_to: the last token a
-// row of a chain sees; sees: a row of the mask.
-template <int C>
-__device__ __forceinline__ void sight(const hfrk_attention_args& a, const Sequence& s, int first, bool page, const int (&seen_to)[C],
-                                      const uint8_t* const (&sees)[C], uint32_t (&seen)[C]) {
+// Of the eight cached tokens from `first` on, those that a row sees: bit j token first + j.  page: they have one; seen_to: the last token the row of a
+// chain sees; sees: the row of the mask.
+__device__ __forceinline__ uint32_t sight(const hfrk_attention_args& a, const Sequence& s, int first, bool page, int seen_to, const uint8_t* sees) {
     const auto first_of_8 = [](int n) { return (1u << min(max(n, 0), 8)) - 1u; };
+    const uint32_t here = page ? first_of_8(s.length - first) : 0u;
+    if (!a.mask) return first_of_8(seen_to + 1 - first) & here;
     const int at = first - s.drafted;  // of the first token among the drafted ones
     const int known = min(s.count, a.mask_columns);
-    const uint32_t here = page ? first_of_8(s.length - first) : 0u;
+    uint32_t bits = 0;
+    if (known > 0) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        if (a.mask) {
-            uint32_t bits = 0;
-            if (known > 0) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) bits |= min((uint32_t)sees[c][min(max(at + j, 0), known - 1)], 1u) << j;
-            }
-            seen[c] = ((bits & first_of_8(known - at)) | first_of_8(-at)) & here;
-        } else {
-            seen[c] = first_of_8(seen_to[c] + 1 - first) & here;
-        }
+        for (int j = 0; j < 8; ++j) bits |= min((uint32_t)sees[min(max(at + j, 0), known - 1)], 1u) << j;
     }
+    return ((bits & first_of_8(known - at)) | first_of_8(-at)) & here;
+}
+
+// Values without infinities and NaN.
+template <int DT>
+__device__ __forceinline__ v4i cleaned(v4i v) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] &= (int)~halves(unbounded<DT>((uint32_t)v[q]));
+    return v;
+}
+
+// Infinities and NaN of an operand of V^T as ones, those of a sign and NaN.
+template <int DT>
+__device__ __forceinline__ void counted4(v4i v, v4i& plus, v4i& minus) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t bits = unbounded<DT>((uint32_t)v[q]);
+        plus[q] = (int)counted<DT>((uint32_t)v[q], bits, 0u);
+        minus[q] = (int)counted<DT>((uint32_t)v[q], bits, 0x80008000u);
+    }
+}
+
+// What is seen of eight tokens, as ones.
+template <int DT>
+__device__ __forceinline__ v4i seen4(uint32_t seen) {
+    constexpr uint32_t one = DT == HFRK_BF16 ? 0x3f80u : 0x3c00u;
+    v4i sights;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sights[q] = (int)(((seen >> 2 * q & 1u) | (seen >> (2 * q + 1) & 1u) << 16) * one);
+    return sights;
 }
 
 // Infinities and NaN among drafted tokens' values: which of a lane's sums one of either sign has reached (a NaN counts as both), a bit for each.
@@ -131,22 +153,13 @@ struct Marks {
     // `values`: in LDS, the lane's part of the operand of V^T's first 16-row block, the others 1 KB apart.  One block at a time, in a loop: unrolled, this
     // rare path takes the registers of the usual one.
     __device__ __forceinline__ void note(const uint32_t (&seen)[C], const v4i* values) {
-        constexpr uint32_t one = DT == HFRK_BF16 ? 0x3f80u : 0x3c00u;
 #pragma unroll 1
         for (int f = 0; f < kCols; ++f) {
-            const v4i v = values[f * kWave];
             v4i plus, minus;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t bits = unbounded<DT>((uint32_t)v[q]);
-                plus[q] = (int)counted<DT>((uint32_t)v[q], bits, 0u);
-                minus[q] = (int)counted<DT>((uint32_t)v[q], bits, 0x80008000u);
-            }
+            counted4<DT>(values[f * kWave], plus, minus);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                v4i sights;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) sights[q] = (int)(((seen[c] >> 2 * q & 1u) | (seen[c] >> (2 * q + 1) & 1u) << 16) * one);
+                const v4i sights = seen4<DT>(seen[c]);
                 const v4f none = {0.f, 0.f, 0.f, 0.f};
                 const v4f up = mfma16<DT>(plus, sights, none), down = mfma16<DT>(minus, sights, none);
 #pragma unroll
@@ -156,13 +169,6 @@ struct Marks {
                 }
             }
         }
-    }
-
-    // The same values without them.
-    static __device__ __forceinline__ v4i cleaned(v4i v) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] &= (int)~halves(unbounded<DT>((uint32_t)v[q]));
-        return v;
     }
 
     __device__ __forceinline__ void apply(v4f (&out)[C][kCols]) const {
@@ -282,7 +288,7 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
     float top[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        top[c] = -INFINITY;
+        top[c] = kNothing;
         sum[c] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int f = 0; f < kCols; ++f) out[c][f] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -335,9 +341,9 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
         const bool some = t0 + kWaveTokens > drafted || __any(lost);
         uint32_t seen[C];
         if (some) {
-            sight<C>(a, s, t0 + value_token, now.value >= 0, seen_to, sees, seen);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
+                seen[c] = sight(a, s, t0 + value_token, now.value >= 0, seen_to[c], sees[c]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (!(seen[c] >> j & 1)) score[c][j / 4][j % 4] = -INFINITY;
@@ -354,16 +360,15 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
             // a row's scale follows its largest score when a lane has found one 2^8 above it, not with every step
             if (__any(most > top[c] + kHeadroom)) {
                 const float grown = fmaxf(top[c], row_max(most));
-                const float shrink = top[c] == grown ? 1.f : __builtin_amdgcn_exp2f(top[c] - grown);
+                const float shrink = __builtin_amdgcn_exp2f(top[c] - grown);
                 top[c] = grown;
                 sum[c] *= shrink;
 #pragma unroll
                 for (int f = 0; f < kCols; ++f) out[c][f] *= shrink;
             }
-            const float base = top[c] == -INFINITY ? 0.f : top[c];
             float w[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(score[c][j / 4][j % 4], scale, -base));
+            for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(score[c][j / 4][j % 4], scale, -top[c]));
             weight[c] = v4i{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
         }
 
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
                 for (int f = 0; f < kCols; ++f) parked[f * kWave] = turned[f];
                 marks.note(seen, parked);
 #pragma unroll
-                for (int f = 0; f < kCols; ++f) turned[f] = Marks<DT, DP, C>::cleaned(parked[f * kWave]);
+                for (int f = 0; f < kCols; ++f) turned[f] = cleaned<DT>(parked[f * kWave]);
             }
         }
 
@@ -449,7 +454,7 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
 #pragma unroll
             for (int w = 0; w < kAttentionWaves; ++w) {
                 const float part_top = statistics[w][r][0];
-                const float share = part_top == most ? 1.f : __builtin_amdgcn_exp2f(part_top - most);  // (equal: both may be -infinity)
+                const float share = __builtin_amdgcn_exp2f(part_top - most);
                 total += share * statistics[w][r][1];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] += share * merged[w][r][d + j];
