@@ -5,17 +5,18 @@
 
 namespace hfrk {
 
-constexpr int kAttentionThreads = 256;
-constexpr int kAttentionWaves = kAttentionThreads / kWave;
-constexpr int kWaveTokens = 32;                                   // cached tokens a wave takes at a time
-constexpr int kTileTokens = kWaveTokens * kAttentionWaves;        // and a workgroup
+constexpr int kWaveTokens = 32;  // cached tokens a wave takes at a time
+// Waves of a workgroup that holds keys and values in registers: two a SIMD, or one where a wave needs more than half of them.
+constexpr int direct_waves(int padded_head) { return padded_head <= 128 ? 8 : 4; }
 
 struct AttentionArgs {
     hfrk_attention_args a;
     float log2_scale;         // softmax scale * log2(e)
     int group;                // query heads per key head
     int rows;                 // rows of a block: C * 16, each a (token, head of the group)
-    int work;                 // tiles per workgroup are chosen so that about this many have some
+    int tile;                 // cached tokens that work is dealt out in
+    int work;                 // workgroups the card has room for at once
+    int least;                // tiles that are not worth splitting
     int slots;                // partial results the workspace holds, per key head
     uint32_t page_magic;      // (t / 8) / (page_size / 8) as a multiplication: n * magic >> (32 + page_shift), or n >> page_shift where magic is 0
     int page_shift;
@@ -50,24 +51,34 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& p, int b) {
 // What a workgroup does: row block `block` of sequence `b`, cached tokens [from, to).
 struct Part {
     int b, block, split, splits, slot;   // slot: where its partial result goes (splits > 1)
-    int from, to;                        // in tiles of kTileTokens
+    int from, to;                        // its tokens; from >= to: none
     Sequence s;
     bool any;
 };
 
-template <typename T>
-__device__ __forceinline__ T lane_prefix(T v, int lane) {  // inclusive sum over the wave's lanes
+__device__ __forceinline__ int lane_prefix(int v, int lane) {  // inclusive sum over the wave's lanes
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
-        const T below = __shfl_up(v, d);
+        const int below = __shfl_up(v, d);
         if (lane >= d) v += below;
     }
     return v;
 }
 
-// The list of work: for every sequence row blocks x splits of its tiles.  The tiles a workgroup takes follow from all sequences' lengths as they are
-// now (in a captured graph too), so that a long one does not keep a few workgroups busy while the others are done.  Each wave makes the list by
-// itself: lanes are sequences.
+__device__ __forceinline__ uint32_t lanes_sum(uint32_t v) {  // over the wave; as wave_sum
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = halves[0] + halves[1];
+    const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = rows[0] + rows[1];
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x128, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x124, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x122, 0xf, 0xf, true);
+    return v + __builtin_amdgcn_update_dpp(0u, v, 0x121, 0xf, 0xf, true);
+}
+
+// The list of work: for every sequence row blocks x splits of its tiles.  How many tiles a workgroup takes follows from all sequences' lengths as they
+// are now (in a captured graph too), so that a long one does not keep a few workgroups busy while the others are done: the share of the whole, and then
+// more until all workgroups find room at once, where that is possible.  Each wave makes the list by itself: lanes are sequences.
 __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
     const int lane = threadIdx.x & (kWave - 1);
     Part part = {};
@@ -77,30 +88,38 @@ __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
         if (b < p.a.seqs) {
             s = sequence(p, b);
             blocks = (int)(((long)s.count * p.group + p.rows - 1) / p.rows);
-            tiles = (s.length + kTileTokens - 1) / kTileTokens;
+            tiles = (s.length + p.tile - 1) / p.tile;
         }
         return s;
     };
-    long total = 0;
+    auto splits_of = [](int tiles, int chunk) { return max(1, (int)((uint32_t)(tiles + chunk - 1) / (uint32_t)chunk)); };
+    uint32_t total = 0, least_items = 0;  // (the host has bounded blocks * tiles)
     for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
         int blocks, tiles;
         amount(b0 + lane, blocks, tiles);
-        long mine = (long)blocks * tiles;
-        if (p.a.seqs > 1) {
-#pragma unroll
-            for (int d = 1; d < kWave; d <<= 1) mine += __shfl_xor(mine, d);
-            total += mine;
-        } else {
-            total = __shfl(mine, 0);
+        total += lanes_sum((uint32_t)(blocks * tiles));
+        least_items += lanes_sum((uint32_t)blocks);
+    }
+    const uint32_t room = (uint32_t)max(1, p.work / p.a.kv_heads);
+    int chunk = max(p.least, (int)((total + room - 1) / room));
+    if (least_items <= room) {
+        for (int round = 0; round < 4; ++round) {
+            uint32_t items = 0;
+            for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
+                int blocks, tiles;
+                amount(b0 + lane, blocks, tiles);
+                items += lanes_sum((uint32_t)(blocks * splits_of(tiles, chunk)));
+            }
+            if (items <= room) break;
+            chunk = (int)((uint64_t)chunk * items / room) + 1;
         }
     }
-    const long share = (total * p.a.kv_heads + p.work - 1) / p.work;
-    const int chunk = __builtin_amdgcn_readfirstlane(share < 1 ? 1 : (int)share);
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
     int items = 0, slots = 0;
     for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
         int blocks, tiles;
         const Sequence s = amount(b0 + lane, blocks, tiles);
-        const int splits = max(1, (tiles + chunk - 1) / chunk);
+        const int splits = splits_of(tiles, chunk);
         const int n = blocks * splits, held = splits > 1 ? n : 0;
         const int items_to = items + (p.a.seqs > 1 ? lane_prefix(n, lane) : n);
         const int slots_to = slots + (p.a.seqs > 1 ? lane_prefix(held, lane) : held);
@@ -108,14 +127,15 @@ __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
         if (found) {
             const int who = __ffsll((unsigned long long)found) - 1;
             const auto of = [who](int v) { return __builtin_amdgcn_readlane(v, who); };  // (into scalar registers: the same for the whole workgroup)
-            const int at = item - (of(items_to) - of(n));
+            const int at = item - (of(items_to) - of(n)), all = of(tiles);
             part.b = b0 + who;
             part.splits = of(splits);
             part.block = (uint32_t)at / (uint32_t)part.splits;
             part.split = at - part.block * part.splits;
             part.slot = of(slots_to) - of(held) + at;
-            part.from = part.split * chunk;
-            part.to = min(part.from + chunk, of(tiles));
+            const int even = (int)((uint32_t)(all + part.splits - 1) / (uint32_t)part.splits);
+            part.from = part.split * even * p.tile;
+            part.to = min((part.split + 1) * even, all) * p.tile;
             part.s = {of(s.first), of(s.count), of(s.length), of(s.drafted)};
             part.any = true;
             return part;

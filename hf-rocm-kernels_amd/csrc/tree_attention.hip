@@ -1,6 +1,9 @@
 // Attention over a paged cache: checks, the choice of kernel, and the kernel that joins the parts of a row.
 #include "tree_attention_kernel.h"
 
+#ifndef V_LEAST
+#define V_LEAST 4
+#endif
 namespace hfrk {
 
 extern template int launch_attention<64>(const AttentionArgs& p, int col_blocks, int grid, hipStream_t stream);
@@ -10,51 +13,92 @@ extern template int launch_attention_shared<64>(const AttentionArgs& p, int grid
 extern template int launch_attention_shared<128>(const AttentionArgs& p, int grid, hipStream_t stream);
 extern template int launch_attention_shared<256>(const AttentionArgs& p, int grid, hipStream_t stream);
 
-// One wave per row of the result whose tokens were split: a lane has eight columns, lane groups take the splits in turn.  The order of
-// the sums is fixed, so equal calls give equal bits.
-template <int DT>
-__global__ void __launch_bounds__(kAttentionThreads) attention_join_kernel(const AttentionArgs p) {
+// Joins the parts of the rows whose tokens were split.  A row's columns are eight a lane, side by side in 16 lanes (32 above 128 columns); PER such groups
+// of lanes take a row's parts in turn: one (many rows), as many as a wave has, or those of a whole workgroup (few rows, many parts).  The order of the
+// sums is fixed, so equal calls give equal bits.
+constexpr int kJoinThreads = 256;
+
+template <int DT, int WIDTH, int PER>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttentionArgs p) {
+    constexpr int kInWave = kWave / WIDTH, kGroups = kJoinThreads / WIDTH;
+    static_assert(PER == 1 || PER == kInWave || PER == kGroups, "a row is a group's, a wave's or a workgroup's");
+    __shared__ float parked[PER == kGroups ? kJoinThreads / kWave : 1][WIDTH][10];
     const hfrk_attention_args& a = p.a;
-    const int lane = threadIdx.x & (kWave - 1);
-    const long index = (long)blockIdx.x * kAttentionWaves + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, group = threadIdx.x / WIDTH;
+    const long index = (long)blockIdx.x * (kGroups / PER) + group / PER;
     const long row = index / a.kv_heads;
     const int head = (int)(index - row * a.kv_heads);
     if (row >= (long)a.tokens * p.group) return;
     const int token = (int)(row / p.group), member = (int)(row - (long)token * p.group);
-    if (a.starts && (token < a.starts[0] || token >= a.starts[a.seqs])) return;  // of no sequence
     const int4 info = p.row_info[row];
+    if (a.starts && (token < a.starts[0] || token >= a.starts[a.seqs])) return;  // of no sequence
     const int first = info.x, splits = info.y;
     if (splits <= 1 || first < 0 || splits > p.slots - first || (uint32_t)info.z >= (uint32_t)p.rows) return;
     const long at = ((long)first * a.kv_heads + head) * p.rows + info.z, step = (long)a.kv_heads * p.rows;
 
-    float most = -INFINITY;
-    for (int s = lane; s < splits; s += kWave) most = fmaxf(most, p.partial_ml[at + s * step].x);
-    most = wave_max(most);
-    const int width = a.head_dim <= 128 ? 16 : 32, d = 8 * (lane & (width - 1));
-    float total = 0.f, o[8] = {};
-    for (int s = lane / width; s < splits; s += kWave / width) {
-        const float2 ml = p.partial_ml[at + s * step];
-        const float share = __builtin_amdgcn_exp2f(ml.x - most);
-        total += share * ml.y;
-        if (d < a.head_dim) {
-            const v4f* const from = reinterpret_cast<const v4f*>(p.partial + (at + s * step) * a.head_dim + d);
-            const v4f lo = from[0], hi = from[1];
+    const int d = 8 * (lane & (WIDTH - 1));
+    const bool column = d < a.head_dim;
+    float top = kNothing, total = 0.f, o[8] = {};
+    auto merge = [&](float other_top, float other_total, const float (&other)[8]) {
+        const float most = fmaxf(top, other_top), mine = __builtin_amdgcn_exp2f(top - most), its = __builtin_amdgcn_exp2f(other_top - most);
+        top = most;
+        total = mine * total + its * other_total;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                o[j] += share * lo[j];
-                o[4 + j] += share * hi[j];
-            }
+        for (int j = 0; j < 8; ++j) o[j] = mine * o[j] + its * other[j];
+    };
+#pragma unroll 4
+    for (int s = group % PER; s < splits; s += PER) {
+        const float2 ml = p.partial_ml[at + s * step];
+        const v4f* const from = reinterpret_cast<const v4f*>(p.partial + (at + s * step) * a.head_dim + (column ? d : 0));
+        const v4f lo = from[0], hi = from[1];
+        const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        merge(ml.x, ml.y, x);
+    }
+    if constexpr (PER > 1) {
+#pragma unroll
+        for (int by = WIDTH; by < kWave; by <<= 1) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __shfl_xor(o[j], by);
+            merge(__shfl_xor(top, by), __shfl_xor(total, by), x);
         }
     }
-    for (int by = width; by < kWave; by <<= 1) {
-        total += __shfl_xor(total, by);
+    if constexpr (PER == kGroups) {
+        if (lane < WIDTH) {
+            float* const to = parked[wave][lane];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] += __shfl_xor(o[j], by);
+            for (int j = 0; j < 8; ++j) to[j] = o[j];
+            to[8] = top;
+            to[9] = total;
+        }
+        __syncthreads();
+        if (wave > 0 || lane >= WIDTH) return;
+#pragma unroll
+        for (int w = 1; w < kJoinThreads / kWave; ++w) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = parked[w][lane][j];
+            merge(parked[w][lane][8], parked[w][lane][9], x);
+        }
     }
-    if (lane >= width || d >= a.head_dim) return;
+    if (!column || (PER > 1 && lane >= WIDTH)) return;
     const bool fp8 = a.cache_dtype == HFRK_FP8_E4M3FN;
     store_row<DT>(a, token, head * p.group + member, d, o, total, fp8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f,
                   a.out_scale ? 1.f / a.out_scale[0] : 1.f);
+}
+
+template <int DT, int WIDTH>
+static int launch_join(const AttentionArgs& p, hipStream_t stream) {
+    constexpr int kGroups = kJoinThreads / WIDTH;
+    const long rows = (long)p.a.tokens * p.a.heads;
+    // A wave a row from one wave per compute unit's SIMD on, a group a row from four waves on: below, more lanes a row find room beside each other.
+    const int per = rows < 4 * kNumCU ? kGroups : rows < 16 * kNumCU ? kWave / WIDTH : 1;
+    const dim3 grid((unsigned)((rows * per + kGroups - 1) / kGroups)), threads(kJoinThreads);
+    if (per == kGroups) hipLaunchKernelGGL((attention_join_kernel<DT, WIDTH, kGroups>), grid, threads, 0, stream, p);
+    else if (per > 1) hipLaunchKernelGGL((attention_join_kernel<DT, WIDTH, kWave / WIDTH>), grid, threads, 0, stream, p);
+    else hipLaunchKernelGGL((attention_join_kernel<DT, WIDTH, 1>), grid, threads, 0, stream, p);
+    HFRK_HIP_TRY(hipGetLastError());
+    return HFRK_SUCCESS;
 }
 
 static int check(const hfrk_attention_args& a) {
@@ -66,6 +110,7 @@ static int check(const hfrk_attention_args& a) {
     if (a.head_dim < 16 || a.head_dim > 256 || a.head_dim % (fp8 || a.head_dim > 128 ? 16 : 8) != 0) return HFRK_BAD_SHAPE;
     if (a.page_size < 8 || a.page_size % 8 != 0 || a.pages < 0 || a.table_columns < 0) return HFRK_BAD_SHAPE;
     if ((long)a.table_columns * a.page_size > (1L << 30) || (long)a.tokens * a.heads > (1L << 28) || a.seqs > (1 << 20)) return HFRK_BAD_SHAPE;
+    // (row blocks times tiles, summed over sequences, stay below 2^32)
     if (!(a.scale > 0.f)) return HFRK_BAD_SHAPE;
     if (a.tokens == 0) return HFRK_SUCCESS;
     if (a.seqs < 1 || (!a.starts && a.tokens % a.seqs != 0)) return HFRK_BAD_SHAPE;
@@ -83,8 +128,8 @@ static int check(const hfrk_attention_args& a) {
 
 // Rows of a block, the work list's bounds and the workspace, from what the host knows: sizes, not lengths.
 struct Decomposition {
-    bool shared;
-    int rows, work, grid, slots;
+    bool shared, fits;
+    int rows, tile, work, least, grid, slots;
     size_t partial, ml, info;  // bytes
 };
 
@@ -101,14 +146,17 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     d.shared = per > 32 && narrow(a.key_page_stride, a.key_place_stride, a.page_size, size) &&
                narrow(a.value_page_stride, a.value_place_stride, a.page_size, size);
     d.rows = per <= 16 ? 16 : per <= 32 || !d.shared ? 32 : per <= 128 || a.head_dim > 128 ? 128 : 256;
-    d.work = d.shared ? 512 : 1024;
+    d.tile = d.shared ? 128 : kWaveTokens * direct_waves(a.head_dim <= 128 ? 128 : 256);
+    d.work = d.rows == 128 ? 2 * kNumCU : kNumCU;
+    d.least = V_LEAST;
     const int rows = d.rows;
     const long blocks = (long)a.tokens * group / rows + a.seqs;
-    const long tiles = ((long)a.table_columns * a.page_size + kTileTokens - 1) / kTileTokens;
+    const long tiles = ((long)a.table_columns * a.page_size + d.tile - 1) / d.tile;
     // sequences' splits are rounded up: one more than their share of the work each, and of those that are split at most twice their share
     const long items = d.work / a.kv_heads + 1 + blocks;
+    d.fits = blocks * tiles < (1L << 31) && items * a.kv_heads < (1L << 31);
     d.grid = (int)(items * a.kv_heads);
-    if (tiles > 1) {
+    if (tiles > d.least) {
         const long slots = 2 * (d.work / a.kv_heads + 1);
         d.slots = (int)(slots < blocks * tiles ? slots : blocks * tiles);
         d.partial = (size_t)d.slots * a.kv_heads * rows * a.head_dim * sizeof(float);
@@ -136,6 +184,7 @@ extern "C" int hfrk_tree_attention(const hfrk_attention_args* args, void* worksp
     p.a = *args;
     const hfrk_attention_args& a = p.a;
     const Decomposition d = decompose(a);
+    if (!d.fits) return HFRK_BAD_SHAPE;
     if (d.slots > 0) {
         if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)) return HFRK_BAD_ALIGNMENT;
         if (workspace_bytes < d.partial + d.info + d.ml) return HFRK_EXCEEDS_SCRATCH;
@@ -147,7 +196,9 @@ extern "C" int hfrk_tree_attention(const hfrk_attention_args* args, void* worksp
     p.log2_scale = a.scale * 1.4426950408889634f;
     p.group = a.heads / a.kv_heads;
     p.rows = d.rows;
+    p.tile = d.tile;
     p.work = d.work;
+    p.least = d.least;
     p.slots = d.slots;
     const uint32_t size = a.cache_dtype == HFRK_FP8_E4M3FN ? 1 : 2;
     p.key_page_bytes = (uint32_t)a.key_page_stride * size;
@@ -174,10 +225,6 @@ extern "C" int hfrk_tree_attention(const hfrk_attention_args* args, void* worksp
                    : a.head_dim <= 128 ? launch_attention<128>(p, d.rows / 16, d.grid, s) : launch_attention<256>(p, d.rows / 16, d.grid, s);
     }
     if (launched != HFRK_SUCCESS || d.slots == 0) return launched;
-    const long waves = (long)a.tokens * a.heads;
-    const dim3 grid((unsigned)((waves + kAttentionWaves - 1) / kAttentionWaves));
-    if (a.dtype == HFRK_BF16) hipLaunchKernelGGL(attention_join_kernel<HFRK_BF16>, grid, dim3(kAttentionThreads), 0, s, p);
-    else hipLaunchKernelGGL(attention_join_kernel<HFRK_F16>, grid, dim3(kAttentionThreads), 0, s, p);
-    HFRK_HIP_TRY(hipGetLastError());
-    return HFRK_SUCCESS;
+    if (a.dtype == HFRK_BF16) return a.head_dim <= 128 ? launch_join<HFRK_BF16, 16>(p, s) : launch_join<HFRK_BF16, 32>(p, s);
+    return a.head_dim <= 128 ? launch_join<HFRK_F16, 16>(p, s) : launch_join<HFRK_F16, 32>(p, s);
 }

@@ -201,14 +201,15 @@ struct CachedTile {
 };
 
 template <int DT, bool FP8, int DP, int C>
-__global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1) attention_kernel(const AttentionArgs p) {
+__global__ void __launch_bounds__(kWave * direct_waves(DP)) attention_kernel(const AttentionArgs p) {
+    constexpr int kWaves = direct_waves(DP), kThreads = kWave * kWaves, kAllTokens = kWaveTokens * kWaves;
     constexpr int kSteps = DP / 32;   // products of 32 columns in K Q^T
     constexpr int kCols = DP / 16;    // V^T's 16-row blocks, and the neighbouring columns a lane loads
     constexpr int kSize = FP8 ? 1 : 2;
     constexpr int kPad = DP + 4;
     typedef CachedTile<DP, FP8> Tile;
-    __shared__ __align__(16) float merged[kAttentionWaves][16][kPad];
-    __shared__ float statistics[kAttentionWaves][16][2];
+    __shared__ __align__(16) float merged[kWaves][16][kPad];
+    __shared__ float statistics[kWaves][16][2];
 
     const hfrk_attention_args& a = p.a;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
@@ -298,22 +299,22 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
 
     Marks<DT, DP, C> marks;
     // a chain's rows see nothing behind the block's last token
-    int end = min(part.to * kTileTokens, s.length);
+    int end = min(part.to, s.length);
     if (!a.mask) end = min(end, drafted + (min(row0 + p.rows, rows) - 1) / p.group + 1);
-    int t0 = part.from * kTileTokens + wave * kWaveTokens;
+    int t0 = part.from + wave * kWaveTokens;
     Tile tile;
     Pages now = {-1, -1}, next = {-1, -1};
     if (t0 < end) {
         now = pages_of(t0);
         load_keys(tile, t0, now.key);
         load_values(tile, t0, now.value);
-        if (t0 + kTileTokens < end) next = pages_of(t0 + kTileTokens);
+        if (t0 + kAllTokens < end) next = pages_of(t0 + kAllTokens);
     }
-    for (; t0 < end; t0 += kTileTokens) {
-        const int t1 = t0 + kTileTokens;
+    for (; t0 < end; t0 += kAllTokens) {
+        const int t1 = t0 + kAllTokens;
         const bool more = t1 < end;
         Pages after = {-1, -1};
-        if (t1 + kTileTokens < end) after = pages_of(t1 + kTileTokens);
+        if (t1 + kAllTokens < end) after = pages_of(t1 + kAllTokens);
 
         v4f score[C][2];
 #pragma unroll
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
 
     marks.apply(out);
 
-    // The four waves' parts of a row: scaled to the largest of their largest scores and added, 16 rows at a time.
+    // The waves' parts of a row: scaled to the largest of their largest scores and added, 16 rows at a time.
     const float value_scale = FP8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f;
     const float inv_out_scale = a.out_scale ? 1.f / a.out_scale[0] : 1.f;
 #pragma unroll
@@ -444,15 +445,15 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
             for (int f = 0; f < kCols; f += 4)
                 *reinterpret_cast<v4f*>(&merged[wave][col][(4 * g + r) * kCols + f]) = v4f{out[c][f][r], out[c][f + 1][r], out[c][f + 2][r], out[c][f + 3][r]};
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * (DP / 8); i += kAttentionThreads) {
+        for (int i = threadIdx.x; i < 16 * (DP / 8); i += kThreads) {
             const int r = i / (DP / 8), d = 8 * (i - r * (DP / 8)), row = row0 + c * 16 + r;
             if (row >= rows || d >= a.head_dim) continue;
             float most = statistics[0][r][0];
 #pragma unroll
-            for (int w = 1; w < kAttentionWaves; ++w) most = fmaxf(most, statistics[w][r][0]);
+            for (int w = 1; w < kWaves; ++w) most = fmaxf(most, statistics[w][r][0]);
             float total = 0.f, o[8] = {};
 #pragma unroll
-            for (int w = 0; w < kAttentionWaves; ++w) {
+            for (int w = 0; w < kWaves; ++w) {
                 const float part_top = statistics[w][r][0];
                 const float share = __builtin_amdgcn_exp2f(part_top - most);
                 total += share * statistics[w][r][1];
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(kAttentionThreads, C <= 2 && DP <= 128 ? 2 : 1
         }
     }
     if (p.row_info && part.split == 0 && head == 0) {
-        for (int r = threadIdx.x; r < p.rows && row0 + r < rows; r += kAttentionThreads)
+        for (int r = threadIdx.x; r < p.rows && row0 + r < rows; r += kThreads)
             p.row_info[(long)s.first * p.group + row0 + r] = make_int4(part.slot - part.split, part.splits, r, 0);
     }
 }
@@ -482,8 +483,8 @@ int launch_attention(const AttentionArgs& p, int col_blocks, int grid, hipStream
     const bool fp8 = p.a.cache_dtype == HFRK_FP8_E4M3FN;
 #define HFRK_ATTENTION(DT, FP8)                                                                                                             \
     do {                                                                                                                                    \
-        if (col_blocks == 1) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 1>), dim3(grid), dim3(kAttentionThreads), 0, stream, p);      \
-        else hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(kAttentionThreads), 0, stream, p);                      \
+        if (col_blocks == 1) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 1>), dim3(grid), dim3(kWave * direct_waves(DP)), 0, stream, p);      \
+        else hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(kWave * direct_waves(DP)), 0, stream, p);                      \
     } while (0)
     if (p.a.dtype == HFRK_BF16) {
         if (fp8) HFRK_ATTENTION(HFRK_BF16, true);

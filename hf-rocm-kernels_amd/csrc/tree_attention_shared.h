@@ -258,9 +258,9 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) attention_share
     float sum = 0.f, top = kNothing, bound = kNothing;  // bound: the raw score from which on the row's scale has to follow
     WideMarks<DT, DP> marks;
 
-    int end = min(part.to * kTileTokens, s.length);
+    int end = min(part.to, s.length);
     if (!a.mask) end = min(end, drafted + (min(block0 + p.rows, rows) - 1) / p.group + 1);  // a chain's rows see nothing behind the block's last token
-    const int begin = part.from * kTileTokens;
+    const int begin = part.from;
     const int steps = begin < end ? (end - begin + 31) / 32 : 0, tiles_here = (steps + 1) / 2;
     const int plain_to = min(drafted, s.length);  // tokens in front of it are seen by all, where they have a page
     if (steps > 0) {
