@@ -6,8 +6,7 @@
 namespace hfrk {
 
 constexpr int kWaveTokens = 32;  // cached tokens a wave takes at a time
-// Waves of a workgroup that holds keys and values in registers: two a SIMD, or one where a wave needs more than half of them.
-constexpr int direct_waves(int padded_head) { return padded_head <= 128 ? 8 : 4; }
+constexpr int kDirectWaves = 4;  // of a workgroup that holds keys and values in registers
 
 struct AttentionArgs {
     hfrk_attention_args a;
@@ -16,7 +15,7 @@ struct AttentionArgs {
     int rows;                 // rows of a block: C * 16, each a (token, head of the group)
     int tile;                 // cached tokens that work is dealt out in
     int work;                 // workgroups the card has room for at once
-    int least;                // tiles that are not worth splitting
+    int shares;               // into how many workgroups one's share may be cut
     int slots;                // partial results the workspace holds, per key head
     uint32_t page_magic;      // (t / 8) / (page_size / 8) as a multiplication: n * magic >> (32 + page_shift), or n >> page_shift where magic is 0
     int page_shift;
@@ -56,13 +55,15 @@ struct Part {
     bool any;
 };
 
-__device__ __forceinline__ int lane_prefix(int v, int lane) {  // inclusive sum over the wave's lanes
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int below = __shfl_up(v, d);
-        if (lane >= d) v += below;
-    }
-    return v;
+// Inclusive sum over the wave's lanes: within rows of 16 by shifts of 1, 2, 4, 8, then the first and third row's last lane to the rows behind them, then the
+// first half's to the second half.  (By exchanges through LDS a workgroup's start took 0.5 us longer.)
+__device__ __forceinline__ int lane_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 
 __device__ __forceinline__ uint32_t lanes_sum(uint32_t v) {  // over the wave; as wave_sum
@@ -77,57 +78,77 @@ __device__ __forceinline__ uint32_t lanes_sum(uint32_t v) {  // over the wave; a
 }
 
 // The list of work: for every sequence row blocks x splits of its tiles.  How many tiles a workgroup takes follows from all sequences' lengths as they
-// are now (in a captured graph too), so that a long one does not keep a few workgroups busy while the others are done: the share of the whole, and then
-// more until all workgroups find room at once, where that is possible.  Each wave makes the list by itself: lanes are sequences.
+// are now (in a captured graph too), so that a long one does not keep a few workgroups busy while the others are done.  Each wave makes the list by
+// itself: lanes are sequences.
+//
+// Of the whole's share of a workgroup, a half and so on of it (p.shares), and of what lets all workgroups run at once, that is taken which ends
+// first: where all run at once, with the longest; else with the whole's share and half a workgroup more.  A workgroup costs about two tiles by itself.
+// (64 lengths from 1 to 8192 in fp8: all at once 131 us, the share 101, half of it 97, a quarter 110.)
 __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
     const int lane = threadIdx.x & (kWave - 1);
     Part part = {};
-    auto amount = [&](int b, int& blocks, int& tiles) {
-        blocks = tiles = 0;
-        Sequence s = {0, 0, 0, 0};
-        if (b < p.a.seqs) {
-            s = sequence(p, b);
-            blocks = (int)(((long)s.count * p.group + p.rows - 1) / p.rows);
-            tiles = (s.length + p.tile - 1) / p.tile;
-        }
-        return s;
+    struct Amount {
+        int blocks, tiles;
+        Sequence s;
     };
-    auto splits_of = [](int tiles, int chunk) { return max(1, (int)((uint32_t)(tiles + chunk - 1) / (uint32_t)chunk)); };
+    auto look = [&](int b) {
+        Amount m = {};
+        if (b < p.a.seqs) {
+            m.s = sequence(p, b);
+            m.blocks = (int)((uint32_t)(m.s.count * p.group + p.rows - 1) / (uint32_t)p.rows);
+            m.tiles = (int)((uint32_t)(m.s.length + p.tile - 1) / (uint32_t)p.tile);
+        }
+        return m;
+    };
+    const Amount first = look(lane);  // the first 64 sequences stay in registers, mostly all
+    auto amount = [&](int b0) { return b0 == 0 ? first : look(b0 + lane); };
+    // ceil(tiles / chunk); the half keeps the quotient's rounding from an integer for tiles + chunk below 2^21
+    auto splits_of = [](int tiles, int chunk) { return max(1, (int)(((float)(tiles + chunk) - 0.5f) * __builtin_amdgcn_rcpf((float)chunk))); };
     uint32_t total = 0, least_items = 0;  // (the host has bounded blocks * tiles)
     for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
-        int blocks, tiles;
-        amount(b0 + lane, blocks, tiles);
-        total += lanes_sum((uint32_t)(blocks * tiles));
-        least_items += lanes_sum((uint32_t)blocks);
+        const Amount m = amount(b0);
+        total += lanes_sum((uint32_t)(m.blocks * m.tiles));
+        least_items += lanes_sum((uint32_t)m.blocks);
     }
+    auto items_of = [&](int chunk) {
+        uint32_t items = 0;
+        for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
+            const Amount m = amount(b0);
+            items += lanes_sum((uint32_t)(m.blocks * splits_of(m.tiles, chunk)));
+        }
+        return items;
+    };
     const uint32_t room = (uint32_t)max(1, p.work / p.a.kv_heads);
-    int chunk = max(p.least, (int)((total + room - 1) / room));
-    if (least_items <= room) {
-        for (int round = 0; round < 4; ++round) {
-            uint32_t items = 0;
-            for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
-                int blocks, tiles;
-                amount(b0 + lane, blocks, tiles);
-                items += lanes_sum((uint32_t)(blocks * splits_of(tiles, chunk)));
+    int chunk = max(1, (int)((total + room - 1) / room));
+    if (p.shares > 1 && least_items > 0) {
+        const int share = chunk;
+        float best = 3e38f;
+        uint32_t at_once = 0;
+        for (int k = 1; k <= p.shares + 1; ++k) {
+            const int now = k <= p.shares ? (share + k - 1) / k : (int)((uint64_t)share * at_once / room) + 1;
+            if (k > p.shares && (at_once <= room || least_items > room)) break;
+            const uint32_t items = items_of(now);
+            if (k == 1) at_once = items;
+            const float ends = items <= room ? (float)now : ((float)total + 2.f * (float)items) * __builtin_amdgcn_rcpf((float)room) + 0.5f * (float)now;
+            if (ends < best) {
+                best = ends;
+                chunk = now;
             }
-            if (items <= room) break;
-            chunk = (int)((uint64_t)chunk * items / room) + 1;
         }
     }
     chunk = __builtin_amdgcn_readfirstlane(chunk);
     int items = 0, slots = 0;
     for (int b0 = 0; b0 < p.a.seqs; b0 += kWave) {
-        int blocks, tiles;
-        const Sequence s = amount(b0 + lane, blocks, tiles);
-        const int splits = splits_of(tiles, chunk);
-        const int n = blocks * splits, held = splits > 1 ? n : 0;
-        const int items_to = items + (p.a.seqs > 1 ? lane_prefix(n, lane) : n);
-        const int slots_to = slots + (p.a.seqs > 1 ? lane_prefix(held, lane) : held);
+        const Amount m = amount(b0);
+        const Sequence s = m.s;
+        const int splits = splits_of(m.tiles, chunk);
+        const int n = m.blocks * splits, held = splits > 1 ? n : 0;
+        const int items_to = items + lane_prefix(n), slots_to = slots + lane_prefix(held);
         const uint64_t found = __ballot(n > 0 && item >= items_to - n && item < items_to);
         if (found) {
             const int who = __ffsll((unsigned long long)found) - 1;
             const auto of = [who](int v) { return __builtin_amdgcn_readlane(v, who); };  // (into scalar registers: the same for the whole workgroup)
-            const int at = item - (of(items_to) - of(n)), all = of(tiles);
+            const int at = item - (of(items_to) - of(n)), all = of(m.tiles);
             part.b = b0 + who;
             part.splits = of(splits);
             part.block = (uint32_t)at / (uint32_t)part.splits;
@@ -140,8 +161,8 @@ __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
             part.any = true;
             return part;
         }
-        items = __builtin_amdgcn_readlane(items_to, p.a.seqs > 1 ? kWave - 1 : 0);
-        slots = __builtin_amdgcn_readlane(slots_to, p.a.seqs > 1 ? kWave - 1 : 0);
+        items = __builtin_amdgcn_readlane(items_to, kWave - 1);
+        slots = __builtin_amdgcn_readlane(slots_to, kWave - 1);
     }
     return part;
 }

@@ -1,8 +1,8 @@
 // Attention over a paged cache: checks, the choice of kernel, and the kernel that joins the parts of a row.
 #include "tree_attention_kernel.h"
 
-#ifndef V_LEAST
-#define V_LEAST 4
+#ifndef V_W
+#define V_W 2
 #endif
 namespace hfrk {
 
@@ -109,7 +109,7 @@ static int check(const hfrk_attention_args& a) {
     if (a.tokens < 0 || a.seqs < 0 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.heads > 65536) return HFRK_BAD_SHAPE;
     if (a.head_dim < 16 || a.head_dim > 256 || a.head_dim % (fp8 || a.head_dim > 128 ? 16 : 8) != 0) return HFRK_BAD_SHAPE;
     if (a.page_size < 8 || a.page_size % 8 != 0 || a.pages < 0 || a.table_columns < 0) return HFRK_BAD_SHAPE;
-    if ((long)a.table_columns * a.page_size > (1L << 30) || (long)a.tokens * a.heads > (1L << 28) || a.seqs > (1 << 20)) return HFRK_BAD_SHAPE;
+    if ((long)a.table_columns * a.page_size > (1L << 27) || (long)a.tokens * a.heads > (1L << 28) || a.seqs > (1 << 20)) return HFRK_BAD_SHAPE;
     // (row blocks times tiles, summed over sequences, stay below 2^32)
     if (!(a.scale > 0.f)) return HFRK_BAD_SHAPE;
     if (a.tokens == 0) return HFRK_SUCCESS;
@@ -129,7 +129,7 @@ static int check(const hfrk_attention_args& a) {
 // Rows of a block, the work list's bounds and the workspace, from what the host knows: sizes, not lengths.
 struct Decomposition {
     bool shared, fits;
-    int rows, tile, work, least, grid, slots;
+    int rows, tile, work, shares, grid, slots;
     size_t partial, ml, info;  // bytes
 };
 
@@ -146,19 +146,19 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     d.shared = per > 32 && narrow(a.key_page_stride, a.key_place_stride, a.page_size, size) &&
                narrow(a.value_page_stride, a.value_place_stride, a.page_size, size);
     d.rows = per <= 16 ? 16 : per <= 32 || !d.shared ? 32 : per <= 128 || a.head_dim > 128 ? 128 : 256;
-    d.tile = d.shared ? 128 : kWaveTokens * direct_waves(a.head_dim <= 128 ? 128 : 256);
-    d.work = d.rows == 128 ? 2 * kNumCU : kNumCU;
-    d.least = V_LEAST;
+    d.tile = d.shared ? 128 : kWaveTokens * kDirectWaves;
+    d.work = d.rows == 256 || a.head_dim > 128 ? kNumCU : V_W * kNumCU;
     const int rows = d.rows;
     const long blocks = (long)a.tokens * group / rows + a.seqs;
     const long tiles = ((long)a.table_columns * a.page_size + d.tile - 1) / d.tile;
-    // sequences' splits are rounded up: one more than their share of the work each, and of those that are split at most twice their share
-    const long items = d.work / a.kv_heads + 1 + blocks;
+    // Workgroups take the whole's share or a part of it (find_part).  Splits are rounded up: one more than that a block, and of those that are split at
+    // most twice as many.
+    d.shares = a.seqs > 1 ? 2 : 1;
+    const long most = (long)d.shares * (d.work / a.kv_heads > 1 ? d.work / a.kv_heads : 1), items = most + blocks < blocks * tiles ? most + blocks : blocks * (tiles > 0 ? tiles : 1);
     d.fits = blocks * tiles < (1L << 31) && items * a.kv_heads < (1L << 31);
     d.grid = (int)(items * a.kv_heads);
-    if (tiles > d.least) {
-        const long slots = 2 * (d.work / a.kv_heads + 1);
-        d.slots = (int)(slots < blocks * tiles ? slots : blocks * tiles);
+    if (tiles > 1) {
+        d.slots = (int)(2 * most < blocks * tiles ? 2 * most : blocks * tiles);
         d.partial = (size_t)d.slots * a.kv_heads * rows * a.head_dim * sizeof(float);
         d.ml = (size_t)d.slots * a.kv_heads * rows * sizeof(float2);
         d.info = (size_t)a.tokens * group * sizeof(int4);
@@ -198,7 +198,7 @@ extern "C" int hfrk_tree_attention(const hfrk_attention_args* args, void* worksp
     p.rows = d.rows;
     p.tile = d.tile;
     p.work = d.work;
-    p.least = d.least;
+    p.shares = d.shares;
     p.slots = d.slots;
     const uint32_t size = a.cache_dtype == HFRK_FP8_E4M3FN ? 1 : 2;
     p.key_page_bytes = (uint32_t)a.key_page_stride * size;

@@ -6,7 +6,7 @@
 // scaled down).
 // A row is one drafted token and one of the query heads that share a key head, so a group of heads reads its keys and values once.
 //
-// Each wave takes 32 cached tokens at a time and C blocks of 16 rows, straight from memory to registers and without LDS:
+// Each wave takes 32 cached tokens at a time and C blocks of 16 rows, from memory to its own registers; keys go through its own part of LDS:
 //   S^T = K Q^T   keys are the A operand.  Row r of the two 16-row products is token 8 (r / 4) + 4 t + r % 4, so that a lane's eight scores are those
 //                 of eight tokens in a row, 8 g .. 8 g + 7 for lane group g = lane / 16, all of query row lane % 16
 //   O^T += V^T P  these eight are, rounded to 16 bits, already the B operand of the second product.  Its A operand is V^T: a lane has loaded
@@ -194,15 +194,13 @@ struct Marks {
 // One wave's operands of 32 cached tokens.
 template <int DP, bool FP8>
 struct CachedTile {
-    static constexpr int kKeyLoads = FP8 ? DP / 64 : DP / 32;   // 16-byte pieces of a key a lane holds
-    static constexpr int kValueWords = (FP8 ? DP / 16 : DP / 8) / 4;  // words of a value
-    v4i key[2][kKeyLoads];
-    uint32_t value[8][kValueWords];
+    static constexpr int kWords = (FP8 ? DP / 16 : DP / 8) / 4;  // of a lane's columns of one token
+    uint32_t key[8][kWords], value[8][kWords];
 };
 
 template <int DT, bool FP8, int DP, int C>
-__global__ void __launch_bounds__(kWave * direct_waves(DP)) attention_kernel(const AttentionArgs p) {
-    constexpr int kWaves = direct_waves(DP), kThreads = kWave * kWaves, kAllTokens = kWaveTokens * kWaves;
+__global__ void __launch_bounds__(kWave * kDirectWaves, DP <= 128 ? 2 : 1) attention_kernel(const AttentionArgs p) {
+    constexpr int kWaves = kDirectWaves, kThreads = kWave * kWaves, kAllTokens = kWaveTokens * kWaves;
     constexpr int kSteps = DP / 32;   // products of 32 columns in K Q^T
     constexpr int kCols = DP / 16;    // V^T's 16-row blocks, and the neighbouring columns a lane loads
     constexpr int kSize = FP8 ? 1 : 2;
@@ -220,10 +218,7 @@ __global__ void __launch_bounds__(kWave * direct_waves(DP)) attention_kernel(con
     const int row0 = part.block * p.rows, rows = s.count * p.group;
     const int drafted = s.drafted;
 
-    // Lane group g has the columns kWindow g .. of keys and queries, read as whole 16-byte pieces one behind the other.  A head that ends inside
-    // a window: the window is moved to the head's end, and the query is zero in the columns that are not this group's.
-    constexpr int kWindow = DP / 4;
-    const int window = min(kWindow * g, a.head_dim - kWindow);
+    // queries: lane group g has 8 columns of each product's 32
     v4i query[C][kSteps];
     int seen_to[C];      // chain: the last token this lane's row sees (-1: no row)
     const uint8_t* sees[C];  // tree: its row of the mask
@@ -237,50 +232,65 @@ __global__ void __launch_bounds__(kWave * direct_waves(DP)) attention_kernel(con
                                                                                   (long)(head * p.group + member) * a.query_head_stride : 0);
 #pragma unroll
         for (int step = 0; step < kSteps; ++step) {
-            const int d = window + 8 * step;
-            query[c][step] = real && d >= kWindow * g ? *reinterpret_cast<const v4i*>(q + d) : v4i{0, 0, 0, 0};
+            const int d = 32 * step + 8 * g;
+            query[c][step] = real && d < a.head_dim ? *reinterpret_cast<const v4i*>(q + d) : v4i{0, 0, 0, 0};
         }
     }
     const float scale = p.log2_scale * (FP8 && a.key_scale ? a.key_scale[head * a.key_scale_stride] : 1.f);
 
-    // where a lane reads: keys of two tokens, values of eight
-    const int key_token = 8 * (col >> 2) + (col & 3), value_token = 8 * g;
-    const int value_column = col * kCols < a.head_dim ? col * kCols : 0;  // (columns a head does not have are read elsewhere and not stored)
-    const uint8_t* const keys = static_cast<const uint8_t*>(a.key_cache) + ((long)head * a.key_cache_head_stride + window) * kSize;
-    const uint8_t* const values = static_cast<const uint8_t*>(a.value_cache) + ((long)head * a.value_cache_head_stride + value_column) * kSize;
+    // A lane reads kCols columns of eight tokens, keys and values alike: whole rows side by side in 16 lanes.  (As operands of K Q^T, 16 rows side by side,
+    // neighbouring lanes read 64 places apart, and a compute unit took requests at a quarter of the rate.)
+    const int token8 = 8 * g;
+    const bool column = col * kCols < a.head_dim;  // columns a head does not have are read elsewhere; keys are cleared there, values not stored
+    const uint8_t* const keys = static_cast<const uint8_t*>(a.key_cache) + ((long)head * a.key_cache_head_stride + (column ? col * kCols : 0)) * kSize;
+    const uint8_t* const values = static_cast<const uint8_t*>(a.value_cache) + ((long)head * a.value_cache_head_stride + (column ? col * kCols : 0)) * kSize;
     const int32_t* const table = a.page_table + (long)part.b * a.table_stride;
-
-    struct Pages {
-        int key, value;
-    };
-    auto page_of = [&](int token) {
+    auto index_of = [&](int token) {
         const uint32_t n = (uint32_t)token >> 3;
         return (int)(p.page_magic ? __umulhi(n, p.page_magic) >> p.page_shift : n >> p.page_shift);
     };
-    auto entry = [&](int token) {  // -1: no such page
-        const int at = page_of(token);
-        const int page = at < a.table_columns ? table[at] : -1;
-        return page >= 0 && page < a.pages ? page : -1;
+    auto page_of = [&](int t0) {  // of the lane's eight tokens; -1: none
+        const int at = index_of(t0 + token8);
+        const int page = table[min(at, a.table_columns - 1)];
+        return at < a.table_columns && (uint32_t)page < (uint32_t)a.pages ? page : -1;
     };
-    auto pages_of = [&](int t0) { return Pages{entry(t0 + key_token), entry(t0 + value_token)}; };
-    auto load_keys = [&](Tile& tile, int t0, int page) {
-        const int token = t0 + key_token, in_page = token - page_of(token) * a.page_size;
-        const uint8_t* at = keys + ((long)max(page, 0) * a.key_page_stride + (long)in_page * a.key_place_stride) * kSize;
+    auto load = [&](uint32_t (&to)[8][Tile::kWords], const uint8_t* cache, long page_stride, long place_stride, int t0, int page) {
+        const int token = t0 + token8, in_page = token - index_of(token) * a.page_size;
+        const uint8_t* at = cache + ((long)max(page, 0) * page_stride + (long)in_page * place_stride) * kSize;
 #pragma unroll
-        for (int t = 0; t < 2; ++t, at += 4 * a.key_place_stride * kSize)
+        for (int j = 0; j < 8; ++j, at += place_stride * kSize) {
+            if constexpr (Tile::kWords == 1) to[j][0] = *reinterpret_cast<const uint32_t*>(at);
+            if constexpr (Tile::kWords == 2) *reinterpret_cast<uint2*>(to[j]) = *reinterpret_cast<const uint2*>(at);
+            if constexpr (Tile::kWords >= 4) {
 #pragma unroll
-            for (int i = 0; i < Tile::kKeyLoads; ++i) tile.key[t][i] = *reinterpret_cast<const v4i*>(at + 16 * i);
+                for (int w = 0; w < Tile::kWords; w += 4) *reinterpret_cast<uint4*>(to[j] + w) = *reinterpret_cast<const uint4*>(at + 4 * w);
+            }
+        }
     };
-    auto load_values = [&](Tile& tile, int t0, int page) {
-        const int token = t0 + value_token, in_page = token - page_of(token) * a.page_size;
-        const uint8_t* at = values + ((long)max(page, 0) * a.value_page_stride + (long)in_page * a.value_place_stride) * kSize;
+    auto load_keys = [&](Tile& tile, int t0, int page) { load(tile.key, keys, a.key_page_stride, a.key_place_stride, t0, page); };
+    auto load_values = [&](Tile& tile, int t0, int page) { load(tile.value, values, a.value_page_stride, a.value_place_stride, t0, page); };
+    // The wave's own LDS turns keys from rows to operands: token 8 g + j is row 4 g + j % 4 of product j / 4; pieces of eight columns change places by the row,
+    // which spreads a product's rows over the banks.
+    uint8_t* const own = reinterpret_cast<uint8_t*>(&merged[wave][0][0]);
+    constexpr int kChunks = DP / 8;
+    auto piece_at = [](int token, int row, int chunk) { return (token * kChunks + (chunk ^ (DP == 64 ? row / 2 : row))) * 16; };
+    auto turn_keys = [&](const Tile& tile) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j, at += a.value_place_stride * kSize) {
-            if constexpr (Tile::kValueWords == 1) tile.value[j][0] = *reinterpret_cast<const uint32_t*>(at);
-            if constexpr (Tile::kValueWords == 2) *reinterpret_cast<uint2*>(tile.value[j]) = *reinterpret_cast<const uint2*>(at);
-            if constexpr (Tile::kValueWords >= 4) {
+        for (int j = 0; j < 8; ++j) {
+            const int token = token8 + j, row = 4 * g + j % 4;
+            uint32_t x[kCols / 2];
 #pragma unroll
-                for (int w = 0; w < Tile::kValueWords; w += 4) *reinterpret_cast<uint4*>(tile.value[j] + w) = *reinterpret_cast<const uint4*>(at + 4 * w);
+            for (int w = 0; w < kCols / 2; ++w) {
+                if constexpr (FP8) x[w] = w % 2 == 0 ? widen2<DT, false>(tile.key[j][w / 2]) : widen2<DT, true>(tile.key[j][w / 2]);
+                else x[w] = tile.key[j][w];
+                if (!column) x[w] = 0;
+            }
+            if constexpr (kCols == 4) {
+                *reinterpret_cast<uint2*>(own + piece_at(token, row, col / 2) + col % 2 * 8) = make_uint2(x[0], x[1]);
+            } else {
+#pragma unroll
+                for (int w = 0; w < kCols / 2; w += 4)
+                    *reinterpret_cast<uint4*>(own + piece_at(token, row, col * (kCols / 8) + w / 4)) = make_uint4(x[w], x[w + 1], x[w + 2], x[w + 3]);
             }
         }
     };
@@ -303,48 +313,45 @@ __global__ void __launch_bounds__(kWave * direct_waves(DP)) attention_kernel(con
     if (!a.mask) end = min(end, drafted + (min(row0 + p.rows, rows) - 1) / p.group + 1);
     int t0 = part.from + wave * kWaveTokens;
     Tile tile;
-    Pages now = {-1, -1}, next = {-1, -1};
+    int now = -1, next = -1;
     if (t0 < end) {
-        now = pages_of(t0);
-        load_keys(tile, t0, now.key);
-        load_values(tile, t0, now.value);
-        if (t0 + kAllTokens < end) next = pages_of(t0 + kAllTokens);
+        now = page_of(t0);
+        load_keys(tile, t0, now);
+        load_values(tile, t0, now);
+        next = page_of(t0 + kAllTokens);
     }
+    // The queries are here before the loop: waited for within it, a wait would take in the next tokens' requests as well.
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) asm volatile("" : "+v"(query[c][step]));
     for (; t0 < end; t0 += kAllTokens) {
         const int t1 = t0 + kAllTokens;
         const bool more = t1 < end;
-        Pages after = {-1, -1};
-        if (t1 + kAllTokens < end) after = pages_of(t1 + kAllTokens);
+        const int after = page_of(t1 + kAllTokens);  // (always: a wait for it alone)
 
+        turn_keys(tile);
+        if (more) load_keys(tile, t1, next);
         v4f score[C][2];
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) score[c][0] = score[c][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                v4f acc = {0.f, 0.f, 0.f, 0.f};
+                const v4i k = *reinterpret_cast<const v4i*>(own + piece_at(8 * (col >> 2) + 4 * t + (col & 3), col, 4 * step + g));
 #pragma unroll
-                for (int step = 0; step < kSteps; ++step) {
-                    v4i k;
-                    if constexpr (FP8) {
-                        const int lo = tile.key[t][step / 2][2 * (step % 2)], hi = tile.key[t][step / 2][2 * (step % 2) + 1];
-                        k = v4i{widen2<DT, false>(lo), widen2<DT, true>(lo), widen2<DT, false>(hi), widen2<DT, true>(hi)};
-                    } else {
-                        k = tile.key[t][step];
-                    }
-                    acc = mfma16<DT>(k, query[c][step], acc);
-                }
-                score[c][t] = acc;
+                for (int c = 0; c < C; ++c) score[c][t] = mfma16<DT>(k, query[c][step], score[c][t]);
             }
-        if (more) load_keys(tile, t1, next.key);
 
         // Tokens that some row does not see: drafted ones, those behind the end, those without a page.
-        const bool lost = now.value < 0 || t0 + value_token + 7 >= s.length;
+        const bool lost = now < 0 || t0 + token8 + 7 >= s.length;
         const bool some = t0 + kWaveTokens > drafted || __any(lost);
         uint32_t seen[C];
         if (some) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                seen[c] = sight(a, s, t0 + value_token, now.value >= 0, seen_to[c], sees[c]);
+                seen[c] = sight(a, s, t0 + token8, now >= 0, seen_to[c], sees[c]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (!(seen[c] >> j & 1)) score[c][j / 4][j % 4] = -INFINITY;
@@ -390,12 +397,12 @@ __global__ void __launch_bounds__(kWave * direct_waves(DP)) attention_kernel(con
                 turned[f][q] = (int)__builtin_amdgcn_perm(odd, even, 0x05040100u);
                 turned[f + 1][q] = (int)__builtin_amdgcn_perm(odd, even, 0x07060302u);
             }
-        if (more) load_values(tile, t1, next.value);
+        if (C == 1 && more) load_values(tile, t1, next);  // (two blocks of rows: behind the products, whose operands take the registers)
 
         if (some) {
             // Weights of zero do not keep an infinity or a NaN out of the sums.  Memory behind the end and without a page is cleared; a drafted
             // token's own are noted for the rows that see it, and taken out.
-            const int left = now.value < 0 ? 0 : min(max(s.length - (t0 + value_token), 0), 8);
+            const int left = now < 0 ? 0 : min(max(s.length - (t0 + token8), 0), 8);
             uint32_t bad = 0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -422,6 +429,7 @@ __global__ void __launch_bounds__(kWave * direct_waves(DP)) attention_kernel(con
 #pragma unroll
             for (int f = 0; f < kCols; ++f) out[c][f] = mfma16<DT>(turned[f], weight[c], out[c][f]);
         }
+        if (C == 2 && more) load_values(tile, t1, next);
         now = next;
         next = after;
     }
@@ -483,8 +491,8 @@ int launch_attention(const AttentionArgs& p, int col_blocks, int grid, hipStream
     const bool fp8 = p.a.cache_dtype == HFRK_FP8_E4M3FN;
 #define HFRK_ATTENTION(DT, FP8)                                                                                                             \
     do {                                                                                                                                    \
-        if (col_blocks == 1) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 1>), dim3(grid), dim3(kWave * direct_waves(DP)), 0, stream, p);      \
-        else hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(kWave * direct_waves(DP)), 0, stream, p);                      \
+        if (col_blocks == 1) hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 1>), dim3(grid), dim3(kWave * kDirectWaves), 0, stream, p);      \
+        else hipLaunchKernelGGL((attention_kernel<DT, FP8, DP, 2>), dim3(grid), dim3(kWave * kDirectWaves), 0, stream, p);                      \
     } while (0)
     if (p.a.dtype == HFRK_BF16) {
         if (fp8) HFRK_ATTENTION(HFRK_BF16, true);

@@ -32,7 +32,7 @@ def tree_attention_checks(
     assert page_table.dim() == 2 and page_table.dtype == torch.int32, f"Expected page_table to be (seqs, columns) int32 but got {page_table.shape} {page_table.dtype}"
     assert page_table.size(1) <= 1 or page_table.stride(1) == 1, f"Expected page_table to have unit stride along its rows but got {page_table.stride()}"
     seqs = page_table.size(0)
-    assert page_table.size(1) * page_size <= 1 << 30, f"Expected at most 2^30 places in a row of page_table: {page_table.shape = }, {page_size = }"
+    assert page_table.size(1) * page_size <= 1 << 27, f"Expected at most 2^27 places in a row of page_table: {page_table.shape = }, {page_size = }"
     assert tokens * heads <= 1 << 28, f"Expected at most 2^28 query heads in a call: {query.shape = }"
     assert tokens == 0 or (key_cache.size(0) >= 1 and page_table.size(1) >= 1), "Expected a page and a column of page_table at least"
     for name, x, count in (("lengths", lengths, seqs), ("starts", starts, seqs + 1)):

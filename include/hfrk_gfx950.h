@@ -442,7 +442,7 @@ int hfrk_append_kv(const hfrk_append_args* args, void* stream);
  * Lengths, starts and tables are read on the device: a captured call may be replayed with others.  The number of parts that a sequence's tokens are
  * split into follows from all lengths of the call, and with it the order of the sums; equal calls give equal bits.
  * head_dim at least 16, a multiple of 8 up to 128, of 16 (e4m3fn caches: always) up to 256; page_size a multiple of 8; query, caches and 16-bit output on 16-byte
- * boundaries with strides of whole 16-byte pieces; scale > 0; table_columns * page_size <= 2^30, tokens * heads <= 2^28.
+ * boundaries with strides of whole 16-byte pieces; scale > 0; table_columns * page_size <= 2^27, tokens * heads <= 2^28.
  * workspace: hfrk_tree_attention_workspace_bytes of it (0: none), 16-byte aligned, any contents, used by one call at a time. */
 typedef struct hfrk_attention_args {
     const void* query;

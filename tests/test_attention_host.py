@@ -97,7 +97,7 @@ def _caches(*shape, dtype=BF16):
     (_caches(0, 16, 2, 64), "a page"),
     (dict(page_table=torch.zeros(2, 3, dtype=torch.long)), "page_table"),
     (dict(page_table=torch.zeros(3, 2, dtype=torch.int32).t()), "unit stride"),
-    (dict(page_table=torch.zeros(1, dtype=torch.int32).expand(2, (1 << 26) + 1)), "unit stride|2\\^30"),
+    (dict(page_table=torch.zeros(1, dtype=torch.int32).expand(2, (1 << 23) + 1)), "unit stride|2\\^27"),
     (dict(lengths=torch.ones(3, dtype=torch.int32)), "lengths"),
     (dict(lengths=torch.ones(2, dtype=torch.long)), "lengths"),
     (dict(starts=torch.ones(2, dtype=torch.int32)), "starts"),
@@ -161,7 +161,7 @@ def _attention_args(**changes):
     (dict(heads=3), _capi.BAD_SHAPE), (dict(head_dim=8), _capi.BAD_SHAPE), (dict(head_dim=68), _capi.BAD_SHAPE), (dict(head_dim=136), _capi.BAD_SHAPE),
     (dict(head_dim=264), _capi.BAD_SHAPE), (dict(head_dim=72, cache_dtype=_capi.FP8_E4M3FN), _capi.BAD_SHAPE), (dict(page_size=4), _capi.BAD_SHAPE),
     (dict(page_size=20), _capi.BAD_SHAPE), (dict(pages=0), _capi.BAD_SHAPE), (dict(table_columns=0), _capi.BAD_SHAPE),
-    (dict(table_columns=1 << 27), _capi.BAD_SHAPE), (dict(tokens=3), _capi.BAD_SHAPE), (dict(seqs=0), _capi.BAD_SHAPE), (dict(scale=0.0), _capi.BAD_SHAPE),
+    (dict(table_columns=(1 << 23) + 1), _capi.BAD_SHAPE), (dict(tokens=3), _capi.BAD_SHAPE), (dict(seqs=0), _capi.BAD_SHAPE), (dict(scale=0.0), _capi.BAD_SHAPE),
     (dict(scale=math.nan), _capi.BAD_SHAPE), (dict(tokens=1 << 27, seqs=1 << 20), _capi.BAD_SHAPE), (dict(query=None), _capi.BAD_SHAPE),
     (dict(lengths=None), _capi.BAD_SHAPE), (dict(query=4104), _capi.BAD_ALIGNMENT), (dict(key_cache=4104), _capi.BAD_ALIGNMENT),
     (dict(output=4104), _capi.BAD_ALIGNMENT), (dict(query_head_stride=68), _capi.BAD_ALIGNMENT), (dict(value_place_stride=66), _capi.BAD_ALIGNMENT),
@@ -184,7 +184,7 @@ def test_attention_workspace():
     assert lib.hfrk_tree_attention_workspace_bytes(ctypes.byref(_attention_args(tokens=0))) == 0
     assert lib.hfrk_tree_attention_workspace_bytes(ctypes.byref(_attention_args(heads=3))) == 0
     # it is bounded by the work that the card can have at once, not by the lengths
-    assert lib.hfrk_tree_attention_workspace_bytes(ctypes.byref(_attention_args(table_columns=1 << 26, head_dim=256, tokens=64))) < 300 << 20
+    assert lib.hfrk_tree_attention_workspace_bytes(ctypes.byref(_attention_args(table_columns=1 << 23, head_dim=256, tokens=64))) < 300 << 20
 
 
 # ---- tracing ------------------------------------------------------------------------------------------------------------
