@@ -1,9 +1,6 @@
 // Attention over a paged cache: checks, the choice of kernel, and the kernel that joins the parts of a row.
 #include "tree_attention_kernel.h"
 
-#ifndef V_W
-#define V_W 2
-#endif
 namespace hfrk {
 
 extern template int launch_attention<64>(const AttentionArgs& p, int col_blocks, int grid, hipStream_t stream);
@@ -145,9 +142,16 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     const int size = a.cache_dtype == HFRK_FP8_E4M3FN ? 1 : 2;
     d.shared = per > 32 && narrow(a.key_page_stride, a.key_place_stride, a.page_size, size) &&
                narrow(a.value_page_stride, a.value_place_stride, a.page_size, size);
+    // A block of rows reads its keys once, so it is as large as the rows fill: 64 sequences x 2731 tokens, 8 key heads, 128 columns, us
+    //     rows a sequence           32 fp8   64   64 fp8   128   256   400
+    //     16 a block, direct           111
+    //     32 a block, direct            84  199      119
+    //     128 a block, shared          138  154      127   164   288   492
+    //     256 a block, shared               217      195   229   262   441
     d.rows = per <= 16 ? 16 : per <= 32 || !d.shared ? 32 : per <= 128 || a.head_dim > 128 ? 128 : 256;
     d.tile = d.shared ? 128 : kWaveTokens * kDirectWaves;
-    d.work = d.rows == 256 || a.head_dim > 128 ? kNumCU : V_W * kNumCU;
+    // (256 rows are eight waves, and heads of more than 128 columns fill the registers: one such workgroup a compute unit)
+    d.work = d.rows == 256 || a.head_dim > 128 ? kNumCU : 2 * kNumCU;
     const int rows = d.rows;
     const long blocks = (long)a.tokens * group / rows + a.seqs;
     const long tiles = ((long)a.table_columns * a.page_size + d.tile - 1) / d.tile;
