@@ -240,6 +240,63 @@ def test_offsets_past_32_bits():
     assert torch.equal(got, tree_attention(**args))
 
 
+@pytest.mark.parametrize("pages_far", [True, False])
+@pytest.mark.parametrize("counts", [[2], [70]])
+def test_wide_strides(pages_far, counts):
+    """Strides of pages that 32 bits just hold in bytes, strides of places that they do not: the kernels of few and of many rows."""
+    step = Step([100], counts, 4, 2, 64, 8 if not pages_far else 16, seed=2)
+    args = step.args()
+    pages = step.key.size(0)
+    far = {}
+    for name in ("key_cache", "value_cache"):
+        if pages_far:
+            strides = (1 << 30, 128, 64, 1)
+            memory = torch.zeros(((pages - 1) << 30) + 16 * 128, dtype=torch.bfloat16, device="cuda")
+        else:
+            strides = (128, 1 << 27, 64, 1)
+            memory = torch.zeros(8 << 27, dtype=torch.bfloat16, device="cuda")
+        far[name] = memory.as_strided(step.key.shape, strides)
+        far[name].copy_(args[name])
+    assert torch.equal(far["key_cache"].nan_to_num(7.0), args["key_cache"].nan_to_num(7.0))
+    got = tree_attention(**{**args, **far})
+    if pages_far or sum(counts) == 2:
+        assert torch.equal(got, tree_attention(**args))  # the same kernel: the same bits
+    step.check(got)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_many_rows_in_graphs_on_two_streams(head_dim, tree):
+    """The kernel of many rows: two captured calls replayed at once, with other lengths, pages and masks than at the capture."""
+    step = Step([2000, 700], [50, 90], 8, 2, head_dim, 16, tree="full" if tree else None, seed=6)
+    args = step.args()
+    tree_attention(**args)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(tree_attention(**args))
+        graphs.append(graph)
+    for i, lengths in enumerate(([2000, 700], [50, 90], [1333, 100])):
+        args["lengths"].copy_(torch.tensor(lengths))
+        if tree and i:
+            args["mask"].copy_(~args["mask"])
+        if i == 2:
+            args["page_table"].copy_(args["page_table"].flip(0))
+            args["lengths"].copy_(torch.tensor([600, 1900]))
+        want = tree_attention(**args)
+        for out in outs:
+            out.fill_(math.nan)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(want).all() and all(torch.equal(out, want) for out in outs)
+
+
 def test_nothing_to_do():
     step = Step([5], [1], 4, 2, 64, 16, uniform=True)
     args = step.args()
