@@ -140,7 +140,15 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     const int group = a.heads / a.kv_heads;
     const long per = (a.tokens + a.seqs - 1) / a.seqs * (long)group;  // rows of a sequence, on average
     const int size = a.cache_dtype == HFRK_FP8_E4M3FN ? 1 : 2;
-    d.shared = per > 32 && narrow(a.key_page_stride, a.key_place_stride, a.page_size, size) &&
+    // With little work a workgroup has a tile or two, and what counts is how soon it has done one: the direct kernel, though its blocks of 32 rows read keys
+    // more often.  From tiles of about 24 a compute unit on (4 where heads of more than 128 columns leave room for one workgroup) sharing pays, us:
+    //     sequences x rows x tokens   4 x 48 x 2000   4 x 108 x 4000   8 x 108 x 2500   1 x 4096 x 1024   16 x 48 x 2731
+    //     tiles a compute unit             8               22               23               33                30 (bf16, 128 columns)
+    //     direct                         23.3             34.3             39.7             47.7              47.1
+    //     shared                         24.4             37.3             38.2             50.5              44.3
+    // (fp8: 20.7 and 25.1, 31.1 and 34.9, 34.9 and 35.8, 40.7 and 51.3.)  The host knows the table's columns, not the lengths.
+    const long few = ((long)a.tokens * group / 32 + a.seqs) * (((long)a.table_columns * a.page_size + 127) / 128) * a.kv_heads;
+    d.shared = per > 32 && few > (a.head_dim > 128 ? 4 : 24) * kNumCU && narrow(a.key_page_stride, a.key_place_stride, a.page_size, size) &&
                narrow(a.value_page_stride, a.value_place_stride, a.page_size, size);
     // A block of rows reads its keys once, so it is as large as the rows fill: 64 sequences x 2731 tokens, 8 key heads, 128 columns, us
     //     rows a sequence           32 fp8   64   64 fp8   128   256   400

@@ -10,19 +10,20 @@ from oracle import attention as oracle
 pytestmark = pytest.mark.gpu
 
 FP8 = torch.float8_e4m3fn
+LONG = 1 << 20  # places in a table's row with which a call counts as much work, whatever the lengths are: many rows take the kernel with LDS
 
 
 class Step:
     """A step's queries and the cache they read, on the CPU: pages in a random order, memory that nobody may read filled with NaN."""
 
     def __init__(self, lengths, counts, heads, kv_heads, head_dim, page, dtype=torch.bfloat16, cache=None, layout="tokens", tree=None, seed=0, extra=0,
-                 uniform=False, loud=1.0):
+                 uniform=False, loud=1.0, places=0):
         g = self.g = torch.Generator().manual_seed(seed)
         cache = cache or dtype
         self.dtype, self.cache, self.lengths, self.counts = dtype, cache, lengths, counts
         seqs, total = len(lengths), sum(counts)
         need = [-(-n // page) for n in lengths]
-        columns = max(max(need), 1) + 1
+        columns = max(max(need) + 1, places // page, 2)
         order = torch.randperm(sum(need) + 3, generator=g).tolist()
         pages = len(order)
         self.table = torch.full((seqs, columns), -1, dtype=torch.int32)
@@ -111,11 +112,12 @@ def test_head_groups_and_pages(heads, kv_heads, page, layout):
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 @pytest.mark.parametrize("counts", [[3, 1, 5], [9, 16, 1, 0, 7], [27, 40], [70, 1, 0, 33]])
 @pytest.mark.parametrize("tree", [False, True])
-def test_chains_and_trees(dtype, cache, head_dim, counts, tree):
-    """Blocks of 16, 32 and 64 rows, the last of a sequence ragged; sequences with no token, masks with empty rows, rows of nobody behind the last."""
+@pytest.mark.parametrize("places", [0, LONG])
+def test_chains_and_trees(dtype, cache, head_dim, counts, tree, places):
+    """Blocks of 16, 32, 128 and 256 rows, the last of a sequence ragged; sequences with no token, masks with empty rows, rows of nobody behind the last."""
     lengths = [n + 37 * (i + 1) for i, n in enumerate(counts)]
     lengths[0] = counts[0]  # nothing in front of the step: rows that see nothing
-    step = Step(lengths, counts, 8, 2, head_dim, 16, dtype, cache, tree="full" if tree else None, seed=sum(counts), extra=2)
+    step = Step(lengths, counts, 8, 2, head_dim, 16, dtype, cache, tree="full" if tree else None, seed=sum(counts), extra=2, places=places)
     if tree:
         step.mask[1] = False
     out = torch.full(step.query.shape, 7.0, dtype=dtype, device="cuda")
@@ -138,9 +140,10 @@ def test_many_sequences(seqs, most):
 
 @pytest.mark.parametrize("dtype,cache", TYPES)
 @pytest.mark.parametrize("counts,length", [([1], 5000), ([20], 3000), ([6, 1], 2500)])
-def test_long_caches_split_between_workgroups(dtype, cache, counts, length):
+@pytest.mark.parametrize("places", [0, LONG])
+def test_long_caches_split_between_workgroups(dtype, cache, counts, length, places):
     lengths = [length - 700 * i for i in range(len(counts))]
-    step = Step(lengths, counts, 4, 1, 128, 32, dtype, cache, seed=length, loud=3.0)
+    step = Step(lengths, counts, 4, 1, 128, 32, dtype, cache, seed=length, loud=3.0, places=places)
     first = tree_attention(**step.args())
     step.check(first)
     again = tree_attention(**step.args())
@@ -148,16 +151,18 @@ def test_long_caches_split_between_workgroups(dtype, cache, counts, length):
 
 
 @pytest.mark.parametrize("dtype,cache", [(torch.bfloat16, None), (torch.float16, FP8)])
-def test_output_in_fp8(dtype, cache):
-    step = Step([300, 20, 0], [2, 5, 1], 8, 2, 128, 16, dtype, cache, seed=4)
+@pytest.mark.parametrize("counts,places", [([2, 5, 1], 0), ([2, 50, 1], LONG)])
+def test_output_in_fp8(dtype, cache, counts, places):
+    step = Step([300, 20 if places == 0 else 60, 0], counts, 8, 2, 128, 16, dtype, cache, seed=4, places=places)
     for s in (0.004, 0.0002):  # the second saturates
         got = tree_attention(**step.args(), out_scale=torch.tensor([s], device="cuda"))
         assert got.dtype == FP8
         step.check(got.float(), out_scale=float(torch.tensor(s)))
 
 
-def test_a_step_longer_than_its_cache_and_pages_that_are_missing():
-    step = Step([3, 90, 60, 50], [6, 2, 2, 4], 4, 2, 64, 16, seed=2)
+@pytest.mark.parametrize("heads,places", [(4, 0), (32, LONG)])
+def test_a_step_longer_than_its_cache_and_pages_that_are_missing(heads, places):
+    step = Step([3, 90, 60, 50], [6, 2, 2, 4], heads, 2, 64, 16, seed=2, places=places)
     step.table[1, 2] = -1          # a hole
     step.table[2, :] = 10 ** 6     # no page of it exists: zeros
     step.table[3, 0] = -2147483648
@@ -170,8 +175,9 @@ def test_a_step_longer_than_its_cache_and_pages_that_are_missing():
 
 
 @pytest.mark.parametrize("width", [0, 2])
-def test_masks_with_fewer_columns_than_the_step(width):
-    step = Step([40, 6], [5, 6], 4, 2, 64, 16, tree=width, seed=6)
+@pytest.mark.parametrize("counts,places", [([5, 6], 0), ([30, 26], LONG)])
+def test_masks_with_fewer_columns_than_the_step(width, counts, places):
+    step = Step([40, counts[1]], counts, 4, 2, 64, 16, tree=width, seed=6, places=places)
     step.check(tree_attention(**step.args()))
     step.mask = (step.mask * 255).to(torch.uint8)  # bytes, any but zero
     step.check(tree_attention(**step.args()))
@@ -180,9 +186,10 @@ def test_masks_with_fewer_columns_than_the_step(width):
 @pytest.mark.parametrize("dtype,cache,what", [(d, None, w) for d in (torch.bfloat16, torch.float16) for w in (math.nan, math.inf, -math.inf)] +
                          [(torch.bfloat16, FP8, math.nan)])  # (e4m3fn has no infinities)
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
-def test_infinities_and_nan_of_drafted_tokens_reach_only_those_who_see_them(dtype, cache, what, head_dim):
+@pytest.mark.parametrize("places", [0, LONG])
+def test_infinities_and_nan_of_drafted_tokens_reach_only_those_who_see_them(dtype, cache, what, head_dim, places):
     for counts in ([5, 1], [20, 3], [40]):
-        step = Step([n + 30 for n in counts], counts, 4, 2, head_dim, 8, dtype, cache, tree="full", seed=9)
+        step = Step([n + 30 for n in counts], counts, 4, 2, head_dim, 8, dtype, cache, tree="full", seed=9, places=places)
         token = step.lengths[0] - counts[0] + 2  # the third drafted token
         page, place = int(step.table[0, token // 8]), token % 8
         if cache == FP8:
@@ -244,7 +251,7 @@ def test_offsets_past_32_bits():
 @pytest.mark.parametrize("counts", [[2], [70]])
 def test_wide_strides(pages_far, counts):
     """Strides of pages that 32 bits just hold in bytes, strides of places that they do not: the kernels of few and of many rows."""
-    step = Step([100], counts, 4, 2, 64, 8 if not pages_far else 16, seed=2)
+    step = Step([100], counts, 4, 2, 64, 8 if not pages_far else 16, seed=2, places=LONG if counts == [70] else 0)
     args = step.args()
     pages = step.key.size(0)
     far = {}
@@ -268,7 +275,7 @@ def test_wide_strides(pages_far, counts):
 @pytest.mark.parametrize("head_dim", [64, 128])
 def test_many_rows_in_graphs_on_two_streams(head_dim, tree):
     """The kernel of many rows: two captured calls replayed at once, with other lengths, pages and masks than at the capture."""
-    step = Step([2000, 700], [50, 90], 8, 2, head_dim, 16, tree="full" if tree else None, seed=6)
+    step = Step([2000, 700], [50, 90], 8, 2, head_dim, 16, tree="full" if tree else None, seed=6, places=LONG)
     args = step.args()
     tree_attention(**args)
     torch.cuda.synchronize()
