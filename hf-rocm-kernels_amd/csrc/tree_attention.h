@@ -158,7 +158,9 @@ __device__ __forceinline__ Part find_part(const AttentionArgs& p, int item) {
             part.from = part.split * even * p.tile;
             part.to = min((part.split + 1) * even, all) * p.tile;
             part.s = {of(s.first), of(s.count), of(s.length), of(s.drafted)};
-            part.any = true;
+            // The workspace has room for every list of starts that do not decrease; with others the sums may wrap, and what has no room is left out.
+            const int slot0 = part.slot - part.split;
+            part.any = part.splits == 1 || (slot0 >= 0 && part.splits <= p.slots - slot0);
             return part;
         }
         items = __builtin_amdgcn_readlane(items_to, kWave - 1);

@@ -84,7 +84,7 @@ def append_kv(
             not written.  Two tokens in one slot leave values of either there
         - positions, frequencies, interleaved, magnitude: as in `rotary`; None: keys are stored as they are
         - query: (tokens, heads, head_dim), rotated into query_output (None: a new tensor; query itself: in place)
-        - key_scale, value_scale: for float8_e4m3fn caches, float32 tensors of one value or one per key head: x / scale is stored,
+        - key_scale, value_scale: for float8_e4m3fn caches, positive float32 tensors of one value or one per key head: x / scale is stored,
             saturating at +-448; None: 1
     Outputs:
         - the rotated queries, None without a query

@@ -398,7 +398,7 @@ int hfrk_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, vo
  *                   strides (elements) between pages, a page's places and heads: tokens-major or heads-major pages
  *   slots           [tokens] int32, or int64 with slots_wide != 0: token t goes to place slot % page_size of page slot / page_size; a slot that is
  *                   negative or past the last page is not written (padding).  Slots that name one place twice leave either's values there
- *   key_scale, value_scale   e4m3fn caches: e4m3fn(clamp(x / scale, +-448)), fp32 scales on the device, one (stride 0) or one a head (1); NULL: 1
+ *   key_scale, value_scale   e4m3fn caches: e4m3fn(clamp(x / scale, +-448)), fp32 scales > 0 on the device, one (stride 0) or one a head (1); NULL: 1
  *   query, query_output      as x and output of hfrk_rotary
  * Nothing may overlap but query and query_output where they are the same. */
 typedef struct hfrk_append_args {
@@ -442,7 +442,8 @@ int hfrk_append_kv(const hfrk_append_args* args, void* stream);
  * Lengths, starts and tables are read on the device: a captured call may be replayed with others.  The number of parts that a sequence's tokens are
  * split into follows from all lengths of the call, and with it the order of the sums; equal calls give equal bits.
  * head_dim at least 16, a multiple of 8 up to 128, of 16 (e4m3fn caches: always) up to 256; page_size a multiple of 8; query, caches and 16-bit output on 16-byte
- * boundaries with strides of whole 16-byte pieces; scale > 0; table_columns * page_size <= 2^27, tokens * heads <= 2^28.
+ * boundaries with strides of whole 16-byte pieces; scale > 0; table_columns * page_size <= 2^27, tokens * heads <= 2^28, and
+ * (tokens * heads / kv_heads / 16 + seqs) * table_columns * page_size / 128 below 2^31.
  * workspace: hfrk_tree_attention_workspace_bytes of it (0: none), 16-byte aligned, any contents, used by one call at a time. */
 typedef struct hfrk_attention_args {
     const void* query;

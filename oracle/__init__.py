@@ -12,6 +12,7 @@ Modules (each function cites the reference lines it follows):
   residual_rms.py `reference_residual_rms`, `precise_residual_rms`
   swiglu.py       `reference_swiglu`
   llama_mlp.py    the four-op chain
+  attention.py    rotary positions, attention over a paged cache, in float64, with the sizes their tolerances are made of
   weight_format.py packed tile layout (pack / unpack / element offset) and e4m3fnuz -> e4m3fn re-encoding
   c/hfrk_oracle.c plain-C restatement (integer-exact GEMM, scalar RMSNorm/SwiGLU) used to pin the above
 
@@ -26,6 +27,7 @@ How each function is pinned (see tests/test_oracle_*.py):
   weight format   fnuz decode table == torch's float8_e4m3fnuz view for all 256 codes and == fn/2 on the same
                   bits; re-encode table == torch's fnuz -> float -> fn casts for all 256 codes; layout: reshape
                   implementation == element-offset formula written from the MFMA operand definition, round trip
+  attention       the same in whole-tensor torch operators, float64 (tests/test_attention_host.py)
   llama MLP       composition of the pinned parts; the reference holds no test or fixture for the chain, so
                   the composition itself (which buffer feeds which op) is "parity unpinned" beyond that
 """

@@ -113,11 +113,15 @@ def test_captured_steps_and_padding():
     still = padded(held)
     table = layer.table.cuda()
     layer.table = table  # (its address is the captured one)
-    layer(hidden, residual.clone(), still)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        layer(hidden, residual.clone(), still)  # eager on the stream of the capture: the projections' workspace
     torch.cuda.synchronize()
     residual_in = residual.clone()
+    torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.cuda.graph(graph, stream=stream):
         out, _ = layer(hidden, residual_in, still)
     up = (torch.randn(2 * 512, HIDDEN, device="cuda") * 4).to(FP8).t()
     down = (torch.randn(HIDDEN, 512, device="cuda") * 4).to(FP8).t()

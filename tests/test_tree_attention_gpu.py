@@ -304,6 +304,18 @@ def test_many_rows_in_graphs_on_two_streams(head_dim, tree):
         assert torch.isfinite(want).all() and all(torch.equal(out, want) for out in outs)
 
 
+def test_starts_that_go_back_write_no_other_rows():
+    """Starts have to rise; others give rows that mean nothing, but no row of no sequence is written and the next call is as it was."""
+    step = Step([600] * 30, [2] * 30, 4, 2, 64, 16, extra=5)
+    args = step.args()
+    want = tree_attention(**args)
+    out = torch.full(step.query.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    back = torch.tensor([0 if i % 2 == 0 else 60 for i in range(31)], dtype=torch.int32, device="cuda")
+    tree_attention(**{**args, "starts": back}, output=out)
+    assert (out[60:] == 7.0).all()
+    assert torch.equal(tree_attention(**args)[:60], want[:60])
+
+
 def test_nothing_to_do():
     step = Step([5], [1], 4, 2, 64, 16, uniform=True)
     args = step.args()
