@@ -53,11 +53,11 @@ def llama_attention_combined_ops(
     kv_heads, head_dim = key_cache.size(2), key_cache.size(3)
     normalized, residual = residual_rms(input=hidden, residual=residual, weight=rms_weight, epsilon=rms_epsilon, scale_tensor=qkv_input_scale)
     qkv = apply_fp8_linear(normalized, qkv_weight, qkv_weight_scale, qkv_input_scale, out_dtype=hidden.dtype)
-    assert qkv.size(1) % head_dim == 0 and qkv.size(1) // head_dim > 2 * kv_heads, \
-        f"Expected qkv_weight to have rows of more than {2 * kv_heads} heads of {head_dim} but got {qkv.size(1)}"
-    query, key, value = qkv.view(tokens, -1, head_dim).split((qkv.size(1) // head_dim - 2 * kv_heads, kv_heads, kv_heads), dim=1)
+    heads = qkv.size(1) // head_dim - 2 * kv_heads
+    assert qkv.size(1) % head_dim == 0 and heads > 0, f"Expected qkv_weight to have rows of more than {2 * kv_heads} heads of {head_dim} but got {qkv.size(1)}"
+    query, key, value = qkv.view(tokens, heads + 2 * kv_heads, head_dim).split((heads, kv_heads, kv_heads), dim=1)
     query = append_kv(key, value, key_cache, value_cache, slots, positions, frequencies, interleaved, magnitude, query=query, key_scale=key_scale,
                       value_scale=value_scale)
     attended = tree_attention(query, key_cache, value_cache, page_table, lengths, starts, mask, scale, key_scale, value_scale, out_scale=o_input_scale)
-    attn_output = apply_fp8_linear(attended.view(tokens, -1), o_weight, o_weight_scale, o_input_scale, out_dtype=hidden.dtype)
+    attn_output = apply_fp8_linear(attended.view(tokens, heads * head_dim), o_weight, o_weight_scale, o_input_scale, out_dtype=hidden.dtype)
     return attn_output, residual

@@ -205,6 +205,22 @@ def test_wrappers_under_fake_tensors():
         assert tree_attention(query, *args, out_scale=empty(1, dtype=torch.float32)).dtype == FP8
 
 
+@pytest.mark.parametrize("tokens", [6, 0, 700])
+def test_the_attention_block_under_fake_tensors(tokens):
+    from hf_rocm_kernels.combined_ops.llama_attention import llama_attention_combined_ops
+    with FakeTensorMode():
+        def empty(*shape, dtype=BF16):
+            return torch.empty(*shape, device="cuda", dtype=dtype)
+        scale = empty(1, dtype=torch.float32)
+        hidden, residual = empty(tokens, 512), empty(tokens, 512)
+        out, residual_out = llama_attention_combined_ops(
+            hidden, residual, empty(512), 1e-5, empty(768, 512, dtype=FP8), empty(768, dtype=torch.float32), scale, empty(512, 512, dtype=FP8), scale,
+            scale, empty(10, 16, 2, 64, dtype=FP8), empty(10, 16, 2, 64, dtype=FP8), empty(tokens, dtype=torch.int32), empty(tokens, dtype=torch.long),
+            empty(32, dtype=torch.float64), empty(2, 5, dtype=torch.int32), empty(2, dtype=torch.int32), empty(3, dtype=torch.int32),
+            empty(tokens, 9, dtype=torch.bool), key_scale=scale, value_scale=scale)
+        assert out.shape == hidden.shape and out.dtype == BF16 and residual_out is residual
+
+
 # ---- frequencies and the Torch forms --------------------------------------------------------------------------------------
 
 def test_frequencies():

@@ -38,7 +38,7 @@ class Layer:
         """The arguments of a step that appends counts[b] tokens to sequence b, which holds held[b]."""
         at = [(b, t) for b in range(2) for t in range(held[b], held[b] + counts[b])]
         return dict(slots=torch.tensor([int(self.table[b, t // PAGE]) * PAGE + t % PAGE for b, t in at], dtype=torch.int32, device="cuda"),
-                    positions=torch.tensor([t for _, t in at], device="cuda"),
+                    positions=torch.tensor([t for _, t in at], dtype=torch.long, device="cuda"),
                     lengths=torch.tensor([h + n for h, n in zip(held, counts)], dtype=torch.int32, device="cuda"),
                     starts=torch.tensor([0, counts[0], sum(counts)], dtype=torch.int32, device="cuda"))
 
@@ -144,6 +144,12 @@ def test_captured_steps_and_padding():
         mlp, _ = llama_mlp_combined_ops(got[:2].clone(), residual_in[:2].clone(), layer.norm, 1e-5, up, s[0], s[1], down, s[2], s[3], fused=True)
         assert torch.isfinite(mlp).all()
         held = [h + 1 for h in held]
+
+
+def test_no_tokens():
+    layer = Layer(FP8)
+    out, _ = layer(*layer.rows(0), layer.step([0, 0], [0, 0]))
+    assert out.shape == (0, HIDDEN)
 
 
 def test_refuses_projections_without_query_heads():

@@ -304,6 +304,36 @@ def test_many_rows_in_graphs_on_two_streams(head_dim, tree):
         assert torch.isfinite(want).all() and all(torch.equal(out, want) for out in outs)
 
 
+def test_a_long_prompt():
+    """Blocks of rows over every length of the triangle, against float64 on the whole scores; two sequences share their first pages."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tokens, heads, head_dim, page, shared = 3000, 4, 128, 32, 1024
+    lengths = [shared + tokens, shared + 700]
+    need = [-(-n // page) for n in lengths]
+    own = torch.randperm(sum(need), generator=g, device="cuda").int()
+    table = torch.full((2, max(need)), -1, dtype=torch.int32, device="cuda")
+    table[0, :need[0]], table[1, :need[1]] = own[:need[0]], own[need[0]:]
+    table[1, :shared // page] = table[0, :shared // page]
+    cache = [torch.randn(sum(need), page, 1, head_dim, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    query = torch.randn(tokens + 700, heads, head_dim, generator=g, device="cuda").to(torch.bfloat16)
+    starts = torch.tensor([0, tokens, tokens + 700], dtype=torch.int32, device="cuda")
+    got = tree_attention(query, *cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), starts)
+    for b, length in enumerate(lengths):
+        first, last = (0, tokens) if b == 0 else (tokens, tokens + 700)
+        k, v = (c[table[b, :need[b]].long(), :, 0].reshape(-1, head_dim)[:length].double() for c in cache)
+        sees = torch.ones(last - first, length, dtype=torch.bool, device="cuda").tril(shared)
+        for h in range(heads):
+            q = query[first:last, h].double()
+            score = (q @ k.T) * head_dim ** -0.5
+            # a score's error as in the oracle
+            off = ((q.abs() @ k.abs().T) * head_dim ** -0.5).masked_fill(~sees, 0).amax(1) * (head_dim + 4) * 2.0 ** -24
+            off = off + (score.abs().masked_fill(~sees, 0).amax(1) * 4 + 4) * 2.0 ** -23
+            p = torch.softmax(score.masked_fill(~sees, -math.inf), 1)
+            found = p @ v, p @ v.abs(), off, v.abs().amax(0).expand(last - first, -1)
+            tol = oracle.attention_tolerance(found, torch.bfloat16, length)
+            assert float(((got[first:last, h].double() - found[0]).abs() / tol).max()) <= 1.0
+
+
 def test_starts_that_go_back_write_no_other_rows():
     """Starts have to rise; others give rows that mean nothing, but no row of no sequence is written and the next call is as it was."""
     step = Step([600] * 30, [2] * 30, 4, 2, 64, 16, extra=5)
