@@ -75,7 +75,8 @@ def tree_attention(
     (decode), a chain of tokens (a prompt's chunk, a linear draft) or a tree of drafted tokens.
     Args:
         - query: a 16-bit (bfloat16 or float16) tensor of shape (tokens, heads, head_dim), heads a multiple of the cache's kv_heads
-        - key_cache, value_cache: as `append_kv` writes them, of the query's dtype or float8_e4m3fn
+        - key_cache, value_cache: as `append_kv` writes them, of the query's dtype or float8_e4m3fn; page_size a multiple of 8, head_dim one from 16 on
+            (of 16 with float8_e4m3fn and above 128) up to 256
         - page_table: (seqs, columns) int32: a sequence's pages in order.  Entries that are no page (-1) hold nothing that is seen
         - lengths: (seqs, ) int32, the cached tokens of each sequence, those of this step included: they are its last ones
         - starts: (seqs + 1, ) int32: sequence b's tokens are rows starts[b] .. starts[b+1] of query; None: the same number each
@@ -83,7 +84,7 @@ def tree_attention(
             has (columns that are missing are not seen); None: a chain, each sees itself and those in front.  Tokens in front of the step are
             seen by all of it
         - scale: the scores' factor, 1/sqrt(head_dim) when None
-        - key_scale, value_scale: the scales of float8_e4m3fn caches, as in `append_kv`
+        - key_scale, value_scale: the positive scales of float8_e4m3fn caches, as in `append_kv`
         - out_scale: one float32: the result is divided by it and converted to float8_e4m3fn, as the projection behind it takes it
         - output: a tensor to write to; None: a new one
     Outputs:
