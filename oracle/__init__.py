@@ -14,6 +14,7 @@ Modules (each function cites the reference lines it follows):
   llama_mlp.py    the four-op chain
   attention.py    rotary positions, attention over a paged cache, in float64, with the sizes their tolerances are made of
   weight_format.py packed tile layout (pack / unpack / element offset) and e4m3fnuz -> e4m3fn re-encoding
+  lane_run.py     the attention and append kernels' own sources run lane by lane on the CPU (lanes/), tensors between pages nothing may touch
   c/hfrk_oracle.c plain-C restatement (integer-exact GEMM, scalar RMSNorm/SwiGLU) used to pin the above
 
 How each function is pinned (see tests/test_oracle_*.py):

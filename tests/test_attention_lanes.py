@@ -1,0 +1,142 @@
+"""The kernels of attention and append from their own sources, lane by lane on the CPU, against float64, with every tensor flush with pages that nothing
+may touch: in front of it in one run, behind it in the other.  No GPU."""
+import random
+
+import pytest
+import torch
+
+from hf_rocm_kernels import rotary_frequencies
+from hf_rocm_kernels.operators.append_kv import reference_append_kv
+from oracle import attention as oracle
+from oracle import lane_run
+from test_tree_attention_gpu import FP8, LONG, TYPES, Step
+
+BOTH_ENDS = (True, False)
+
+
+def attend(step, at_end, **more):
+    call = dict(query=step.query, key_cache=step.key, value_cache=step.value, page_table=step.table, lengths=torch.tensor(step.lengths, dtype=torch.int32),
+                starts=step.starts, mask=step.mask, key_scale=step.key_scale, value_scale=step.value_scale)
+    return lane_run.attention(**{**call, **more}, at_end=at_end)
+
+
+def run(step, out_scale=None):
+    """Both runs: right values, rows of nobody left alone, and the same bits whatever the workspace held."""
+    results = []
+    for at_end in BOTH_ENDS:
+        scale = None if out_scale is None else torch.tensor([out_scale])
+        out = torch.full(step.query.shape, 7.0).to(step.dtype if scale is None else FP8)
+        got = attend(step, at_end, output=out, out_scale=scale, noise=0xff if at_end else 0x3f)
+        step.check(got.float() if out_scale else got, out_scale=None if out_scale is None else float(torch.tensor(out_scale)))
+        assert (got[sum(step.counts):].float() == 7.0).all()
+        results.append(got.contiguous().view(torch.uint8))
+    assert torch.equal(*results)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("head_dim", [16, 80, 128, 256])
+def test_few_rows(dtype, cache, head_dim):
+    run(Step([1, 7, 9, 31, 33, 129, 0, 300], [1] * 8, 8, 2, head_dim, 24, dtype, cache, uniform=True, seed=head_dim))
+    run(Step([41, 70, 3], [3, 12, 0], 6, 3, head_dim, 8, dtype, cache, layout="heads", tree="full", seed=head_dim, extra=1))
+
+
+@pytest.mark.parametrize("dtype,cache,head_dim", [(torch.float16, None, 64), (torch.bfloat16, FP8, 96), (torch.float16, FP8, 256), (torch.bfloat16, None, 144)])
+@pytest.mark.parametrize("counts", [[33, 0, 40], [70, 1]])
+@pytest.mark.parametrize("tree", [None, "full"])
+def test_many_rows(dtype, cache, head_dim, counts, tree):
+    """128 and (70 tokens of four heads, up to 128 columns) 256 rows a block."""
+    lengths = [n + 37 * (i + 1) for i, n in enumerate(counts)]
+    lengths[0] = counts[0]
+    step = Step(lengths, counts, 8, 2, head_dim, 16, dtype, cache, tree=tree, seed=sum(counts), extra=2, places=LONG)
+    if tree:
+        step.mask[1] = False
+    run(step)
+
+
+@pytest.mark.parametrize("heads,kv_heads,counts,places", [(4, 1, [1], 0), (8, 2, [2, 70], 0), (8, 2, [40, 90], LONG), (64, 1, [70], LONG)])
+def test_rows_split_between_workgroups(heads, kv_heads, counts, places):
+    """Parts joined by a workgroup, a wave or a group of lanes a row (4 to 4480 rows)."""
+    run(Step([700 - 100 * i for i in range(len(counts))], counts, heads, kv_heads, 64, 32, torch.float16, seed=3, places=places))
+
+
+@pytest.mark.parametrize("heads,places", [(4, 0), (32, LONG)])
+def test_pages_that_are_missing(heads, places):
+    step = Step([3, 90, 60, 50], [6, 2, 2, 4], heads, 2, 64, 16, seed=2, places=places)
+    step.table[1, 2], step.table[2, :], step.table[3, 0] = -1, 10 ** 6, -2147483648
+    step.lengths[3] = 10 ** 9 if places == 0 else 64
+    run(step)
+
+
+@pytest.mark.parametrize("heads,places", [(4, 0), (32, LONG)])
+def test_starts_that_go_back(heads, places):
+    """Rows that mean nothing, but no access outside."""
+    step = Step([300] * 12, [3] * 12, heads, 2, 64, 16, places=places)
+    step.starts = torch.tensor([0 if i % 2 == 0 else 36 for i in range(13)], dtype=torch.int32)
+    for at_end in BOTH_ENDS:
+        attend(step, at_end)
+
+
+def test_more_sequences_than_lanes_and_fp8_results():
+    g = torch.Generator().manual_seed(3)
+    counts = torch.randint(0, 3, (70,), generator=g).tolist()
+    run(Step([n + 5 * i % 40 for i, n in enumerate(counts)], counts, 4, 2, 64, 16, torch.float16, seed=1))
+    run(Step([200, 20], [2, 5], 8, 2, 128, 16, torch.bfloat16, FP8, seed=4), out_scale=0.004)
+
+
+@pytest.mark.parametrize("seed", range(5))
+def test_drawn(seed):
+    r = random.Random(seed)
+    for _ in range(3):
+        dtype, cache = r.choice(TYPES)
+        kv_heads, group, seqs = r.choice([1, 2, 3]), r.choice([1, 2, 5, 7, 17]), r.choice([1, 2, 5])
+        head_dim = r.choice([16, 48, 64, 112, 144] if cache == FP8 else [16, 24, 40, 72, 104, 144])
+        counts = [r.randint(0, r.choice([1, 2, 9, 20])) for _ in range(seqs)]
+        counts[r.randrange(seqs)] += 1
+        lengths = [max(0, n + r.choice([-2, 0, 30, 200, 400])) for n in counts]
+        step = Step(lengths, counts, kv_heads * group, kv_heads, head_dim, r.choice([8, 24, 40, 1000]), dtype, cache, r.choice(["tokens", "heads"]),
+                    r.choice([None, None, "full", 2, 0]), r.randrange(1000), r.choice([0, 3]), places=r.choice([0, LONG]))
+        if r.random() < 0.4:
+            step.table[r.randrange(seqs), r.randrange(step.table.size(1))] = r.choice([-1, 10 ** 6])
+        run(step)
+
+
+# ---- append -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cache", [None, FP8])
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+@pytest.mark.parametrize("tokens,heads,kv_heads,head_dim,rotated,interleaved", [
+    (1, 8, 2, 128, 128, False), (6, 35, 5, 96, 48, True), (260, 3, 1, 16, 16, False), (5, 4, 4, 80, 0, False), (3, 3, 1, 36, 20, True), (2, 2, 1, 1024, 512, True)])
+def test_append(cache, layout, tokens, heads, kv_heads, head_dim, rotated, interleaved):
+    g = torch.Generator().manual_seed(tokens)
+    dtype, page, pages = torch.float16, 24, 13
+    query, key, value = (torch.randn(tokens, n, head_dim, generator=g).to(dtype) for n in (heads, kv_heads, kv_heads))
+    shape = (pages, page, kv_heads, head_dim) if layout == "tokens" else (pages, kv_heads, page, head_dim)
+    caches = [torch.zeros(shape).to(cache or dtype) for _ in range(2)]
+    if layout == "heads":
+        caches = [c.transpose(1, 2) for c in caches]
+    slots = torch.randperm(pages * page, generator=g)[:tokens]
+    slots[0] = pages * page - 1
+    if tokens > 4:
+        slots[1], slots[3] = -1, pages * page
+    scales = dict(key_scale=torch.rand(kv_heads, generator=g) + 0.01, value_scale=torch.tensor([0.01])) if cache else {}
+    turn = dict(positions=torch.randint(0, 1000, (tokens,), generator=g), frequencies=rotary_frequencies(rotated, device="cpu")[0], interleaved=interleaved) \
+        if rotated else {}
+    want = [c.clone() for c in caches]
+    reference_append_kv(key, value, *want, slots, query=query if rotated else None, **turn, **scales)
+    for at_end in BOTH_ENDS:
+        got = [c.clone() for c in caches]
+        out = torch.zeros_like(query) if rotated else None
+        lane_run.append(key, value, *got, slots, query=query if rotated else None, query_output=out, at_end=at_end, **turn, **scales)
+        for mine, theirs in zip(got, want):  # (what a rounding is off by may round to the neighbouring value)
+            mine, theirs = mine.float(), theirs.float()
+            assert ((mine - theirs).abs() <= theirs.abs() * torch.finfo(cache or dtype).eps + 2.0 ** -9).all() and torch.equal(mine != 0, theirs != 0)
+        if rotated:
+            turned, size = oracle.rotary(query, turn["positions"], turn["frequencies"], interleaved)
+            assert ((out.double() - turned).abs() <= oracle.rotary_tolerance(turned, size, dtype)).all()
+
+
+def test_an_access_outside_is_seen():
+    """The check itself: eight sequences, lengths for four."""
+    step = Step([5] * 8, [1] * 8, 4, 2, 64, 16, uniform=True)
+    with pytest.raises(AssertionError, match="signal 11"):
+        attend(step, True, lengths=torch.full((4,), 5, dtype=torch.int32))
