@@ -21,7 +21,7 @@ struct AttentionArgs {
     int page_shift;
     uint32_t key_page_bytes, key_place_bytes, value_page_bytes, value_place_bytes;  // strides, where 32 bits hold them (`narrow`)
     float* partial;           // [slots * kv_heads][rows][head_dim], divided by nothing
-    float2* partial_ml;       // [slots * kv_heads][rows]: largest score (in log2 units) and sum
+    float2* partial_ml;       // [slots * kv_heads][rows]: the scale that weights were made with (in log2 units) and their sum
     int4* row_info;           // [tokens * group]: first slot, splits, row in its block
 };
 

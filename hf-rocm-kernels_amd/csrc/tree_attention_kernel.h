@@ -3,7 +3,7 @@
 //   o_i = sum_j 2^(c s_ij - m_i) v_j / sum_j 2^(c s_ij - m_i),  s_ij = q_i . k_j,  c = scale * key_scale * log2(e)
 //
 // over the cached tokens j that row i sees, m_i the largest c s_ij so far or less by at most 8 (one pass: when it follows, what has been summed is
-// scaled down).
+// scaled down); in fp16 7 below that, as its weights have to be held above 2^-25.
 // A row is one drafted token and one of the query heads that share a key head, so a group of heads reads its keys and values once.
 //
 // Each wave takes 32 cached tokens at a time and C blocks of 16 rows, from memory to its own registers; keys go through its own part of LDS:
@@ -12,8 +12,9 @@
 //   O^T += V^T P  these eight are, rounded to 16 bits, already the B operand of the second product.  Its A operand is V^T: a lane has loaded
 //                 the same eight tokens' values of DP / 16 neighbouring columns, and turns that block within its own registers
 //   l += 1 P      the sum of the weights, as rounded, by one more product with ones
-// Scores, sums and statistics are fp32.  The weights are rounded to the cache's 16-bit type (half a step of 2^-8 or 2^-11 each, and the same
-// rounded weights make the sum, so that the rounding does not tilt the mean).
+// Scores, sums and statistics are fp32.  The weights are rounded to the query's 16-bit type (half a step of 2^-8 or 2^-11 each, and the same
+// rounded weights make the sum, so that the rounding does not tilt the mean).  In fp16 they lie between 2^7, or more, for a row's largest and 2^15, so that
+// one of 2^-32 of the largest still counts: with 1 to 2^8 a flat tail of 131071 tokens 2^25 below a first one was lost, 0.4 % of the sum.
 //
 // The next tokens' keys are requested before the present scores are made, their values behind the products: a wave has up to 16 KB (128 columns, 16
 // bits) in flight, and bytes bound the kernel.  Values are widened and turned two columns at a time beside the products: held turned, they
@@ -25,7 +26,11 @@
 
 namespace hfrk {
 
-constexpr float kHeadroom = 8.f;    // weights may grow to 2^8 before a row's scale follows
+// A row's scale is set so that its largest weight is 2^lift, and follows when one is 2^8 above that.
+template <int DT>
+constexpr float kLift = DT == HFRK_F16 ? 7.f : 0.f;
+template <int DT>
+constexpr float kHeadroom = 8.f + kLift<DT>;
 constexpr float kNothing = -1e38f;  // the scale of a row that has seen nothing; finite, so that nothing has to be told apart
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
@@ -379,8 +384,8 @@ __global__ void __launch_bounds__(kWave * kDirectWaves, DP <= 128 ? 2 : 1) atten
             for (int j = 1; j < 8; ++j) most = fmaxf(most, score[c][j / 4][j % 4]);
             most *= scale;
             // a row's scale follows its largest score when a lane has found one 2^8 above it, not with every step
-            if (__any(most > top[c] + kHeadroom)) {
-                const float grown = fmaxf(top[c], row_max(most));
+            if (__any(most > top[c] + kHeadroom<DT>)) {
+                const float grown = fmaxf(top[c], row_max(most) - kLift<DT>);
                 const float shrink = __builtin_amdgcn_exp2f(top[c] - grown);
                 top[c] = grown;
                 sum[c] *= shrink;

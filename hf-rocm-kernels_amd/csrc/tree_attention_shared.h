@@ -336,10 +336,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) attention_share
 #pragma unroll
         for (int j = 1; j < 16; ++j) most = fmaxf(most, score[j]);
         if (__any(most > bound)) {
-            const float grown = fmaxf(top, of_both(most * scale, [](float x, float y) { return fmaxf(x, y); }));
+            const float grown = fmaxf(top, of_both(most * scale, [](float x, float y) { return fmaxf(x, y); }) - kLift<DT>);
             const float shrink = __builtin_amdgcn_exp2f(top - grown);
             top = grown;
-            bound = (grown + kHeadroom) / scale;
+            bound = (grown + kHeadroom<DT>) / scale;
             sum *= shrink;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) out[b] *= shrink;

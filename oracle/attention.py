@@ -94,12 +94,12 @@ def attention_tolerance(found, dtype: torch.dtype, length: int, out_dtype: Optio
     """How far a kernel may be that keeps scores and sums in fp32 and rounds the weights to `dtype` and the result to `out_dtype`.
 
     A weight is off by half a step u and by the score's error e (relative), in the sum above the line and in the one below: 2 (u + e) of
-    sum p |v|; sums of `length` terms in fp32 2^-24 each above and below; a weight below fp16's normal values by half its smallest step of the largest
-    weight, which is at most the sum: length * 2^-25 * largest |v| (bf16 reaches as far down as fp32).  Then one rounding."""
+    sum p |v|; sums of `length` terms in fp32 2^-24 each above and below; a weight below fp16's normal values by half its smallest step, 2^-25,
+    where the largest weight, which is at most the sum, is 2^7 or more: length * 2^-32 * largest |v| (bf16 reaches as far down as fp32).  Then one rounding."""
     out, spread, off, most = found
     u = half_step(dtype)
     inner = 2 * (u + off[..., None]) * (1 + u) * spread + 2 * length * 2.0 ** -24 * spread
-    inner = inner + (2 * length * smallest_step(dtype) * most if dtype == torch.float16 else 0.0)
+    inner = inner + (2 * length * smallest_step(dtype) * 2.0 ** -7 * most if dtype == torch.float16 else 0.0)
     if out_dtype is None:
         return inner + (out.abs() + inner) * half_step(dtype) * (1 + 2.0 ** -10) + smallest_step(dtype)
     return inner + (out.abs() + inner) * half_step(out_dtype) * (1 + 2.0 ** -10) + out_scale * smallest_step(out_dtype)

@@ -9,7 +9,7 @@ from hf_rocm_kernels import rotary_frequencies
 from hf_rocm_kernels.operators.append_kv import reference_append_kv
 from oracle import attention as oracle
 from oracle import lane_run
-from test_tree_attention_gpu import FP8, LONG, TYPES, Step
+from test_tree_attention_gpu import FP8, LONG, TYPES, Step, check_small_weights, small_weights
 
 BOTH_ENDS = (True, False)
 
@@ -140,3 +140,13 @@ def test_an_access_outside_is_seen():
     step = Step([5] * 8, [1] * 8, 4, 2, 64, 16, uniform=True)
     with pytest.raises(AssertionError, match="signal 11"):
         attend(step, True, lengths=torch.full((4,), 5, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("far", [21.5, 23.5, 24.6, 25.0, 28.0])
+@pytest.mark.parametrize("tokens,heads,cache", [(1, 2, None), (3, 8, FP8), (40, 8, None)])
+def test_many_small_weights_beside_a_large_one_in_fp16(far, tokens, heads, cache):
+    """A first token with a large score and a value of zero, and a flat tail `far` powers of two below it: the tail is the result."""
+    length, page = 300, 16
+    step = small_weights(far, length, page, tokens, heads, cache or torch.float16, places=LONG if tokens == 40 else 0)
+    got = lane_run.attention(*step[0])
+    check_small_weights(got, *step[1:])

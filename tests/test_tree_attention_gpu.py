@@ -448,3 +448,39 @@ def test_whole_calls_and_general_ones_give_the_same_bits(monkeypatch):
     got = calls()
     monkeypatch.setattr(wrapped, "_tree_attention_new", lambda *args: None)
     assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+
+
+def small_weights(far, length, page, tokens, heads, cache, places=0):
+    """(arguments, head groups' far, first row's place): queries and keys whose scores are in powers of two: `far` for the first token, 0 for the others, the first token's
+    value is 0 and the others' 448.  The step is a chain."""
+    pages = -(-length // page)
+    key, value = torch.zeros(pages, page, 1, 16), torch.full((pages, page, 1, 16), 448.0)
+    key[0, 0, 0, :2] = torch.tensor([far // 8 * 8, far % 8]) if cache != FP8 else torch.tensor([8.0, 8.0])
+    value[0, 0] = 0.0
+    query = torch.zeros(tokens, heads, 16)
+    query[..., :2] = 1.0 if cache != FP8 else far / 16
+    query = query.to(torch.float16)
+    columns = max(pages, places // page)
+    table = torch.zeros(1, columns, dtype=torch.int32)
+    table[0, :pages] = torch.arange(pages)
+    far = (query[0, 0].double() * key[0, 0, 0].to(cache).double()).sum()
+    return (query, key.to(cache), value.to(cache), table, torch.tensor([length], dtype=torch.int32), None, None, math.log(2.0)), far, length - tokens
+
+
+def check_small_weights(got, far, front):
+    """A weight in fp16 is off by half a step of itself and by 2^-25 where the largest is at least 2^7, in the sum above and in the one below the line; the scale ln 2 is a
+    float, as are the score and the exponential (2^-24 of `far` each, and 2^-22): then one rounding."""
+    weight = 2.0 ** -float(far)
+    tail = torch.arange(front, front + got.size(0), dtype=torch.float64)  # tokens behind the first that a row sees
+    want = 448.0 * tail * weight / (1.0 + tail * weight)
+    off = 2 * (2.0 ** -11 + 2.0 ** -32 / weight + 4 * float(far) * 2.0 ** -24 + 2.0 ** -22) + 2 * float(tail.max()) * 2.0 ** -24
+    tolerance = want * (off * (1 + 2.0 ** -8) + 2.0 ** -11) + oracle.smallest_step(torch.float16)
+    assert ((got.cpu().double() - want[:, None, None]).abs() <= tolerance[:, None, None]).all()
+
+
+@pytest.mark.parametrize("far", [21.5, 23.5, 24.6, 25.0, 28.0])
+@pytest.mark.parametrize("tokens,heads,cache", [(1, 2, torch.float16), (3, 8, FP8), (70, 8, torch.float16), (20, 8, FP8)])
+def test_many_small_weights_beside_a_large_one_in_fp16(far, tokens, heads, cache):
+    """Rows far longer than fp16 has steps below the largest weight: a first token with a large score and a value of zero, and a flat tail."""
+    args, far, front = small_weights(far, 131072, 64, tokens, heads, cache)
+    check_small_weights(tree_attention(*[t.cuda() if torch.is_tensor(t) else t for t in args]), far, front)
