@@ -298,3 +298,44 @@ def test_whole_call_operators_take_no_meta_tensor_among_others():
         assert call(*tensors("cpu", "meta", at)) is None
     for at in (1, 2, 3, 4):
         assert append(*tensors("cpu", "meta", at)) == (False, None)
+
+
+YARN = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+
+
+@pytest.mark.parametrize("changes,magnitude", [
+    (dict(mscale=1.0, mscale_all_dim=1.0), 1.0), (dict(mscale=0.707, mscale_all_dim=0.707), 1.0),
+    (dict(mscale=1.0, mscale_all_dim=0.5), (0.1 * math.log(40.0) + 1.0) / (0.05 * math.log(40.0) + 1.0)),
+    (dict(mscale=1.0, mscale_all_dim=0.5, factor=0.5), 1.0), (dict(mscale=1.0, mscale_all_dim=0.5, attention_factor=0.25), 0.25),
+    (dict(mscale=1.0), 0.1 * math.log(40.0) + 1.0), (dict(mscale=None, mscale_all_dim=None, truncate=None), 0.1 * math.log(40.0) + 1.0),
+    (dict(mscale=0.0, mscale_all_dim=0), 0.1 * math.log(40.0) + 1.0)])
+def test_magnitude_of_yarn_entries(changes, magnitude):
+    assert math.isclose(rotary_frequencies(64, scaling={**YARN, **changes}, device="cpu")[1], magnitude, rel_tol=1e-15)
+
+
+def test_a_yarn_ramp_between_whole_pairs():
+    """truncate false: the ramp's ends are not rounded outwards."""
+    plain = rotary_frequencies(64, device="cpu")[0]
+    got = rotary_frequencies(64, scaling={**YARN, "truncate": False, "beta_fast": 16, "beta_slow": 2}, device="cpu")[0]
+    first, last = (64 * math.log(4096 / (n * 2 * math.pi)) / (2 * math.log(10000.0)) for n in (16, 2))
+    for j in range(32):
+        divided = min(max((j - first) / (last - first), 0.0), 1.0)
+        assert math.isclose(float(got[j]), float(plain[j]) * (1 - divided + divided / 40), rel_tol=1e-13)
+    assert not torch.equal(got, rotary_frequencies(64, scaling={**YARN, "beta_fast": 16, "beta_slow": 2}, device="cpu")[0])
+
+
+@pytest.mark.parametrize("scaling,says", [
+    ({**YARN, "mscale": 0.7}, "mscale_all_dim"), ({**YARN, "mscale_all_dim": 1.0}, "mscale_all_dim"), ({**YARN, "long_factor": [1.0]}, "long_factor"),
+    ({"rope_type": "linear", "factor": 2.0, "attention_factor": 1.5}, "attention_factor"), ({"type": "default", "mrope_section": [16, 24, 24]}, "mrope_section"),
+    ({"rope_type": "default", "factor": 4.0}, "factor"), ({**YARN, "rope_theta": 500000.0}, "rope_theta"),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": 1024, "truncate": False}, "truncate")])
+def test_entries_that_are_not_understood_are_refused(scaling, says):
+    with pytest.raises(ValueError, match=says):
+        rotary_frequencies(64, scaling=scaling, device="cpu")
+
+
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "default", "rope_theta": 10000.0}, {"type": "default", "factor": 1.0, "original_max_position_embeddings": 2048, "finetuned": True},
+    {"rope_type": "linear", "factor": 1.0, "attention_factor": None, "partial_rotary_factor": 0.5}])
+def test_entries_with_keys_that_change_nothing(scaling):
+    assert torch.equal(rotary_frequencies(64, scaling=scaling, device="cpu")[0], rotary_frequencies(64, device="cpu")[0])
