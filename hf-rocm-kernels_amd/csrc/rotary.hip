@@ -11,6 +11,7 @@
 // The angle in 32 bits is off by 2^-24 of itself, 0.008 at position 131072: more than bf16's rounding of the result.  Position and frequency are
 // multiplied in double, in turns; what is left of the turn fits a float, and an eighth of a turn either way is a short series.
 #include "hfrk_internal.h"
+#include "overlap.h"
 
 namespace hfrk {
 
@@ -312,6 +313,7 @@ extern "C" int hfrk_append_kv(const hfrk_append_args* args, void* stream) {
         if (!a.key || !a.value || !a.key_cache || !a.value_cache || !a.slots || a.pages < 0 || a.page_size < 1) return HFRK_BAD_SHAPE;
         if (!fp8 && (a.key_scale || a.value_scale)) return HFRK_BAD_DTYPE;
     }
+    if (append_overlap(a)) return HFRK_BAD_SHAPE;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a.dtype == HFRK_F16) return fp8 ? launch_append<HFRK_F16, true>(a, s) : launch_append<HFRK_F16, false>(a, s);
     return fp8 ? launch_append<HFRK_BF16, true>(a, s) : launch_append<HFRK_BF16, false>(a, s);

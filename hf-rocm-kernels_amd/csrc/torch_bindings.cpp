@@ -4,7 +4,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -13,6 +12,7 @@
 #include <cmath>
 
 #include "hfrk_gfx950.h"
+#include "overlap.h"
 
 namespace {
 
@@ -795,21 +795,10 @@ bool heads_16bit(const at::Tensor& t) {
     return t.dim() == 3 && is_16bit(t.scalar_type()) && (t.size(2) <= 1 || t.stride(2) == 1);
 }
 
-bool repeats_itself(const at::Tensor& t) { return t.numel() > 0 && at::has_internal_overlap(t) == at::MemOverlap::Yes; }
-
-// Whether the memory from a tensor's first to its last element meets another's.
-bool meets(const at::Tensor& a, const at::Tensor& b) {
-    if (a.numel() == 0 || b.numel() == 0) return false;
-    auto end = [](const at::Tensor& t) {
-        int64_t last = 0;
-        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-        return static_cast<const uint8_t*>(t.data_ptr()) + (last + 1) * (int64_t)t.element_size();
-    };
-    return static_cast<const uint8_t*>(a.data_ptr()) < end(b) && static_cast<const uint8_t*>(b.data_ptr()) < end(a);
-}
-
-bool same_memory(const at::Tensor& a, const at::Tensor& b) {
-    return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && stride_of(a, 0) == stride_of(b, 0) && stride_of(a, 1) == stride_of(b, 1);
+hfrk::Extent extent(const at::Tensor& t) {  // unit stride along the last of three or four dimensions
+    const int64_t size = t.element_size();
+    auto dim = [&](int64_t i) { return hfrk::Extent::Dim{t.size(i), t.stride(i) * size}; };
+    return t.dim() == 4 ? hfrk::Extent(t.data_ptr(), t.size(3) * size, {dim(0), dim(1), dim(2)}) : hfrk::Extent(t.data_ptr(), t.size(2) * size, {dim(0), dim(1)});
 }
 
 bool is_index(const at::Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
@@ -851,7 +840,6 @@ const char* turned_args(hfrk_append_args& a, const at::Tensor& heads, const at::
     if (!heads_16bit(heads)) return "heads to rotate must be a float16 or bfloat16 [tokens, heads, head_dim] tensor with unit stride along head_dim";
     if (!heads_16bit(output) || output.sizes() != heads.sizes() || output.scalar_type() != heads.scalar_type() || output.device() != heads.device())
         return "the rotated heads' output must have their shape, dtype and device and unit stride along head_dim";
-    if (repeats_itself(output) || (meets(heads, output) && !same_memory(heads, output))) return "the rotated heads' output must be the input itself or lie apart from it";
     if (heads.size(0) >= (int64_t(1) << 31) || heads.size(1) > 65536 || heads.size(2) > 1024 || heads.size(2) < 1) return "at most 65536 heads of 1 to 1024 values";
     a.query = heads.data_ptr();
     a.query_token_stride = stride_of(heads, 0);
@@ -903,17 +891,11 @@ const char* append_args(hfrk_append_args& a, const at::Tensor& key, const at::Te
         if (const char* why = turned_args(a, *query, query_output)) return why;
         if (query->size(0) != tokens || query->size(2) != head_dim || query->scalar_type() != key.scalar_type() || query->device() != key.device())
             return "query must have as many tokens as key, its head_dim, dtype and device";
-        if (!same_memory(*query, query_output) && (meets(query_output, key) || meets(query_output, value))) return "query_output must lie apart from key and value";
     }
     CacheArgs k, v;
     if (const char* why = cache_arg(key_cache, key, kv_heads, head_dim, k)) return why;
     if (const char* why = cache_arg(value_cache, key, kv_heads, head_dim, v)) return why;
     if (const char* why = caches_alike(key_cache, value_cache)) return why;
-    for (const at::Tensor* cache : {&key_cache, &value_cache}) {
-        if (repeats_itself(*cache) || meets(*cache, key) || meets(*cache, value) || (query.has_value() && (meets(*cache, *query) || meets(*cache, query_output))))
-            return "the caches must lie apart from the step's tensors and not overlap themselves";
-    }
-    if (key_cache.numel() > 0 && key_cache.data_ptr() == value_cache.data_ptr()) return "key_cache and value_cache must not be the same memory";
     if (slots.dim() != 1 || slots.size(0) != tokens || !is_index(slots) || !slots.is_contiguous() || slots.device() != key.device())
         return "slots must be a contiguous int32 or int64 tensor with one element per token, on the tensors' device";
     if (const char* why = rotation_args(a, key, tokens, positions, frequencies, magnitude, interleaved)) return why;
@@ -991,7 +973,9 @@ const char* attention_args(hfrk_attention_args& a, const at::Tensor& query, cons
     if (output.dim() != 3 || output.sizes() != query.sizes() || (head_dim > 1 && output.stride(2) != 1) || output.device() != query.device() ||
         output.scalar_type() != (out_scale.has_value() ? at::kFloat8_e4m3fn : query.scalar_type()))
         return "output must have the query's shape, device and dtype (float8_e4m3fn with out_scale) and unit stride along head_dim";
-    if (repeats_itself(output) || meets(output, query) || meets(output, key_cache) || meets(output, value_cache)) return "output must lie apart from the query and the caches";
+    const hfrk::Extent written = extent(output);
+    if (hfrk::repeats(written) || hfrk::meets(written, extent(query)) || hfrk::meets(written, extent(key_cache)) || hfrk::meets(written, extent(value_cache)))
+        return "output must lie apart from the query and the caches and not overlap itself";
     if (tokens >= (int64_t(1) << 31) || heads > 65536 || seqs > (1 << 20) || page_table.size(1) >= (int64_t(1) << 31)) return "too many tokens, heads or sequences";
     a.query = query.data_ptr();
     a.query_token_stride = stride_of(query, 0);
@@ -1024,6 +1008,14 @@ const char* attention_args(hfrk_attention_args& a, const at::Tensor& query, cons
     return nullptr;
 }
 
+// The C entry refuses tensors that share memory; what they are is said here.
+void run_append(const hfrk_append_args& a, const at::Tensor& on, const char* op) {
+    const int status = hfrk_append_kv(&a, current_stream(on));
+    const char* const why = status == HFRK_BAD_SHAPE ? hfrk::append_overlap(a) : nullptr;
+    TORCH_CHECK(!why, why);
+    raise_on(status, op);
+}
+
 // The workspace is the call's own, from torch's allocator: calls on several streams, and captured graphs, do not share it.
 int run_attention(const hfrk_attention_args& a, const at::Tensor& query) {
     const size_t bytes = hfrk_tree_attention_workspace_bytes(&a);
@@ -1037,7 +1029,7 @@ void rotary(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& 
     const char* const why = rotary_args(a, x, positions, frequencies, magnitude, interleaved, output);
     TORCH_CHECK(!why, why);
     DeviceScope scope(x);
-    raise_on(hfrk_append_kv(&a, current_stream(x)), "rotary");
+    run_append(a, x, "rotary");
 }
 
 void append_kv(const at::Tensor& key, const at::Tensor& value, at::Tensor& key_cache, at::Tensor& value_cache, const at::Tensor& slots,
@@ -1050,7 +1042,7 @@ void append_kv(const at::Tensor& key, const at::Tensor& value, at::Tensor& key_c
                                         query_output.has_value() ? *query_output : key, key_scale, value_scale);
     TORCH_CHECK(!why, why);
     DeviceScope scope(key);
-    raise_on(hfrk_append_kv(&a, current_stream(key)), "append_kv");
+    run_append(a, key, "append_kv");
 }
 
 void tree_attention(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& page_table,

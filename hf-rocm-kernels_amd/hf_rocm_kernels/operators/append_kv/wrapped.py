@@ -86,6 +86,8 @@ def append_kv(
         - query: (tokens, heads, head_dim), rotated into query_output (None: a new tensor; query itself: in place)
         - key_scale, value_scale: for float8_e4m3fn caches, positive float32 tensors of one value or one per key head: x / scale is stored,
             saturating at +-448; None: 1
+    The caches and query_output may share memory with nothing else that the call takes (slices of one tensor that lie between each other do not); refused
+    otherwise.
     Outputs:
         - the rotated queries, None without a query
     """

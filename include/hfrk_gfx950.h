@@ -383,7 +383,7 @@ int hfrk_quantize_fp8(const void* input, const float* static_scale, void* output
  *   (x, y) -> magnitude * (x cos - y sin, y cos + x sin);   pairs (j, j + rotated/2), or (2j, 2j+1) where interleaved != 0
  * The values behind them are copied.  The angle is formed in double, so far positions lose nothing.
  *   x, output     16-bit (dtype) [tokens, heads, head_dim], unit stride in a head, strides between tokens and heads in elements; output may be x
- *                 itself and must not overlap it otherwise
+ *                 itself and must not overlap it, or itself, otherwise (HFRK_BAD_SHAPE)
  *   positions     [tokens] int32, or int64 with positions_wide != 0
  *   frequencies   [rotated/2] radians per position, fp32, or fp64 with frequencies_wide != 0
  * head_dim <= 1024.  Heads of whole 16 values on 16-byte boundaries take the vectorised kernel. */
@@ -400,7 +400,8 @@ int hfrk_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, vo
  *                   negative or past the last page is not written (padding).  Slots that name one place twice leave either's values there
  *   key_scale, value_scale   e4m3fn caches: e4m3fn(clamp(x / scale, +-448)), fp32 scales > 0 on the device, one (stride 0) or one a head (1); NULL: 1
  *   query, query_output      as x and output of hfrk_rotary
- * Nothing may overlap but query and query_output where they are the same. */
+ * Nothing that is written (query_output, the caches) may share memory with anything else or repeat itself, but query_output may be query: HFRK_BAD_SHAPE.  Tensors
+ * whose elements lie between each other's (slices of a projection's output, keys and values side by side in a page) share none. */
 typedef struct hfrk_append_args {
     const void* query;
     int64_t query_token_stride, query_head_stride;

@@ -23,7 +23,7 @@ _ROOT = os.path.dirname(_HERE)
 _CSRC = os.path.join(_ROOT, "hf-rocm-kernels_amd", "csrc")
 _LANES = os.path.join(_HERE, "lanes")
 _BUILD = os.path.join(_HERE, "_build")
-_HEADERS = ("hfrk_internal.h", "tree_attention.h", "tree_attention_kernel.h", "tree_attention_shared.h")
+_HEADERS = ("hfrk_internal.h", "overlap.h", "tree_attention.h", "tree_attention_kernel.h", "tree_attention_shared.h")
 _SOURCES = ("rotary.hip", "tree_attention.hip", *(f"tree_attention_{kind}d{n}.hip" for kind in ("", "shared_") for n in (64, 128, 256)))
 _PAGE = mmap.PAGESIZE
 _MARGIN = 16 * _PAGE  # in front of a tensor and behind it
@@ -171,16 +171,12 @@ def attention(query, key_cache, value_cache, page_table, lengths, starts=None, m
     return output
 
 
-def append(key, value, key_cache, value_cache, slots, positions=None, frequencies=None, interleaved=False, magnitude=1.0, query=None, query_output=None,
-           key_scale=None, value_scale=None, at_end=True):
-    """hfrk_append_kv of CPU tensors (key None: hfrk_rotary); writes to the caches and to query_output, which must be tensors of their own."""
-    m = Memory(at_end)
+def _append_args(at, key, value, key_cache, value_cache, slots, positions, frequencies, interleaved, magnitude, query, query_output, key_scale, value_scale):
+    """at: a tensor's address."""
     a = _capi.AppendArgs()
-    written = [(t, m.copy(t)) for t in (key_cache, value_cache, query_output) if t is not None]
-    at = {id(t): p for t, p in written}
     for name, t in (("query", query), ("query_output", query_output), ("key", key), ("value", value), ("key_cache", key_cache), ("value_cache", value_cache),
                     ("slots", slots), ("positions", positions), ("frequencies", frequencies), ("key_scale", key_scale), ("value_scale", value_scale)):
-        setattr(a, name, at[id(t)] if id(t) in at else m.copy(t))
+        setattr(a, name, None if t is None else at(t))
     if query is not None:
         a.query_token_stride, a.query_head_stride = query.stride()[:2]
         a.output_token_stride, a.output_head_stride = query_output.stride()[:2]
@@ -200,9 +196,27 @@ def append(key, value, key_cache, value_cache, slots, positions=None, frequencie
         a.rotated, a.magnitude, a.interleaved = 2 * frequencies.numel(), magnitude, int(interleaved)
     for name, t in (("key_scale_stride", key_scale), ("value_scale_stride", value_scale)):
         setattr(a, name, int(t is not None and t.numel() > 1))
+    return a
+
+
+def append(key, value, key_cache, value_cache, slots, positions=None, frequencies=None, interleaved=False, magnitude=1.0, query=None, query_output=None,
+           key_scale=None, value_scale=None, at_end=True):
+    """hfrk_append_kv of CPU tensors (key None: hfrk_rotary), each in memory of its own; writes to the caches and to query_output."""
+    m = Memory(at_end)
+    written = [(t, m.copy(t)) for t in (key_cache, value_cache, query_output) if t is not None]
+    at = {id(t): p for t, p in written}
+    a = _append_args(lambda t: at[id(t)] if id(t) in at else m.copy(t), key, value, key_cache, value_cache, slots, positions, frequencies, interleaved, magnitude,
+                     query, query_output, key_scale, value_scale)
     lib = _load()
     _run(lambda: lib.hfrk_append_kv(ctypes.byref(a), None))
     for t, p in written:
         storage = t.untyped_storage()
         ctypes.memmove(storage.data_ptr(), p - t.storage_offset() * t.element_size(), storage.nbytes())
     return query_output
+
+
+def append_where_they_are(key, value, key_cache, value_cache, slots, positions=None, frequencies=None, interleaved=False, magnitude=1.0, query=None,
+                          query_output=None, key_scale=None, value_scale=None) -> int:
+    """The same on the tensors' own memory, which they may share; its status."""
+    return _load().hfrk_append_kv(ctypes.byref(_append_args(lambda t: t.data_ptr(), key, value, key_cache, value_cache, slots, positions, frequencies, interleaved,
+                                                            magnitude, query, query_output, key_scale, value_scale)), None)

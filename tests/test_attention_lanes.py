@@ -5,7 +5,7 @@ import random
 import pytest
 import torch
 
-from hf_rocm_kernels import rotary_frequencies
+from hf_rocm_kernels import _capi, rotary_frequencies
 from hf_rocm_kernels.operators.append_kv import reference_append_kv
 from oracle import attention as oracle
 from oracle import lane_run
@@ -150,3 +150,122 @@ def test_many_small_weights_beside_a_large_one_in_fp16(far, tokens, heads, cache
     step = small_weights(far, length, page, tokens, heads, cache or torch.float16, places=LONG if tokens == 40 else 0)
     got = lane_run.attention(*step[0])
     check_small_weights(got, *step[1:])
+
+
+# ---- memory that tensors share --------------------------------------------------------------------------------------------
+
+def shared_step(layout, tokens=3):
+    """(query, key, value, key cache, value cache), views of one projection's output and one cache's memory, in a layout that is in use."""
+    rows = torch.arange(tokens * 8 * 16, dtype=torch.float32).remainder(251).to(torch.float16)
+    if layout == "grouped":          # [tokens, head, (query, key, value)]
+        rows = rows[:tokens * 6 * 16].view(tokens, 2, 3, 16)
+        step = rows[:, :, 0], rows[:, :, 1], rows[:, :, 2]
+    elif layout == "key and value in turn":
+        rows = rows.view(tokens, 8, 16)
+        step = rows[:, :4], rows[:, 4::2], rows[:, 5::2]
+    else:
+        rows = rows.view(tokens, 8, 16)
+        step = rows[:, :4], rows[:, 4:6], rows[:, 6:]
+    memory = torch.zeros(4 * 8 * 2 * 2 * 16, dtype=torch.float16)
+    if layout == "pages in turn":
+        both = memory.view(4, 2, 8, 2, 16)
+        caches = both[:, 0], both[:, 1]
+    elif layout == "heads side by side":
+        both = memory.view(4, 8, 4, 16)
+        caches = both[:, :, :2], both[:, :, 2:]
+    elif layout == "columns side by side":
+        both = memory.view(4, 8, 2, 32)
+        caches = both[..., :16], both[..., 16:]
+    elif layout == "keys by heads, values by tokens":
+        both = memory.view(4, 2, 256)
+        caches = both[:, 0].view(4, 2, 8, 16).transpose(1, 2), both[:, 1].view(4, 8, 2, 16)
+    elif layout == "layers in turn":
+        both = memory.view(2, 4, 8, 2, 16)
+        caches = both[0], both[1]
+    else:
+        caches = memory[:1024].view(4, 8, 2, 16), memory[1024:].view(4, 8, 2, 16)
+    return (*step, *caches)
+
+
+SLOTS, TURN = torch.tensor([5, 31, 8]), dict(positions=torch.tensor([1, 7, 30]), frequencies=torch.tensor([0.5] * 8, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("tokens", [3, 1])
+@pytest.mark.parametrize("layout", ["plain", "grouped", "key and value in turn", "pages in turn", "heads side by side", "columns side by side",
+                                    "keys by heads, values by tokens", "layers in turn"])
+def test_views_of_one_memory_that_lie_between_each_other(layout, tokens):
+    query, key, value, *caches = shared_step(layout, tokens)
+    turn = dict(positions=TURN["positions"][:tokens], frequencies=TURN["frequencies"])
+    want = [c.clone() for c in caches]
+    turned = reference_append_kv(key, value, *want, SLOTS[:tokens], query=query, **turn)
+    assert lane_run.append_where_they_are(key, value, *caches, SLOTS[:tokens], query=query, query_output=query, **turn) == _capi.SUCCESS
+    assert (query.float() - turned.float()).abs().max() <= 0.25 and all((a.float() - b.float()).abs().max() <= 0.25 for a, b in zip(caches, want))
+
+
+def overlapping(case):
+    query, key, value, key_cache, value_cache = shared_step("plain")
+    rows = query.as_strided((3, 8, 16), (128, 16, 1), 0)
+    memory = key_cache.as_strided((2048,), (1,), 0)
+    call = dict(query=query, query_output=query, key=key, value=value, key_cache=key_cache, value_cache=value_cache)
+    if case == "in place over a key head":
+        call.update(query=rows[:, :5], query_output=rows[:, :5])
+    elif case == "in place, the keys themselves":
+        call.update(query=key, query_output=key)
+    elif case == "in place over a value head of another token":
+        call.update(value=rows.as_strided((2, 2, 16), (128, 16, 1), 128), key=key[1:], query=query[:2], query_output=rows.as_strided((2, 4, 16), (128, 16, 1), 64))
+        call.update(query=call["query_output"])
+    elif case == "an output shifted by a head":
+        call.update(query=rows[:, :3], query_output=rows[:, 1:4])
+    elif case == "an output whose heads overlap":
+        call.update(query_output=torch.zeros(400, dtype=torch.float16).as_strided((3, 4, 16), (64, 8, 1)))
+    elif case == "an output whose tokens overlap":
+        call.update(query_output=torch.zeros(400, dtype=torch.float16).as_strided((3, 4, 16), (32, 16, 1)))
+    elif case == "caches a page apart":
+        call.update(key_cache=memory[:1024].view(4, 8, 2, 16), value_cache=memory[256:1280].view(4, 8, 2, 16))
+    elif case == "caches a head apart":
+        call.update(key_cache=memory.view(4, 8, 4, 16)[:, :, :2], value_cache=memory.view(4, 8, 4, 16)[:, :, 1:3])
+    elif case == "caches eight columns apart":
+        call.update(key_cache=memory.view(4, 8, 2, 32)[..., :16], value_cache=memory.view(4, 8, 2, 32)[..., 8:24])
+    elif case == "one cache":
+        call.update(value_cache=key_cache)
+    elif case == "places that overlap":
+        call.update(key_cache=memory.as_strided((4, 8, 2, 16), (256, 16, 16, 1)))
+    elif case == "pages that overlap":
+        call.update(value_cache=memory[1024:].as_strided((4, 8, 2, 16), (128, 32, 16, 1)))
+    elif case == "a cache and the step":
+        call.update(key_cache=rows.as_strided((1, 8, 2, 16), (0, 32, 16, 1), 100))
+        call.update(value_cache=value_cache[:1])
+    return call
+
+
+@pytest.mark.parametrize("case", ["in place over a key head", "in place, the keys themselves", "in place over a value head of another token",
+                                  "an output shifted by a head", "an output whose heads overlap", "an output whose tokens overlap", "caches a page apart",
+                                  "caches a head apart", "caches eight columns apart", "one cache", "places that overlap", "pages that overlap",
+                                  "a cache and the step"])
+def test_memory_that_is_written_and_used_by_others_is_refused(case):
+    call = overlapping(case)
+    n = call["key"].size(0)
+    assert lane_run.append_where_they_are(**call, slots=SLOTS[:n], positions=TURN["positions"][:n], frequencies=TURN["frequencies"]) == _capi.BAD_SHAPE
+
+
+def test_what_meets_by_counting_bytes():
+    """Drawn views of one buffer: refused where two of a launch's threads use a byte that one of them writes, and, the strides lying within each
+    other, nowhere else."""
+    r = random.Random(1)
+    memory = torch.zeros(4096, dtype=torch.float16)
+    refused = 0
+    for _ in range(400):
+        token, head = r.choice([64, 128, 200]), r.choice([16, 32, 48])
+        def view(n):
+            return memory.as_strided((r.choice([1, 2, 3]), n, 16), (token, head, 1), r.randrange(0, 256, 8))
+        query, output = view(r.choice([1, 2])), view(2)
+        output = output[:query.size(0), :query.size(1)]
+        query = query[:output.size(0)]
+        if (output.size(1) - 1) * head + 16 > token:
+            continue
+        used = [{int(x) for x in (torch.arange(4096).as_strided(t.shape, t.stride(), t.storage_offset())).flatten()} for t in (query, output)]
+        apart = not (used[0] & used[1]) or (query.storage_offset() == output.storage_offset())
+        status = lane_run.append_where_they_are(None, None, None, None, None, torch.arange(query.size(0)), TURN["frequencies"], query=query, query_output=output)
+        assert status == (_capi.SUCCESS if apart else _capi.BAD_SHAPE)
+        refused += not apart
+    assert 50 < refused < 350

@@ -237,3 +237,24 @@ def test_refused_on_the_device():
     with pytest.raises(RuntimeError, match="query_output"):
         append_kv(rows[:, 2:4], rows[:, 4:], cache, torch.zeros_like(cache), positions, positions, frequencies, query=rows[:, :2].clone(),
                   query_output=rows[:, 3:5])
+
+
+def test_shared_memory_is_refused_on_the_device():
+    rows = torch.zeros(3, 8, 64, dtype=torch.bfloat16, device="cuda")
+    memory = torch.zeros(4, 8, 4, 64, dtype=torch.bfloat16, device="cuda")
+    turn = dict(positions=torch.zeros(3, dtype=torch.long, device="cuda"), frequencies=torch.ones(32, device="cuda"))
+    slots = torch.arange(3, device="cuda")
+    with pytest.raises(RuntimeError, match="query_output must lie apart"):  # a key's head is turned by one thread and read by another
+        append_kv(rows[:, 4:6], rows[:, 6:], memory[:, :, :2], memory[:, :, 2:], slots, query=rows[:, :5], query_output=rows[:, :5], **turn)
+    with pytest.raises(RuntimeError, match="same memory"):
+        append_kv(rows[:, 4:6], rows[:, 6:], memory[:, :, :2], memory[:, :, 1:3], slots)
+    with pytest.raises(RuntimeError, match="overlap themselves"):
+        append_kv(rows[:, 4:6], rows[:, 6:], memory[:2, :, :2].as_strided((2, 8, 2, 64), (256, 64, 64, 1)), memory[2:, :, :2], slots)
+    with pytest.raises(RuntimeError, match="apart"):
+        rotary(rows, **turn, output=rows.as_strided((3, 8, 64), (512, 32, 1)))
+    # heads in groups of (query, key, value), turned where they are, and caches side by side in a head
+    grouped = torch.randn(3, 2, 3, 64, device="cuda").to(torch.bfloat16)
+    want = rotary(grouped[:, :, 0].contiguous(), **turn)
+    query = grouped[:, :, 0]
+    append_kv(grouped[:, :, 1], grouped[:, :, 2], memory[:, :, :2], memory[:, :, 2:], slots, query=query, query_output=query, **turn)
+    assert torch.equal(query, want) and torch.equal(memory[0, :3, 2:], grouped[:, :, 2])
