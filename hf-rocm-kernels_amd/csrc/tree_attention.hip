@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Atte
     }
     if (!column || (PER > 1 && lane >= WIDTH)) return;
     const bool fp8 = a.cache_dtype == HFRK_FP8_E4M3FN;
-    store_row<DT>(a, token, head * p.group + member, d, o, total, fp8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f,
+    store_row<DT>(a, token, head * p.group + member, d, o, top, total, fp8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f,
                   a.out_scale ? 1.f / a.out_scale[0] : 1.f);
 }
 

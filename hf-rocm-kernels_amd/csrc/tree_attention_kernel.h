@@ -32,6 +32,7 @@ constexpr float kLift = DT == HFRK_F16 ? 7.f : 0.f;
 template <int DT>
 constexpr float kHeadroom = 8.f + kLift<DT>;
 constexpr float kNothing = -1e38f;  // the scale of a row that has seen nothing; finite, so that nothing has to be told apart
+constexpr float kSunk = -0.9e38f;   // of one that has seen scores of minus infinity only: more than nothing, less than all others
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -67,11 +68,12 @@ __device__ __forceinline__ float row_max(float v) {
     return fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
 }
 
-// Eight values of a row of the result: divided by the sum of the weights, times the values' scale; a row that saw nothing is zero.
+// Eight values of a row of the result: divided by the sum of the weights, times the values' scale; a row that saw nothing is zero, one that saw scores of
+// minus infinity only has no sum to divide by and is NaN.
 template <int DT>
-__device__ __forceinline__ void store_row(const hfrk_attention_args& a, long token, int head, int d, const float (&o)[8], float total, float value_scale,
-                                          float inv_out_scale) {
-    const float by = total == 0.f ? 0.f : value_scale / total;
+__device__ __forceinline__ void store_row(const hfrk_attention_args& a, long token, int head, int d, const float (&o)[8], float top, float total,
+                                          float value_scale, float inv_out_scale) {
+    const float by = total != 0.f ? value_scale / total : top > kNothing ? NAN : 0.f;
     const long at = token * a.output_token_stride + head * a.output_head_stride + d;
     if (a.out_scale) {
         uint32_t w[2];
@@ -123,6 +125,19 @@ __device__ __forceinline__ uint32_t sight(const hfrk_attention_args& a, const Se
         for (int j = 0; j < 8; ++j) bits |= min((uint32_t)sees[min(max(at + j, 0), known - 1)], 1u) << j;
     }
     return ((bits & first_of_8(known - at)) | first_of_8(-at)) & here;
+}
+
+// Whether a row sees a cached token that has a page, of the lane's eight from `first` on and those `step` behind them each time, in any part of its sequence (the
+// first that is looked at, mostly).  For rows that have met no finite score, behind the loop: noted in it, it took registers that the loop does not have
+// (16 trees of 64: 347 -> 351 us).
+__device__ __forceinline__ bool sees_some(const AttentionArgs& p, const Sequence& s, const int32_t* table, int first, int step, int seen_to, const uint8_t* sees) {
+    for (const int end = p.a.mask ? s.length : min(s.length, seen_to + 1); first < end; first += step) {
+        if (sight(p.a, s, first, true, seen_to, sees) == 0) continue;
+        const uint32_t eights = (uint32_t)first >> 3;
+        const int at = (int)(p.page_magic ? __umulhi(eights, p.page_magic) >> p.page_shift : eights >> p.page_shift);
+        if (at < p.a.table_columns && (uint32_t)table[at] < (uint32_t)p.a.pages) return true;
+    }
+    return false;
 }
 
 // Values without infinities and NaN.
@@ -466,6 +481,11 @@ __global__ void __launch_bounds__(kWave * kDirectWaves, DP <= 128 ? 2 : 1) atten
     }
 
     marks.apply(out);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const bool lost = top[c] == kNothing;
+        if (__any(lost)) top[c] = fmaxf(top[c], row_max(lost && sees_some(p, s, table, token8, kWaveTokens, seen_to[c], sees[c]) ? kSunk : kNothing));
+    }
 
     // The waves' parts of a row: scaled to the largest of their largest scores and added, 16 rows at a time.
     const float value_scale = FP8 && a.value_scale ? a.value_scale[head * a.value_scale_stride] : 1.f;
@@ -507,7 +527,7 @@ __global__ void __launch_bounds__(kWave * kDirectWaves, DP <= 128 ? 2 : 1) atten
                 if (d == 0) p.partial_ml[at] = make_float2(most, total);
             } else {
                 const int token = row / p.group, member = row - token * p.group;
-                store_row<DT>(a, s.first + token, head * p.group + member, d, o, total, value_scale, inv_out_scale);
+                store_row<DT>(a, s.first + token, head * p.group + member, d, o, most, total, value_scale, inv_out_scale);
             }
         }
     }

@@ -385,6 +385,18 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) attention_share
     }
     sum = of_both(sum, [](float x, float y) { return x + y; });
     marks.apply(out);
+    const bool lost = top == kNothing;
+    if (__any(lost)) {
+        bool some;
+        if constexpr (DP <= 64) {
+            some = lost && sees_some(p, s, table, 8 * h, 16, seen_to, sees);
+        } else {  // looked up again: held through the loop, the sequence took a register more of each lane (16 trees of 64: 344 -> 347 us; with heads of 64 there is room)
+            const Sequence again = sequence(p, part.b);
+            some = lost && real && sees_some(p, again, a.page_table + (long)part.b * a.table_stride, 8 * h, 16, again.drafted + row_token,
+                                             static_cast<const uint8_t*>(a.mask) + (long)(again.first + row_token) * a.mask_stride);
+        }
+        top = fmaxf(top, of_both(some ? kSunk : kNothing, [](float x, float y) { return fmaxf(x, y); }));
+    }
 
     // a lane has two runs of DP / 4 neighbouring columns of its row
     if (!real) return;
@@ -409,7 +421,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) attention_share
                 *reinterpret_cast<v4f*>(to) = v4f{o[0], o[1], o[2], o[3]};
                 *reinterpret_cast<v4f*>(to + 4) = v4f{o[4], o[5], o[6], o[7]};
             } else {
-                store_row<DT>(a, s.first + row_token, head * p.group + member, d, o, sum, value_scale, inv_out_scale);
+                store_row<DT>(a, s.first + row_token, head * p.group + member, d, o, top, sum, value_scale, inv_out_scale);
             }
         }
 }

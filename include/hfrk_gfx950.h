@@ -431,7 +431,8 @@ int hfrk_append_kv(const hfrk_append_args* args, void* stream);
 /* Attention of a step's queries over a paged cache that holds the step's own keys and values too.
  *   Sequence b has lengths[b] cached tokens; the last of them are its step's: rows starts[b] .. starts[b+1] of query.  Row i of a sequence (0 the first)
  *   sees every token in front of the step's, and of the step's the j <= i (mask NULL: one token, or a chain), or the j with mask[row][j] != 0 (a tree).
- *   output[row, head] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * key_scale * (q . k_j));  zero where a row sees nothing
+ *   output[row, head] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * key_scale * (q . k_j));  zero where a row sees nothing, NaN where all that it sees
+ *   has a score of minus infinity (0 / 0)
  *   query         16-bit (dtype) [tokens, heads, head_dim]; heads a multiple of kv_heads, query heads h * heads/kv_heads ... share key head h
  *   output        [tokens, heads, head_dim] of dtype, or e4m3fn(clamp(result / out_scale[0], +-448)) where out_scale is not NULL.  Rows of no
  *                 sequence are left as they are

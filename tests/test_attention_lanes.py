@@ -9,7 +9,7 @@ from hf_rocm_kernels import _capi, rotary_frequencies
 from hf_rocm_kernels.operators.append_kv import reference_append_kv
 from oracle import attention as oracle
 from oracle import lane_run
-from test_tree_attention_gpu import FP8, LONG, TYPES, Step, check_small_weights, small_weights
+from test_tree_attention_gpu import FP8, LONG, TYPES, Step, check_small_weights, minus_infinities, small_weights
 
 BOTH_ENDS = (True, False)
 
@@ -98,6 +98,13 @@ def test_drawn(seed):
         if r.random() < 0.4:
             step.table[r.randrange(seqs), r.randrange(step.table.size(1))] = r.choice([-1, 10 ** 6])
         run(step)
+
+
+@pytest.mark.parametrize("counts,front,heads,head_dim,places", [([1, 1], 40, 4, 64, 0), ([3, 2], 0, 4, 16, 0), ([5, 9], 300, 8, 64, 0), ([40, 36], 0, 8, 64, LONG),
+                                                                ([40, 70], 100, 8, 64, LONG)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_scores_of_minus_infinity(counts, front, heads, head_dim, places, tree):
+    run(minus_infinities(torch.float16 if tree else torch.bfloat16, counts, front, heads, head_dim, tree, places))
 
 
 # ---- append -------------------------------------------------------------------------------------------------------------

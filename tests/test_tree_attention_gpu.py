@@ -484,3 +484,25 @@ def test_many_small_weights_beside_a_large_one_in_fp16(far, tokens, heads, cache
     """Rows far longer than fp16 has steps below the largest weight: a first token with a large score and a value of zero, and a flat tail."""
     args, far, front = small_weights(far, 131072, 64, tokens, heads, cache)
     check_small_weights(tree_attention(*[t.cuda() if torch.is_tensor(t) else t for t in args]), far, front)
+
+
+def minus_infinities(dtype, counts, front, heads, head_dim, tree, places):
+    """The first sequence's keys are minus infinity, its queries positive: rows of it that see something have no softmax, and rows that see nothing are zero.  The
+    second's are so up to its step, which counts for nothing beside a finite score."""
+    step = Step([n + front for n in counts], counts, heads, 2, head_dim, 16, dtype, tree="full" if tree else None, seed=7, places=places)
+    step.query = step.query.abs() + 0.25
+    for b, end in ((0, step.lengths[0]), (1, front)):
+        for t in range(end):
+            step.key[int(step.table[b, t // 16]), t % 16] = -math.inf
+    if tree:
+        step.mask[1] = False
+    return step
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts,front,heads,head_dim,places", [([1, 1], 40, 4, 64, 0), ([3, 2], 0, 4, 128, 0), ([5, 9], 700, 8, 256, 0), ([40, 36], 0, 8, 64, LONG),
+                                                                ([40, 70], 300, 8, 128, LONG), ([33, 40], 20, 4, 256, LONG)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_scores_of_minus_infinity(dtype, counts, front, heads, head_dim, places, tree):
+    step = minus_infinities(dtype, counts, front, heads, head_dim, tree, places)
+    step.check(tree_attention(**step.args()))
