@@ -167,7 +167,10 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     // most twice as many.
     d.shares = a.seqs > 1 ? 2 : 1;
     const long most = (long)d.shares * (d.work / a.kv_heads > 1 ? d.work / a.kv_heads : 1), items = most + blocks < blocks * tiles ? most + blocks : blocks * (tiles > 0 ? tiles : 1);
-    d.fits = blocks * tiles < (1L << 31) && items * a.kv_heads < (1L << 31);
+    // Every workgroup makes the list of work from all sequences: 0.25, 3.1 and 50 ms for 1024, 4096 and 16384 sequences of 16 tokens, 8 key heads, where the last
+    // is 2^31 workgroups times sequences.  (1024 sequences of 1000 to 2000 tokens, 1.23 ms, are at the rate of their bytes.)  At 2^36 a call would take
+    // 1.6 s; it is refused from there on, as it would soon look as if it hung.
+    d.fits = blocks * tiles < (1L << 31) && items * a.kv_heads < (1L << 31) && items * a.kv_heads * a.seqs <= (1L << 36);
     d.grid = (int)(items * a.kv_heads);
     if (tiles > 1) {
         d.slots = (int)(2 * most < blocks * tiles ? 2 * most : blocks * tiles);

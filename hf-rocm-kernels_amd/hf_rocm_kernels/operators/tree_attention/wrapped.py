@@ -90,6 +90,7 @@ def tree_attention(
     Outputs:
         - (tokens, heads, head_dim) of the query's dtype, or float8_e4m3fn with out_scale.  A token that sees nothing gets zeros; rows behind
           the last sequence's are not written
+    A batch of some thousand short sequences is slow, as every workgroup looks at all of them; one of 65536 with more than about 15 kv_heads is refused.
     Lengths, starts and page_table stay on the device: no call waits for them, and a captured call may be replayed with others.  The result does not depend
     on other streams' calls (each has a workspace of its own), but how a sequence's tokens are split, and with it the last bits, depends on all lengths.
     """

@@ -445,7 +445,8 @@ int hfrk_append_kv(const hfrk_append_args* args, void* stream);
  * split into follows from all lengths of the call, and with it the order of the sums; equal calls give equal bits.
  * head_dim at least 16, a multiple of 8 up to 128, of 16 (e4m3fn caches: always) up to 256; page_size a multiple of 8; query, caches and 16-bit output on 16-byte
  * boundaries with strides of whole 16-byte pieces; scale > 0; table_columns * page_size <= 2^27, tokens * heads <= 2^28, and
- * (tokens * heads / kv_heads / 16 + seqs) * table_columns * page_size / 128 below 2^31.
+ * (tokens * heads / kv_heads / 16 + seqs) * table_columns * page_size / 128 below 2^31.  Every workgroup looks at every sequence: a batch of some thousand short
+ * ones is slow (4096 of 16 tokens 3 ms), and workgroups times seqs above 2^36 (about 65536 sequences of a token with 15 key heads) are refused: HFRK_BAD_SHAPE.
  * workspace: hfrk_tree_attention_workspace_bytes of it (0: none), 16-byte aligned, any contents, used by one call at a time. */
 typedef struct hfrk_attention_args {
     const void* query;

@@ -339,3 +339,12 @@ def test_entries_that_are_not_understood_are_refused(scaling, says):
     {"rope_type": "linear", "factor": 1.0, "attention_factor": None, "partial_rotary_factor": 0.5}])
 def test_entries_with_keys_that_change_nothing(scaling):
     assert torch.equal(rotary_frequencies(64, scaling=scaling, device="cpu")[0], rotary_frequencies(64, device="cpu")[0])
+
+
+@pytest.mark.parametrize("tokens,seqs,kv_heads,status", [
+    (1 << 16, 1 << 16, 8, _capi.BAD_ALIGNMENT), (1 << 18, 1 << 18, 2, _capi.BAD_SHAPE), (1 << 17, 1 << 17, 8, _capi.BAD_SHAPE),
+    (1 << 20, 1 << 20, 1, _capi.BAD_SHAPE), (1 << 15, 1 << 14, 64, _capi.BAD_ALIGNMENT), (1 << 16, 1 << 16, 64, _capi.BAD_SHAPE)])
+def test_batches_whose_list_of_work_would_take_seconds_are_refused(tokens, seqs, kv_heads, status):
+    """Every workgroup makes the list: workgroups times sequences are bounded.  (Those that are taken lack a workspace here.)"""
+    a = _attention_args(tokens=tokens, seqs=seqs, heads=kv_heads, kv_heads=kv_heads)
+    assert _capi.load().hfrk_tree_attention(ctypes.byref(a), None, 0, None) == status
