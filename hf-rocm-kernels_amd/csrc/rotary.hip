@@ -275,8 +275,33 @@ static bool pieces_of_16(const hfrk_append_args& a, bool fp8) {
     return a.head_dim % 16 == 0 && a.rotated % 16 == 0 && (addresses & 15) == 0 && (strides & 7) == 0;
 }
 
+// The same from token `first` on.
+static hfrk_append_args behind(hfrk_append_args a, int first, int tokens) {
+    auto ahead = [](const void* p, int64_t bytes) { return p ? static_cast<const uint8_t*>(p) + bytes : nullptr; };
+    a.query = ahead(a.query, 2 * first * a.query_token_stride);
+    a.query_output = const_cast<uint8_t*>(ahead(a.query_output, 2 * first * a.output_token_stride));
+    a.key = ahead(a.key, 2 * first * a.key_token_stride);
+    a.value = ahead(a.value, 2 * first * a.value_token_stride);
+    a.slots = ahead(a.slots, (a.slots_wide ? 8L : 4L) * first);
+    a.positions = ahead(a.positions, (a.positions_wide ? 8L : 4L) * first);
+    a.tokens = tokens;
+    return a;
+}
+
+// A launch's threads are counted in 32 bits, and one of 2^24 + n workgroups of 256 runs n of them, without an error.
+constexpr int kTokensOfALaunch = 1 << 23;
+
 template <int DT, bool FP8>
 static int launch_append(const hfrk_append_args& a, hipStream_t stream) {
+    if (a.tokens > kTokensOfALaunch) {
+        for (int first = 0; first < a.tokens;) {
+            const int tokens = a.tokens - first < kTokensOfALaunch ? a.tokens - first : kTokensOfALaunch;
+            const int status = launch_append<DT, FP8>(behind(a, first, tokens), stream);
+            if (status != HFRK_SUCCESS) return status;
+            first += tokens;
+        }
+        return HFRK_SUCCESS;
+    }
     const size_t lds = (size_t)a.rotated * sizeof(float);
     const int heads = a.heads + 2 * a.kv_heads;
     if (pieces_of_16(a, FP8)) {

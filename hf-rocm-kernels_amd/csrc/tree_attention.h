@@ -23,6 +23,7 @@ struct AttentionArgs {
     float* partial;           // [slots * kv_heads][rows][head_dim], divided by nothing
     float2* partial_ml;       // [slots * kv_heads][rows]: the scale that weights were made with (in log2 units) and their sum
     int4* row_info;           // [tokens * group]: first slot, splits, row in its block
+    long join_first;          // the first (row, key head) of a join's launch
 };
 
 // A sequence's drafted tokens (rows first .. first + count of the query), its cached ones (these included) as far as its row of the page table

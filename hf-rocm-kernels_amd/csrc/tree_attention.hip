@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Atte
     __shared__ float parked[PER == kGroups ? kJoinThreads / kWave : 1][WIDTH][10];
     const hfrk_attention_args& a = p.a;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, group = threadIdx.x / WIDTH;
-    const long index = (long)blockIdx.x * (kGroups / PER) + group / PER;
+    const long index = p.join_first + (long)blockIdx.x * (kGroups / PER) + group / PER;
     const long row = index / a.kv_heads;
     const int head = (int)(index - row * a.kv_heads);
     if (row >= (long)a.tokens * p.group) return;
@@ -85,12 +85,18 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Atte
 }
 
 template <int DT, int WIDTH>
-static int launch_join(const AttentionArgs& p, hipStream_t stream) {
+static int launch_join(AttentionArgs p, hipStream_t stream) {
     constexpr int kGroups = kJoinThreads / WIDTH;
     const long rows = (long)p.a.tokens * p.a.heads;
     // A wave a row from one wave per compute unit's SIMD on, a group a row from four waves on: below, more lanes a row find room beside each other.
     const int per = rows < 4 * kNumCU ? kGroups : rows < 16 * kNumCU ? kWave / WIDTH : 1;
-    const dim3 grid((unsigned)((rows * per + kGroups - 1) / kGroups)), threads(kJoinThreads);
+    const dim3 threads(kJoinThreads);
+    const long most = (1L << 23) * kGroups / per;  // of a launch, whose threads are counted in 32 bits
+    for (; rows - p.join_first > most; p.join_first += most) {  // (so many rows have a group each)
+        hipLaunchKernelGGL((attention_join_kernel<DT, WIDTH, 1>), dim3(1 << 23), threads, 0, stream, p);
+        HFRK_HIP_TRY(hipGetLastError());
+    }
+    const dim3 grid((unsigned)(((rows - p.join_first) * per + kGroups - 1) / kGroups));
     if (per == kGroups) hipLaunchKernelGGL((attention_join_kernel<DT, WIDTH, kGroups>), grid, threads, 0, stream, p);
     else if (per > 1) hipLaunchKernelGGL((attention_join_kernel<DT, WIDTH, kWave / WIDTH>), grid, threads, 0, stream, p);
     else hipLaunchKernelGGL((attention_join_kernel<DT, WIDTH, 1>), grid, threads, 0, stream, p);
@@ -170,7 +176,8 @@ static Decomposition decompose(const hfrk_attention_args& a) {
     // Every workgroup makes the list of work from all sequences: 0.25, 3.1 and 50 ms for 1024, 4096 and 16384 sequences of 16 tokens, 8 key heads, where the last
     // is 2^31 workgroups times sequences.  (1024 sequences of 1000 to 2000 tokens, 1.23 ms, are at the rate of their bytes.)  At 2^36 a call would take
     // 1.6 s; it is refused from there on, as it would soon look as if it hung.
-    d.fits = blocks * tiles < (1L << 31) && items * a.kv_heads < (1L << 31) && items * a.kv_heads * a.seqs <= (1L << 36);
+    // (A launch's threads are counted in 32 bits; more run as the rest, without an error.)
+    d.fits = blocks * tiles < (1L << 31) && items * a.kv_heads * (rows == 256 ? 512 : 256) < (1L << 32) && items * a.kv_heads * a.seqs <= (1L << 36);
     d.grid = (int)(items * a.kv_heads);
     if (tiles > 1) {
         d.slots = (int)(2 * most < blocks * tiles ? 2 * most : blocks * tiles);

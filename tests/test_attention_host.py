@@ -348,3 +348,10 @@ def test_batches_whose_list_of_work_would_take_seconds_are_refused(tokens, seqs,
     """Every workgroup makes the list: workgroups times sequences are bounded.  (Those that are taken lack a workspace here.)"""
     a = _attention_args(tokens=tokens, seqs=seqs, heads=kv_heads, kv_heads=kv_heads)
     assert _capi.load().hfrk_tree_attention(ctypes.byref(a), None, 0, None) == status
+
+
+@pytest.mark.parametrize("seqs,kv_heads,status", [(1024, 8192, _capi.BAD_ALIGNMENT), (2048, 8192, _capi.BAD_SHAPE)])
+def test_launches_of_more_threads_than_32_bits_count_are_refused(seqs, kv_heads, status):
+    """A launch of 2^24 + n workgroups of 256 threads runs n of them, without an error."""
+    a = _attention_args(tokens=seqs, seqs=seqs, heads=kv_heads, kv_heads=kv_heads)
+    assert _capi.load().hfrk_tree_attention(ctypes.byref(a), None, 0, None) == status

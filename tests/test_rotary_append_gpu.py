@@ -258,3 +258,21 @@ def test_shared_memory_is_refused_on_the_device():
     query = grouped[:, :, 0]
     append_kv(grouped[:, :, 1], grouped[:, :, 2], memory[:, :, :2], memory[:, :, 2:], slots, query=query, query_output=query, **turn)
     assert torch.equal(query, want) and torch.equal(memory[0, :3, 2:], grouped[:, :, 2])
+
+
+def test_more_tokens_than_a_launch_has_workgroups():
+    """2^24 workgroups of 256 threads are more than 32 bits count."""
+    tokens = (1 << 24) + 5
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows = torch.randn(tokens, 3, 2, generator=g, device="cuda").to(torch.float16)
+    positions = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    frequencies = torch.tensor([0.37], dtype=torch.float64, device="cuda")
+    memory = torch.zeros(2, 1 << 20, 17, 1, 2, dtype=torch.float16, device="cuda")
+    got = append_kv(rows[:, 1:2], rows[:, 2:], memory[0], memory[1], positions, positions, frequencies, query=rows[:, :1])
+    some = torch.cat((torch.arange(3), (1 << 23) + torch.arange(-3, 3), (1 << 24) + torch.arange(-3, 5)))
+    x = rows[some.cuda()].cpu()
+    want, size = oracle.rotary(x[:, :2], some, frequencies.cpu(), False)
+    mine = torch.cat((got[some.cuda()].cpu(), memory[0].view(-1, 1, 2)[some.cuda()].cpu()), dim=1)
+    assert ((mine.double() - want).abs() <= oracle.rotary_tolerance(want, size, torch.float16)).all()
+    assert torch.equal(memory[1].view(-1, 1, 2)[:tokens], rows[:, 2:]) and not memory[:, -1].any()
+    assert torch.equal(rotary(rows[:, :1], positions, frequencies), got)

@@ -506,3 +506,23 @@ def minus_infinities(dtype, counts, front, heads, head_dim, tree, places):
 def test_scores_of_minus_infinity(dtype, counts, front, heads, head_dim, places, tree):
     step = minus_infinities(dtype, counts, front, heads, head_dim, tree, places)
     step.check(tree_attention(**step.args()))
+
+
+def test_more_rows_than_a_launch_has_threads():
+    """A last row of 2^27, whose parts are joined: more groups of 32 lanes than 32 bits count threads."""
+    tokens, heads, head_dim, page, long = (1 << 21) + 1, 64, 144, 4096, 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(2)
+    key, value = (torch.randn(1, page, heads, head_dim, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    query = torch.randn(1, heads, head_dim, generator=g, device="cuda").to(torch.bfloat16)
+    table = torch.zeros(2, long // page, dtype=torch.int32, device="cuda")  # one page, over and over
+    starts = torch.tensor([0, tokens - 1, tokens], dtype=torch.int32, device="cuda")
+    out = torch.full((tokens, heads, head_dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    tree_attention(query.expand(tokens, heads, head_dim), key, value, table, torch.tensor([8, long], dtype=torch.int32, device="cuda"), starts, output=out)
+    # the page's weights 1024 times over; products of 16 tokens are added one after the other, 2^18 of them at most
+    q, k, v = query[0].cpu().double(), key[0].cpu().double().transpose(0, 1), value[0].cpu().double().transpose(0, 1)
+    score = torch.matmul(k, q[:, :, None])[..., 0] * head_dim ** -0.5
+    off = torch.matmul(k.abs(), q.abs()[:, :, None])[..., 0].amax(1) * head_dim ** -0.5 * (head_dim + 4) * 2.0 ** -24 + (score.abs().amax(1) * 4 + 4) * 2.0 ** -23
+    p = torch.softmax(score, 1)[:, None]
+    found = torch.matmul(p, v)[:, 0], torch.matmul(p, v.abs())[:, 0], off, v.abs().amax(1)
+    assert ((out[-1].cpu().double() - found[0]).abs() <= oracle.attention_tolerance(found, torch.bfloat16, long // 16)).all()
+    assert not out[:tokens - 9].any()  # rows that see nothing
