@@ -78,6 +78,17 @@ __device__ __forceinline__ uint8_t cvt_fp8(float a) {
     return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(a, a, 0u, false) & 0xffu);
 }
 
+// The same with NaN kept (0x7f or 0xff), for caches and what is read from them: a NaN that turned into a number there would be a fault that nobody sees.
+__device__ __forceinline__ float clamp_fp8_or_nan(float a) { return fabsf(a) > 448.0f ? copysignf(448.0f, a) : a; }
+
+__device__ __forceinline__ uint32_t cvt_pk_fp8_or_nan(float a, float b, uint32_t old, bool high) {
+    a = clamp_fp8_or_nan(a);
+    b = clamp_fp8_or_nan(b);
+    return high ? __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, true) : __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, false);
+}
+
+__device__ __forceinline__ uint8_t cvt_fp8_or_nan(float a) { return (uint8_t)(cvt_pk_fp8_or_nan(a, a, 0u, false) & 0xffu); }
+
 // silu(g) * u * inv_scale in fp32, sigmoid as 1 / (1 + 2^(-g log2 e)) (the reference's form, swiglu_vectorized.cu:27-97)
 __device__ __forceinline__ float silu_mul(float g, float u, float inv_scale) {
     const float e = __builtin_amdgcn_exp2f(-g * 1.44269504089f);

@@ -78,8 +78,8 @@ __device__ __forceinline__ uint2 pack8_fp8(const float (&x)[8], float inv_scale)
     uint32_t w[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        w[j] = cvt_pk_fp8(x[4 * j] * inv_scale, x[4 * j + 1] * inv_scale, 0u, false);
-        w[j] = cvt_pk_fp8(x[4 * j + 2] * inv_scale, x[4 * j + 3] * inv_scale, w[j], true);
+        w[j] = cvt_pk_fp8_or_nan(x[4 * j] * inv_scale, x[4 * j + 1] * inv_scale, 0u, false);
+        w[j] = cvt_pk_fp8_or_nan(x[4 * j + 2] * inv_scale, x[4 * j + 3] * inv_scale, w[j], true);
     }
     return make_uint2(w[0], w[1]);
 }
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kRotaryThreads) append_scalar_kernel(const hfr
     __syncthreads();
 
     auto put = [&](void* to, int at, float x, float inv_scale, bool fp8) {
-        if (FP8 && fp8) static_cast<uint8_t*>(to)[at] = cvt_fp8(x * inv_scale);
+        if (FP8 && fp8) static_cast<uint8_t*>(to)[at] = cvt_fp8_or_nan(x * inv_scale);
         else static_cast<uint16_t*>(to)[at] = store16<DT>(x);
     };
     auto rows = [&](const uint16_t* from, void* to, float inv_scale, bool fp8, int i) {
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kRotaryThreads) append_scalar_kernel(const hfr
         const int h = n / a.head_dim, i = n - h * a.head_dim;
         const long at = page * a.value_page_stride + place * a.value_place_stride + h * a.value_cache_head_stride;
         const uint16_t x = static_cast<const uint16_t*>(a.value)[token * a.value_token_stride + h * a.value_head_stride + i];
-        if (FP8) static_cast<uint8_t*>(a.value_cache)[at + i] = cvt_fp8(load16<DT>(x) * (a.value_scale ? 1.f / a.value_scale[h * a.value_scale_stride] : 1.f));
+        if (FP8) static_cast<uint8_t*>(a.value_cache)[at + i] = cvt_fp8_or_nan(load16<DT>(x) * (a.value_scale ? 1.f / a.value_scale[h * a.value_scale_stride] : 1.f));
         else static_cast<uint16_t*>(a.value_cache)[at + i] = x;
     }
 }

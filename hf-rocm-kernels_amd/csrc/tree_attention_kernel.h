@@ -79,8 +79,8 @@ __device__ __forceinline__ void store_row(const hfrk_attention_args& a, long tok
         uint32_t w[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            w[j] = cvt_pk_fp8(o[4 * j] * by * inv_out_scale, o[4 * j + 1] * by * inv_out_scale, 0u, false);
-            w[j] = cvt_pk_fp8(o[4 * j + 2] * by * inv_out_scale, o[4 * j + 3] * by * inv_out_scale, w[j], true);
+            w[j] = cvt_pk_fp8_or_nan(o[4 * j] * by * inv_out_scale, o[4 * j + 1] * by * inv_out_scale, 0u, false);
+            w[j] = cvt_pk_fp8_or_nan(o[4 * j + 2] * by * inv_out_scale, o[4 * j + 3] * by * inv_out_scale, w[j], true);
         }
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.output) + at) = make_uint2(w[0], w[1]);
     } else {

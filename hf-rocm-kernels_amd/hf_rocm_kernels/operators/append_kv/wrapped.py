@@ -85,7 +85,7 @@ def append_kv(
         - positions, frequencies, interleaved, magnitude: as in `rotary`; None: keys are stored as they are
         - query: (tokens, heads, head_dim), rotated into query_output (None: a new tensor; query itself: in place)
         - key_scale, value_scale: for float8_e4m3fn caches, positive float32 tensors of one value or one per key head: x / scale is stored,
-            saturating at +-448; None: 1
+            saturating at +-448, NaN kept; None: 1
     The caches and query_output may share memory with nothing else that the call takes (slices of one tensor that lie between each other do not); refused
     otherwise.
     Outputs:

@@ -85,7 +85,7 @@ def tree_attention(
             seen by all of it
         - scale: the scores' factor, 1/sqrt(head_dim) when None
         - key_scale, value_scale: the positive scales of float8_e4m3fn caches, as in `append_kv`
-        - out_scale: one float32: the result is divided by it and converted to float8_e4m3fn, as the projection behind it takes it
+        - out_scale: one float32: the result is divided by it and converted to float8_e4m3fn (saturating, NaN kept), as the projection behind it takes it
         - output: a tensor to write to; None: a new one
     Outputs:
         - (tokens, heads, head_dim) of the query's dtype, or float8_e4m3fn with out_scale.  A token that sees nothing gets zeros; rows behind

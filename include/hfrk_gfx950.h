@@ -398,7 +398,7 @@ int hfrk_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, vo
  *                   strides (elements) between pages, a page's places and heads: tokens-major or heads-major pages
  *   slots           [tokens] int32, or int64 with slots_wide != 0: token t goes to place slot % page_size of page slot / page_size; a slot that is
  *                   negative or past the last page is not written (padding).  Slots that name one place twice leave either's values there
- *   key_scale, value_scale   e4m3fn caches: e4m3fn(clamp(x / scale, +-448)), fp32 scales > 0 on the device, one (stride 0) or one a head (1); NULL: 1
+ *   key_scale, value_scale   e4m3fn caches: e4m3fn(clamp(x / scale, +-448)), a NaN stays one; fp32 scales > 0 on the device, one (stride 0) or one a head (1); NULL: 1
  *   query, query_output      as x and output of hfrk_rotary
  * Nothing that is written (query_output, the caches) may share memory with anything else or repeat itself, but query_output may be query: HFRK_BAD_SHAPE.  Tensors
  * whose elements lie between each other's (slices of a projection's output, keys and values side by side in a page) share none. */
@@ -434,7 +434,7 @@ int hfrk_append_kv(const hfrk_append_args* args, void* stream);
  *   output[row, head] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * key_scale * (q . k_j));  zero where a row sees nothing, NaN where all that it sees
  *   has a score of minus infinity (0 / 0)
  *   query         16-bit (dtype) [tokens, heads, head_dim]; heads a multiple of kv_heads, query heads h * heads/kv_heads ... share key head h
- *   output        [tokens, heads, head_dim] of dtype, or e4m3fn(clamp(result / out_scale[0], +-448)) where out_scale is not NULL.  Rows of no
+ *   output        [tokens, heads, head_dim] of dtype, or e4m3fn(clamp(result / out_scale[0], +-448)), NaN kept, where out_scale is not NULL.  Rows of no
  *                 sequence are left as they are
  *   key_cache, value_cache, key_scale, value_scale   as in hfrk_append_kv; the values are scale * e4m3fn
  *   page_table    [seqs, table_columns] int32, rows table_stride elements apart: token t of a sequence is at place t % page_size of page

@@ -90,7 +90,8 @@ inline float from_e4m3(uint8_t b) {
     const float v = e ? ldexpf(1 + m / 8.f, e - 7) : ldexpf(m / 8.f, -6);
     return b & 0x80 ? -v : v;
 }
-inline uint8_t to_e4m3(float f) {  // nearest, ties to even; of finite values up to 448
+inline uint8_t to_e4m3(float f) {  // nearest, ties to even; of NaN and values up to 448
+    if (f != f) return signbit(f) ? 0xff : 0x7f;
     uint8_t best = 0;
     for (int code = 1; code < 127; ++code) {
         const float now = fabsf(fabsf(f) - from_e4m3(code)), before = fabsf(fabsf(f) - from_e4m3(best));

@@ -1,5 +1,6 @@
 """The kernels of attention and append from their own sources, lane by lane on the CPU, against float64, with every tensor flush with pages that nothing
 may touch: in front of it in one run, behind it in the other.  No GPU."""
+import math
 import random
 
 import pytest
@@ -276,3 +277,22 @@ def test_what_meets_by_counting_bytes():
         assert status == (_capi.SUCCESS if apart else _capi.BAD_SHAPE)
         refused += not apart
     assert 50 < refused < 350
+
+
+@pytest.mark.parametrize("head_dim", [16, 18])
+def test_fp8_keeps_nan_and_saturates_infinities(head_dim):
+    """Caches and results in e4m3fn: no NaN becomes a number.  (Vector and scalar kernel.)"""
+    key = torch.zeros(1, 1, head_dim, dtype=torch.float16)
+    key[0, 0, :6] = torch.tensor([math.nan, math.inf, -math.inf, 3e4, -math.nan, 449.0])
+    caches = [torch.zeros(1, 8, 1, head_dim).to(FP8) for _ in range(2)]
+    lane_run.append(key, key, *caches, torch.tensor([3]))
+    for c in caches:
+        got = c[0, 3, 0].float()
+        assert torch.isnan(got[[0, 4]]).all() and torch.equal(got[[1, 2, 3, 5, 6]], torch.tensor([448.0, -448.0, 448.0, 448.0, 0.0]))
+
+
+@pytest.mark.parametrize("places", [0, LONG])
+def test_a_result_in_fp8_keeps_nan(places):
+    step = minus_infinities(torch.bfloat16, [40, 40], 0, 8, 64, False, places)
+    got = attend(step, True, out_scale=torch.tensor([0.01])).float()
+    assert torch.isnan(got[:40]).all() and torch.isfinite(got[40:]).all()

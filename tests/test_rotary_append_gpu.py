@@ -276,3 +276,14 @@ def test_more_tokens_than_a_launch_has_workgroups():
     assert ((mine.double() - want).abs() <= oracle.rotary_tolerance(want, size, torch.float16)).all()
     assert torch.equal(memory[1].view(-1, 1, 2)[:tokens], rows[:, 2:]) and not memory[:, -1].any()
     assert torch.equal(rotary(rows[:, :1], positions, frequencies), got)
+
+
+@pytest.mark.parametrize("head_dim", [16, 18])
+def test_append_in_fp8_keeps_nan_and_saturates_infinities(head_dim):
+    key = torch.zeros(1, 1, head_dim, dtype=torch.float16, device="cuda")
+    key[0, 0, :6] = torch.tensor([math.nan, math.inf, -math.inf, 3e4, -math.nan, 449.0])
+    caches = [torch.zeros(1, 8, 1, head_dim, device="cuda").to(FP8) for _ in range(2)]
+    append_kv(key, key, *caches, torch.tensor([3], device="cuda"))
+    for c in caches:
+        got = c[0, 3, 0].float().cpu()
+        assert torch.isnan(got[[0, 4]]).all() and torch.equal(got[[1, 2, 3, 5, 6]], torch.tensor([448.0, -448.0, 448.0, 448.0, 0.0]))

@@ -526,3 +526,10 @@ def test_more_rows_than_a_launch_has_threads():
     found = torch.matmul(p, v)[:, 0], torch.matmul(p, v.abs())[:, 0], off, v.abs().amax(1)
     assert ((out[-1].cpu().double() - found[0]).abs() <= oracle.attention_tolerance(found, torch.bfloat16, long // 16)).all()
     assert not out[:tokens - 9].any()  # rows that see nothing
+
+
+@pytest.mark.parametrize("places", [0, LONG])
+def test_a_result_in_fp8_keeps_nan(places):
+    step = minus_infinities(torch.bfloat16, [40, 40], 0, 8, 64, False, places)
+    got = tree_attention(**step.args(), out_scale=torch.tensor([0.01], device="cuda")).float()
+    assert torch.isnan(got[:40]).all() and torch.isfinite(got[40:]).all()
