@@ -48,7 +48,7 @@ def llama_attention_combined_ops(
     Rows of padding (a negative slot, behind starts' last) take no part in other rows; theirs of the first output hold nothing.
     Nothing waits for the host, and a captured call can be replayed with other positions, slots, lengths, pages and masks in the same tensors.  Run one eager
     call on the stream of the capture first: the projections' workspace is the stream's.
-    Returns (attn_output, residual)."""
+    Inference only.  Returns (attn_output, residual)."""
     tokens = hidden.size(0)
     kv_heads, head_dim = key_cache.size(2), key_cache.size(3)
     normalized, residual = residual_rms(input=hidden, residual=residual, weight=rms_weight, epsilon=rms_epsilon, scale_tensor=qkv_input_scale)

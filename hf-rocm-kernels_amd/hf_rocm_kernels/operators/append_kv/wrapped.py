@@ -87,7 +87,7 @@ def append_kv(
         - key_scale, value_scale: for float8_e4m3fn caches, positive float32 tensors of one value or one per key head: x / scale is stored,
             saturating at +-448, NaN kept; None: 1
     The caches and query_output may share memory with nothing else that the call takes (slices of one tensor that lie between each other do not); refused
-    otherwise.
+    otherwise.  Inference only: the rotated queries carry no gradient.
     Outputs:
         - the rotated queries, None without a query
     """

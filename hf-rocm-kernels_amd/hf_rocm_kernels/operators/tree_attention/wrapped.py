@@ -88,8 +88,9 @@ def tree_attention(
         - out_scale: one float32: the result is divided by it and converted to float8_e4m3fn (saturating, NaN kept), as the projection behind it takes it
         - output: a tensor to write to; None: a new one
     Outputs:
-        - (tokens, heads, head_dim) of the query's dtype, or float8_e4m3fn with out_scale.  A token that sees nothing gets zeros; rows behind
-          the last sequence's are not written
+        - (tokens, heads, head_dim) of the query's dtype, or float8_e4m3fn with out_scale.  A token that sees nothing gets zeros, one whose scores
+          are all minus infinity NaN; rows behind the last sequence's are not written.  Inference only: the result carries no gradient
+    Each call takes a workspace from torch's allocator for parts of rows: up to about 128 MiB and 16 bytes a token and query head of a group.
     A batch of some thousand short sequences is slow, as every workgroup looks at all of them; one of 65536 with more than about 15 kv_heads is refused.
     Lengths, starts and page_table stay on the device: no call waits for them, and a captured call may be replayed with others.  The result does not depend
     on other streams' calls (each has a workspace of its own), but how a sequence's tokens are split, and with it the last bits, depends on all lengths.

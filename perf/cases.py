@@ -7,7 +7,7 @@ Kinds of case, each with plain sizes and options:
           decode token to a prefill chunk; row-major or packed weight, dynamic per-token or static activation scale,
           optionally a bias or a residual in the epilogue
   mlp     the decoder MLP sub-block, operator by operator (`llama_mlp_combined_ops`) or as a captured graph (`LlamaMlpGraph`)
-  decode  one token step through a few decoder layers without the attention itself (it is not part of this package): per
+  decode  one token step through a few decoder layers without the attention itself (`operators.py` times that): per
           layer RMSNorm, qkv, o_proj, RMSNorm, gate_up, SwiGLU, down with per-token scales, captured in one HIP graph as a
           serving program does.  Each layer starts from a hidden state and residual of its own: chained, the one-step fp8
           flips that another order of sums causes would grow from layer to layer and leave nothing to compare.
@@ -200,7 +200,7 @@ def _prepare_decode(state, case, gen, dtype):
         for i, layer in enumerate(layers):
             q, _, s = residual_rms_dynamic(x[i], residual[i], layer["norm1"], _EPS)
             qkvs.append(layer["qkv"](q, input_scale=s))
-            h = layer["o_proj"](layer["attn"])  # the attention over qkv is other software's: its result is an input here
+            h = layer["o_proj"](layer["attn"])  # the attention over qkv is timed by itself: its result is an input here
             q, _, s = residual_rms_dynamic(h, residual[i], layer["norm2"], _EPS)
             act, s = swiglu_dynamic(layer["gate_up"](q, input_scale=s))
             hiddens.append(layer["down"](act, input_scale=s))
