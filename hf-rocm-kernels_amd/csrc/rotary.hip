@@ -276,14 +276,14 @@ static bool pieces_of_16(const hfrk_append_args& a, bool fp8) {
 }
 
 // The same from token `first` on.
-static hfrk_append_args behind(hfrk_append_args a, int first, int tokens) {
+static hfrk_append_args behind(hfrk_append_args a, int64_t first, int tokens) {
     auto ahead = [](const void* p, int64_t bytes) { return p ? static_cast<const uint8_t*>(p) + bytes : nullptr; };
     a.query = ahead(a.query, 2 * first * a.query_token_stride);
     a.query_output = const_cast<uint8_t*>(ahead(a.query_output, 2 * first * a.output_token_stride));
     a.key = ahead(a.key, 2 * first * a.key_token_stride);
     a.value = ahead(a.value, 2 * first * a.value_token_stride);
-    a.slots = ahead(a.slots, (a.slots_wide ? 8L : 4L) * first);
-    a.positions = ahead(a.positions, (a.positions_wide ? 8L : 4L) * first);
+    a.slots = ahead(a.slots, (a.slots_wide ? 8 : 4) * first);
+    a.positions = ahead(a.positions, (a.positions_wide ? 8 : 4) * first);
     a.tokens = tokens;
     return a;
 }

@@ -287,3 +287,17 @@ def test_append_in_fp8_keeps_nan_and_saturates_infinities(head_dim):
     for c in caches:
         got = c[0, 3, 0].float().cpu()
         assert torch.isnan(got[[0, 4]]).all() and torch.equal(got[[1, 2, 3, 5, 6]], torch.tensor([448.0, -448.0, 448.0, 448.0, 0.0]))
+
+
+def test_a_launch_whose_first_token_is_past_31_bits_of_bytes():
+    """Slices of a call that begin 2^30 tokens in, or later: their offsets in bytes need more than 32 bits."""
+    tokens = (1 << 30) + (1 << 23) + 5
+    x = torch.empty(tokens, 1, 2, dtype=torch.float16, device="cuda")
+    some = torch.cat((torch.arange(3), (1 << 30) + torch.arange(-3, 3), tokens + torch.arange(-8, 0)))
+    x[some.cuda()] = torch.randn(some.numel(), 1, 2, generator=torch.Generator().manual_seed(1)).to(torch.float16).cuda()
+    positions = torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    positions[some.cuda()] = torch.arange(some.numel(), dtype=torch.int32, device="cuda")
+    frequencies = torch.tensor([0.37], dtype=torch.float64, device="cuda")
+    before = x[some.cuda()].cpu()
+    assert rotary(x, positions, frequencies, output=x) is x
+    _check_rotated(x[some.cuda()], before, torch.arange(some.numel()), frequencies.cpu(), False)
