@@ -2,6 +2,7 @@
 may touch: in front of it in one run, behind it in the other.  No GPU."""
 import math
 import random
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -22,16 +23,19 @@ def attend(step, at_end, **more):
 
 
 def run(step, out_scale=None):
-    """Both runs: right values, rows of nobody left alone, and the same bits whatever the workspace held."""
-    results = []
-    for at_end in BOTH_ENDS:
-        scale = None if out_scale is None else torch.tensor([out_scale])
+    """Both runs, side by side: right values, rows of nobody left alone, and the same bits whatever the workspace held."""
+    scale = None if out_scale is None else torch.tensor([out_scale])
+
+    def one(at_end):
         out = torch.full(step.query.shape, 7.0).to(step.dtype if scale is None else FP8)
-        got = attend(step, at_end, output=out, out_scale=scale, noise=0xff if at_end else 0x3f)
-        step.check(got.float() if out_scale else got, out_scale=None if out_scale is None else float(torch.tensor(out_scale)))
-        assert (got[sum(step.counts):].float() == 7.0).all()
-        results.append(got.contiguous().view(torch.uint8))
-    assert torch.equal(*results)
+        return attend(step, at_end, output=out, out_scale=scale, noise=0xff if at_end else 0x3f)
+
+    with ThreadPoolExecutor(2) as pool:
+        results = list(pool.map(one, BOTH_ENDS))
+    assert torch.equal(*(r.contiguous().view(torch.uint8) for r in results))
+    got = results[0]
+    step.check(got.float() if out_scale else got, out_scale=None if out_scale is None else float(torch.tensor(out_scale)))
+    assert (got[sum(step.counts):].float() == 7.0).all()
 
 
 @pytest.mark.parametrize("dtype,cache", TYPES)
