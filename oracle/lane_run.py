@@ -12,6 +12,8 @@ import os
 import re
 import shutil
 import subprocess
+import tempfile
+import threading
 from concurrent.futures import ThreadPoolExecutor
 
 import torch
@@ -28,6 +30,7 @@ _SOURCES = ("rotary.hip", "tree_attention.hip", *(f"tree_attention_{kind}d{n}.hi
 _PAGE = mmap.PAGESIZE
 _MARGIN = 16 * _PAGE  # in front of a tensor and behind it
 _lib = None
+_loading = threading.Lock()
 
 
 def _text(name):
@@ -52,8 +55,8 @@ def build() -> str:
     lib = os.path.join(_BUILD, f"lanes_{digest.hexdigest()[:16]}.so")
     if os.path.exists(lib):
         return lib
-    work = f"{lib}.{os.getpid()}"
-    os.makedirs(work)
+    os.makedirs(_BUILD, exist_ok=True)
+    work = tempfile.mkdtemp(dir=_BUILD)
     try:
         for name, text in texts.items():
             with open(os.path.join(work, name), "w") as f:
@@ -80,9 +83,11 @@ def build() -> str:
 
 def _load():
     global _lib
-    if _lib is None:
-        _lib = ctypes.CDLL(build())
-        _lib.hfrk_tree_attention_workspace_bytes.restype = ctypes.c_size_t
+    with _loading:
+        if _lib is None:
+            lib = ctypes.CDLL(build())
+            lib.hfrk_tree_attention_workspace_bytes.restype = ctypes.c_size_t
+            _lib = lib
     return _lib
 
 
