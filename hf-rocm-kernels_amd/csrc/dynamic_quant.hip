@@ -3,7 +3,7 @@
 //   residual_rms_dynamic:  residual <- input + residual;  y = rmsnorm(residual) * weight
 //   swiglu_dynamic:        y = silu(gate) * up
 //   quantize_fp8:          y = x   (also with one static scale: the reference's fp8_quantize, utils/fp8.py:6-29, on device)
-// and in both:            scale[row] = max(amax_row |y| / 448, FLT_MIN);  output = e4m3fn(y / scale[row])
+// (the last two also to int8: scale[row] = max(amax / 127, FLT_MIN), output = rint(y / scale[row])) and in both:            scale[row] = max(amax_row |y| / 448, FLT_MIN);  output = e4m3fn(y / scale[row])
 // The per-row scales feed the GEMM's per-token scale_a directly, so no activation scale has to be calibrated ahead
 // of time.  The reference only has the static-scale forms (one scale_tensor for the whole tensor:
 // operators/residual_rms/wrapped.py:94-95, operators/swiglu/wrapped.py:49-84); these kernels have no counterpart
@@ -33,11 +33,29 @@ __device__ __forceinline__ void dyn_zero_row(uint16_t* next_buffer, int buffer_c
     for (int i = head + body * 8 + threadIdx.x; i < buffer_cols; i += blockDim.x) row[i] = 0;
 }
 
+// Four int8 codes rint(y / scale) in a word, lowest first, +-127 at most (NaN: -127).  The quotient is y * inv corrected by its remainder, so that
+// values next to the middle between two codes go where the quotient rounded to fp32 goes; adding 1.5 * 2^23 leaves the integer, ties to even, in the low bits.
+__device__ __forceinline__ uint32_t four_int8(const float* y, float scale, float inv) {
+    uint32_t code[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        const float q = __builtin_amdgcn_fmed3f(y[v] * inv, 1e4f, -1e4f);  // (finite, so that the remainder is)
+        const float c = __builtin_amdgcn_fmed3f(fmaf(fmaf(-q, scale, y[v]), inv, q), 127.0f, -127.0f);
+        code[v] = __float_as_uint(c + 12582912.0f);
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(code[1], code[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(code[3], code[2], 0x04000c0cu);
+    return lo | hi;
+}
+
 // Quantise the cached row: scale from the row maximum, 8 values per 8-byte store.
-template <int ITERS>
-__device__ __forceinline__ void dyn_store_row(const float (&y)[ITERS][8], float inv, __amdgpu_buffer_rsrc_t out_row) {
+template <int ITERS, int OUT>
+__device__ __forceinline__ void dyn_store_row(const float (&y)[ITERS][8], float scale, float inv, __amdgpu_buffer_rsrc_t out_row) {
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
+        if constexpr (OUT == HFRK_INT8) {
+            store_fp8_piece(out_row, threadIdx.x + it * blockDim.x, make_uint2(four_int8(y[it], scale, inv), four_int8(y[it] + 4, scale, inv)));
+            continue;
+        }
         uint32_t p0 = cvt_pk_fp8(y[it][0] * inv, y[it][1] * inv, 0u, false);
         p0 = cvt_pk_fp8(y[it][2] * inv, y[it][3] * inv, p0, true);
         uint32_t p1 = cvt_pk_fp8(y[it][4] * inv, y[it][5] * inv, 0u, false);
@@ -46,12 +64,24 @@ __device__ __forceinline__ void dyn_store_row(const float (&y)[ITERS][8], float 
     }
 }
 
-template <int ITERS>
-__device__ __forceinline__ void dyn_quantise_row(const float (&y)[ITERS][8], float amax, __amdgpu_buffer_rsrc_t out_row, float* scales) {
-    const float scale = fmaxf(amax / 448.0f, FLT_MIN);
+// int8: a row with an infinity or a NaN (`bad`, the sum of y * 0) gets the scale NaN, as its codes cannot say so.
+template <int ITERS, int OUT>
+__device__ __forceinline__ void dyn_quantise_row(const float (&y)[ITERS][8], float amax, float bad, __amdgpu_buffer_rsrc_t out_row, float* scales) {
+    const float scale = fmaxf(amax / (OUT == HFRK_INT8 ? 127.0f : 448.0f), FLT_MIN);
     const float inv = 1.0f / scale;
-    if (threadIdx.x == 0) scales[blockIdx.x] = scale;
-    dyn_store_row<ITERS>(y, inv, out_row);
+    if (threadIdx.x == 0) scales[blockIdx.x] = OUT == HFRK_INT8 ? scale + bad : scale;
+    dyn_store_row<ITERS, OUT>(y, scale, inv, out_row);
+}
+
+// The sum of y * 0 over the row: 0, or NaN where a value is none or infinite.
+template <int ITERS>
+__device__ __forceinline__ float dyn_bad_values(const float (&y)[ITERS][8], float* red) {
+    float bad = 0.f;
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+        for (int v = 0; v < 8; ++v) bad += y[it][v] * 0.f;
+    return block_sum(bad, red);
 }
 
 template <int DT, int ITERS>
@@ -104,11 +134,11 @@ __global__ void __launch_bounds__(kDynMaxThreads) residual_rms_dynamic_kernel(
         }
     }
     amax = block_max(amax, red_max);
-    dyn_quantise_row<ITERS>(y, amax, make_rsrc(output + row_off, (uint32_t)cols), scales);
+    dyn_quantise_row<ITERS, HFRK_FP8_E4M3FN>(y, amax, 0.f, make_rsrc(output + row_off, (uint32_t)cols), scales);
     dyn_zero_row(next_buffer, buffer_cols);
 }
 
-template <int DT, int ITERS>
+template <int DT, int ITERS, int OUT>
 __global__ void __launch_bounds__(kDynMaxThreads) swiglu_dynamic_kernel(
     const uint16_t* __restrict__ gate_up, uint8_t* __restrict__ output, float* __restrict__ scales,
     uint16_t* __restrict__ next_buffer, int cols, int buffer_cols) {
@@ -135,14 +165,19 @@ __global__ void __launch_bounds__(kDynMaxThreads) swiglu_dynamic_kernel(
         }
     }
     amax = block_max(amax, red_max);
-    dyn_quantise_row<ITERS>(y, amax, make_rsrc(output + (long)blockIdx.x * cols, (uint32_t)cols), scales);
+    float bad = 0.f;
+    if constexpr (OUT == HFRK_INT8) {
+        __shared__ __align__(16) float red_bad[16];
+        bad = dyn_bad_values<ITERS>(y, red_bad);
+    }
+    dyn_quantise_row<ITERS, OUT>(y, amax, bad, make_rsrc(output + (long)blockIdx.x * cols, (uint32_t)cols), scales);
     dyn_zero_row(next_buffer, buffer_cols);
 }
 
 // Plain quantisation of a 16-bit activation block (what sits between an attention output and the o_proj GEMM):
 // dynamic (static_scale == nullptr): scales[row] = max(amax_row |x| / 448, FLT_MIN), output = e4m3fn(x / scales[row]);
 // static: output = e4m3fn(x / static_scale[0]), saturating, scales untouched.
-template <int DT, int ITERS>
+template <int DT, int ITERS, int OUT>
 __global__ void __launch_bounds__(kDynMaxThreads) quantize_rows_kernel(
     const uint16_t* __restrict__ input, const float* __restrict__ static_scale, uint8_t* __restrict__ output,
     float* __restrict__ scales, int cols) {
@@ -165,11 +200,16 @@ __global__ void __launch_bounds__(kDynMaxThreads) quantize_rows_kernel(
         }
     }
     if (static_scale) {
-        dyn_store_row<ITERS>(y, 1.0f / static_scale[0], rout);
+        dyn_store_row<ITERS, OUT>(y, static_scale[0], 1.0f / static_scale[0], rout);
         return;
     }
     amax = block_max(amax, red_max);
-    dyn_quantise_row<ITERS>(y, amax, rout, scales);
+    float bad = 0.f;
+    if constexpr (OUT == HFRK_INT8) {
+        __shared__ __align__(16) float red_bad[16];
+        bad = dyn_bad_values<ITERS>(y, red_bad);
+    }
+    dyn_quantise_row<ITERS, OUT>(y, amax, bad, rout, scales);
 }
 
 static bool dyn_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -221,9 +261,11 @@ extern "C" int hfrk_residual_rms_dynamic(const void* input, void* residual, cons
     return HFRK_SUCCESS;
 }
 
-extern "C" int hfrk_swiglu_dynamic(const void* gate_up, void* output, float* scales, void* next_buffer, int rows, int cols,
-                                   int buffer_cols, int io_dtype, void* stream) {
-    using namespace hfrk;
+namespace hfrk {
+
+template <int OUT>
+static int run_swiglu_dynamic(const void* gate_up, void* output, float* scales, void* next_buffer, int rows, int cols, int buffer_cols, int io_dtype,
+                              void* stream) {
     if (rows < 0 || cols < 1 || buffer_cols < 0 || cols % 8 != 0) return HFRK_BAD_SHAPE;
     if (rows == 0) return HFRK_SUCCESS;
     if (!gate_up || !output || !scales) return HFRK_BAD_SHAPE;
@@ -236,8 +278,8 @@ extern "C" int hfrk_swiglu_dynamic(const void* gate_up, void* output, float* sca
     const uint16_t* in = static_cast<const uint16_t*>(gate_up);
     uint8_t* out = static_cast<uint8_t*>(output);
     uint16_t* nb = static_cast<uint16_t*>(next_buffer);
-#define HFRK_DYN_SWIGLU(DT_, IT_)                                                                                    \
-    hipLaunchKernelGGL((swiglu_dynamic_kernel<DT_, IT_>), dim3(rows), dim3(threads), 0, s, in, out, scales, nb, cols, \
+#define HFRK_DYN_SWIGLU(DT_, IT_)                                                                                           \
+    hipLaunchKernelGGL((swiglu_dynamic_kernel<DT_, IT_, OUT>), dim3(rows), dim3(threads), 0, s, in, out, scales, nb, cols, \
                        buffer_cols)
     if (io_dtype == HFRK_F16) {
         if (iters == 1) HFRK_DYN_SWIGLU(HFRK_F16, 1); else if (iters == 2) HFRK_DYN_SWIGLU(HFRK_F16, 2); else HFRK_DYN_SWIGLU(HFRK_F16, 4);
@@ -249,9 +291,8 @@ extern "C" int hfrk_swiglu_dynamic(const void* gate_up, void* output, float* sca
     return HFRK_SUCCESS;
 }
 
-extern "C" int hfrk_quantize_fp8(const void* input, const float* static_scale, void* output, float* scales, int rows, int cols,
-                                 int io_dtype, void* stream) {
-    using namespace hfrk;
+template <int OUT>
+static int run_quantize(const void* input, const float* static_scale, void* output, float* scales, int rows, int cols, int io_dtype, void* stream) {
     if (rows < 0 || cols < 1 || cols % 8 != 0) return HFRK_BAD_SHAPE;
     if (rows == 0) return HFRK_SUCCESS;
     if (!input || !output || (!static_scale && !scales)) return HFRK_BAD_SHAPE;
@@ -263,7 +304,7 @@ extern "C" int hfrk_quantize_fp8(const void* input, const float* static_scale, v
     const uint16_t* in = static_cast<const uint16_t*>(input);
     uint8_t* out = static_cast<uint8_t*>(output);
 #define HFRK_QUANT(DT_, IT_) \
-    hipLaunchKernelGGL((quantize_rows_kernel<DT_, IT_>), dim3(rows), dim3(threads), 0, s, in, static_scale, out, scales, cols)
+    hipLaunchKernelGGL((quantize_rows_kernel<DT_, IT_, OUT>), dim3(rows), dim3(threads), 0, s, in, static_scale, out, scales, cols)
     if (io_dtype == HFRK_F16) {
         if (iters == 1) HFRK_QUANT(HFRK_F16, 1); else if (iters == 2) HFRK_QUANT(HFRK_F16, 2); else HFRK_QUANT(HFRK_F16, 4);
     } else {
@@ -272,4 +313,24 @@ extern "C" int hfrk_quantize_fp8(const void* input, const float* static_scale, v
 #undef HFRK_QUANT
     HFRK_HIP_TRY(hipGetLastError());
     return HFRK_SUCCESS;
+}
+
+}  // namespace hfrk
+
+extern "C" int hfrk_swiglu_dynamic(const void* gate_up, void* output, float* scales, void* next_buffer, int rows, int cols,
+                                   int buffer_cols, int io_dtype, void* stream) {
+    return hfrk::run_swiglu_dynamic<HFRK_FP8_E4M3FN>(gate_up, output, scales, next_buffer, rows, cols, buffer_cols, io_dtype, stream);
+}
+
+extern "C" int hfrk_swiglu_dynamic_int8(const void* gate_up, void* output, float* scales, int rows, int cols, int io_dtype, void* stream) {
+    return hfrk::run_swiglu_dynamic<HFRK_INT8>(gate_up, output, scales, nullptr, rows, cols, 0, io_dtype, stream);
+}
+
+extern "C" int hfrk_quantize_fp8(const void* input, const float* static_scale, void* output, float* scales, int rows, int cols,
+                                 int io_dtype, void* stream) {
+    return hfrk::run_quantize<HFRK_FP8_E4M3FN>(input, static_scale, output, scales, rows, cols, io_dtype, stream);
+}
+
+extern "C" int hfrk_quantize_int8(const void* input, const float* static_scale, void* output, float* scales, int rows, int cols, int io_dtype, void* stream) {
+    return hfrk::run_quantize<HFRK_INT8>(input, static_scale, output, scales, rows, cols, io_dtype, stream);
 }

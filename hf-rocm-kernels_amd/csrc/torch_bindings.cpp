@@ -1097,6 +1097,343 @@ at::Tensor tree_attention_new(const at::Tensor& query, const at::Tensor& key_cac
     return run_attention(a, query) == HFRK_SUCCESS ? output : at::Tensor();
 }
 
+// ---- 8-bit integers and experts -------------------------------------------------------------------------------------------------
+// As above: the `_new` forms take what is certain to run, allocate and launch in one native operator, and answer everything else with no tensor.
+
+bool is_8bit(at::ScalarType t) { return t == at::kFloat8_e4m3fn || t == at::kChar; }
+
+// Whether a contiguous result lies on an operand's memory (first to last byte).
+bool meets(const at::Tensor& result, const at::Tensor& t) {
+    if (result.numel() == 0 || t.numel() == 0) return false;
+    int64_t span = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) span += (t.size(d) - 1) * t.stride(d);
+    const char *r0 = static_cast<const char*>(result.data_ptr()), *t0 = static_cast<const char*>(t.data_ptr());
+    return r0 < t0 + span * (int64_t)t.element_size() && t0 < r0 + result.numel() * (int64_t)result.element_size();
+}
+
+bool meets(const at::Tensor& result, const std::optional<at::Tensor>& t) { return t.has_value() && meets(result, *t); }
+
+void quantize_int8(at::Tensor& input, const std::optional<at::Tensor>& scale_tensor, at::Tensor& output, at::Tensor& scales) {
+    TORCH_CHECK(input.dim() == 2 && input.is_contiguous(), "input must be a contiguous [rows, cols] tensor");
+    const int io = dtype16(input, "input");
+    TORCH_CHECK(output.scalar_type() == at::kChar && output.sizes() == input.sizes() && output.is_contiguous(), "output must be int8, match input and be contiguous");
+    check_same_device(input, output, "output");
+    if (scale_tensor.has_value()) {
+        TORCH_CHECK(scale_tensor->numel() == 1 && scale_tensor->scalar_type() == at::kFloat, "scale_tensor must be one float32");
+        check_same_device(input, *scale_tensor, "scale_tensor");
+    } else {
+        TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.numel() == input.size(0),
+                    "scales must be a contiguous float32 tensor with one element per row");
+        check_same_device(input, scales, "scales");
+    }
+    TORCH_CHECK(!meets(output, input) && !meets(output, scales) && !meets(scales, input), "output, scales and input must not share memory");
+    DeviceScope scope(input);
+    raise_on(hfrk_quantize_int8(input.data_ptr(), scale_tensor.has_value() ? scale_tensor->data_ptr<float>() : nullptr, output.data_ptr(),
+                                scale_tensor.has_value() ? nullptr : scales.data_ptr<float>(), (int)input.size(0), (int)input.size(1), io, current_stream(input)),
+             "quantize_int8");
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_int8_new(const at::Tensor& input) {
+    if (!plain_rows(input) || !dynamic_columns(input.size(1))) return {};
+    DeviceScope scope(input);
+    at::Tensor output = at::empty(input.sizes(), input.options().dtype(at::kChar));
+    at::Tensor scales = at::empty({input.size(0)}, input.options().dtype(at::kFloat));
+    if (hfrk_quantize_int8(input.data_ptr(), nullptr, output.data_ptr(), scales.data_ptr<float>(), (int)input.size(0), (int)input.size(1), dtype16(input, "input"),
+                           current_stream(input)) != HFRK_SUCCESS)
+        return {};
+    return {output, scales};
+}
+
+void swiglu_dynamic_int8(at::Tensor& gate_up, at::Tensor& output, at::Tensor& scales) {
+    TORCH_CHECK(gate_up.dim() == 2 && gate_up.is_contiguous() && gate_up.size(1) % 2 == 0, "gate_up must be a contiguous [rows, 2*cols] tensor");
+    const int io = dtype16(gate_up, "gate_up");
+    const int64_t rows = gate_up.size(0), cols = gate_up.size(1) / 2;
+    TORCH_CHECK(output.scalar_type() == at::kChar && output.dim() == 2 && output.size(0) == rows && output.size(1) == cols && output.is_contiguous(),
+                "output must be a contiguous [rows, cols] int8 tensor");
+    TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.numel() == rows,
+                "scales must be a contiguous float32 tensor with one element per row");
+    check_same_device(gate_up, output, "output");
+    check_same_device(gate_up, scales, "scales");
+    TORCH_CHECK(!meets(output, gate_up) && !meets(output, scales) && !meets(scales, gate_up), "output, scales and gate_up must not share memory");
+    DeviceScope scope(gate_up);
+    raise_on(hfrk_swiglu_dynamic_int8(gate_up.data_ptr(), output.data_ptr(), scales.data_ptr<float>(), (int)rows, (int)cols, io, current_stream(gate_up)),
+             "swiglu_dynamic_int8");
+}
+
+std::tuple<at::Tensor, at::Tensor> swiglu_dynamic_int8_new(const at::Tensor& gate_up) {
+    if (!plain_rows(gate_up) || gate_up.size(1) % 2 != 0 || !dynamic_columns(gate_up.size(1) / 2)) return {};
+    DeviceScope scope(gate_up);
+    const int64_t rows = gate_up.size(0), cols = gate_up.size(1) / 2;
+    at::Tensor output = at::empty({rows, cols}, gate_up.options().dtype(at::kChar));
+    at::Tensor scales = at::empty({rows}, gate_up.options().dtype(at::kFloat));
+    if (hfrk_swiglu_dynamic_int8(gate_up.data_ptr(), output.data_ptr(), scales.data_ptr<float>(), (int)rows, (int)cols, dtype16(gate_up, "gate_up"),
+                                 current_stream(gate_up)) != HFRK_SUCCESS)
+        return {};
+    return {output, scales};
+}
+
+// D = (base ? base : 0) + scale_a x scale_b x A.B on int8 codes: A [m, k], B [k, n] with unit stride along k, base [n] or [m, n].
+const char* int8_operands(const at::Tensor& A, const at::Tensor& B, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
+                          const std::optional<at::Tensor>& scale_b, at::ScalarType dtype) {
+    if (A.dim() != 2 || !A.is_contiguous() || A.scalar_type() != at::kChar) return "A must be a contiguous [m, k] int8 tensor";
+    const int64_t m = A.size(0), k = A.size(1);
+    if (B.dim() != 2 || B.scalar_type() != at::kChar || B.size(0) != k || (k > 1 && B.stride(0) != 1)) return "B must be [k, n] int8 with unit stride along k";
+    const int64_t n = B.size(1);
+    if (m >= (int64_t(1) << 31) || n >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || (n > 1 && (B.stride(1) < k || B.stride(1) >= (int64_t(1) << 31))))
+        return "A, B or B's rows are larger than the kernel's limits";
+    if (!is_16bit(dtype)) return "the result must be float16 or bfloat16";
+    if (!float_vector(scale_a, m, A)) return "scale_a must be float32 on A's device with 1 or m elements";
+    if (scale_b.has_value() && !float_vector(*scale_b, n, A)) return "scale_b must be float32 on A's device with 1 or n elements";
+    if (base.has_value() && !(base->is_contiguous() && base->scalar_type() == dtype && base->device() == A.device() &&
+                              ((base->dim() == 1 && base->size(0) == n) || (base->dim() == 2 && base->size(0) == m && base->size(1) == n))))
+        return "base must be a contiguous [n] or [m, n] tensor of the result's dtype on A's device";
+    if (B.device() != A.device()) return "B must be on A's device";
+    return nullptr;
+}
+
+int run_int8_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tensor& D, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
+                  const std::optional<at::Tensor>& scale_b) {
+    const int m = (int)A.size(0), n = (int)B.size(1), k = (int)A.size(1);
+    return hfrk_int8_gemm(A.data_ptr(), B.data_ptr(), D.data_ptr(), base.has_value() ? base->data_ptr() : nullptr,
+                          base.has_value() && base->dim() == 2 ? n : 0, scale_a.data_ptr<float>(), scale_a.numel() == 1 ? 0 : 1,
+                          scale_b.has_value() ? scale_b->data_ptr<float>() : nullptr, scale_b.has_value() && scale_b->numel() != 1 ? 1 : 0, m, n, k,
+                          n > 1 ? (int)B.stride(1) : k, D.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, current_stream(A));
+}
+
+void int8_gemm(const at::Tensor& A, const at::Tensor& B, at::Tensor& D, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
+               const std::optional<at::Tensor>& scale_b) {
+    const char* const why = int8_operands(A, B, base, scale_a, scale_b, D.scalar_type());
+    TORCH_CHECK(!why, why);
+    TORCH_CHECK(D.dim() == 2 && D.size(0) == A.size(0) && D.size(1) == B.size(1) && D.is_contiguous(), "D must be a contiguous [m, n] tensor");
+    check_same_device(A, D, "D");
+    TORCH_CHECK(!meets(D, A) && !meets(D, B) && !meets(D, scale_a) && !meets(D, scale_b), "D must share no memory with the operands");
+    TORCH_CHECK(!meets(D, base) || (base->data_ptr() == D.data_ptr() && base->dim() == 2), "D may be base but not share part of it");
+    if (A.size(0) == 0) return;
+    DeviceScope scope(A);
+    raise_on(run_int8_gemm(A, B, D, base, scale_a, scale_b), "int8_gemm");
+}
+
+// As fp8_linear: input [..., k] 16-bit (quantised here, with input_scale or per row) or int8 with its scale(s); weight [n, k] int8.
+at::Tensor int8_linear(const at::Tensor& input, const at::Tensor& weight, const std::optional<at::Tensor>& weight_scale,
+                       const std::optional<at::Tensor>& input_scale, const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& residual,
+                       std::optional<at::ScalarType> out_dtype) {
+    const bool quantised = input.scalar_type() == at::kChar;
+    if (!input.is_cuda() || input.dim() < 1 || input.numel() == 0 || !input.is_contiguous() || weight.dim() != 2) return {};
+    if (!quantised && !is_16bit(input.scalar_type())) return {};
+    if ((quantised && !input_scale.has_value()) || (bias.has_value() && residual.has_value())) return {};
+    const int64_t k = input.size(-1), m = input.numel() / k, n = weight.size(0);
+    if (n < 1 || m >= (int64_t(1) << 31)) return {};
+    if (!quantised && (!dynamic_columns(k) || (input_scale.has_value() && !one_float(*input_scale, input)))) return {};
+    const at::ScalarType dtype = out_dtype.value_or(quantised ? at::kBFloat16 : input.scalar_type());
+    std::optional<at::Tensor> base;
+    if (residual.has_value()) {
+        if (residual->numel() != m * n || !residual->is_contiguous()) return {};
+        base = residual->view({m, n});
+    } else if (bias.has_value()) {
+        if (bias->dim() != 1) return {};
+        base = bias;
+    }
+    DeviceScope scope(input);
+    at::Tensor codes, scales;
+    if (quantised) {
+        codes = input.dim() == 2 ? input : input.view({m, k});
+        scales = *input_scale;
+    } else {
+        codes = at::empty({m, k}, input.options().dtype(at::kChar));
+        scales = input_scale.has_value() ? *input_scale : at::empty({m}, input.options().dtype(at::kFloat));
+    }
+    const at::Tensor B = weight.t();
+    if (int8_operands(codes, B, base, scales, weight_scale, dtype)) return {};
+    at::DimVector sizes(input.sizes());
+    sizes.back() = n;
+    at::Tensor out = at::empty(sizes, input.options().dtype(dtype));
+    if (!quantised && hfrk_quantize_int8(input.data_ptr(), input_scale.has_value() ? scales.data_ptr<float>() : nullptr, codes.data_ptr(),
+                                         input_scale.has_value() ? nullptr : scales.data_ptr<float>(), (int)m, (int)k,
+                                         input.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, current_stream(input)) != HFRK_SUCCESS)
+        return {};
+    return run_int8_gemm(codes, B, out, base, scales, weight_scale) == HFRK_SUCCESS ? out : at::Tensor();
+}
+
+// a [a_rows, k], b [experts, k, n] with unit stride along k, offsets [experts + 1], rows [count] or none, output [count, n].
+const char* grouped_args(hfrk_grouped_args& g, const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a, const std::optional<at::Tensor>& scale_b,
+                         const at::Tensor& offsets, const std::optional<at::Tensor>& rows, at::ScalarType dtype) {
+    constexpr int64_t kMost = int64_t(1) << 31;
+    if (a.dim() != 2 || !a.is_contiguous() || !is_8bit(a.scalar_type())) return "a must be a contiguous [rows, k] float8_e4m3fn or int8 tensor";
+    const int64_t a_rows = a.size(0), k = a.size(1);
+    if (b.dim() != 3 || b.scalar_type() != a.scalar_type() || b.size(1) != k || (k > 1 && b.stride(1) != 1))
+        return "b must be [experts, k, n] of a's dtype with unit stride along k";
+    const int64_t experts = b.size(0), n = b.size(2);
+    if (experts < 1 || n < 1 || a_rows >= kMost || k >= kMost || n >= kMost || (n > 1 && (b.stride(2) < k || b.stride(2) >= kMost)) || b.stride(0) < 0)
+        return "a, b or b's rows are outside the kernel's limits";
+    if (!is_16bit(dtype)) return "the result must be float16 or bfloat16";
+    if (!float_vector(scale_a, a_rows, a)) return "scale_a must be float32 on a's device with 1 element or one for each row of a";
+    if (offsets.dim() != 1 || offsets.size(0) != experts + 1 || offsets.scalar_type() != at::kInt || !offsets.is_contiguous() || offsets.device() != a.device())
+        return "offsets must be experts + 1 int32 values on a's device";
+    if (rows.has_value() && (rows->dim() != 1 || rows->scalar_type() != at::kInt || !rows->is_contiguous() || rows->device() != a.device() || rows->size(0) >= kMost))
+        return "rows must be a contiguous vector of int32 values on a's device";
+    if (b.device() != a.device()) return "b must be on a's device";
+    g.a = a.data_ptr();
+    g.b = b.data_ptr();
+    g.expert_stride = experts > 1 ? b.stride(0) : 0;
+    g.b_stride = n > 1 ? (int)b.stride(2) : (int)k;
+    g.scale_a = scale_a.data_ptr<float>();
+    g.scale_a_stride = scale_a.numel() == 1 ? 0 : 1;
+    if (scale_b.has_value()) {
+        const at::Tensor& s = *scale_b;
+        if (s.scalar_type() != at::kFloat || s.device() != a.device() || s.dim() < 1 || s.dim() > 2 || s.size(0) != experts || (s.dim() == 2 && s.size(1) != n) ||
+            (s.dim() == 2 && n > 1 && s.stride(1) != 1) || s.stride(0) < 0)
+            return "scale_b must be float32 (experts,) or (experts, n) on a's device, unit stride along n";
+        g.scale_b = s.data_ptr<float>();
+        g.scale_b_expert_stride = experts > 1 ? s.stride(0) : 0;
+        g.scale_b_stride = s.dim() == 2 ? 1 : 0;
+    }
+    g.offsets = offsets.data_ptr<int32_t>();
+    g.rows = rows.has_value() ? rows->data_ptr<int32_t>() : nullptr;
+    g.count = (int)(rows.has_value() ? rows->size(0) : a_rows);
+    g.a_rows = (int)a_rows;
+    g.experts = (int)std::min<int64_t>(experts, 1 << 30);
+    g.n = (int)n;
+    g.k = (int)k;
+    g.type = a.scalar_type() == at::kChar ? HFRK_INT8 : HFRK_FP8_E4M3FN;
+    g.dtype = dtype == at::kBFloat16 ? HFRK_BF16 : HFRK_F16;
+    return nullptr;
+}
+
+void grouped_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a, const std::optional<at::Tensor>& scale_b, const at::Tensor& offsets,
+                  const std::optional<at::Tensor>& rows, at::Tensor& output) {
+    hfrk_grouped_args g = {};
+    const char* const why = grouped_args(g, a, b, scale_a, scale_b, offsets, rows, output.scalar_type());
+    TORCH_CHECK(!why, why);
+    TORCH_CHECK(output.dim() == 2 && output.size(0) == g.count && output.size(1) == g.n && output.is_contiguous(), "output must be a contiguous [rows, n] tensor");
+    check_same_device(a, output, "output");
+    TORCH_CHECK(!meets(output, a) && !meets(output, b) && !meets(output, scale_a) && !meets(output, scale_b) && !meets(output, offsets) && !meets(output, rows),
+                "output must share no memory with the operands");
+    g.output = output.data_ptr();
+    DeviceScope scope(a);
+    raise_on(hfrk_grouped_gemm(&g, current_stream(a)), "grouped_gemm");
+}
+
+at::Tensor grouped_gemm_new(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a, const std::optional<at::Tensor>& scale_b,
+                            const at::Tensor& offsets, const std::optional<at::Tensor>& rows, at::ScalarType dtype) {
+    hfrk_grouped_args g = {};
+    if (!a.is_cuda() || grouped_args(g, a, b, scale_a, scale_b, offsets, rows, dtype)) return {};
+    DeviceScope scope(a);
+    at::Tensor output = at::empty({g.count, g.n}, a.options().dtype(dtype));
+    g.output = output.data_ptr();
+    return hfrk_grouped_gemm(&g, current_stream(a)) == HFRK_SUCCESS ? output : at::Tensor();
+}
+
+const char* route_args(hfrk_route_args& r, const at::Tensor& logits, int64_t top, const std::optional<at::Tensor>& bias, bool sigmoid, bool renormalize,
+                       double factor, const std::optional<at::Tensor>& mask) {
+    const at::ScalarType type = logits.scalar_type();
+    if (logits.dim() != 2 || !(is_16bit(type) || type == at::kFloat)) return "logits must be a [tokens, experts] float16, bfloat16 or float32 tensor";
+    const int64_t tokens = logits.size(0), experts = logits.size(1);
+    if (experts > 1 && logits.stride(1) != 1) return "logits must have unit stride along the experts";
+    if (top < 1 || top > HFRK_MAX_TOP || top > experts || tokens > (int64_t(1) << 28)) return "top must be between 1 and the number of experts, 32 at most";
+    if (bias.has_value() && (bias->dim() != 1 || bias->size(0) != experts || bias->scalar_type() != at::kFloat || !bias->is_contiguous() ||
+                             bias->device() != logits.device()))
+        return "bias must be one float32 for each expert on the logits' device";
+    if (mask.has_value() && (mask->dim() != 1 || mask->size(0) != tokens || (mask->scalar_type() != at::kBool && mask->scalar_type() != at::kByte) ||
+                             !mask->is_contiguous() || mask->device() != logits.device()))
+        return "mask must be one bool or uint8 for each token on the logits' device";
+    r.logits = logits.data_ptr();
+    r.logits_stride = tokens > 1 ? logits.stride(0) : 0;
+    r.bias = bias.has_value() ? bias->data_ptr<float>() : nullptr;
+    r.mask = mask.has_value() ? mask->data_ptr() : nullptr;
+    r.tokens = (int)tokens;
+    r.num_experts = (int)std::min<int64_t>(experts, 1 << 30);
+    r.top = (int)top;
+    r.dtype = type == at::kFloat ? HFRK_FP32 : type == at::kBFloat16 ? HFRK_BF16 : HFRK_F16;
+    r.sigmoid = sigmoid;
+    r.renormalize = renormalize;
+    r.factor = (float)factor;
+    return nullptr;
+}
+
+int run_route(hfrk_route_args& r, const at::Tensor& logits, const at::Tensor& weights, const at::Tensor& experts, const at::Tensor& places,
+              const at::Tensor& rows, const at::Tensor& offsets) {
+    r.weights = weights.data_ptr<float>();
+    r.experts = experts.data_ptr<int32_t>();
+    r.places = places.data_ptr<int32_t>();
+    r.rows = rows.data_ptr<int32_t>();
+    r.offsets = offsets.data_ptr<int32_t>();
+    return hfrk_route_experts(&r, current_stream(logits));
+}
+
+void route_experts(const at::Tensor& logits, int64_t top, const std::optional<at::Tensor>& bias, bool sigmoid, bool renormalize, double factor,
+                   const std::optional<at::Tensor>& mask, at::Tensor& weights, at::Tensor& experts, at::Tensor& places, at::Tensor& rows, at::Tensor& offsets) {
+    hfrk_route_args r = {};
+    const char* const why = route_args(r, logits, top, bias, sigmoid, renormalize, factor, mask);
+    TORCH_CHECK(!why, why);
+    TORCH_CHECK(weights.scalar_type() == at::kFloat && weights.numel() == r.tokens * top && weights.is_contiguous(), "weights must be tokens * top float32");
+    for (const at::Tensor* t : {&experts, &places, &rows})
+        TORCH_CHECK(t->scalar_type() == at::kInt && t->numel() == r.tokens * top && t->is_contiguous(), "experts, places and rows must be tokens * top int32");
+    TORCH_CHECK(offsets.scalar_type() == at::kInt && offsets.numel() == r.num_experts + 1 && offsets.is_contiguous(), "offsets must be experts + 1 int32");
+    const at::Tensor* const results[] = {&weights, &experts, &places, &rows, &offsets};
+    for (const at::Tensor* t : results) {
+        check_same_device(logits, *t, "a result");
+        TORCH_CHECK(!meets(*t, logits) && !meets(*t, bias) && !meets(*t, mask), "results must share no memory with the operands");
+        for (const at::Tensor* u : results) TORCH_CHECK(t == u || !meets(*t, *u), "results must share no memory with each other");
+    }
+    DeviceScope scope(logits);
+    raise_on(run_route(r, logits, weights, experts, places, rows, offsets), "route_experts");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_experts_new(const at::Tensor& logits, int64_t top,
+                                                                                         const std::optional<at::Tensor>& bias, bool sigmoid,
+                                                                                         bool renormalize, double factor,
+                                                                                         const std::optional<at::Tensor>& mask) {
+    hfrk_route_args r = {};
+    if (!logits.is_cuda() || route_args(r, logits, top, bias, sigmoid, renormalize, factor, mask)) return {};
+    DeviceScope scope(logits);
+    const auto ints = logits.options().dtype(at::kInt);
+    at::Tensor weights = at::empty({r.tokens, top}, logits.options().dtype(at::kFloat));
+    at::Tensor experts = at::empty({r.tokens, top}, ints), places = at::empty({r.tokens, top}, ints), rows = at::empty({r.tokens * top}, ints),
+               offsets = at::empty({logits.size(1) + 1}, ints);
+    if (run_route(r, logits, weights, experts, places, rows, offsets) != HFRK_SUCCESS) return {};
+    return {weights, experts, places, rows, offsets};
+}
+
+const char* combine_operands(const at::Tensor& y, const at::Tensor& weights, const at::Tensor& places, const std::optional<at::Tensor>& base) {
+    if (y.dim() != 2 || !y.is_contiguous() || !is_16bit(y.scalar_type())) return "y must be a contiguous [rows, cols] float16 or bfloat16 tensor";
+    if (places.dim() != 2 || places.scalar_type() != at::kInt || !places.is_contiguous() || places.device() != y.device())
+        return "places must be a contiguous [tokens, top] int32 tensor on y's device";
+    if (weights.sizes() != places.sizes() || weights.scalar_type() != at::kFloat || !weights.is_contiguous() || weights.device() != y.device())
+        return "weights must be float32, contiguous, of places' shape and on y's device";
+    if (base.has_value() && (base->dim() != 2 || base->size(0) != places.size(0) || base->size(1) != y.size(1) || !base->is_contiguous() ||
+                             base->scalar_type() != y.scalar_type() || base->device() != y.device()))
+        return "base must be a contiguous [tokens, cols] tensor of y's dtype on its device";
+    if (y.size(0) >= (int64_t(1) << 31) || y.size(1) < 1 || y.size(1) >= (int64_t(1) << 31) || places.size(0) >= (int64_t(1) << 31) || places.size(1) > HFRK_MAX_TOP)
+        return "y or places is outside the kernel's limits";
+    return nullptr;
+}
+
+int run_combine(const at::Tensor& y, const at::Tensor& weights, const at::Tensor& places, const std::optional<at::Tensor>& base, const at::Tensor& output) {
+    return hfrk_combine_experts(y.data_ptr(), weights.data_ptr<float>(), places.data_ptr<int32_t>(), base.has_value() ? base->data_ptr() : nullptr,
+                                output.data_ptr(), (int)places.size(0), (int)places.size(1), (int)y.size(1), (int)y.size(0),
+                                y.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, current_stream(y));
+}
+
+void combine_experts(const at::Tensor& y, const at::Tensor& weights, const at::Tensor& places, const std::optional<at::Tensor>& base, at::Tensor& output) {
+    const char* const why = combine_operands(y, weights, places, base);
+    TORCH_CHECK(!why, why);
+    TORCH_CHECK(output.dim() == 2 && output.size(0) == places.size(0) && output.size(1) == y.size(1) && output.is_contiguous() &&
+                    output.scalar_type() == y.scalar_type(),
+                "output must be a contiguous [tokens, cols] tensor of y's dtype");
+    check_same_device(y, output, "output");
+    TORCH_CHECK(!meets(output, y) && !meets(output, weights) && !meets(output, places) && (!meets(output, base) || base->data_ptr() == output.data_ptr()),
+                "output may be base and must share no other memory");
+    DeviceScope scope(y);
+    raise_on(run_combine(y, weights, places, base, output), "combine_experts");
+}
+
+at::Tensor combine_experts_new(const at::Tensor& y, const at::Tensor& weights, const at::Tensor& places, const std::optional<at::Tensor>& base) {
+    if (!y.is_cuda() || combine_operands(y, weights, places, base)) return {};
+    DeviceScope scope(y);
+    at::Tensor output = at::empty({places.size(0), y.size(1)}, y.options());
+    return run_combine(y, weights, places, base, output) == HFRK_SUCCESS ? output : at::Tensor();
+}
+
 }  // namespace
 
 TORCH_LIBRARY(_HFRK_C, ops) {
@@ -1218,6 +1555,40 @@ TORCH_LIBRARY(_HFRK_C, ops) {
 
     ops.def("quantize_fp8(Tensor input, Tensor? scale_tensor, Tensor! output, Tensor! scales) -> ()");
     ops.impl("quantize_fp8", c10::kCUDA, &quantize_fp8);
+
+    ops.def("quantize_int8(Tensor input, Tensor? scale_tensor, Tensor! output, Tensor! scales) -> ()");
+    ops.impl("quantize_int8", c10::kCUDA, &quantize_int8);
+    ops.def("swiglu_dynamic_int8(Tensor gate_up, Tensor! output, Tensor! scales) -> ()");
+    ops.impl("swiglu_dynamic_int8", c10::kCUDA, &swiglu_dynamic_int8);
+    ops.def("int8_gemm(Tensor A, Tensor B, Tensor(a!) D, Tensor? base, Tensor scale_a, Tensor? scale_b) -> ()");
+    ops.impl("int8_gemm", c10::kCUDA, &int8_gemm);
+    ops.def("grouped_gemm(Tensor a, Tensor b, Tensor scale_a, Tensor? scale_b, Tensor offsets, Tensor? rows, Tensor(a!) output) -> ()");
+    ops.impl("grouped_gemm", c10::kCUDA, &grouped_gemm);
+    ops.def(
+        "route_experts(Tensor logits, int top, Tensor? bias, bool sigmoid, bool renormalize, float factor, Tensor? mask, Tensor(a!) weights, "
+        "Tensor(b!) experts, Tensor(c!) places, Tensor(d!) rows, Tensor(e!) offsets) -> ()");
+    ops.impl("route_experts", c10::kCUDA, &route_experts);
+    ops.def("combine_experts(Tensor y, Tensor weights, Tensor places, Tensor? base, Tensor(a!) output) -> ()");
+    ops.impl("combine_experts", c10::kCUDA, &combine_experts);
+
+    ops.def("quantize_int8_new(Tensor input) -> (Tensor, Tensor)");
+    ops.impl("quantize_int8_new", c10::kCUDA, &quantize_int8_new);
+    ops.def("swiglu_dynamic_int8_new(Tensor gate_up) -> (Tensor, Tensor)");
+    ops.impl("swiglu_dynamic_int8_new", c10::kCUDA, &swiglu_dynamic_int8_new);
+    ops.def(
+        "int8_linear(Tensor input, Tensor weight, Tensor? weight_scale, Tensor? input_scale, Tensor? bias, Tensor? residual, "
+        "ScalarType? out_dtype) -> Tensor");
+    ops.impl("int8_linear", c10::kCUDA, &int8_linear);
+    ops.def("grouped_gemm_new(Tensor a, Tensor b, Tensor scale_a, Tensor? scale_b, Tensor offsets, Tensor? rows, ScalarType dtype) -> Tensor");
+    ops.impl("grouped_gemm_new", c10::kCUDA, &grouped_gemm_new);
+    ops.def(
+        "route_experts_new(Tensor logits, int top, Tensor? bias, bool sigmoid, bool renormalize, float factor, Tensor? mask) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor)");
+    ops.impl("route_experts_new", c10::kCUDA, &route_experts_new);
+    ops.def("combine_experts_new(Tensor y, Tensor weights, Tensor places, Tensor? base) -> Tensor");
+    ops.impl("combine_experts_new", c10::kCUDA, &combine_experts_new);
+    for (const char* name : {"quantize_int8_new", "swiglu_dynamic_int8_new", "int8_linear", "grouped_gemm_new", "route_experts_new", "combine_experts_new"})
+        ops.impl(name, torch::dispatch(c10::DispatchKey::Autograd, torch::CppFunction::makeFallthrough()));
 }
 
 // nothing_intercepts() -> bool: whether an operator called now, on plain tensors, runs its kernel and is seen by nobody else.  Whatever

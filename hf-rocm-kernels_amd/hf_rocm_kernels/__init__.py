@@ -8,7 +8,10 @@ from .operators.increment import increment
 from .operators.residual_rms import residual_rms, residual_rms_dynamic
 from .operators.swiglu import swiglu, swiglu_dynamic
 from .operators.skinny_gemm import skinny_gemm, skinny_gemm_add, skinny_gemm_rms, skinny_gemm_scaled, skinny_gemm_swiglu
-from .operators.quantize import quantize_fp8
+from .operators.quantize import quantize_fp8, quantize_int8
+from .operators.int8_gemm import int8_gemm
+from .operators.grouped_gemm import grouped_gemm
+from .operators.experts import ExpertRoute, combine_experts, route_experts
 from .operators.rotary import rotary, rotary_frequencies
 from .operators.append_kv import append_kv
 from .operators.tree_attention import tree_attention
@@ -20,4 +23,4 @@ plan_table.load_from_environment()  # HFRK_PLAN_TABLE=<json>: tuned GEMM decompo
 
 __all__ = ["increment", "residual_rms", "swiglu", "skinny_gemm", "skinny_gemm_scaled", "skinny_gemm_add",
            "skinny_gemm_swiglu", "skinny_gemm_rms", "residual_rms_dynamic", "swiglu_dynamic", "quantize_fp8", "rotary",
-           "rotary_frequencies", "append_kv", "tree_attention"]
+           "rotary_frequencies", "append_kv", "tree_attention", "quantize_int8", "int8_gemm", "grouped_gemm", "ExpertRoute", "route_experts", "combine_experts"]

@@ -30,6 +30,8 @@ EXCEEDS_SCRATCH = 14
 F16 = 0
 BF16 = 1
 FP8_E4M3FN = 2
+INT8 = 3
+FP32 = 4
 
 # enum hfrk_epilogue
 EPILOGUE_NONE = 0
@@ -40,6 +42,8 @@ WEIGHT_E4M3FN = 0
 WEIGHT_E4M3FNUZ = 1
 
 GEMM_MAX_M = 64
+MAX_EXPERTS = 512
+MAX_TOP = 32
 SCALES_IN_PACKED_BUFFER = -1  # sb_stride of hfrk_skinny_gemm_packed: use the scales hfrk_pack_weight_scaled stored
 
 
@@ -96,6 +100,18 @@ class AttentionArgs(ctypes.Structure):
                        "cache_dtype")]
 
 
+class GroupedArgs(ctypes.Structure):
+    """struct hfrk_grouped_args"""
+    _fields_ = [*_pointers("a", "rows", "b"), *_strides("expert_stride"), *_pointers("output", "scale_a", "scale_b"), *_strides("scale_b_expert_stride"),
+                *_pointers("offsets"), *_ints("scale_a_stride", "scale_b_stride", "b_stride", "count", "a_rows", "experts", "n", "k", "type", "dtype")]
+
+
+class RouteArgs(ctypes.Structure):
+    """struct hfrk_route_args"""
+    _fields_ = [*_pointers("logits"), *_strides("logits_stride"), *_pointers("bias", "mask", "weights", "experts", "places", "rows", "offsets"),
+                *_ints("tokens", "num_experts", "top", "dtype", "sigmoid", "renormalize"), ("factor", ctypes.c_float)]
+
+
 _i, _p, _f = ctypes.c_int, ctypes.c_void_p, ctypes.c_float
 
 # name -> (restype, argtypes); every symbol the header declares
@@ -143,6 +159,12 @@ SIGNATURES = {
     "hfrk_append_kv": (_i, [ctypes.POINTER(AppendArgs), _p]),
     "hfrk_tree_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
     "hfrk_tree_attention": (_i, [ctypes.POINTER(AttentionArgs), _p, ctypes.c_size_t, _p]),
+    "hfrk_quantize_int8": (_i, [_p, _p, _p, _p, _i, _i, _i, _p]),
+    "hfrk_swiglu_dynamic_int8": (_i, [_p, _p, _p, _i, _i, _i, _p]),
+    "hfrk_int8_gemm": (_i, [_p, _p, _p, _p, _i, _p, _i, _p] + [_i] * 6 + [_p]),
+    "hfrk_grouped_gemm": (_i, [ctypes.POINTER(GroupedArgs), _p]),
+    "hfrk_route_experts": (_i, [ctypes.POINTER(RouteArgs), _p]),
+    "hfrk_combine_experts": (_i, [_p] * 5 + [_i] * 5 + [_p]),
     "hfrk_plan_table_load": (_i, [ctypes.c_char_p, _i, ctypes.POINTER(_i)]),
 }
 

@@ -21,6 +21,7 @@ from ..operators.skinny_gemm.wrapped import scale_vectors, skinny_gemm_checks
 from ..utils.dispatch import runs_now
 from ..utils.fp8 import amax_scale, fp8_quantize
 from ..utils.weight_format import PackedWeight, pack_weight
+from .int8_linear import Int8Linear
 
 Weight = Union[Tensor, PackedWeight]
 _fp8_linear = torch.ops._HFRK_C.fp8_linear.default
@@ -180,11 +181,14 @@ class Fp8Linear(torch.nn.Module):
 
 
 def convert_linear_layers(module: torch.nn.Module, per_channel: bool = True, packed: bool = False,
-                          skip: Sequence[str] = ()) -> int:
-    """Replace, in place and recursively, every nn.Linear under `module` that the FP8 path can take (in_features a
-    multiple of 16 -- of 256 for packed weights -- and at most 32768, 16-bit weight) by an Fp8Linear quantised from it; returns how many were replaced.
+                          skip: Sequence[str] = (), dtype: torch.dtype = torch.float8_e4m3fn) -> int:
+    """Replace, in place and recursively, every nn.Linear under `module` that the 8-bit path can take (in_features a
+    multiple of 16 -- of 256 for packed weights -- and at most 32768, 16-bit weight) by an Fp8Linear (with dtype=torch.int8 an Int8Linear, which has no packed form) quantised from it;
+    returns how many were replaced.
     skip: layers whose dotted name ends with one of these strings stay as they are (e.g. ("lm_head",)).
     The counterpart, without the serving stack, of switching a model's linear method (reference README.md:95-97)."""
+    assert dtype in (torch.float8_e4m3fn, torch.int8), f"Expected {dtype = } to be torch.float8_e4m3fn or torch.int8"
+    assert not packed or dtype == torch.float8_e4m3fn, "packed weights are float8_e4m3fn"
     replaced = 0
 
     def visit(parent: torch.nn.Module, prefix: str) -> None:
@@ -196,7 +200,10 @@ def convert_linear_layers(module: torch.nn.Module, per_channel: bool = True, pac
                 usable = (child.in_features % (256 if packed else 16) == 0 and child.in_features <= 32768
                           and child.weight.dtype in (torch.float16, torch.bfloat16))
                 if usable and not any(full.endswith(suffix) for suffix in skip):
-                    setattr(parent, name, Fp8Linear.from_float(child, per_channel=per_channel, packed=packed))
+                    if dtype == torch.int8:
+                        setattr(parent, name, Int8Linear.from_float(child, per_channel=per_channel))
+                    else:
+                        setattr(parent, name, Fp8Linear.from_float(child, per_channel=per_channel, packed=packed))
                     replaced += 1
             else:
                 visit(child, full)

@@ -9,6 +9,7 @@ from .binding import _swiglu
 
 _swiglu_new = torch.ops._HFRK_C.swiglu_new.default
 _swiglu_dynamic_new = torch.ops._HFRK_C.swiglu_dynamic_new.default
+_swiglu_dynamic_int8_new = torch.ops._HFRK_C.swiglu_dynamic_int8_new.default
 MAX_THREADS_PER_SM = 1024
 _IO_DTYPES = (torch.bfloat16, torch.float16)
 
@@ -90,9 +91,14 @@ def swiglu(
 def swiglu_dynamic(
     gate_up_proj: Tensor,
     next_buffer: Optional[Tensor] = None,
+    dtype: torch.dtype = torch.float8_e4m3fn,
 ) -> Tuple[Tensor, Tensor]:
-    """SwiGLU with per-row dynamic quantisation to float8_e4m3fn (scale = row amax / 448).
-    Returns (output fp8 (rows, cols), scales fp32 (rows,)).  cols % 8 == 0 and cols <= 32768."""
+    """SwiGLU with per-row dynamic quantisation to float8_e4m3fn (scale = row amax / 448) or, with dtype=torch.int8, to int8 (row amax / 127; a row
+    that holds an infinity or a NaN has the scale NaN; no next_buffer).
+    Returns (output (rows, cols), scales fp32 (rows,)).  cols % 8 == 0 and cols <= 32768."""
+    if dtype == torch.int8:
+        return _swiglu_dynamic_int8(gate_up_proj, next_buffer)
+    assert dtype == torch.float8_e4m3fn, f"Expected {dtype = } to be torch.float8_e4m3fn or torch.int8"
     if next_buffer is None and runs_now(gate_up_proj):
         output, scales = _swiglu_dynamic_new(gate_up_proj)
         if output is not None:
@@ -105,4 +111,20 @@ def swiglu_dynamic(
     output = torch.empty(size=(rows, cols), dtype=torch.float8_e4m3fn, device=gate_up_proj.device)
     scales = torch.empty(size=(rows,), dtype=torch.float32, device=gate_up_proj.device)
     torch.ops._HFRK_C.swiglu_dynamic(gate_up_proj, output, scales, next_buffer)
+    return output, scales
+
+
+def _swiglu_dynamic_int8(gate_up_proj: Tensor, next_buffer: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    assert next_buffer is None, "Expected no next_buffer with dtype=torch.int8"
+    if runs_now(gate_up_proj):
+        output, scales = _swiglu_dynamic_int8_new(gate_up_proj)
+        if output is not None:
+            return output, scales
+    next_buffer = torch.empty(size=(gate_up_proj.size(0), 0), device=gate_up_proj.device, dtype=gate_up_proj.dtype)
+    swiglu_checks(gate_up_proj, torch.empty(1, dtype=torch.float32, device=gate_up_proj.device), next_buffer)
+    rows, cols = gate_up_proj.size(0), gate_up_proj.size(1) // 2
+    assert cols % 8 == 0 and 0 < cols <= 32768, f"Expected cols % 8 == 0 and 0 < cols <= 32768: {gate_up_proj.shape = }"
+    output = torch.empty(size=(rows, cols), dtype=torch.int8, device=gate_up_proj.device)
+    scales = torch.empty(size=(rows,), dtype=torch.float32, device=gate_up_proj.device)
+    torch.ops._HFRK_C.swiglu_dynamic_int8(gate_up_proj, output, scales)
     return output, scales

@@ -47,7 +47,7 @@ enum hfrk_status {
 };
 
 /* Element types of 16-bit tensors. */
-enum hfrk_dtype { HFRK_F16 = 0, HFRK_BF16 = 1, HFRK_FP8_E4M3FN = 2 };
+enum hfrk_dtype { HFRK_F16 = 0, HFRK_BF16 = 1, HFRK_FP8_E4M3FN = 2, HFRK_INT8 = 3, HFRK_FP32 = 4 };
 
 /* What happens to the product before it is stored (hfrk_skinny_gemm_fused). */
 enum hfrk_epilogue { HFRK_EPILOGUE_NONE = 0, HFRK_EPILOGUE_SWIGLU = 1 };
@@ -473,6 +473,85 @@ typedef struct hfrk_attention_args {
 
 size_t hfrk_tree_attention_workspace_bytes(const hfrk_attention_args* args);
 int hfrk_tree_attention(const hfrk_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- 8-bit integers ---------------------------------------------------------------------------------------------------------------------
+ * The quantisers above with int8 codes: scales[r] = max(amax_c |y[r,c]| / 127, FLT_MIN), output = rint(y / scale), ties to even, +-127 at most.
+ * A row that holds an infinity or a NaN gets the scale NaN (its codes mean nothing), so that a product's row is NaN too.  With a static scale, results
+ * saturate and a NaN becomes -127.  Same limits: cols % 8 == 0, cols <= 32768, 16-byte aligned input, 8-byte aligned output. */
+int hfrk_quantize_int8(const void* input, const float* static_scale, void* output, float* scales, int rows, int cols, int io_dtype, void* stream);
+int hfrk_swiglu_dynamic_int8(const void* gate_up, void* output, float* scales, int rows, int cols, int io_dtype, void* stream);
+
+/* D[m,n] = (base ? base[m,n] : 0) + sa[m] * sb[n] * sum_k A[m,k] * W[n,k], int8 codes summed exactly in int32, the rest in fp32, one rounding to 16 bits.
+ *   A [m,k] int8, rows of k bytes;  B [n,k] int8, rows b_stride bytes apart;  D [m,n] of d_dtype
+ *   base of d_dtype, rows base_stride elements apart (0: one row for all, a bias), or NULL
+ *   scale_a fp32 [m] (sa_stride 1) or one (0); scale_b [n] (1), one (0) or NULL: 1
+ * Any number of rows.  k a multiple of 16 up to 131056, n up to 2^21, b_stride a multiple of 16 up to 2^21, A and B on 16-byte boundaries.  No workspace. */
+int hfrk_int8_gemm(const void* A, const void* B, void* D, const void* base, int base_stride, const float* scale_a, int sa_stride, const float* scale_b,
+                   int sb_stride, int m, int n, int k, int b_stride, int d_dtype, void* stream);
+
+/* ---- an MLP of experts ------------------------------------------------------------------------------------------------------------------
+ * Products of rows grouped by expert:
+ *   output[i, c] = scale_a[r] * scale_b[e, c] * sum_k a[r, k] * b[e, c, k]      for offsets[e] <= i < offsets[e + 1],  r = rows ? rows[i] : i
+ *   a        [a_rows, k] codes of `type`: HFRK_FP8_E4M3FN (sums in fp32) or HFRK_INT8 (sums in int32)
+ *   rows     [count] int32 or NULL.  A number that is no row of a gives a row of zeros
+ *   b        [experts, n, k] codes, experts expert_stride bytes apart, rows b_stride bytes
+ *   scale_a  fp32 [a_rows] (stride 1) or one (0);  scale_b fp32, element (e, c) at e * scale_b_expert_stride + c * scale_b_stride (stride 1, or 0: one an
+ *            expert), or NULL: 1
+ *   offsets  [experts + 1] int32, not decreasing, read on the device (a captured call may be replayed with others).  Rows behind offsets[experts], and
+ *            those in front of offsets[0], are left as they are; offsets are cut to 0 .. count
+ *   output   [count, n] of dtype (16-bit); shares no memory with the rest
+ * experts <= 512; k, n, strides as in hfrk_int8_gemm (fp8: k up to 2^21); with rows, a_rows * k below 2^31 - 2^22; count up to a_rows without.  No workspace. */
+typedef struct hfrk_grouped_args {
+    const void* a;
+    const int32_t* rows;
+    const void* b;
+    int64_t expert_stride;
+    void* output;
+    const float* scale_a;
+    const float* scale_b;
+    int64_t scale_b_expert_stride;
+    const int32_t* offsets;
+    int scale_a_stride, scale_b_stride, b_stride;
+    int count, a_rows, experts, n, k, type, dtype;
+} hfrk_grouped_args;
+
+int hfrk_grouped_gemm(const hfrk_grouped_args* args, void* stream);
+
+/* Which experts the tokens go to, and the tokens in the experts' order.
+ *   logits   [tokens, num_experts] of dtype (HFRK_F16, HFRK_BF16 or HFRK_FP32), rows logits_stride elements apart
+ *   s        softmax of a row (sigmoid != 0: of each value 1 / (1 + e^-x)), fp32
+ *   experts  [tokens, top] int32: the choices, largest logit first or, with bias (fp32 [num_experts]), largest s + bias (made and compared in 64 bits); of
+ *            equals the lowest index first.  An expert whose logit (or s + bias) is minus infinity or NaN is never chosen: -1 where none is left
+ *   weights  [tokens, top] fp32: factor * s of the choice, with renormalize divided by the sum of the row's choices (where that is not 0); 0 for -1.  A
+ *            NaN among a row's logits makes its weights NaN
+ *   mask     [tokens] bytes or NULL: a token whose byte is 0 is padding: experts -1, weights 0
+ *   offsets  [num_experts + 1] int32: expert e has the pairs offsets[e] .. offsets[e+1]; offsets[0] = 0
+ *   rows     [tokens * top] int32: the token of each pair, in the experts' order and within an expert in the tokens'; -1 behind the last pair
+ *   places   [tokens, top] int32: where each pair is in that order, -1 for those of no expert
+ * num_experts <= 512, top <= HFRK_MAX_TOP and num_experts, tokens <= 2^24, tokens * top <= 2^28.  Results share no memory with each other or the rest.  No workspace, no
+ * atomics: equal calls give equal bits. */
+#define HFRK_MAX_TOP 32
+typedef struct hfrk_route_args {
+    const void* logits;
+    int64_t logits_stride;
+    const float* bias;
+    const void* mask;
+    float* weights;
+    int32_t* experts;
+    int32_t* places;
+    int32_t* rows;
+    int32_t* offsets;
+    int tokens, num_experts, top, dtype, sigmoid, renormalize;
+    float factor;
+} hfrk_route_args;
+
+int hfrk_route_experts(const hfrk_route_args* args, void* stream);
+
+/* output[t] = (base ? base[t] : 0) + sum_j weights[t, j] * y[places[t, j]], fp32, one rounding.
+ *   y [y_rows, cols], base [tokens, cols] or NULL, output [tokens, cols] of dtype (16-bit), rows side by side; weights [tokens, top] fp32, places [tokens, top]
+ *   int32: a number that is no row of y counts as a row of zeros.  output may be base and shares no other memory.  top <= HFRK_MAX_TOP, cols <= 2^21, tokens < 2^24. */
+int hfrk_combine_experts(const void* y, const float* weights, const int32_t* places, const void* base, void* output, int tokens, int top, int cols, int y_rows,
+                         int dtype, void* stream);
 
 #ifdef __cplusplus
 }
