@@ -1,10 +1,11 @@
 // Products of rows grouped by expert, and of 8-bit integers: launch arguments, and how a workgroup finds its group.
 #pragma once
 
-#include "skinny_gemm_args.h"
+#include "tiled_gemm.h"
 
 namespace hfrk {
 
+// What the groups are: the same fields for the rows kernel and the tiled one.
 struct GroupedArgs {
     const uint8_t* A;
     const uint8_t* B;
@@ -22,6 +23,13 @@ struct GroupedArgs {
     int d_dtype;
     int vec;                 // rows of D and base take whole 8-byte pieces
     int tiles_n;
+};
+
+struct TiledGroupedArgs : TiledGemmArgs {
+    const int32_t* offsets;
+    const int32_t* rows;
+    int64_t expert_stride, sb_expert_stride;
+    int count, a_rows, experts;
 };
 
 constexpr int kMaxExperts = 512;
@@ -53,8 +61,8 @@ __device__ __forceinline__ int xcd_range_id(int block, int total) {
 // device only, so a launch has a workgroup for every tile there can be (grouped_tiles_bound) and those behind the last one find none.  Each
 // wave looks for itself, a lane at up to EPL experts.  Offsets that do not increase, or pass the rows, cannot lead outside: each is cut to 0 .. count, and a tile is one of a
 // group's own or none.
-template <int EPL>
-__device__ __forceinline__ bool find_tile_of(const GroupedArgs& a, int bm, GroupTile* t) {
+template <int EPL, typename Args>
+__device__ __forceinline__ bool find_tile_of(const Args& a, int bm, GroupTile* t) {
     const int lane = threadIdx.x & 63;
     int edge[EPL + 1], tiles[EPL];
 #pragma unroll
@@ -95,7 +103,8 @@ __device__ __forceinline__ bool find_tile_of(const GroupedArgs& a, int bm, Group
     return found;
 }
 
-__device__ __forceinline__ bool find_tile(const GroupedArgs& a, int bm, GroupTile* t) {
+template <typename Args>
+__device__ __forceinline__ bool find_tile(const Args& a, int bm, GroupTile* t) {
     if (!a.offsets) {
         t->expert = 0;
         t->first = 0;
@@ -109,5 +118,10 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs& a, int bm, GroupTil
 
 // The most tiles of `bm` rows that groups of `count` rows together can have: every group's last one may be partly filled.
 inline long grouped_tiles_bound(int count, int experts, int bm) { return (long)count / bm + (experts < count ? experts : count); }
+
+// tiled_grouped_fp8.hip, tiled_grouped_int8.hip, tiled_int8.hip: the tiled kernel on groups and on one int8 weight.
+int launch_tiled_grouped_fp8(const TiledGroupedArgs& args, int shape, long grid, hipStream_t stream);
+int launch_tiled_grouped_int8(const TiledGroupedArgs& args, int shape, long grid, hipStream_t stream);
+int launch_tiled_int8(const TiledGemmArgs& args, int shape, hipStream_t stream);
 
 }  // namespace hfrk

@@ -3,16 +3,18 @@
 // codes of float8_e4m3fn (sums in fp32) or int8 (sums in int32: exact up to k = 131071, then one conversion), scales applied to the whole sum, one
 // rounding to 16 bits.  No counterpart in the reference, whose GEMM has one fp8 weight.
 //
-// grouped_rows_kernel: a workgroup takes 16 MT rows of a group by 16 RT columns, and its eight waves take the 128-byte chunks of k in turn, so that at
-// any time the workgroup reads a run of 1 KB of each weight row.  Operands go from memory to registers (lane l of a 16 x 16 tile holds pieces l / 16 and
-// l / 16 + 4 of row l % 16: which bytes of k a lane has does not matter as long as both operands agree); the waves' sums meet in LDS, in wave order.
+// grouped_rows_kernel: a workgroup takes 16 MT rows of a group; each of its waves takes 16 RT columns and every KW-th 128-byte chunk of k, so that KW waves
+// read a run of KW * 128 bytes of each weight row at a time.  Operands go from memory to registers (lane l of a 16 x 16 tile holds pieces l / 16 and
+// l / 16 + 4 of row l % 16: which bytes of k a lane has does not matter as long as both operands agree), one tile's chunk ahead of the one that is
+// multiplied; the sums of the waves along k meet in LDS, in wave order.  Bound by memory: 5.8 TB/s on 940 MB of weights.  More rows a group go to the tiled
+// kernel (tiled_gemm_kernel.h).
 #include <limits.h>
+#include <math.h>
 
 #include "grouped_gemm.h"
 
 namespace hfrk {
 
-constexpr int kRowsWaves = 8;
 constexpr int kRowsChunk = 128;  // bytes of k that a wave takes at a time
 
 template <int DT>
@@ -20,23 +22,28 @@ __device__ __forceinline__ uint32_t two_to_16bit(float lo, float hi) {
     return (uint32_t)store16<DT>(lo) | (uint32_t)store16<DT>(hi) << 16;
 }
 
-template <bool INT8, int MT, int RT>
-__global__ void __launch_bounds__(64 * kRowsWaves) grouped_rows_kernel(const GroupedArgs a) {
-    constexpr int U = MT * RT >= 4 ? 2 : 4;  // chunks requested together
-    static_assert(MT * RT <= kRowsWaves, "the epilogue has a thread for every four values");
-    __shared__ v4i sums[kRowsWaves][MT * RT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// KW waves split k, CW of them the columns.
+template <bool INT8, int MT, int RT, int KW, int CW>
+__global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_rows_kernel(const GroupedArgs a) {
+    constexpr int WAVES = KW * CW, TILES = CW * MT * RT;  // matrix tiles of 16 x 16 of the workgroup
+    constexpr int EACH = (TILES + WAVES - 1) / WAVES;     // tiles whose sums a wave finishes
+    constexpr int BM = 16 * MT, BN = 16 * RT * CW;
+    __shared__ v4i sums[KW][TILES][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = wave % KW, cw = wave / KW;
 
     GroupTile t;
-    if (!find_tile(a, 16 * MT, &t)) return;
-    const int m0 = t.tile % t.tiles_m * 16 * MT, n0 = t.tile / t.tiles_m * 16 * RT;
-    const int row0 = t.first + m0, rows = min(16 * MT, t.rows - m0), cols = min(16 * RT, a.n - n0);
+    if (!find_tile(a, BM, &t)) return;
+    const int m0 = t.tile % t.tiles_m * BM, n0 = t.tile / t.tiles_m * BN;
+    const int row0 = t.first + m0, rows = min(BM, t.rows - m0), cols = min(BN, a.n - n0);
 
-    // which row of A a row of the tile is; rows that are none read as zero
-    auto row_of_a = [&](int r) __attribute__((always_inline)) {
-        const int i = r < rows ? (a.rows ? a.rows[row0 + r] : row0 + r) : -1;
-        return (uint32_t)i < (uint32_t)a.a_rows ? i : -1;
-    };
+    // Which row of A a row of the tile is, -1: none.  The numbers come through a buffer over the tile's own, so that none is read behind them.
+    const __amdgpu_buffer_rsrc_t rnumbers = make_rsrc(a.rows + row0, a.rows ? (uint32_t)rows * 4u : 0u);
+    auto number_of = [&](int r) __attribute__((always_inline)) { return a.rows ? __builtin_amdgcn_raw_buffer_load_b32(rnumbers, r * 4, 0, 0) : row0 + r; };
+    auto row_of = [&](int r, int number) __attribute__((always_inline)) { return r < rows && (uint32_t)number < (uint32_t)a.a_rows ? number : -1; };
+    int number[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) number[i] = number_of(i * 16 + (lane & 15));
+
     // gathered rows lie anywhere in A (below 2 GB); others behind the tile's first
     const long a_from = a.rows ? 0 : row0;
     const __amdgpu_buffer_rsrc_t ra = make_rsrc(a.A + a_from * a.k, (uint32_t)((a.rows ? a.a_rows : rows) * (long)a.k));
@@ -45,120 +52,259 @@ __global__ void __launch_bounds__(64 * kRowsWaves) grouped_rows_kernel(const Gro
     const int piece = (lane >> 4) * 16;
     uint32_t va[MT], vb[RT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int r = row_of_a(i * 16 + (lane & 15));
-        va[i] = r >= 0 ? (uint32_t)((r - a_from) * a.k + piece) : (uint32_t)kOutsideBuffer;
-    }
-#pragma unroll
-    for (int j = 0; j < RT; ++j) vb[j] = (uint32_t)(j * 16 + (lane & 15)) * (uint32_t)a.b_stride + piece;
+    for (int j = 0; j < RT; ++j) vb[j] = (uint32_t)((cw * RT + j) * 16 + (lane & 15)) * (uint32_t)a.b_stride + piece;
 
-    // what the epilogue needs of this thread's four values, requested ahead
-    const int e_tile = threadIdx.x >> 6, e_m = e_tile / RT * 16 + (lane & 15), e_n = e_tile % RT * 16 + (lane >> 4) * 4;
-    const bool writes = e_tile < MT * RT && e_m < rows && e_n < cols;
-    float sa = 0.f, sb[4];
-    if (writes) {
-        const int r = row_of_a(e_m);
-        sa = r >= 0 ? a.scale_a[(long)r * a.sa_stride] : 0.f;
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-            sb[v] = a.scale_b ? a.scale_b[t.expert * a.sb_expert_stride + (long)min(n0 + e_n + v, a.n - 1) * a.sb_stride] : 1.0f;
-    }
-
-    typedef int acc_i __attribute__((ext_vector_type(4)));
     typedef float acc_f __attribute__((ext_vector_type(4)));
-    using Acc = std::conditional_t<INT8, acc_i, acc_f>;
+    using Acc = std::conditional_t<INT8, v4i, acc_f>;
     Acc acc[MT][RT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < RT; ++j) acc[i][j] = Acc{0, 0, 0, 0};
 
-    const int chunks = (a.k + kRowsChunk - 1) / kRowsChunk;
-#pragma unroll 1
-    for (int c = wave; c < chunks; c += kRowsWaves * U) {
-        v4i fa[U][MT][2], fb[U][RT][2];
+    // registers of the tile that is multiplied and of the next one: a tile's own, or with one tile those of every other chunk
+    v4i fa[2][MT][2], fb[RT == 1 ? 2 : RT][2];
+    auto get_b = [&](int set, int j, int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kb = (c + u * kRowsWaves) * kRowsChunk;
+        for (int h = 0; h < 2; ++h) {
+            const int by = c * kRowsChunk + h * 64;
+            fb[RT == 1 ? set : j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, by + piece < a.k ? vb[j] + (uint32_t)by : (uint32_t)kOutsideBuffer, 0, 0);
+        }
+    };
+    auto get_a = [&](int set, int c) __attribute__((always_inline)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bool inside = kb + h * 64 + piece < a.k;
-                const uint32_t by = (uint32_t)(kb + h * 64);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < RT; ++j) fb[u][j][h] = __builtin_amdgcn_raw_buffer_load_b128(rb, inside ? vb[j] + by : (uint32_t)kOutsideBuffer, 0, 0);
+            for (int i = 0; i < MT; ++i) {
+                const int by = c * kRowsChunk + h * 64;
+                fa[set][i][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, by + piece < a.k ? va[i] + (uint32_t)by : (uint32_t)kOutsideBuffer, 0, 0);
+            }
+    };
+    auto multiply = [&](int set, int j) __attribute__((always_inline)) {
+        const v4i(&b)[2] = fb[RT == 1 ? set : j];
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fa[u][i][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, inside ? va[i] + by : (uint32_t)kOutsideBuffer, 0, 0);
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (INT8) {
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[0], fa[set][i][0], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[1], fa[set][i][1], acc[i][j], 0, 0, 0);
+            } else {
+                auto join = [](v4i lo, v4i hi) __attribute__((always_inline)) { return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}; };
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(b[0], b[1]), join(fa[set][i][0], fa[set][i][1]), acc[i][j], 0, 0, 0, 0, 0, 0);
             }
         }
+    };
+
+    // The weight is requested in front of the rows, whose numbers are still on their way.
+    const int chunks = (a.k + kRowsChunk - 1) / kRowsChunk;
+    get_b(0, 0, kw);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+    for (int i = 0; i < MT; ++i) {
+        const int r = row_of(i * 16 + (lane & 15), number[i]);
+        va[i] = r >= 0 ? (uint32_t)((r - a_from) * a.k + piece) : (uint32_t)kOutsideBuffer;
+    }
+    get_a(0, kw);
+    for (int c = kw; c < chunks; c += 2 * KW) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+        for (int half = 0; half < 2; ++half) {
+            get_a(half ^ 1, c + (half + 1) * KW);
 #pragma unroll
-                for (int j = 0; j < RT; ++j) {
-                    if constexpr (INT8) {
-                        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u][j][0], fa[u][i][0], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[u][j][1], fa[u][i][1], acc[i][j], 0, 0, 0);
-                    } else {
-                        auto join = [](v4i lo, v4i hi) __attribute__((always_inline)) { return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}; };
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(fb[u][j][0], fb[u][j][1]), join(fa[u][i][0], fa[u][i][1]),
-                                                                                      acc[i][j], 0, 0, 0, 0, 0, 0);
-                    }
-                }
+            for (int j = 0; j < RT; ++j) {
+                get_b((half + (j + 1) / RT) & 1, (j + 1) % RT, c + (half + (j + 1) / RT) * KW);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(half, j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < RT; ++j) sums[wave][i * RT + j][lane] = __builtin_bit_cast(v4i, acc[i][j]);
+        for (int j = 0; j < RT; ++j) sums[kw][cw * MT * RT + i * RT + j][lane] = __builtin_bit_cast(v4i, acc[i][j]);
+    // what the epilogue needs of this thread's values: tile e of the workgroup is wave e / (MT RT)'s tile e % (MT RT)
+    int e_m[EACH], e_n[EACH];
+    float sa[EACH], sb[EACH][4];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int tile = wave + e * WAVES, of = tile % (MT * RT);
+        e_m[e] = of / RT * 16 + (lane & 15);
+        e_n[e] = (tile / (MT * RT) * RT + of % RT) * 16 + (lane >> 4) * 4;
+        const int r = row_of(e_m[e], number_of(e_m[e]));
+        sa[e] = r >= 0 ? a.scale_a[(long)r * a.sa_stride] : 0.f;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            sb[e][v] = a.scale_b ? a.scale_b[t.expert * a.sb_expert_stride + (long)min(n0 + e_n[e] + v, a.n - 1) * a.sb_stride] : 1.0f;
+    }
     __syncthreads();
-    if (!writes) return;
-    Acc total = Acc{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < kRowsWaves; ++w) total += __builtin_bit_cast(Acc, sums[w][e_tile][lane]);
-
-    const long at = (long)(row0 + e_m) * a.n + n0 + e_n, base_at = (long)(row0 + e_m) * a.base_stride + n0 + e_n;
-    uint16_t* const d = static_cast<uint16_t*>(a.D) + at;
-    const uint16_t* const base = a.base ? static_cast<const uint16_t*>(a.base) + base_at : nullptr;
-    auto finish = [&](auto dt) __attribute__((always_inline)) {
-        constexpr int DT = decltype(dt)::value;
-        float x[4];
+    for (int e = 0; e < EACH; ++e) {
+        const int tile = wave + e * WAVES;
+        if (tile >= TILES || e_m[e] >= rows || e_n[e] >= cols) continue;
+        Acc total = Acc{0, 0, 0, 0};
 #pragma unroll
-        for (int v = 0; v < 4; ++v) x[v] = (float)total[v] * (sa * sb[v]);
-        if (a.vec) {
-            if (base) {
-                const uint2 b = *reinterpret_cast<const uint2*>(base);
-                x[0] += load16<DT>((uint16_t)(b.x & 0xffff));
-                x[1] += load16<DT>((uint16_t)(b.x >> 16));
-                x[2] += load16<DT>((uint16_t)(b.y & 0xffff));
-                x[3] += load16<DT>((uint16_t)(b.y >> 16));
+        for (int w = 0; w < KW; ++w) total += __builtin_bit_cast(Acc, sums[w][tile][lane]);
+        const long at = (long)(row0 + e_m[e]) * a.n + n0 + e_n[e], base_at = (long)(row0 + e_m[e]) * a.base_stride + n0 + e_n[e];
+        uint16_t* const d = static_cast<uint16_t*>(a.D) + at;
+        const uint16_t* const base = a.base ? static_cast<const uint16_t*>(a.base) + base_at : nullptr;
+        auto finish = [&](auto dt) __attribute__((always_inline)) {
+            constexpr int DT = decltype(dt)::value;
+            float x[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) x[v] = (float)total[v] * (sa[e] * sb[e][v]);
+            if (a.vec) {
+                if (base) {
+                    const uint2 b = *reinterpret_cast<const uint2*>(base);
+                    x[0] += load16<DT>((uint16_t)(b.x & 0xffff));
+                    x[1] += load16<DT>((uint16_t)(b.x >> 16));
+                    x[2] += load16<DT>((uint16_t)(b.y & 0xffff));
+                    x[3] += load16<DT>((uint16_t)(b.y >> 16));
+                }
+                *reinterpret_cast<uint2*>(d) = make_uint2(two_to_16bit<DT>(x[0], x[1]), two_to_16bit<DT>(x[2], x[3]));
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if (e_n[e] + v < cols) d[v] = store16<DT>(x[v] + (base ? load16<DT>(base[v]) : 0.f));
             }
-            *reinterpret_cast<uint2*>(d) = make_uint2(two_to_16bit<DT>(x[0], x[1]), two_to_16bit<DT>(x[2], x[3]));
-        } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-                if (n0 + e_n + v < a.n) d[v] = store16<DT>(x[v] + (base ? load16<DT>(base[v]) : 0.f));
-        }
-    };
-    if (a.d_dtype == HFRK_BF16) finish(std::integral_constant<int, HFRK_BF16>{});
-    else finish(std::integral_constant<int, HFRK_F16>{});
+        };
+        if (a.d_dtype == HFRK_BF16) finish(std::integral_constant<int, HFRK_BF16>{});
+        else finish(std::integral_constant<int, HFRK_F16>{});
+    }
 }
 
-template <bool INT8, int MT, int RT>
+template <bool INT8, int MT, int RT, int KW, int CW>
 static int launch_rows(GroupedArgs a, hipStream_t stream) {
-    a.tiles_n = (a.n + 16 * RT - 1) / (16 * RT);
+    constexpr int BN = 16 * RT * CW, THREADS = 64 * KW * CW;
+    a.tiles_n = (a.n + BN - 1) / BN;
     const long tiles = (a.offsets ? grouped_tiles_bound(a.count, a.experts, 16 * MT) : ((long)a.count + 16 * MT - 1) / (16 * MT)) * a.tiles_n;
-    if (tiles * 64 * kRowsWaves > (long)UINT_MAX) return HFRK_BAD_SHAPE;
-    hipLaunchKernelGGL((grouped_rows_kernel<INT8, MT, RT>), dim3((unsigned)tiles), dim3(64 * kRowsWaves), 0, stream, a);
+    if (tiles * THREADS > (long)UINT_MAX) return HFRK_BAD_SHAPE;
+    hipLaunchKernelGGL((grouped_rows_kernel<INT8, MT, RT, KW, CW>), dim3((unsigned)tiles), dim3(THREADS), 0, stream, a);
     HFRK_HIP_TRY(hipGetLastError());
     return HFRK_SUCCESS;
 }
 
+// Which rows kernel: `groups` of rows, each a tile high.  With enough workgroups, 64 columns in four tiles a wave, eight waves along k; a wave asks for one
+// tile's chunk at a time, and it is the six waves of a SIMD that keep memory busy: with all four tiles' chunks requested together and two sets of registers 100
+// tokens on 6 of 160 experts of 3008 x 5120 take 471 us instead of 376 (5.9 TB/s), 32 on 2 of 8 of 28672 x 4096 177 and 164.  With few workgroups, one
+// tile of 16 columns a wave spreads them (one token on 2 of 8 experts of 28672 x 4096 38.2 -> 32.0 us, on 6 of 64 of 2816 x 2048 12.0 -> 9.0, 8 tokens on 2 of 8 of
+// 4096 x 14336 74 -> 62), as long as a workgroup's 16 k bytes outweigh its start and end (4 tokens on 8 of 128 of 1536 x 2048: 17.0 us with 64 columns, 19.6 with
+// 16).  A k of up to eight chunks gives eight waves one each: four waves take it then, and the others other columns (4 tokens on 8 of 128 of 2048 x 768 15.3 ->
+// 12.0, one token 7.1 -> 5.8); a long one on a few workgroups is read by sixteen waves (1 x 10000 x 5136 int8 13.0 -> 11.9, 1 x 4096 x 14336 13.3 -> 12.3).
 template <bool INT8>
-static int launch_grouped(const GroupedArgs& a, hipStream_t stream) {
-    return launch_rows<INT8, 1, 2>(a, stream);
+static int launch_few_rows(const GroupedArgs& a, int groups, hipStream_t stream) {
+    const long tiles64 = (long)groups * ((a.n + 63) / 64), tiles16 = (long)groups * ((a.n + 15) / 16);
+    const bool spread = tiles64 <= 512 || (tiles64 <= 1024 && a.k >= 4096);
+    if (a.k <= 1024) return spread ? launch_rows<INT8, 1, 1, 4, 2>(a, stream) : launch_rows<INT8, 1, 4, 4, 2>(a, stream);
+    if (!spread) return launch_rows<INT8, 1, 4, 8, 1>(a, stream);
+    return a.k >= 5120 && tiles16 <= 1024 ? launch_rows<INT8, 1, 1, 16, 1>(a, stream) : launch_rows<INT8, 1, 1, 8, 1>(a, stream);
 }
 
-static int grouped_run(GroupedArgs& a, int type, hipStream_t stream) {
+// The tile shape with the smallest predicted time, in us: rounds of workgroups, each a start and end and k's stages, or the weights' way from memory.  Group sizes
+// are not known here: groups of the mean size are assumed, of whose rows of tiles half a one more is partly filled.  Constants fitted to 38 sizes (16 to 2048
+// rows a group, k 256 to 14336): the choice is 0.8 % slower than the best shape in the mean, 22 % on the worst (512 tokens, 2 of 8, 4096 x 14336 of very uneven
+// popularity: whether a group passes 256 rows decides there).
+static int grouped_shape(const GroupedArgs& a, int groups) {
+    struct Shape { float fixed, stage, pair_fixed, pair_stage; };  // pair: two workgroups on a compute unit against one
+    static constexpr Shape kShape[kGroupedShapeCount] = {{11.2f, 1.26f, 1, 1}, {10.0f, .625f, 1, 1}, {4.87f, .478f, 1, 1}, {2.78f, .393f, 1.26f, 1.74f}, {4.14f, .465f, 1.32f, 2.27f}};
+    constexpr int kOrder[kGroupedShapeCount] = {2, 4, 0, 1, 3};  // (of equals the first)
+    const float mean = (float)a.count / groups, stages = (float)((a.k + kTiledStage - 1) / kTiledStage);
+    const float stream = (float)groups * a.n * a.k / 6.0e6f + 3.f;
+    int best = 2;
+    float least = INFINITY;
+    for (int shape : kOrder) {
+        const TiledShape& s = kGroupedShapes[shape];
+        const float tiles = groups * fmaxf(1.f, mean / s.bm + .5f) * ((a.n + s.bn - 1) / s.bn), slots = (float)(kNumCU * s.per_cu);
+        auto round_us = [&](float count) {
+            const bool pair = count > kNumCU;
+            return count <= 0 ? 0.f : kShape[shape].fixed * (pair ? kShape[shape].pair_fixed : 1.f) + stages * kShape[shape].stage * (pair ? kShape[shape].pair_stage : 1.f);
+        };
+        const float rounds = floorf(tiles / slots), t = fmaxf(rounds * round_us(slots) + round_us(tiles - rounds * slots), stream);
+        if (t < least) {
+            least = t;
+            best = shape;
+        }
+    }
+    return best;
+}
+
+// The tiled kernel on groups.
+static int launch_grouped_tiles(const GroupedArgs& a, bool int8, int groups, hipStream_t stream) {
+    const int shape = grouped_shape(a, groups);
+    const TiledShape& s = kGroupedShapes[shape];
+    const long grid = grouped_tiles_bound(a.count, a.experts, s.bm) * ((a.n + s.bn - 1) / s.bn);
+    if (grid * s.threads > (long)UINT_MAX) return HFRK_BAD_SHAPE;
+    TiledGroupedArgs t{};
+    t.A = a.A;
+    t.B = a.B;
+    t.D = a.D;
+    t.scale_a = a.scale_a;
+    t.scale_b = a.scale_b;
+    t.sa_stride = a.sa_stride;
+    t.sb_stride = a.sb_stride;
+    t.m = a.count;
+    t.n = a.n;
+    t.k = a.k;
+    t.b_stride = a.b_stride;
+    t.d_dtype = a.d_dtype;
+    t.vec = a.n % 8 == 0 && (reinterpret_cast<uintptr_t>(a.D) & 15) == 0;
+    t.tiles_m = ((a.count - 1) / groups + s.bm) / s.bm;  // of a group of the mean size: what the walk of the tiles and of k goes by
+    t.tiles_n = (a.n + s.bn - 1) / s.bn;
+    const int square = s.bm == s.bn ? 6 : 4;
+    t.group_m = t.tiles_m < square ? t.tiles_m : square;
+    t.splits = 1;
+    t.stages_q = (a.k + kTiledStage - 1) / kTiledStage;
+    turn_k(&t, s, false);
+    t.offsets = a.offsets;
+    t.rows = a.rows;
+    t.expert_stride = a.expert_stride;
+    t.sb_expert_stride = a.sb_expert_stride;
+    t.count = a.count;
+    t.a_rows = a.a_rows;
+    t.experts = a.experts;
+    return int8 ? launch_tiled_grouped_int8(t, shape, grid, stream) : launch_tiled_grouped_fp8(t, shape, grid, stream);
+}
+
+// Up to ten rows a group go to the rows kernel: its workgroup streams a weight for 16 rows at most (64 tokens on 2 of
+// 8 experts of 28672 x 4096, 16 rows each: 213 us, tiles 182; 8 rows each 164 and 180; 128 on 6 of 64 of 2816 x 2048, 12 each, 76.9 and 75.3).
+constexpr int kFewRowsPerGroup = 10;
+
+template <bool INT8>
+static int launch_grouped(const GroupedArgs& a, hipStream_t stream) {
+    const int groups = a.experts < a.count ? a.experts : a.count;
+    return a.count / groups <= kFewRowsPerGroup ? launch_few_rows<INT8>(a, groups, stream) : launch_grouped_tiles(a, INT8, groups, stream);
+}
+
+// One int8 weight: up to 16 rows the rows kernel, more the tiled one, k in parts where that is worth clearing their counters (a launch of 2 us) and the caller gave
+// memory for them.
+constexpr int kDenseFewRows = 16;
+
+static hfrk_tiled_plan int8_plan(int m, int n, int k, bool split) {
+    hfrk_tiled_plan whole, parts;
+    const float t = make_tiled_plan(m, n, k, 1, &whole);
+    return split && make_tiled_plan(m, n, k, kTiledMaxSplits, &parts) + 2.f < t ? parts : whole;
+}
+
+static size_t int8_workspace_bytes(const hfrk_tiled_plan& p, int m, int n) { return tiled_plan_ws_bytes(p, m, n) + (size_t)tiled_plan_counters(p, m, n) * sizeof(int); }
+
+__global__ void __launch_bounds__(256) clear_counters_kernel(int* counters, int count) {
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) counters[i] = 0;
+}
+
+static int launch_int8(const GroupedArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (a.count <= kDenseFewRows) return launch_few_rows<true>(a, 1, stream);
+    if (!tiled_size_ok(a.count, a.n, a.k)) return HFRK_BAD_SHAPE;
+    hfrk_tiled_plan p = int8_plan(a.count, a.n, a.k, workspace != nullptr);
+    if (int8_workspace_bytes(p, a.count, a.n) > workspace_bytes) p = int8_plan(a.count, a.n, a.k, false);
+    const size_t partials = tiled_plan_ws_bytes(p, a.count, a.n);
+    int* const counters = p.splits > 1 ? reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + partials) : nullptr;
+    if (counters) {
+        const int count = (int)tiled_plan_counters(p, a.count, a.n);
+        hipLaunchKernelGGL(clear_counters_kernel, dim3(count > 2048 ? 8 : 1), dim3(256), 0, stream, counters, count);
+        HFRK_HIP_TRY(hipGetLastError());
+    }
+    return tiled_launch(a.A, a.B, false, a.D, a.base, a.base_stride, a.scale_a, a.sa_stride, a.scale_b, a.sb_stride, a.count, a.n, a.k, a.b_stride, a.d_dtype, p,
+                        static_cast<float*>(workspace), partials, counters, stream, true);
+}
+
+static int grouped_run(GroupedArgs& a, int type, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     // offsets inside a tile's buffers stay below 2^31, and the largest int8 product, 2^14 k, below it too
     constexpr int kMost = 1 << 21;
     if (a.count < 0 || a.a_rows < 0 || a.experts < 1 || a.experts > kMaxExperts || a.n < 1 || a.n > kMost || a.k < 1 || a.k > kMost) return HFRK_BAD_SHAPE;
@@ -179,6 +325,7 @@ static int grouped_run(GroupedArgs& a, int type, hipStream_t stream) {
         return HFRK_BAD_ALIGNMENT;
     if (!a.base) a.base_stride = 0;
     a.vec = a.n % 4 == 0 && a.base_stride % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.D) | reinterpret_cast<uintptr_t>(a.base)) & 7) == 0;
+    if (!a.offsets) return launch_int8(a, workspace, workspace_bytes, stream);
     return type == HFRK_INT8 ? launch_grouped<true>(a, stream) : launch_grouped<false>(a, stream);
 }
 
@@ -207,11 +354,18 @@ int hfrk_grouped_gemm(const hfrk_grouped_args* args, void* stream) {
     a.n = args->n;
     a.k = args->k;
     a.d_dtype = args->dtype;
-    return hfrk::grouped_run(a, args->type, static_cast<hipStream_t>(stream));
+    return hfrk::grouped_run(a, args->type, nullptr, 0, static_cast<hipStream_t>(stream));
+}
+
+size_t hfrk_int8_gemm_workspace_bytes(int m, int n, int k) {
+    using namespace hfrk;
+    if (m <= kDenseFewRows || !tiled_size_ok(m, n, k)) return 0;
+    return int8_workspace_bytes(int8_plan(m, n, k, true), m, n);
 }
 
 int hfrk_int8_gemm(const void* A, const void* B, void* D, const void* base, int base_stride, const float* scale_a, int sa_stride, const float* scale_b,
-                   int sb_stride, int m, int n, int k, int b_stride, int d_dtype, void* stream) {
+                   int sb_stride, int m, int n, int k, int b_stride, int d_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return HFRK_BAD_ALIGNMENT;
     hfrk::GroupedArgs a{};
     a.A = static_cast<const uint8_t*>(A);
     a.B = static_cast<const uint8_t*>(B);
@@ -228,7 +382,7 @@ int hfrk_int8_gemm(const void* A, const void* B, void* D, const void* base, int 
     a.n = n;
     a.k = k;
     a.d_dtype = d_dtype;
-    return hfrk::grouped_run(a, HFRK_INT8, static_cast<hipStream_t>(stream));
+    return hfrk::grouped_run(a, HFRK_INT8, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -53,6 +53,17 @@ constexpr bool tiled_half_stages(int tm, int waves) { return tm * waves >= 32; }
 // Waves of a workgroup that only load, beside the WM x WN that multiply (tiled_gemm_kernel.h).
 constexpr int tiled_loader_waves(int tm) { return tm < 4 ? 4 : 0; }
 
+// Groups (grouped_gemm.hip): the four largest shapes, and 128 x 128 in five halves of stages, 80 KB, whose waves load for themselves, so that two workgroups share
+// a compute unit and one multiplies while the other starts or ends.  A group has few tiles and often a short k: start and end are a third of the time
+// there (333 rows of 60 experts, 4 each, 2816 x 2048 fp8: 128 x 128 84.4 -> 76.9 us; 512 tokens, 8 of 128, 2048 x 768 83.9 -> 63.5; 8 x 28672 x 4096 with 250 tokens
+// each 323 -> 310).
+#define HFRK_TILED_GROUPED(X) \
+    X(0, 4, 2, 2, 4, 5, 1)    \
+    X(1, 2, 2, 4, 2, 3, 1)    \
+    X(2, 2, 2, 2, 2, 5, 1)    \
+    X(3, 2, 1, 2, 2, 3, 2)
+#define HFRK_TILED_PAIRED(X) X(4, 2, 2, 2, 2, 5, 2)
+
 struct TiledShape {
     int bm, bn, stages, per_cu;
     bool halves;
@@ -60,6 +71,10 @@ struct TiledShape {
 };
 #define HFRK_TILED_ROW(I, TM, TN, WM, WN, NST, WGS) {32 * TM * WM, 32 * TN * WN, NST, WGS, tiled_half_stages(TM, WM * WN), 64 * (WM * WN + tiled_loader_waves(TM))},
 constexpr TiledShape kTiledShapes[] = {HFRK_TILED_SHAPES(HFRK_TILED_ROW)};
+#define HFRK_TILED_PAIR(I, TM, TN, WM, WN, NST, WGS) {32 * TM * WM, 32 * TN * WN, NST, WGS, true, 64 * WM * WN},
+constexpr TiledShape kGroupedShapes[] = {HFRK_TILED_GROUPED(HFRK_TILED_ROW) HFRK_TILED_PAIRED(HFRK_TILED_PAIR)};
+constexpr int kGroupedShapeCount = sizeof(kGroupedShapes) / sizeof(kGroupedShapes[0]);
+#undef HFRK_TILED_PAIR
 #undef HFRK_TILED_ROW
 #define HFRK_TILED_SAME(I, TM, TN, WM, WN, NST, WGS) \
     static_assert(kTiledShapes[I].bm == 32 * TM * WM && kTiledShapes[I].bn == 32 * TN * WN && kTiledShapes[I].stages == NST && kTiledShapes[I].per_cu == WGS);
@@ -73,12 +88,17 @@ constexpr int tiled_lds_bytes(const TiledShape& s) { return (s.bm + s.bn) * (s.h
 bool tiled_size_ok(int m, int n, int k);
 // Whether the tiled GEMM is the faster one for a call that the skinny GEMM would run under `skinny`, and the plan it then takes.
 bool tiled_instead(int m, int n, int k, const hfrk_gemm_plan& skinny, hfrk_tiled_plan* plan);
+// The plan that the costs name, k in `max_splits` parts at most, and its cost in us.
+constexpr int kTiledMaxSplits = 8;
+float make_tiled_plan(int m, int n, int k, int max_splits, hfrk_tiled_plan* plan);
+// Where in k the workgroups of a launch start (tiles_m, tiles_n, group_m and splits are set); `small`: 64 x 64 tiles.
+void turn_k(TiledGemmArgs* a, const TiledShape& s, bool small);
 size_t tiled_plan_ws_bytes(const hfrk_tiled_plan& p, int m, int n);
 long tiled_plan_counters(const hfrk_tiled_plan& p, int m, int n);
 // The launch alone: arguments are checked and the plan fits them and the workspace.
 int tiled_launch(const void* A, const void* B, bool packed, void* D, const void* base, int base_stride, const float* scale_a, int sa_stride,
                  const float* scale_b, int sb_stride, int m, int n, int k, int b_stride, int d_dtype, const hfrk_tiled_plan& p, float* ws, size_t ws_bytes,
-                 int* counters, hipStream_t stream);
+                 int* counters, hipStream_t stream, bool int8 = false);
 int launch_tiled_rowmajor(const TiledGemmArgs& args, int shape, hipStream_t stream);  // tiled_gemm_rowmajor.hip
 int launch_tiled_packed(const TiledGemmArgs& args, int shape, hipStream_t stream);    // tiled_gemm_packed.hip
 

@@ -1,7 +1,7 @@
 // Host side of the tiled GEMM: plan and entry points (the kernel is in tiled_gemm_kernel.h).
 #include <math.h>
 
-#include "tiled_gemm.h"
+#include "grouped_gemm.h"
 
 namespace hfrk {
 
@@ -60,8 +60,6 @@ static float tiled_cost(int m, int n, int k, int shape, int splits) {
     if (splits > 1) t += .451f + .797f * splits + (float)wgs * s.bm * s.bn * 8.f / kShares;
     return t;
 }
-
-constexpr int kTiledMaxSplits = 8;
 
 // Up to 64 rows: one row of tiles streams the weight.  64 x 64 tiles with k in up to 8 parts of 4 stages or more on at most 512 workgroups, or,
 // where they take a second round, 128 x 64 tiles, two on a compute unit.  In us, the constants fitted to 1300 sizes of 17 to 64 rows with weights from
@@ -150,13 +148,10 @@ bool tiled_instead(int m, int n, int k, const hfrk_gemm_plan& skinny, hfrk_tiled
     return margin * make_few_rows_plan(m, n, k, kTiledMaxSplits, plan) < workgroup_kernel_cost(m, n, k, skinny);
 }
 
-static void make_tiled_plan(int m, int n, int k, int max_splits, hfrk_tiled_plan* plan) {
+float make_tiled_plan(int m, int n, int k, int max_splits, hfrk_tiled_plan* plan) {
     float best = INFINITY;
     const int stages = div_up(k, kTiledStage);
-    if (m <= 64) {  // (the fit below starts at 65 rows)
-        make_few_rows_plan(m, n, k, max_splits, plan);
-        return;
-    }
+    if (m <= 64) return make_few_rows_plan(m, n, k, max_splits, plan);  // (the fit below starts at 65 rows)
     for (int shape = 0; shape < kTiledShapeCount; ++shape) {
         const TiledShape& s = kTiledShapes[shape];
         const int tiles_m = div_up(m, s.bm);
@@ -176,6 +171,7 @@ static void make_tiled_plan(int m, int n, int k, int max_splits, hfrk_tiled_plan
             }
         }
     }
+    return best;
 }
 
 // The workgroups of an XCD share rows of A and of the weight.  Walking k in step they all ask for a line while it is on its way into their
@@ -187,21 +183,20 @@ static void make_tiled_plan(int m, int n, int k, int max_splits, hfrk_tiled_plan
 // 16.0 -> 16.3.  Windows of 400 KB gain a third of that, of 1.2 to 3 MB as much on the sizes above and lose up to 7 % on others (1192 x 5488 x 2048 23.1 ->
 // 24.6); k turned as a whole loses up to twice the time where it does not fit L2.  64 x 64 tiles start together: they lose 1 to 3 % by it
 // (187 x 4024 x 7872 21.6 -> 22.2, 317 x 1800 x 6400 18.2 -> 18.7).
-static void turn_k(TiledGemmArgs* a, int shape) {
-    const TiledShape& s = kTiledShapes[shape];
+void turn_k(TiledGemmArgs* a, const TiledShape& s, bool small) {
     const int grid = a->tiles_m * a->tiles_n * a->splits, resident = kNumCU * s.per_cu;
     const int per_xcd = div_up(grid < resident ? grid : resident, 8);
     int columns = div_up(per_xcd, a->group_m);
     columns = columns < a->tiles_n ? columns : a->tiles_n;
     a->phase_m = 65536 / a->group_m;
     a->phase_n = 65536 / columns;
-    a->window = shape == 4 ? 1 : (int)(700 * 1024 / (((long)a->group_m * s.bm + (long)columns * s.bn) * kTiledStage));
+    a->window = small ? 1 : (int)(700 * 1024 / (((long)a->group_m * s.bm + (long)columns * s.bn) * kTiledStage));
     a->window = a->window < 1 ? 1 : a->window;
 }
 
 int tiled_launch(const void* A, const void* B, bool packed, void* D, const void* base, int base_stride, const float* scale_a, int sa_stride,
                  const float* scale_b, int sb_stride, int m, int n, int k, int b_stride, int d_dtype, const hfrk_tiled_plan& p, float* ws, size_t ws_bytes,
-                 int* counters, hipStream_t stream) {
+                 int* counters, hipStream_t stream, bool int8) {
     const TiledShape& s = kTiledShapes[p.shape];
     const int row_tiles = div_up(m, s.bm);
     if ((uint64_t)row_tiles * div_up(n, s.bn) * p.splits * s.threads >> 32) {
@@ -212,7 +207,7 @@ int tiled_launch(const void* A, const void* B, bool packed, void* D, const void*
             const hfrk_tiled_plan q{p.shape, p.splits, p.group_m < half ? p.group_m : half};
             return tiled_launch(static_cast<const uint8_t*>(A) + (size_t)row * k, B, packed, static_cast<uint8_t*>(D) + (size_t)row * n * 2,
                                 base ? static_cast<const uint8_t*>(base) + (size_t)row * base_stride * 2 : base, base_stride, scale_a + (size_t)row * sa_stride,
-                                sa_stride, scale_b, sb_stride, count, n, k, b_stride, d_dtype, q, ws, ws_bytes, counters, stream);
+                                sa_stride, scale_b, sb_stride, count, n, k, b_stride, d_dtype, q, ws, ws_bytes, counters, stream, int8);
         };
         const int rc = part(0, rows);
         return rc == HFRK_SUCCESS ? part(rows, m - rows) : rc;
@@ -243,8 +238,9 @@ int tiled_launch(const void* A, const void* B, bool packed, void* D, const void*
     args.counters = counters;
     args.stages_q = stages / p.splits;
     args.stages_r = stages % p.splits;
-    turn_k(&args, p.shape);
-    return packed ? launch_tiled_packed(args, p.shape, stream)
+    turn_k(&args, s, p.shape == 4);
+    return int8 ? launch_tiled_int8(args, p.shape, stream)
+         : packed ? launch_tiled_packed(args, p.shape, stream)
                   : launch_tiled_rowmajor(args, p.shape, stream);
 }
 

@@ -53,11 +53,13 @@
 // purpose: with a branch per value for NaN and 64-bit addresses it took 18 us of a 256 x 256 tile, now 7.
 #pragma once
 
+#include "grouped_gemm.h"
 #include "tiled_gemm.h"
 
 namespace hfrk {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 
 // One 16-byte-per-lane load from memory straight into LDS: lane l's piece lands at lds_base + 16 l.  As inline assembly because the
 // compiler, when it knows of such a load, waits for it before every LDS read that follows; the waits are placed by hand here.  m0 is
@@ -89,9 +91,9 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2h));
 }
 
-// LW: waves that only load.
-template <int TM, int TN, int WM, int WN, int NST, int WGS, bool PACKED, int LW>
-__global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4) tiled_gemm_kernel(const TiledGemmArgs a) {
+// LW: waves that only load.  INT8: codes are int8, sums int32.  GROUPED: rows grouped by expert, a weight for each (grouped_gemm.h); k is not split then.
+template <int TM, int TN, int WM, int WN, int NST, int WGS, bool PACKED, int LW, bool INT8 = false, bool GROUPED = false, bool HALF = tiled_half_stages(TM, WM * WN)>
+__global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4) tiled_gemm_kernel(const std::conditional_t<GROUPED, TiledGroupedArgs, TiledGemmArgs> a) {
     constexpr int NW = WM * WN, NL = LW ? LW : NW;  // waves that multiply, that load
     constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
     constexpr int KB = kTiledStage;
@@ -99,7 +101,6 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
     constexpr int LA = A_BYTES / (1024 * NL), LB = B_BYTES / (1024 * NL);  // load instructions per loading wave and stage, 1 KB each
     constexpr int NMMA = TM * TN;
     // NST counts whole stages, or (HALF) the halves of stages, 64 bytes of k each, that LDS holds.
-    constexpr bool HALF = tiled_half_stages(TM, NW);
     constexpr int ROW = HALF ? KB / 2 : KB, SLOT = HALF ? STAGE / 2 : STAGE, RING = NST * SLOT, AHEAD = HALF ? NST / 2 : NST;  // AHEAD: stages requested in front
     constexpr int kOutside = 0x7ffffff0;  // beyond any tile's range
 
@@ -114,32 +115,65 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
 
     // ---- which tile, which part of k ---------------------------------------------------------------------------------
     int id = blockIdx.x;
-    {
+    GroupTile group;  // (GROUPED)
+    if constexpr (GROUPED) {
+        if (!find_tile(a, BM, &group)) return;
+        id = group.tile;
+    } else {
         const int per = (int)gridDim.x >> 3, extra = (int)gridDim.x & 7, x = id & 7;  // XCD x works on one contiguous range of ids
         id = x * per + min(x, extra) + (id >> 3);
     }
-    const int tiles = a.tiles_m * a.tiles_n;
-    const int split = a.splits == 1 ? 0 : id / tiles, tile = id - split * tiles;  // neighbours work on the same part of k
+    int tiles_m;
+    if constexpr (GROUPED) tiles_m = group.tiles_m;
+    else tiles_m = a.tiles_m;
+    const int tiles = tiles_m * a.tiles_n;
+    const int split = GROUPED || a.splits == 1 ? 0 : id / tiles, tile = id - split * tiles;  // neighbours work on the same part of k
     const int group_tiles = a.group_m * a.tiles_n;
     const int grp = tile / group_tiles, in_grp = tile - grp * group_tiles;
-    const int gm = min(a.group_m, a.tiles_m - grp * a.group_m);
+    const int gm = min(a.group_m, tiles_m - grp * a.group_m);
     const int tn = in_grp / gm, tm = grp * a.group_m + in_grp - tn * gm;
-    const int m0 = tm * BM, n0 = tn * BN;
+    // m0: the tile's first row of D; rows_a: how many there are
+    int m0 = tm * BM, rows_a;
+    const int n0 = tn * BN;
+    const uint8_t* weight = a.B;
+    const float* scales_b = a.scale_b;
+    if constexpr (GROUPED) {
+        rows_a = min(BM, group.rows - m0);
+        m0 += group.first;
+        weight += group.expert * a.expert_stride;
+        if (scales_b) scales_b += group.expert * a.sb_expert_stride;
+    } else {
+        rows_a = min(BM, a.m - m0);
+    }
+    // (GROUPED) which row of A row r of the tile is, -1: none.  The numbers come through a buffer over the tile's own: no branch, so that several are
+    // requested together.
+    auto row_number = [&](int r) __attribute__((always_inline)) {
+        if constexpr (GROUPED) return __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(a.rows + m0, (uint32_t)rows_a * 4u), r * 4, 0, 0);
+        else return r;
+    };
+    auto row_of_number = [&](int r, int number) __attribute__((always_inline)) {
+        if constexpr (GROUPED) return (uint32_t)r < (uint32_t)rows_a && (uint32_t)number < (uint32_t)a.a_rows ? number : -1;
+        else return number;
+    };
+    bool gathers = false;
+    if constexpr (GROUPED) gathers = a.rows != nullptr;
     const uint32_t phase = ((uint32_t)(in_grp - tn * gm) * (uint32_t)a.phase_m + (uint32_t)tn * (uint32_t)a.phase_n) & 0xffff;  // in 65536ths
     const int s_begin = split * a.stages_q + min(split, a.stages_r), s_end = s_begin + a.stages_q + (split < a.stages_r ? 1 : 0);
 
     // ---- operand streams ---------------------------------------------------------------------------------------------
     // buffers over this tile's rows, moved to the stage that is requested
-    const int rows_a = min(BM, a.m - m0);
     v4i ra = tile_rsrc(a.A + (long)m0 * a.k, (uint32_t)rows_a * (uint32_t)a.k);
+    if constexpr (GROUPED) {
+        if (gathers) ra = tile_rsrc(a.A, (uint32_t)a.a_rows * (uint32_t)a.k);
+    }
     v4i rb;
     constexpr int kStepB = PACKED ? 2048 : KB;  // a stage of a packed 16-row tile is half of a 4 KB chunk
     if constexpr (PACKED) {
         const int tiles16 = min(BN / 16, (a.n + 15) / 16 - n0 / 16);
-        rb = tile_rsrc(a.B + (long)(n0 / 16) * a.k * 16, (uint32_t)tiles16 * (uint32_t)a.k * 16u);
+        rb = tile_rsrc(weight + (long)(n0 / 16) * a.k * 16, (uint32_t)tiles16 * (uint32_t)a.k * 16u);
     } else {
         const int rows_b = min(BN, a.n - n0);
-        rb = tile_rsrc(a.B + (long)n0 * a.b_stride, (uint32_t)(rows_b - 1) * (uint32_t)a.b_stride + (uint32_t)a.k);
+        rb = tile_rsrc(weight + (long)n0 * a.b_stride, (uint32_t)(rows_b - 1) * (uint32_t)a.b_stride + (uint32_t)a.k);
     }
     int va[LA], vb[LB];
     int pa[LA], pb[LB];  // k byte of the lane's piece within its stage (for the last, partial stage)
@@ -148,6 +182,21 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
         const int row = HALF ? ((q >> 1) * NL + loader) * 16 + (lane >> 2) : (q * NL + loader) * 8 + (lane >> 3);
         pa[q] = HALF ? ((lane & 3) ^ ((row >> 2) & 3)) * 16 + (q & 1) * ROW : ((lane & 7) ^ ((row >> 1) & 7)) * 16;
         va[q] = row * a.k + pa[q];
+    }
+    if constexpr (GROUPED) {
+        if (gathers && loader >= 0) {  // (a wave that only multiplies has no rows to load: its numbers are below zero)
+            int number[LA];
+            auto row_of_load = [&](int q) __attribute__((always_inline)) {
+                return HALF ? ((q >> 1) * NL + loader) * 16 + (lane >> 2) : (q * NL + loader) * 8 + (lane >> 3);
+            };
+#pragma unroll
+            for (int q = 0; q < LA; ++q) number[q] = row_number(row_of_load(q));
+#pragma unroll
+            for (int q = 0; q < LA; ++q) {
+                const int from = row_of_number(row_of_load(q), number[q]);
+                va[q] = from >= 0 ? from * a.k + pa[q] : kOutside;
+            }
+        }
     }
 #pragma unroll
     for (int q = 0; q < LB; ++q) {
@@ -230,13 +279,15 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
         }
     };
 
-    v16f acc[TM][TN];
+    using Acc = std::conditional_t<INT8, v16i, v16f>;
+    using Four = std::conditional_t<INT8, v4i, v4f>;
+    Acc acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
 
     // Half a stage (64 bytes of k): multiply the operands read half a stage ago (register set S) while the next half's are read into
     // the other set.  The second half reads from the next stage, so it opens with the wait for that stage and a barrier behind it.  With
@@ -280,7 +331,14 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
                 }
             reads = reads_to;
             loads = loads_to;
-            acc[t / TN][t % TN] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frb[S][t % TN], fra[S][t / TN], acc[t / TN][t % TN], 0, 0, 0, 0, 0, 0);
+            if constexpr (INT8) {  // (half of the lane's bytes at a time: which of them meet does not matter, as both operands agree)
+                const v8i &x = frb[S][t % TN], &y = fra[S][t / TN];
+                Acc& c = acc[t / TN][t % TN];
+                c = __builtin_amdgcn_mfma_i32_32x32x32_i8(v4i{x[0], x[1], x[2], x[3]}, v4i{y[0], y[1], y[2], y[3]}, c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_i32_32x32x32_i8(v4i{x[4], x[5], x[6], x[7]}, v4i{y[4], y[5], y[6], y[7]}, c, 0, 0, 0);
+            } else {
+                acc[t / TN][t % TN] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frb[S][t % TN], fra[S][t / TN], acc[t / TN][t % TN], 0, 0, 0, 0, 0, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (S == 1 && !LW) issue_end();
@@ -329,7 +387,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
     workgroup_barrier();  // LDS is free: no wave reads operands any more, no load is under way
 
     // ---- partial sums of a tile whose k is split -----------------------------------------------------------------------
-    if (a.splits > 1) {
+    if (!GROUPED && a.splits > 1) {
         const __amdgpu_buffer_rsrc_t ws = make_rsrc(a.ws, a.ws_bytes);
         constexpr int kCoherent = 17;  // sc0 | sc1: written through to memory, read past the caches (the XCDs' L2s are not coherent)
         auto ws_off = [&](int sp, int t, int p) __attribute__((always_inline)) {
@@ -339,8 +397,8 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
         for (int t = 0; t < NMMA; ++t)
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                const v16f& x = acc[t / TN][t % TN];
-                const v4f v = {x[4 * p], x[4 * p + 1], x[4 * p + 2], x[4 * p + 3]};
+                const Acc& x = acc[t / TN][t % TN];
+                const Four v = {x[4 * p], x[4 * p + 1], x[4 * p + 2], x[4 * p + 3]};
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, v), ws, ws_off(split, t, p), 0, kCoherent);
             }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -363,9 +421,9 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
         constexpr int CH = NMMA == 1 || WGS * (NW + LW) > 8 || (LW == 0 && NW > 4) ? 1 : 2, FLY = NMMA == 1 ? 7 : 3;
 #pragma unroll
         for (int t0 = 0; t0 < NMMA; t0 += CH) {
-            v4f sum[CH * 4];
+            Four sum[CH * 4];
 #pragma unroll
-            for (int p = 0; p < CH * 4; ++p) sum[p] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int p = 0; p < CH * 4; ++p) sum[p] = Four{0, 0, 0, 0};
             auto add_shares = [&](int first, int end) __attribute__((always_inline)) {
 #pragma unroll 1
                 for (; first < end; first += FLY) {
@@ -381,15 +439,15 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
                     for (int j = 0; j < FLY; ++j)
                         if (first + j < end) {
 #pragma unroll
-                            for (int p = 0; p < CH * 4; ++p) sum[p] += __builtin_bit_cast(v4f, share[j][p]);
+                            for (int p = 0; p < CH * 4; ++p) sum[p] += __builtin_bit_cast(Four, share[j][p]);
                         }
                 }
             };
             add_shares(0, split);
 #pragma unroll
             for (int p = 0; p < CH * 4; ++p) {
-                const v16f& x = acc[(t0 + p / 4) / TN][(t0 + p / 4) % TN];
-                sum[p] += v4f{x[4 * (p % 4)], x[4 * (p % 4) + 1], x[4 * (p % 4) + 2], x[4 * (p % 4) + 3]};
+                const Acc& x = acc[(t0 + p / 4) / TN][(t0 + p / 4) % TN];
+                sum[p] += Four{x[4 * (p % 4)], x[4 * (p % 4) + 1], x[4 * (p % 4) + 2], x[4 * (p % 4) + 3]};
             }
             add_shares(split + 1, a.splits);
 #pragma unroll
@@ -416,22 +474,38 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
     const __amdgpu_buffer_rsrc_t rd = make_rsrc(static_cast<uint16_t*>(a.D) + (long)m0 * a.n, (uint32_t)rows_a * (uint32_t)a.n * 2u);
     const __amdgpu_buffer_rsrc_t rbase = make_rsrc(static_cast<const uint16_t*>(a.base) + (long)m0 * a.base_stride,
                                                    a.base ? (uint32_t)((rows_a - 1) * a.base_stride + a.n) * 2u : 0u);
-    const __amdgpu_buffer_rsrc_t rsa = make_rsrc(a.scale_a + (long)m0 * a.sa_stride, (uint32_t)((rows_a - 1) * a.sa_stride + 1) * 4u);
+    __amdgpu_buffer_rsrc_t rsa = make_rsrc(a.scale_a + (long)m0 * a.sa_stride, (uint32_t)((rows_a - 1) * a.sa_stride + 1) * 4u);
+    if constexpr (GROUPED) {
+        if (gathers) rsa = make_rsrc(a.scale_a, (uint32_t)((a.a_rows - 1) * a.sa_stride + 1) * 4u);
+    }
     float sb[8];
 #pragma unroll
-    for (int v = 0; v < 8; ++v) sb[v] = a.scale_b ? a.scale_b[(long)min(n0 + col + v, a.n - 1) * a.sb_stride] : 1.0f;
+    for (int v = 0; v < 8; ++v) sb[v] = scales_b ? scales_b[(long)min(n0 + col + v, a.n - 1) * a.sb_stride] : 1.0f;
     auto write_back = [&](auto dt) __attribute__((always_inline)) {
         constexpr int DT = decltype(dt)::value;
         // The memory counter retires in order, so a load requested after stores waits for them: scales and addends of 32 rows
         // are requested before the stores of the 32 rows in front.
         v4i add[2][PASSES];
         float sa[2][PASSES];
+        int from[TM * PASSES];  // (GROUPED: rows of the scales, all requested ahead)
+        if constexpr (GROUPED) {
+            if (gathers && a.vec) {
+#pragma unroll
+                for (int r = 0; r < TM * PASSES; ++r) from[r] = row_number(row0 + r * RPI + lane / LPR);
+#pragma unroll
+                for (int r = 0; r < TM * PASSES; ++r) from[r] = row_of_number(row0 + r * RPI + lane / LPR, from[r]);
+            }
+        }
         const uint32_t base_off = ((uint32_t)(row0 + lane / LPR) * (uint32_t)a.base_stride + (uint32_t)(n0 + col)) * 2u | outside;
         const uint32_t base_step = (uint32_t)(RPI * 2) * (uint32_t)a.base_stride;
         auto fetch = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int r = 0; r < PASSES; ++r) {
-                sa[i & 1][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsa, (row0 + i * 32 + r * RPI + lane / LPR) * a.sa_stride * 4, 0, 0));
+                int row = row0 + i * 32 + r * RPI + lane / LPR;
+                if constexpr (GROUPED) {
+                    if (gathers) row = from[i * PASSES + r] < 0 ? kOutside / 4 : from[i * PASSES + r];
+                }
+                sa[i & 1][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsa, row * a.sa_stride * 4, 0, 0));
                 add[i & 1][r] = __builtin_amdgcn_raw_buffer_load_b128(rbase, (int)(base_off + (uint32_t)(i * PASSES + r) * base_step), 0, 0);
             }
         };
@@ -445,7 +519,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
 #pragma unroll
                 for (int p = 0; p < 4; ++p)
                     *reinterpret_cast<v4f*>(stage + lr * RS + j * 32 + lg * 16 + p * 4) =
-                        v4f{acc[i][j][4 * p], acc[i][j][4 * p + 1], acc[i][j][4 * p + 2], acc[i][j][4 * p + 3]};
+                        v4f{(float)acc[i][j][4 * p], (float)acc[i][j][4 * p + 1], (float)acc[i][j][4 * p + 2], (float)acc[i][j][4 * p + 3]};
             if (a.vec && i + 1 < TM) fetch(i + 1);
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -470,8 +544,14 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
                 for (int e = lane; e < 32 * TN * 32; e += 64) {
                     const int r = e / (TN * 32), c = e % (TN * 32);
                     const int m = m0 + row0 + i * 32 + r, n = n0 + wn * TN * 32 + c;
-                    if (m >= a.m || n >= a.n) continue;
-                    float x = stage[r * RS + c] * (a.scale_a[(long)m * a.sa_stride] * (a.scale_b ? a.scale_b[(long)n * a.sb_stride] : 1.0f));
+                    int row = m;
+                    if constexpr (GROUPED) {
+                        if (m >= m0 + rows_a || n >= a.n) continue;
+                        if (gathers) row = max(row_of_number(m - m0, row_number(m - m0)), 0);  // (no row: a sum of zero, times some scale)
+                    } else {
+                        if (m >= a.m || n >= a.n) continue;
+                    }
+                    float x = stage[r * RS + c] * (a.scale_a[(long)row * a.sa_stride] * (scales_b ? scales_b[(long)n * a.sb_stride] : 1.0f));
                     if (a.base) x += load16<DT>(static_cast<const uint16_t*>(a.base)[(long)m * a.base_stride + n]);
                     static_cast<uint16_t*>(a.D)[(long)m * a.n + n] = (uint16_t)pack_pair<DT>(x, 0.f);
                 }
@@ -485,9 +565,10 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
     else write_back(std::integral_constant<int, HFRK_F16>{});
 }
 
-template <int TM, int TN, int WM, int WN, int NST, int WGS, bool PACKED, int LW = tiled_loader_waves(TM)>
-static int launch_tiled_shape(const TiledGemmArgs& args, int lds_bytes, hipStream_t stream) {
-    auto kern = tiled_gemm_kernel<TM, TN, WM, WN, NST, WGS, PACKED, LW>;
+template <int TM, int TN, int WM, int WN, int NST, int WGS, bool PACKED, int LW = tiled_loader_waves(TM), bool INT8 = false, bool GROUPED = false,
+          bool HALF = tiled_half_stages(TM, WM * WN)>
+static int launch_tiled_shape(const std::conditional_t<GROUPED, TiledGroupedArgs, TiledGemmArgs>& args, int lds_bytes, hipStream_t stream, long grid = 0) {
+    auto kern = tiled_gemm_kernel<TM, TN, WM, WN, NST, WGS, PACKED, LW, INT8, GROUPED, HALF>;
     static bool attr_done[kMaxDevices] = {};
     int dev = 0;
     HFRK_HIP_TRY(hipGetDevice(&dev));
@@ -495,25 +576,41 @@ static int launch_tiled_shape(const TiledGemmArgs& args, int lds_bytes, hipStrea
         HFRK_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
         if (dev >= 0 && dev < kMaxDevices) attr_done[dev] = true;
     }
-    hipLaunchKernelGGL(kern, dim3(args.tiles_m * args.tiles_n * args.splits), dim3(64 * (WM * WN + LW)), lds_bytes, stream, args);
+    if (grid == 0) grid = args.tiles_m * args.tiles_n * args.splits;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * (WM * WN + LW)), lds_bytes, stream, args);
     HFRK_HIP_TRY(hipGetLastError());
     return HFRK_SUCCESS;
 }
 
-template <bool PACKED>
+template <bool PACKED, bool INT8 = false>
 static int launch_tiled(const TiledGemmArgs& args, int shape, hipStream_t stream) {
     if (args.stages_q + (args.stages_r ? 1 : 0) <= 2) {
         switch (shape) {
 #define HFRK_TILED_CASE(I, TM, TN, WM, WN, NST, WGS) \
-    case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, PACKED, 0>(args, tiled_lds_bytes(kTiledShapes[I]), stream);
+    case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, PACKED, 0, INT8>(args, tiled_lds_bytes(kTiledShapes[I]), stream);
             HFRK_TILED_SHORT_K(HFRK_TILED_CASE)
 #undef HFRK_TILED_CASE
         }
     }
     switch (shape) {
 #define HFRK_TILED_CASE(I, TM, TN, WM, WN, NST, WGS) \
-    case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, PACKED>(args, tiled_lds_bytes(kTiledShapes[I]), stream);
+    case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, PACKED, tiled_loader_waves(TM), INT8>(args, tiled_lds_bytes(kTiledShapes[I]), stream);
         HFRK_TILED_SHAPES(HFRK_TILED_CASE)
+#undef HFRK_TILED_CASE
+    }
+    return HFRK_INVALID_CONFIG;
+}
+
+template <bool INT8>
+static int launch_tiled_groups(const TiledGroupedArgs& args, int shape, long grid, hipStream_t stream) {
+    switch (shape) {
+#define HFRK_TILED_CASE(I, TM, TN, WM, WN, NST, WGS) \
+    case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, false, tiled_loader_waves(TM), INT8, true>(args, tiled_lds_bytes(kGroupedShapes[I]), stream, grid);
+        HFRK_TILED_GROUPED(HFRK_TILED_CASE)
+#undef HFRK_TILED_CASE
+#define HFRK_TILED_CASE(I, TM, TN, WM, WN, NST, WGS) \
+    case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, false, 0, INT8, true, true>(args, tiled_lds_bytes(kGroupedShapes[I]), stream, grid);
+        HFRK_TILED_PAIRED(HFRK_TILED_CASE)
 #undef HFRK_TILED_CASE
     }
     return HFRK_INVALID_CONFIG;

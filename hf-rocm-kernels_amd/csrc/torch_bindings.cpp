@@ -1194,10 +1194,14 @@ const char* int8_operands(const at::Tensor& A, const at::Tensor& B, const std::o
 int run_int8_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tensor& D, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
                   const std::optional<at::Tensor>& scale_b) {
     const int m = (int)A.size(0), n = (int)B.size(1), k = (int)A.size(1);
+    // (memory of the call's own: streams and graphs share none)
+    const size_t bytes = hfrk_int8_gemm_workspace_bytes(m, n, k);
+    const at::Tensor workspace = bytes ? at::empty({(int64_t)bytes}, A.options().dtype(at::kByte)) : at::Tensor();
     return hfrk_int8_gemm(A.data_ptr(), B.data_ptr(), D.data_ptr(), base.has_value() ? base->data_ptr() : nullptr,
                           base.has_value() && base->dim() == 2 ? n : 0, scale_a.data_ptr<float>(), scale_a.numel() == 1 ? 0 : 1,
                           scale_b.has_value() ? scale_b->data_ptr<float>() : nullptr, scale_b.has_value() && scale_b->numel() != 1 ? 1 : 0, m, n, k,
-                          n > 1 ? (int)B.stride(1) : k, D.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, current_stream(A));
+                          n > 1 ? (int)B.stride(1) : k, D.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, bytes ? workspace.data_ptr() : nullptr, bytes,
+                          current_stream(A));
 }
 
 void int8_gemm(const at::Tensor& A, const at::Tensor& B, at::Tensor& D, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,

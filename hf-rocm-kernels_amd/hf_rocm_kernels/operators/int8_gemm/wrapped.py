@@ -52,7 +52,7 @@ def int8_gemm(
     output: Optional[Tensor] = None,
     out_dtype: torch.dtype = torch.bfloat16,
 ) -> Tensor:
-    """base + scale_a * scale_b * (a @ b) on int8 codes, any number of rows: the sums are exact, scales and addend are applied in fp32, and the result
+    """base + scale_a * scale_b * (a @ b) on int8 codes, from one row to whole prompts (2^24): the sums are exact, scales and addend are applied in fp32, and the result
     is rounded once.
     Args:
         - a: an (m, k) int8 tensor in row-major format, k a multiple of 16 up to 131056
@@ -60,7 +60,7 @@ def int8_gemm(
         - scale_a: float32, one or one per row of a (`quantize_int8` and `swiglu_dynamic` give these); scale_b: one, one per column of b, or None: 1
         - base: an addend of the result's dtype, (m, n) (a residual) or (n,) (a bias)
         - output: a tensor to write to (it may be base), or None for a new one of out_dtype (bfloat16 or float16)
-    Inference only: the result carries no gradient.
+    Where few tiles have a long k a call takes a workspace from torch's allocator (64 MiB at most).  Inference only: the result carries no gradient.
     """
     if output is None and a.dim() == 2 and b.dim() == 2 and runs_now(a) and a.dtype == torch.int8:
         out = _int8_linear(a, b.t(), scale_b, scale_a, None if base is None or base.dim() != 1 else base, base if base is not None and base.dim() == 2 else None,

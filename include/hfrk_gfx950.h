@@ -485,9 +485,13 @@ int hfrk_swiglu_dynamic_int8(const void* gate_up, void* output, float* scales, i
  *   A [m,k] int8, rows of k bytes;  B [n,k] int8, rows b_stride bytes apart;  D [m,n] of d_dtype
  *   base of d_dtype, rows base_stride elements apart (0: one row for all, a bias), or NULL
  *   scale_a fp32 [m] (sa_stride 1) or one (0); scale_b [n] (1), one (0) or NULL: 1
- * Any number of rows.  k a multiple of 16 up to 131056, n up to 2^21, b_stride a multiple of 16 up to 2^21, A and B on 16-byte boundaries.  No workspace. */
+ * m up to 2^24 (and tiles of 64 x 64 below 2^24).  k a multiple of 16 up to 131056, n up to 2^21, b_stride a multiple of 16 up to 2^21, A and B on 16-byte
+ * boundaries.  base may be D.
+ * workspace: hfrk_int8_gemm_workspace_bytes of it lets few tiles with a long k share their k between workgroups (the sums are exact either way: equal bits); fewer, or
+ * NULL, and each has its k to itself.  16-byte aligned, any contents, used by one call at a time. */
+size_t hfrk_int8_gemm_workspace_bytes(int m, int n, int k);
 int hfrk_int8_gemm(const void* A, const void* B, void* D, const void* base, int base_stride, const float* scale_a, int sa_stride, const float* scale_b,
-                   int sb_stride, int m, int n, int k, int b_stride, int d_dtype, void* stream);
+                   int sb_stride, int m, int n, int k, int b_stride, int d_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- an MLP of experts ------------------------------------------------------------------------------------------------------------------
  * Products of rows grouped by expert:

@@ -42,10 +42,11 @@ def test_grouped_gemm_refuses_on_the_host(changes, status):
 
 
 def _int8(**changes):
-    args = dict(A=P, B=P, D=P, base=None, base_stride=0, sa=P, sa_stride=1, sb=P, sb_stride=1, m=8, n=32, k=64, b_stride=64, dtype=_capi.BF16)
+    args = dict(A=P, B=P, D=P, base=None, base_stride=0, sa=P, sa_stride=1, sb=P, sb_stride=1, m=8, n=32, k=64, b_stride=64, dtype=_capi.BF16, workspace=None,
+                bytes=0)
     args.update(changes)
     return LIB.hfrk_int8_gemm(args["A"], args["B"], args["D"], args["base"], args["base_stride"], args["sa"], args["sa_stride"], args["sb"], args["sb_stride"], args["m"],
-                              args["n"], args["k"], args["b_stride"], args["dtype"], None)
+                              args["n"], args["k"], args["b_stride"], args["dtype"], args["workspace"], args["bytes"], None)
 
 
 @pytest.mark.parametrize("changes,status", [
@@ -56,6 +57,13 @@ def _int8(**changes):
 ])
 def test_int8_gemm_refuses_on_the_host(changes, status):
     assert _int8(**changes) == status
+
+
+def test_int8_gemm_workspace():
+    """Few tiles and a long k share it between workgroups; many tiles, few rows and a short k do not."""
+    assert LIB.hfrk_int8_gemm_workspace_bytes(128, 4096, 14336) > 0 and LIB.hfrk_int8_gemm_workspace_bytes(64, 4096, 14336) > 0
+    for m, n, k in ((1, 4096, 14336), (16, 4096, 14336), (4096, 28672, 4096), (512, 8192, 256), (0, 64, 64), (-1, 64, 64), (100, 0, 64), (1 << 30, 64, 64)):
+        assert LIB.hfrk_int8_gemm_workspace_bytes(m, n, k) == 0, (m, n, k)
 
 
 def _route(**changes):
