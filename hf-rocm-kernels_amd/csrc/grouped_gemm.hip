@@ -181,20 +181,41 @@ static int launch_rows(GroupedArgs a, hipStream_t stream) {
     return HFRK_SUCCESS;
 }
 
-// Which rows kernel: `groups` of rows, each a tile high.  With enough workgroups, 64 columns in four tiles a wave, eight waves along k; a wave asks for one
-// tile's chunk at a time, and it is the six waves of a SIMD that keep memory busy: with all four tiles' chunks requested together and two sets of registers 100
-// tokens on 6 of 160 experts of 3008 x 5120 take 471 us instead of 376 (5.9 TB/s), 32 on 2 of 8 of 28672 x 4096 177 and 164.  With few workgroups, one
-// tile of 16 columns a wave spreads them (one token on 2 of 8 experts of 28672 x 4096 38.2 -> 32.0 us, on 6 of 64 of 2816 x 2048 12.0 -> 9.0, 8 tokens on 2 of 8 of
-// 4096 x 14336 74 -> 62), as long as a workgroup's 16 k bytes outweigh its start and end (4 tokens on 8 of 128 of 1536 x 2048: 17.0 us with 64 columns, 19.6 with
-// 16).  A k of up to eight chunks gives eight waves one each: four waves take it then, and the others other columns (4 tokens on 8 of 128 of 2048 x 768 15.3 ->
-// 12.0, one token 7.1 -> 5.8); a long one on a few workgroups is read by sixteen waves (1 x 10000 x 5136 int8 13.0 -> 11.9, 1 x 4096 x 14336 13.3 -> 12.3).
+// Which rows kernel, and its predicted time in us: rounds of workgroups over the compute units, each reading its columns' weights, its rows (with less weight,
+// as they come from L2) and spending the time of 10 KB on its start and end, at 22 KB a us.  `active` groups of `rows` rows.  64 columns a workgroup where there
+// are many, in four tiles a wave; a wave asks for one tile's chunk at a time, and it is the six waves of a SIMD that keep memory busy: with all four tiles'
+// chunks requested together and two sets of registers 100 tokens on 6 of 160 experts of 3008 x 5120 take 471 us instead of 376 (5.9 TB/s), 32 on 2 of 8 of 28672 x
+// 4096 177 and 164.  Fewer columns spread a call over the compute units: one token on 2 of 8 experts of 4096 x 14336 28.9 -> 18.8 us with 32 columns (128 and
+// 256 workgroups), on 6 of 64 of 2816 x 2048 12.2 -> 10.1 with 48, one row of 4096 x 14336 int8 29.2 -> 12.9 with 16; where the rounds do not get fewer they cost (32
+// tokens on 2 of 8 of 4096 x 14336 85 -> 113 with 16 columns).  Up to eight chunks of k leave eight waves one each: four waves take k then, and the others other
+// columns (4 tokens on 8 of 128 of 2048 x 768 15.8 -> 12.0 with 128 columns, one token 7.5 -> 6.5 with 64 of them).
+struct FewRows {
+    int cols, waves_k;
+    float us;
+};
+
+static FewRows few_rows_kernel(int n, int k, float active, float rows) {
+    auto workgroups = [&](int cols) { return active * ((n + cols - 1) / cols); };
+    auto predicted = [&](int cols) { return 1.5f + ceilf(workgroups(cols) / kNumCU) * (cols + .6f * fminf(rows, 16.f) + 1e4f / k) * k / 22e3f; };
+    if (k <= 8 * kRowsChunk) {
+        const int cols = workgroups(128) >= kNumCU ? 128 : 64;
+        return {cols, 4, predicted(cols)};
+    }
+    FewRows best{64, 8, predicted(64)};
+    for (int cols : {48, 32, 16})
+        if (predicted(cols) < best.us) best = {cols, 8, predicted(cols)};
+    return best;
+}
+
 template <bool INT8>
-static int launch_few_rows(const GroupedArgs& a, int groups, hipStream_t stream) {
-    const long tiles64 = (long)groups * ((a.n + 63) / 64), tiles16 = (long)groups * ((a.n + 15) / 16);
-    const bool spread = tiles64 <= 512 || (tiles64 <= 1024 && a.k >= 4096);
-    if (a.k <= 1024) return spread ? launch_rows<INT8, 1, 1, 4, 2>(a, stream) : launch_rows<INT8, 1, 4, 4, 2>(a, stream);
-    if (!spread) return launch_rows<INT8, 1, 4, 8, 1>(a, stream);
-    return a.k >= 5120 && tiles16 <= 1024 ? launch_rows<INT8, 1, 1, 16, 1>(a, stream) : launch_rows<INT8, 1, 1, 8, 1>(a, stream);
+static int launch_few_rows(const GroupedArgs& a, const FewRows& f, hipStream_t stream) {
+    if (f.waves_k == 4) return f.cols == 128 ? launch_rows<INT8, 1, 4, 4, 2>(a, stream) : launch_rows<INT8, 1, 2, 4, 2>(a, stream);
+    switch (f.cols) {
+        case 64: return launch_rows<INT8, 1, 4, 8, 1>(a, stream);
+        case 48: return launch_rows<INT8, 1, 3, 8, 1>(a, stream);
+        case 32: return launch_rows<INT8, 1, 2, 8, 1>(a, stream);
+        default: return launch_rows<INT8, 1, 1, 8, 1>(a, stream);
+    }
 }
 
 // The tile shape with the smallest predicted time, in us: rounds of workgroups, each a start and end and k's stages, or the weights' way from memory.  Group sizes
@@ -269,17 +290,32 @@ constexpr int kFewRowsPerGroup = 10;
 template <bool INT8>
 static int launch_grouped(const GroupedArgs& a, hipStream_t stream) {
     const int groups = a.experts < a.count ? a.experts : a.count;
-    return a.count / groups <= kFewRowsPerGroup ? launch_few_rows<INT8>(a, groups, stream) : launch_grouped_tiles(a, INT8, groups, stream);
+    if (a.count / groups > kFewRowsPerGroup) return launch_grouped_tiles(a, INT8, groups, stream);
+    const float active = a.experts * (1.f - powf(1.f - 1.f / a.experts, (float)a.count));  // groups that have rows, if all are as likely
+    return launch_few_rows<INT8>(a, few_rows_kernel(a.n, a.k, fmaxf(active, 1.f), a.count / fmaxf(active, 1.f)), stream);
 }
 
-// One int8 weight: up to 16 rows the rows kernel, more the tiled one, k in parts where that is worth clearing their counters (a launch of 2 us) and the caller gave
-// memory for them.
+// One int8 weight: up to 16 rows the rows kernel, up to 32 the one with the smaller predicted time (32 x 4096 x 4096 9.1 us, on tiles 11.4; 32 x 28672 x 4096 41.9 and
+// 31.8), more the tiled one, k in parts where that is worth clearing their counters (a launch of 2 us) and the caller gave memory for them.
 constexpr int kDenseFewRows = 16;
 
-static hfrk_tiled_plan int8_plan(int m, int n, int k, bool split) {
+static hfrk_tiled_plan int8_plan(int m, int n, int k, bool split, float* us) {
     hfrk_tiled_plan whole, parts;
-    const float t = make_tiled_plan(m, n, k, 1, &whole);
-    return split && make_tiled_plan(m, n, k, kTiledMaxSplits, &parts) + 2.f < t ? parts : whole;
+    *us = make_tiled_plan(m, n, k, 1, &whole);
+    const float shared = split ? make_tiled_plan(m, n, k, kTiledMaxSplits, &parts) + 2.f : *us;
+    if (shared >= *us) return whole;
+    *us = shared;
+    return parts;
+}
+
+// The plan, or (false) that the rows kernel `few` is to run.
+static bool int8_on_tiles(int m, int n, int k, bool split, hfrk_tiled_plan* p, FewRows* few) {
+    const float tiles16 = (float)((m + 15) / 16);
+    *few = few_rows_kernel(n, k, tiles16, m / tiles16);
+    if (m <= kDenseFewRows) return false;
+    float us;
+    *p = int8_plan(m, n, k, split, &us);
+    return m > 2 * kDenseFewRows || us < few->us;
 }
 
 static size_t int8_workspace_bytes(const hfrk_tiled_plan& p, int m, int n) { return tiled_plan_ws_bytes(p, m, n) + (size_t)tiled_plan_counters(p, m, n) * sizeof(int); }
@@ -289,10 +325,12 @@ __global__ void __launch_bounds__(256) clear_counters_kernel(int* counters, int 
 }
 
 static int launch_int8(const GroupedArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-    if (a.count <= kDenseFewRows) return launch_few_rows<true>(a, 1, stream);
     if (!tiled_size_ok(a.count, a.n, a.k)) return HFRK_BAD_SHAPE;
-    hfrk_tiled_plan p = int8_plan(a.count, a.n, a.k, workspace != nullptr);
-    if (int8_workspace_bytes(p, a.count, a.n) > workspace_bytes) p = int8_plan(a.count, a.n, a.k, false);
+    hfrk_tiled_plan p{};
+    FewRows few;
+    bool tiles = int8_on_tiles(a.count, a.n, a.k, workspace != nullptr, &p, &few);
+    if (tiles && int8_workspace_bytes(p, a.count, a.n) > workspace_bytes) tiles = int8_on_tiles(a.count, a.n, a.k, false, &p, &few);
+    if (!tiles) return launch_few_rows<true>(a, few, stream);
     const size_t partials = tiled_plan_ws_bytes(p, a.count, a.n);
     int* const counters = p.splits > 1 ? reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + partials) : nullptr;
     if (counters) {
@@ -359,8 +397,9 @@ int hfrk_grouped_gemm(const hfrk_grouped_args* args, void* stream) {
 
 size_t hfrk_int8_gemm_workspace_bytes(int m, int n, int k) {
     using namespace hfrk;
-    if (m <= kDenseFewRows || !tiled_size_ok(m, n, k)) return 0;
-    return int8_workspace_bytes(int8_plan(m, n, k, true), m, n);
+    hfrk_tiled_plan p{};
+    FewRows few;
+    return tiled_size_ok(m, n, k) && int8_on_tiles(m, n, k, true, &p, &few) ? int8_workspace_bytes(p, m, n) : 0;
 }
 
 int hfrk_int8_gemm(const void* A, const void* B, void* D, const void* base, int base_stride, const float* scale_a, int sa_stride, const float* scale_b,
