@@ -26,37 +26,20 @@ struct RouteArgs {
     int32_t* places;
     int32_t* rows;
     int32_t* offsets;
-    int64_t stride;  // elements between rows of the logits
+    int32_t* counts;  // workspace: every run's pairs of every expert
+    int64_t stride;   // elements between rows of the logits
     int tokens, count, top, dtype, sigmoid, renormalize;
     float factor;
 };
 
-template <typename T>
-__device__ __forceinline__ T unsigned_max(T a, T b) { return a > b ? a : b; }
-
-template <int CTRL, typename T>
-__device__ __forceinline__ T lanes_moved(T x) {
-    if constexpr (sizeof(T) == 4) {
-        return (T)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
-    } else {
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, 0xf, 0xf, true);
-        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, 0xf, 0xf, true);
-        return (uint64_t)hi << 32 | lo;
-    }
-}
-
-// The largest of the wave's values, the same bits in every lane (rotations within rows of 16 lanes, then the four rows).
-template <typename T>
-__device__ __forceinline__ T wave_max_of(T x) {
-    x = unsigned_max(x, lanes_moved<0x121>(x));
-    x = unsigned_max(x, lanes_moved<0x122>(x));
-    x = unsigned_max(x, lanes_moved<0x124>(x));
-    x = unsigned_max(x, lanes_moved<0x128>(x));
-    auto lane = [&](int l) __attribute__((always_inline)) {
-        if constexpr (sizeof(T) == 4) return (T)__builtin_amdgcn_readlane((int)x, l);
-        else return (T)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l));
-    };
-    return unsigned_max(unsigned_max(lane(0), lane(16)), unsigned_max(lane(32), lane(48)));
+// The largest of the wave's values, the same bits in every lane: rotations within rows of 16 lanes, then the four rows.
+__device__ __forceinline__ uint32_t wave_max_unsigned(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));
+    const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)x, 0), (uint32_t)__builtin_amdgcn_readlane((int)x, 16));
+    return max(a, max((uint32_t)__builtin_amdgcn_readlane((int)x, 32), (uint32_t)__builtin_amdgcn_readlane((int)x, 48)));
 }
 
 // Values as unsigned integers in the same order, above zero; zero for what is never chosen: NaN and minus infinity.  Both zeros are one.
@@ -72,50 +55,138 @@ __device__ __forceinline__ uint64_t order_of(double x) {
     return x > -(double)INFINITY ? b ^ ((b >> 63) ? ~0ull : 1ull << 63) : 0ull;
 }
 
+// e^x as 2^(x log2 e) by the hardware's exponential: off by 2^-23 and by 1.5 |x| 2^-24 of itself, which is least where the result is large.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504089f); }
+
 __device__ __forceinline__ double wave_sum_wide(double v) {
 #pragma unroll
     for (int by = 32; by; by >>= 1) v += __shfl_xor(v, by);
     return v;
 }
 
-// One wave, one token: expert lane + 64 j in register j.  Choice i's expert (-1: there is none) and weight come back in lane i.
+__device__ __forceinline__ float logit_of(const RouteArgs& a, int token, int e) {
+    const long at = token * a.stride + e;
+    if (a.dtype == HFRK_FP32) return static_cast<const float*>(a.logits)[at];
+    return a.dtype == HFRK_BF16 ? load16<HFRK_BF16>(static_cast<const uint16_t*>(a.logits)[at]) : load16<HFRK_F16>(static_cast<const uint16_t*>(a.logits)[at]);
+}
+
+// The `top` largest keys of a wave in order, choice i's expert (`id`) in lane i of `chosen` (-1: there is none).  Keys are hi or (WIDE) hi and lo as one number,
+// zero for what is never chosen.  A lane sorts its own once, so that a choice looks at one value a lane, and of equal ones takes that of the lowest lane, whose experts
+// have the lowest numbers.  GAPS: whether each choice, and the best one left, is further below the one in front than twice what 32 bits may be off: then
+// sums in 64 bits choose the same.
+template <int EPL, bool WIDE, bool GAPS>
+__device__ __forceinline__ bool choose_largest(uint32_t (&hi)[EPL], uint32_t (&lo)[EPL], int (&id)[EPL], int top, int* chosen) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int r = 0; r < EPL; ++r)
+#pragma unroll
+        for (int j = r & 1; j + 1 < EPL; j += 2) {  // neighbours change places where the second is above
+            const bool swap = WIDE ? ((uint64_t)hi[j + 1] << 32 | lo[j + 1]) > ((uint64_t)hi[j] << 32 | lo[j]) : hi[j + 1] > hi[j];
+            auto exchange = [&](auto& p, auto& q) __attribute__((always_inline)) {
+                const auto up = swap ? q : p;
+                q = swap ? p : q;
+                p = up;
+            };
+            exchange(hi[j], hi[j + 1]);
+            if constexpr (WIDE) exchange(lo[j], lo[j + 1]);
+            exchange(id[j], id[j + 1]);
+        }
+    *chosen = -1;
+    bool apart = true;
+    float above = INFINITY;
+    for (int i = 0; i < top + (GAPS ? 1 : 0); ++i) {
+        const uint32_t best = wave_max_unsigned(hi[0]);
+        if (best == 0) break;  // (a key's upper half is above zero: the smallest is that of the lowest number)
+        if constexpr (GAPS) {
+            const float value = __uint_as_float(best ^ ((best >> 31) ? 0x80000000u : 0xffffffffu));
+            apart = apart && above - value > 0x1p-18f * (1.0f + fabsf(value));  // (also false where it is no number)
+            above = value;
+        }
+        uint64_t equal = __ballot(hi[0] == best);
+        if constexpr (WIDE) {
+            if (equal & (equal - 1)) {  // rarely: upper halves are equal
+                const uint32_t low = wave_max_unsigned(hi[0] == best ? lo[0] : 0u);
+                equal = __ballot(hi[0] == best && lo[0] == low);
+            }
+        }
+        const int owner = __builtin_ctzll(equal), expert = __builtin_amdgcn_readlane(id[0], owner);
+        if (!GAPS || i < top) *chosen = lane == i ? expert : *chosen;
+        const bool mine = lane == owner;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+            hi[j] = mine ? (j + 1 < EPL ? hi[j + 1] : 0u) : hi[j];
+            if constexpr (WIDE) lo[j] = mine ? (j + 1 < EPL ? lo[j + 1] : 0u) : lo[j];
+            if (j + 1 < EPL) id[j] = mine ? id[j + 1] : id[j];
+        }
+    }
+    return apart;
+}
+
+// One wave, one token; lane l has the experts EPL l ... in registers.  Choice i's expert (-1: there is none) and weight come back in lane i; what a weight needs is
+// computed for the choices only.  With a bias the choice is made in 32 bits first and is what 64 give where its values lie far enough apart: s is off by
+// less than 2^-19 (e^-y is off by (2 + 1.5 y) 2^-24 e^-y, below 2^-22.5 for any y; the reciprocal by 2^-23 of s; a sum of 512 positive terms along chains of 14 steps by
+// 2^-20 of itself), s + bias by another 2^-24 of itself; a third of a percent of 256 experts' tokens lie closer and are done again.  16000 tokens on 8 of 256 experts 54 -> 28 us with sorted lanes, and with this 28 -> 16.
 template <int EPL, bool BIAS>
 __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, int token, int* chosen, float* weight) {
-    using Key = std::conditional_t<BIAS, uint64_t, uint32_t>;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, first = lane * EPL;
     *chosen = -1;
     *weight = 0.f;
     if (a.mask && !a.mask[token]) return;
-    float x[EPL], score[EPL];
-    Key key[EPL];
+    // through a buffer over the token's row: no branch, so that all are requested together
+    float x[EPL];
+    if (a.dtype == HFRK_FP32) {
+        const __amdgpu_buffer_rsrc_t row = make_rsrc(static_cast<const float*>(a.logits) + token * a.stride, (uint32_t)experts * 4u);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) x[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(row, (first + j) * 4, 0, 0));
+    } else {
+        const __amdgpu_buffer_rsrc_t row = make_rsrc(static_cast<const uint16_t*>(a.logits) + token * a.stride, (uint32_t)experts * 2u);
+        uint16_t h[EPL];
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) h[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(row, (first + j) * 2, 0, 0);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) x[j] = a.dtype == HFRK_BF16 ? load16<HFRK_BF16>(h[j]) : load16<HFRK_F16>(h[j]);
+    }
+    float bias[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-        const int e = lane + 64 * j;
-        const long at = token * a.stride + e;
-        x[j] = -INFINITY;
-        if (e < experts) {
-            if (a.dtype == HFRK_FP32) x[j] = static_cast<const float*>(a.logits)[at];
-            else if (a.dtype == HFRK_BF16) x[j] = load16<HFRK_BF16>(static_cast<const uint16_t*>(a.logits)[at]);
-            else x[j] = load16<HFRK_F16>(static_cast<const uint16_t*>(a.logits)[at]);
+        x[j] = first + j < experts ? x[j] : -INFINITY;
+        bias[j] = BIAS ? a.bias[min(first + j, experts - 1)] : 0.f;
+    }
+    bool none = false;  // a logit is NaN
+    float most = x[0];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        none |= x[j] != x[j];
+        most = fmaxf(most, x[j]);
+    }
+    none = __ballot(none) != 0;
+    float sum = 1.f, e[EPL];
+    if (!a.sigmoid) {
+        most = wave_max(most);
+        if (most == -INFINITY) most = 0.f;
+        float part = 0.f;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+            e[j] = exp_of(x[j] - most);
+            part += e[j];
+        }
+        sum = wave_sum(part);
+    }
+    uint32_t hi[EPL], lo[EPL];
+    int id[EPL];
+    const float each = __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        id[j] = first + j;
+        lo[j] = 0u;
+        if constexpr (BIAS) {
+            const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_of(-x[j])) : e[j] * each;
+            hi[j] = x[j] > -INFINITY ? order_of(s + bias[j]) : 0u;
+        } else {
+            hi[j] = order_of(x[j]);
         }
     }
-    // scores; the sum over all experts is NaN where a logit is
-    float most = x[0], sum = 0.f;
-#pragma unroll
-    for (int j = 1; j < EPL; ++j) most = fmaxf(most, x[j]);
-    most = wave_max(most);
-    if (most == -INFINITY) most = 0.f;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-        score[j] = a.sigmoid ? 1.0f / (1.0f + expf(-x[j])) : expf(x[j] - most);
-        sum += score[j];
-    }
-    sum = wave_sum(sum);
-    if (!a.sigmoid) {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) score[j] = score[j] / sum;
-    }
-    if constexpr (BIAS) {
+    if (!choose_largest<EPL, false, BIAS>(hi, lo, id, a.top, chosen) && BIAS) {
         double wide[EPL], whole = 0.0;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
@@ -125,43 +196,24 @@ __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, 
         if (!a.sigmoid) whole = wave_sum_wide(whole);
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
-            const int e = lane + 64 * j;
             const double s = a.sigmoid ? wide[j] : wide[j] / whole;
-            key[j] = x[j] > -INFINITY ? order_of(s + (double)(e < experts ? a.bias[e] : 0.f)) : 0;
+            const uint64_t key = x[j] > -INFINITY ? order_of(s + (double)bias[j]) : 0;
+            id[j] = first + j;
+            hi[j] = (uint32_t)(key >> 32);
+            lo[j] = (uint32_t)key;
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) key[j] = order_of(x[j]);
+        choose_largest<EPL, true, false>(hi, lo, id, a.top, chosen);
     }
-
-    for (int i = 0; i < a.top; ++i) {
-        Key mine = key[0];
-#pragma unroll
-        for (int j = 1; j < EPL; ++j) mine = unsigned_max(mine, key[j]);
-        const Key best = wave_max_of(mine);
-        if (best == 0) break;
-        bool found = false;
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-            const uint64_t equal = found ? 0 : __ballot(key[j] == best);
-            if (equal) {
-                const int owner = __builtin_ctzll(equal);
-                const float s = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(score[j]), owner));
-                if (lane == owner) key[j] = 0;
-                if (lane == i) {
-                    *chosen = owner + 64 * j;
-                    *weight = s;
-                }
-                found = true;
-            }
-        }
+    if (*chosen >= 0) {
+        const float l = logit_of(a, token, *chosen);
+        *weight = a.sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - most) / sum;
     }
     if (a.renormalize) {
         const float part = wave_sum(*weight);
         if (part != 0.f) *weight = *weight / part;
     }
     *weight *= a.factor;
-    if (sum != sum) *weight = NAN;
+    if (none) *weight = NAN;
 }
 
 // A token a wave; pairs that are nothing get their place here.
@@ -180,51 +232,95 @@ __global__ void __launch_bounds__(256) choose_experts_kernel(const RouteArgs a, 
     }
 }
 
-// Workgroup e puts expert e's pairs in order: it counts the pairs of lower experts and its own, a wave each sixteenth of them, and then goes through
-// its part again.  The last workgroup has what is behind the last expert.
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+// The pairs in the experts' order: each of up to 128 workgroups has a run of pairs.  Each counts its run's pairs of every expert, and in a second launch adds the
+// runs' counts: those in front of its own and all, which say where its pairs begin; then it deals its run out, 1024 pairs at a time, a wave finding the lanes of
+// the same expert by the bits of its number.  (A workgroup an expert, each going through all pairs twice, took 50 us of 128000 pairs and 256 experts, every
+// workgroup counting all pairs in LDS 21; the two launches take 8.)
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortGroups = 128;
 
-__global__ void __launch_bounds__(kSortThreads) sort_pairs_kernel(const RouteArgs a, int experts) {
-    __shared__ int lower[kSortWaves], same[kSortWaves];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = blockIdx.x;
-    const int part = ((a.count + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
-    const int from = min(wave * part, a.count), to = min(from + part, a.count);
-    int below = 0, equal = 0;
-#pragma unroll 8
-    for (int i = from + lane; i < to; i += 64) {
+__global__ void __launch_bounds__(kSortThreads) count_pairs_kernel(const RouteArgs a, int experts, int run) {
+    __shared__ int counts[kMaxExperts];
+    const int tid = threadIdx.x, from = blockIdx.x * run, to = min(from + run, a.count);
+    if (tid < kMaxExperts) counts[tid] = 0;
+    __syncthreads();
+    for (int i = from + tid; i < to; i += kSortThreads) {
         const int e = a.experts[i];
-        below += (uint32_t)e < (uint32_t)mine;
-        equal += e == mine;
-    }
-    below = __builtin_amdgcn_readlane(wave_prefix_sum(below), 63);
-    equal = __builtin_amdgcn_readlane(wave_prefix_sum(equal), 63);
-    if (lane == 0) {
-        lower[wave] = below;
-        same[wave] = equal;
+        if (e >= 0) atomicAdd(&counts[e], 1);  // (of integers: their order does not matter)
     }
     __syncthreads();
-    int start = 0, at = 0;
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-        start += lower[w];
-        at += w < wave ? same[w] : 0;
-    }
-    at += start;
-    if (threadIdx.x == 0) a.offsets[mine] = start;
-    if (mine == experts) {
-        for (int i = start + (int)threadIdx.x; i < a.count; i += kSortThreads) a.rows[i] = -1;
-        return;
-    }
-    if (equal == 0) return;
-    for (int i = from; i < to; i += 64) {
-        const bool hit = i + lane < to && a.experts[i + lane] == mine;
-        const uint64_t hits = __ballot(hit);
-        if (hit) {
-            const int place = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0));
-            a.places[i + lane] = place;
-            a.rows[place] = (i + lane) / a.top;
+    if (tid < experts) a.counts[blockIdx.x * experts + tid] = counts[tid];
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_pairs_kernel(const RouteArgs a, int experts, int run) {
+    __shared__ int before[kMaxExperts], all[kMaxExperts], of_wave[kSortWaves][kMaxExperts];
+    __shared__ int sums[kSortWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int from = blockIdx.x * run, to = min(from + run, a.count);
+    if (tid < kMaxExperts) before[tid] = all[tid] = 0;
+    __syncthreads();
+    {
+        const int shares = kSortThreads / experts, share = tid / experts, e = tid - share * experts;  // threads that share an expert's runs
+        int front = 0, behind = 0;
+        if (share < shares) {
+#pragma unroll 8
+            for (int r = share; r < (int)gridDim.x; r += shares) {
+                const int n = a.counts[r * experts + e];
+                if (r < (int)blockIdx.x) front += n;
+                else behind += n;
+            }
+            atomicAdd(&before[e], front);
+            atomicAdd(&all[e], behind);
         }
-        at += __builtin_popcountll(hits);
+    }
+    __syncthreads();
+    // where each expert begins, and in it this run's pairs
+    const int here = tid < kMaxExperts ? before[tid] + all[tid] : 0;
+    const int upto = wave_prefix_sum(here);
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int start = upto - here;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) start += w < wave ? sums[w] : 0;
+    if (tid < kMaxExperts) before[tid] += start;
+    if (blockIdx.x == 0 && tid <= experts) a.offsets[tid] = start;
+    // rows behind the last pair (the last thread's start is all pairs that have an expert)
+    __syncthreads();
+    if (tid == kSortThreads - 1) sums[0] = start;
+    __syncthreads();
+    const int held = sums[0];
+    for (int i = max(from, held) + tid; i < to; i += kSortThreads) a.rows[i] = -1;
+
+    const int bits = 32 - __builtin_clz(experts);
+    for (int chunk = from; chunk < to; chunk += kSortThreads) {
+        const int i = chunk + tid;
+        const int e = i < to ? a.experts[i] : -1;
+        for (int x = tid; x < kSortWaves * kMaxExperts; x += kSortThreads) (&of_wave[0][0])[x] = 0;
+        __syncthreads();
+        uint64_t same = __ballot(e >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot((e >> b) & 1);
+            same &= (e >> b) & 1 ? set : ~set;
+        }
+        const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+        if (e >= 0 && rank == 0) of_wave[wave][e] = __builtin_popcountll(same);
+        __syncthreads();
+        if (tid < experts) {  // the waves' pairs of an expert one after the other
+            int at = before[tid];
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) {
+                const int n = of_wave[w][tid];
+                of_wave[w][tid] = at;
+                at += n;
+            }
+            before[tid] = at;
+        }
+        __syncthreads();
+        if (e >= 0) {
+            const int place = of_wave[wave][e] + rank;
+            a.places[i] = place;
+            a.rows[place] = i / a.top;
+        }
+        __syncthreads();
     }
 }
 
@@ -272,14 +368,21 @@ __global__ void __launch_bounds__(kSortThreads) route_few_kernel(const RouteArgs
     }
 }
 
+static bool route_few(int tokens, int count) { return count <= kFewPairs && tokens <= 4 * kSortWaves; }
+
+static int route_run(int count) { return ((count + kSortGroups - 1) / kSortGroups + kSortThreads - 1) / kSortThreads * kSortThreads; }
+
 template <int EPL, bool BIAS>
 static int launch_route(const RouteArgs& a, int experts, hipStream_t stream) {
-    if (a.count <= kFewPairs && a.tokens <= 4 * kSortWaves) {
+    if (route_few(a.tokens, a.count)) {
         hipLaunchKernelGGL((route_few_kernel<EPL, BIAS>), dim3(1), dim3(kSortThreads), 0, stream, a, experts);
     } else {
         hipLaunchKernelGGL((choose_experts_kernel<EPL, BIAS>), dim3((a.tokens + 3) / 4), dim3(256), 0, stream, a, experts);
         HFRK_HIP_TRY(hipGetLastError());
-        hipLaunchKernelGGL(sort_pairs_kernel, dim3(experts + 1), dim3(kSortThreads), 0, stream, a, experts);
+        const int run = route_run(a.count), runs = (a.count + run - 1) / run;
+        hipLaunchKernelGGL(count_pairs_kernel, dim3(runs), dim3(kSortThreads), 0, stream, a, experts, run);
+        HFRK_HIP_TRY(hipGetLastError());
+        hipLaunchKernelGGL(sort_pairs_kernel, dim3(runs), dim3(kSortThreads), 0, stream, a, experts, run);
     }
     HFRK_HIP_TRY(hipGetLastError());
     return HFRK_SUCCESS;
@@ -345,11 +448,18 @@ __global__ void __launch_bounds__(256) combine_experts_kernel(const CombineArgs 
 
 extern "C" {
 
-int hfrk_route_experts(const hfrk_route_args* args, void* stream) {
+size_t hfrk_route_experts_workspace_bytes(int tokens, int num_experts, int top) {
+    using namespace hfrk;
+    if (tokens < 1 || num_experts < 1 || num_experts > kMaxExperts || top < 1 || (long)tokens * top > (1L << 28) || route_few(tokens, tokens * top)) return 0;
+    const int run = route_run(tokens * top);
+    return (size_t)((tokens * top + run - 1) / run) * num_experts * sizeof(int32_t);
+}
+
+int hfrk_route_experts(const hfrk_route_args* args, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace hfrk;
     if (!args) return HFRK_BAD_SHAPE;
     RouteArgs a{args->logits, args->bias, static_cast<const uint8_t*>(args->mask), args->weights, args->experts, args->places, args->rows, args->offsets,
-                args->logits_stride, args->tokens, 0, args->top, args->dtype, args->sigmoid, args->renormalize, args->factor};
+                static_cast<int32_t*>(workspace), args->logits_stride, args->tokens, 0, args->top, args->dtype, args->sigmoid, args->renormalize, args->factor};
     const int experts = args->num_experts;
     if (a.tokens < 0 || experts < 1 || experts > kMaxExperts || a.top < 1 || a.top > HFRK_MAX_TOP || a.top > experts) return HFRK_BAD_SHAPE;
     if (a.tokens > (1 << 24) || (long)a.tokens * a.top > (1L << 28) || a.stride < 0) return HFRK_BAD_SHAPE;
@@ -359,6 +469,8 @@ int hfrk_route_experts(const hfrk_route_args* args, void* stream) {
          reinterpret_cast<uintptr_t>(a.places) | reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.offsets)) & 3 ||
         reinterpret_cast<uintptr_t>(a.logits) & (a.dtype == HFRK_FP32 ? 3 : 1))
         return HFRK_BAD_ALIGNMENT;
+    if (workspace_bytes < hfrk_route_experts_workspace_bytes(a.tokens, experts, a.top) || (!workspace && workspace_bytes)) return HFRK_EXCEEDS_SCRATCH;
+    if (reinterpret_cast<uintptr_t>(workspace) & 3) return HFRK_BAD_ALIGNMENT;
     a.count = a.tokens * a.top;
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto with = [&](auto epl) {

@@ -1361,7 +1361,10 @@ int run_route(hfrk_route_args& r, const at::Tensor& logits, const at::Tensor& we
     r.places = places.data_ptr<int32_t>();
     r.rows = rows.data_ptr<int32_t>();
     r.offsets = offsets.data_ptr<int32_t>();
-    return hfrk_route_experts(&r, current_stream(logits));
+    // (memory of the call's own: streams and graphs share none)
+    const size_t bytes = hfrk_route_experts_workspace_bytes(r.tokens, r.num_experts, r.top);
+    const at::Tensor workspace = bytes ? at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte)) : at::Tensor();
+    return hfrk_route_experts(&r, bytes ? workspace.data_ptr() : nullptr, bytes, current_stream(logits));
 }
 
 void route_experts(const at::Tensor& logits, int64_t top, const std::optional<at::Tensor>& bias, bool sigmoid, bool renormalize, double factor,

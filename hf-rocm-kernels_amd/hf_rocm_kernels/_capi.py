@@ -164,7 +164,8 @@ SIGNATURES = {
     "hfrk_int8_gemm_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
     "hfrk_int8_gemm": (_i, [_p, _p, _p, _p, _i, _p, _i, _p] + [_i] * 6 + [_p, ctypes.c_size_t, _p]),
     "hfrk_grouped_gemm": (_i, [ctypes.POINTER(GroupedArgs), _p]),
-    "hfrk_route_experts": (_i, [ctypes.POINTER(RouteArgs), _p]),
+    "hfrk_route_experts_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
+    "hfrk_route_experts": (_i, [ctypes.POINTER(RouteArgs), _p, ctypes.c_size_t, _p]),
     "hfrk_combine_experts": (_i, [_p] * 5 + [_i] * 5 + [_p]),
     "hfrk_plan_table_load": (_i, [ctypes.c_char_p, _i, ctypes.POINTER(_i)]),
 }

@@ -532,8 +532,9 @@ int hfrk_grouped_gemm(const hfrk_grouped_args* args, void* stream);
  *   offsets  [num_experts + 1] int32: expert e has the pairs offsets[e] .. offsets[e+1]; offsets[0] = 0
  *   rows     [tokens * top] int32: the token of each pair, in the experts' order and within an expert in the tokens'; -1 behind the last pair
  *   places   [tokens, top] int32: where each pair is in that order, -1 for those of no expert
- * num_experts <= 512, top <= HFRK_MAX_TOP and num_experts, tokens <= 2^24, tokens * top <= 2^28.  Results share no memory with each other or the rest.  No workspace, no
- * atomics: equal calls give equal bits. */
+ * num_experts <= 512, top <= HFRK_MAX_TOP and num_experts, tokens <= 2^24, tokens * top <= 2^28.  Results share no memory with each other or the rest.
+ * Equal calls give equal bits.  workspace: hfrk_route_experts_workspace_bytes of it (0: none; 256 KB at most), 4-byte aligned, any contents, used by one call at a
+ * time: HFRK_EXCEEDS_SCRATCH. */
 #define HFRK_MAX_TOP 32
 typedef struct hfrk_route_args {
     const void* logits;
@@ -549,7 +550,8 @@ typedef struct hfrk_route_args {
     float factor;
 } hfrk_route_args;
 
-int hfrk_route_experts(const hfrk_route_args* args, void* stream);
+size_t hfrk_route_experts_workspace_bytes(int tokens, int num_experts, int top);
+int hfrk_route_experts(const hfrk_route_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* output[t] = (base ? base[t] : 0) + sum_j weights[t, j] * y[places[t, j]], fp32, one rounding.
  *   y [y_rows, cols], base [tokens, cols] or NULL, output [tokens, cols] of dtype (16-bit), rows side by side; weights [tokens, top] fp32, places [tokens, top]

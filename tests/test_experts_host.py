@@ -70,7 +70,8 @@ def _route(**changes):
     args = dict(logits=P, logits_stride=16, bias=None, mask=None, weights=P, experts=P, places=P, rows=P, offsets=P, tokens=4, num_experts=16, top=2, dtype=_capi.FP32,
                 sigmoid=0, renormalize=1, factor=1.0)
     args.update(changes)
-    return LIB.hfrk_route_experts(ctypes.byref(_capi.RouteArgs(**args)), None)
+    memory = args.pop("workspace", None), args.pop("bytes", 0)
+    return LIB.hfrk_route_experts(ctypes.byref(_capi.RouteArgs(**args)), *memory, None)
 
 
 @pytest.mark.parametrize("changes,status", [
@@ -78,9 +79,16 @@ def _route(**changes):
     ({"top": 33, "num_experts": 64}, _capi.BAD_SHAPE), ({"num_experts": 0}, _capi.BAD_SHAPE), ({"num_experts": 513}, _capi.BAD_SHAPE), ({"tokens": -1}, _capi.BAD_SHAPE),
     ({"tokens": (1 << 24) + 1}, _capi.BAD_SHAPE), ({"tokens": 1 << 24, "num_experts": 64, "top": 17}, _capi.BAD_SHAPE), ({"dtype": _capi.INT8}, _capi.BAD_DTYPE),
     ({"logits": P + 2}, _capi.BAD_ALIGNMENT), ({"rows": P + 1}, _capi.BAD_ALIGNMENT), ({"bias": P + 2}, _capi.BAD_ALIGNMENT), ({"logits_stride": -1}, _capi.BAD_SHAPE),
+    ({"tokens": 1000}, _capi.EXCEEDS_SCRATCH), ({"tokens": 1000, "workspace": P, "bytes": 127}, _capi.EXCEEDS_SCRATCH),
+    ({"tokens": 1000, "workspace": P + 2, "bytes": 4096}, _capi.BAD_ALIGNMENT), ({"bytes": 64}, _capi.EXCEEDS_SCRATCH),
 ])
 def test_route_experts_refuses_on_the_host(changes, status):
     assert _route(**changes) == status
+
+
+def test_route_experts_workspace():
+    sizes = [LIB.hfrk_route_experts_workspace_bytes(*x) for x in ((64, 128, 8), (65, 128, 8), (1000, 16, 2), (1 << 24, 512, 16), (16000, 256, 8), (0, 16, 2), (5, 600, 2))]
+    assert sizes == [0, 128 * 4, 2 * 16 * 4, 128 * 512 * 4, 125 * 256 * 4, 0, 0]
 
 
 def test_combine_and_quantise_refuse_on_the_host():
