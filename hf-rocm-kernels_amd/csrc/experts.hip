@@ -72,10 +72,10 @@ __device__ __forceinline__ float logit_of(const RouteArgs& a, int token, int e) 
 
 // The `top` largest keys of a wave in order, choice i's expert (`id`) in lane i of `chosen` (-1: there is none).  Keys are hi or (WIDE) hi and lo as one number,
 // zero for what is never chosen.  A lane sorts its own once, so that a choice looks at one value a lane, and of equal ones takes that of the lowest lane, whose experts
-// have the lowest numbers.  GAPS: whether each choice, and the best one left, is further below the one in front than twice what 32 bits may be off: then
-// sums in 64 bits choose the same.
+// have the lowest numbers.  GAPS: whether each choice, and the best one left, is further below the one in front than margin * (1 + its size), twice what 32 bits may be
+// off: then sums in 64 bits choose the same.
 template <int EPL, bool WIDE, bool GAPS>
-__device__ __forceinline__ bool choose_largest(uint32_t (&hi)[EPL], uint32_t (&lo)[EPL], int (&id)[EPL], int top, int* chosen) {
+__device__ __forceinline__ bool choose_largest(uint32_t (&hi)[EPL], uint32_t (&lo)[EPL], int (&id)[EPL], int top, float margin, int* chosen) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int r = 0; r < EPL; ++r)
@@ -99,7 +99,7 @@ __device__ __forceinline__ bool choose_largest(uint32_t (&hi)[EPL], uint32_t (&l
         if (best == 0) break;  // (a key's upper half is above zero: the smallest is that of the lowest number)
         if constexpr (GAPS) {
             const float value = __uint_as_float(best ^ ((best >> 31) ? 0x80000000u : 0xffffffffu));
-            apart = apart && above - value > 0x1p-18f * (1.0f + fabsf(value));  // (also false where it is no number)
+            apart = apart && above - value > margin * (1.0f + fabsf(value));  // (also false where it is no number)
             above = value;
         }
         uint64_t equal = __ballot(hi[0] == best);
@@ -122,11 +122,17 @@ __device__ __forceinline__ bool choose_largest(uint32_t (&hi)[EPL], uint32_t (&l
     return apart;
 }
 
+// Twice what s + bias may be off in 32 bits, for a sum of size v as margin * (1 + |v|).  e^-y is off by (2 + y) 2^-24 of itself (exponent rounded, hardware's
+// exponential within a step).  Sigmoid, 1 / (1 + e^-x): s (1 - s) times that is at most 0.6 * 2^-24, the sum 1 + e^-x adds 2^-24 s, the reciprocal 2^-23 s, s + bias
+// 2^-24 |v|: below 2^-22 (1 + |v|).  Softmax: s y is at most 0.37, the sum of up to 512 positive terms along chains of up to 20 is off by 22 * 2^-24 of itself, the
+// reciprocal and the product by 3 * 2^-24: below 2^-19 (1 + |v|).
+__device__ __forceinline__ float margin_of(const RouteArgs& a) { return a.sigmoid ? 0x1p-21f : 0x1p-18f; }
+
 // One wave, one token; lane l has the experts EPL l ... in registers.  Choice i's expert (-1: there is none) and weight come back in lane i; what a weight needs is
-// computed for the choices only.  With a bias the choice is made in 32 bits first and is what 64 give where its values lie far enough apart: s is off by
-// less than 2^-19 (e^-y is off by (2 + 1.5 y) 2^-24 e^-y, below 2^-22.5 for any y; the reciprocal by 2^-23 of s; a sum of 512 positive terms along chains of 14 steps by
-// 2^-20 of itself), s + bias by another 2^-24 of itself; a third of a percent of 256 experts' tokens lie closer and are done again.  16000 tokens on 8 of 256 experts 54 -> 28 us with sorted lanes, and with this 28 -> 16.
-template <int EPL, bool BIAS>
+// computed for the choices only.  With a bias the choice is made in 32 bits first and is what 64 give where its values lie far enough apart; the few tokens of
+// which they do not are done again.  16000 tokens on 8 of 256 experts, choosing in 64 bits at once: 28 us, with this 20.6.
+// AGAIN: 32 bits have left it open already.
+template <int EPL, bool BIAS, bool AGAIN = false>
 __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, int token, int* chosen, float* weight) {
     const int lane = threadIdx.x & 63, first = lane * EPL;
     *chosen = -1;
@@ -174,19 +180,23 @@ __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, 
     }
     uint32_t hi[EPL], lo[EPL];
     int id[EPL];
-    const float each = __builtin_amdgcn_rcpf(sum);
+    bool open = AGAIN;
+    if constexpr (!AGAIN) {
+        const float each = __builtin_amdgcn_rcpf(sum);
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-        id[j] = first + j;
-        lo[j] = 0u;
-        if constexpr (BIAS) {
-            const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_of(-x[j])) : e[j] * each;
-            hi[j] = x[j] > -INFINITY ? order_of(s + bias[j]) : 0u;
-        } else {
-            hi[j] = order_of(x[j]);
+        for (int j = 0; j < EPL; ++j) {
+            id[j] = first + j;
+            lo[j] = 0u;
+            if constexpr (BIAS) {
+                const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_of(-x[j])) : e[j] * each;
+                hi[j] = x[j] > -INFINITY ? order_of(s + bias[j]) : 0u;
+            } else {
+                hi[j] = order_of(x[j]);
+            }
         }
+        open = !choose_largest<EPL, false, BIAS>(hi, lo, id, a.top, margin_of(a), chosen);
     }
-    if (!choose_largest<EPL, false, BIAS>(hi, lo, id, a.top, chosen) && BIAS) {
+    if (open && BIAS) {
         double wide[EPL], whole = 0.0;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
@@ -202,7 +212,7 @@ __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, 
             hi[j] = (uint32_t)(key >> 32);
             lo[j] = (uint32_t)key;
         }
-        choose_largest<EPL, true, false>(hi, lo, id, a.top, chosen);
+        choose_largest<EPL, true, false>(hi, lo, id, a.top, 0.f, chosen);
     }
     if (*chosen >= 0) {
         const float l = logit_of(a, token, *chosen);
@@ -216,7 +226,14 @@ __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, 
     if (none) *weight = NAN;
 }
 
-// A token a wave; pairs that are nothing get their place here.
+__device__ __forceinline__ void store_choice(const RouteArgs& a, int token, int i, int chosen, float weight) {
+    const long at = (long)token * a.top + i;
+    a.weights[at] = weight;
+    a.experts[at] = chosen;
+    if (chosen < 0) a.places[at] = -1;  // pairs that are nothing get their place here
+}
+
+// A token a wave.
 template <int EPL, bool BIAS>
 __global__ void __launch_bounds__(256) choose_experts_kernel(const RouteArgs a, int experts) {
     const int lane = threadIdx.x & 63, token = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -224,11 +241,152 @@ __global__ void __launch_bounds__(256) choose_experts_kernel(const RouteArgs a, 
     int chosen;
     float weight;
     choose_experts<EPL, BIAS>(a, experts, token, &chosen, &weight);
-    if (lane < a.top) {
-        const long at = (long)token * a.top + lane;
-        a.weights[at] = weight;
-        a.experts[at] = chosen;
-        if (chosen < 0) a.places[at] = -1;
+    if (lane < a.top) store_choice(a, token, lane, chosen, weight);
+}
+
+template <typename T, typename OP>
+__device__ __forceinline__ T row_reduce(T v, OP op) {  // over the 16 lanes of a row, every one of which gets it
+    auto rotated = [](T x, auto by) __attribute__((always_inline)) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + decltype(by)::value, 0xf, 0xf, true));
+    };
+    v = op(v, rotated(v, std::integral_constant<int, 1>{}));
+    v = op(v, rotated(v, std::integral_constant<int, 2>{}));
+    v = op(v, rotated(v, std::integral_constant<int, 4>{}));
+    return op(v, rotated(v, std::integral_constant<int, 8>{}));
+}
+
+// Four tokens a wave, 16 lanes each: expert 16 j + lane in register j, sorted within the lane by key and, of equal keys, number.  Many tokens are bound by
+// the instructions of a choice, most of which are the same for one token and for four: 16000 tokens on 8 of 256 experts 15.2 -> 11.0 us, with a bias 21.0 -> 19.1 (of
+// which the tokens that are done again are the end), 4096 on 6 of 64 4.5 -> 3.9.  A single token waits longer for it.  Tokens whose choice 32 bits leave open are done again, a wave each.
+template <int EPL, bool BIAS>
+__global__ void __launch_bounds__(256) choose_many_kernel(const RouteArgs a, int experts) {
+    const int lane = threadIdx.x & 63, in_row = lane & 15, token0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 4, token = token0 + (lane >> 4);
+    if (token0 >= a.tokens) return;
+    const bool real = token < a.tokens && (!a.mask || a.mask[token]);
+    auto add = [](float x, float y) { return x + y; };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
+    auto above = [](uint32_t x, uint32_t y) { return max(x, y); };
+    float x[EPL];
+    {
+        // through a buffer over the wave's rows: no branch, so that all are requested together
+        const int size = a.dtype == HFRK_FP32 ? 4 : 2;
+        const uint32_t rows = (uint32_t)min(4, a.tokens - token0);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(static_cast<const uint8_t*>(a.logits) + token0 * a.stride * size, ((rows - 1) * (uint32_t)a.stride + (uint32_t)experts) * size);
+        const int at = ((lane >> 4) * (int)a.stride + in_row) * size;
+        if (a.dtype == HFRK_FP32) {
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) x[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at + j * 64, 0, 0));
+        } else {
+            uint16_t h[EPL];
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) h[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at + j * 32, 0, 0);
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) x[j] = a.dtype == HFRK_BF16 ? load16<HFRK_BF16>(h[j]) : load16<HFRK_F16>(h[j]);
+        }
+    }
+    bool none = false;
+    float most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        x[j] = j * 16 + in_row < experts ? x[j] : -INFINITY;
+        none |= x[j] != x[j];
+        most = fmaxf(most, x[j]);
+    }
+    none = row_reduce(none ? 1u : 0u, above) != 0u && real;
+    float sum = 1.f, e[EPL];
+    if (!a.sigmoid) {
+        most = row_reduce(most, larger);
+        if (most == -INFINITY) most = 0.f;
+        float part = 0.f;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+            e[j] = exp_of(x[j] - most);
+            part += e[j];
+        }
+        sum = row_reduce(part, add);
+    }
+    uint32_t hi[EPL], lo[EPL];  // the key, and the inverse of the expert's number: as one integer the larger is chosen first
+    const float each = __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        const int expert = j * 16 + in_row;
+        lo[j] = ~(uint32_t)expert;
+        if constexpr (BIAS) {
+            const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_of(-x[j])) : e[j] * each;
+            hi[j] = x[j] > -INFINITY ? order_of(s + a.bias[min(expert, experts - 1)]) : 0u;
+        } else {
+            hi[j] = order_of(x[j]);
+        }
+        hi[j] = real ? hi[j] : 0u;
+    }
+    // Batcher's merge exchange, largest first
+#pragma unroll
+    for (int p = 1; p < EPL; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < EPL; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < EPL && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const int u = i + j, v = i + j + k;
+                        const bool swap = ((uint64_t)hi[v] << 32 | lo[v]) > ((uint64_t)hi[u] << 32 | lo[u]);
+                        const uint32_t h0 = swap ? hi[v] : hi[u], h1 = swap ? hi[u] : hi[v], l0 = swap ? lo[v] : lo[u], l1 = swap ? lo[u] : lo[v];
+                        hi[u] = h0;
+                        hi[v] = h1;
+                        lo[u] = l0;
+                        lo[v] = l1;
+                    }
+    int chosen[2] = {-1, -1};  // choices in_row and in_row + 16
+    bool apart = true;
+    const float margin = margin_of(a);
+    float front = INFINITY;
+    for (int i = 0; i < a.top + (BIAS ? 1 : 0); ++i) {
+        const uint32_t best = row_reduce(hi[0], above);
+        const uint32_t number = row_reduce(hi[0] == best ? lo[0] : 0u, above);
+        if constexpr (BIAS) {
+            const float value = __uint_as_float(best ^ ((best >> 31) ? 0x80000000u : 0xffffffffu));
+            apart = apart && (best == 0 || front - value > margin * (1.0f + fabsf(value)));  // (also false where it is no number)
+            front = value;
+        }
+        const int expert = best ? (int)~number : -1;
+        if (i < 16) chosen[0] = in_row == i ? expert : chosen[0];
+        else if (i < a.top) chosen[1] = in_row == i - 16 ? expert : chosen[1];
+        const bool mine = lo[0] == number && best != 0;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+            hi[j] = mine ? (j + 1 < EPL ? hi[j + 1] : 0u) : hi[j];
+            if (j + 1 < EPL) lo[j] = mine ? lo[j + 1] : lo[j];
+        }
+    }
+    if (BIAS && a.top < 16) chosen[0] = in_row < a.top ? chosen[0] : -1;  // (the one beyond the last was looked at for its distance)
+    float weight[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        if (chosen[c] >= 0) {
+            const float l = logit_of(a, token, chosen[c]);
+            weight[c] = a.sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - most) / sum;
+        }
+    if (a.renormalize) {
+        const float part = row_reduce(weight[0] + weight[1], add);
+        if (part != 0.f) {
+            weight[0] /= part;
+            weight[1] /= part;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        weight[c] = none ? NAN : weight[c] * a.factor;
+        if (token < a.tokens && apart && in_row + 16 * c < a.top) store_choice(a, token, in_row + 16 * c, chosen[c], weight[c]);
+    }
+    if constexpr (BIAS) {
+        for (uint64_t again = __ballot(!apart && in_row == 0 && token < a.tokens); again; again &= again - 1) {
+            const int t = token0 + __builtin_ctzll(again) / 16;
+            int c;
+            float w;
+            choose_experts<(EPL + 3) / 4, true, true>(a, experts, t, &c, &w);
+            if (lane < a.top) store_choice(a, t, lane, c, w);
+        }
     }
 }
 
@@ -377,7 +535,11 @@ static int launch_route(const RouteArgs& a, int experts, hipStream_t stream) {
     if (route_few(a.tokens, a.count)) {
         hipLaunchKernelGGL((route_few_kernel<EPL, BIAS>), dim3(1), dim3(kSortThreads), 0, stream, a, experts);
     } else {
-        hipLaunchKernelGGL((choose_experts_kernel<EPL, BIAS>), dim3((a.tokens + 3) / 4), dim3(256), 0, stream, a, experts);
+        // four tokens a wave need more than 512 waves of them, and rows that a wave's buffer reaches
+        if (EPL <= 4 && a.tokens > 2048 && a.stride < (1 << 26))
+            hipLaunchKernelGGL((choose_many_kernel<EPL <= 4 ? 4 * EPL : 4, BIAS>), dim3((a.tokens + 15) / 16), dim3(256), 0, stream, a, experts);
+        else
+            hipLaunchKernelGGL((choose_experts_kernel<EPL, BIAS>), dim3((a.tokens + 3) / 4), dim3(256), 0, stream, a, experts);
         HFRK_HIP_TRY(hipGetLastError());
         const int run = route_run(a.count), runs = (a.count + run - 1) / run;
         hipLaunchKernelGGL(count_pairs_kernel, dim3(runs), dim3(kSortThreads), 0, stream, a, experts, run);

@@ -113,7 +113,8 @@ __device__ __forceinline__ bool find_tile(const Args& a, int bm, GroupTile* t) {
         t->tile = xcd_range_id(blockIdx.x, t->tiles_m * a.tiles_n);
         return t->tile >= 0;
     }
-    return a.experts <= 64 ? find_tile_of<1>(a, bm, t) : find_tile_of<kMaxExperts / 64>(a, bm, t);
+    if (a.experts <= 64) return find_tile_of<1>(a, bm, t);
+    return a.experts <= 128 ? find_tile_of<2>(a, bm, t) : find_tile_of<kMaxExperts / 64>(a, bm, t);
 }
 
 // The most tiles of `bm` rows that groups of `count` rows together can have: every group's last one may be partly filled.

@@ -35,6 +35,76 @@ def test_route(dtype, tokens, experts, top):
         _check(route_experts(logits, top, **options), logits, top, **options)
 
 
+def _many(logits, top, scoring, bias, mask=None):
+    """A route of many tokens by sorts in 64 bits: (experts, places, rows, offsets)."""
+    x = logits.double()
+    key = x if bias is None else (torch.softmax(x, 1) if scoring == "softmax" else torch.sigmoid(x)) + bias.double()
+    key = torch.where((x > -math.inf) & (key > -math.inf), key, -math.inf)
+    order = torch.sort(key, dim=1, descending=True, stable=True)
+    experts = torch.where(order.values[:, :top] > -math.inf, order.indices[:, :top], -1)
+    if mask is not None:
+        experts = torch.where(mask[:, None], experts, -1)
+    flat = experts.reshape(-1)
+    group = torch.where(flat < 0, logits.size(1), flat)
+    pairs = torch.sort(group, stable=True).indices
+    offsets = torch.searchsorted(group[pairs], torch.arange(logits.size(1) + 1, device=DEV))
+    held = torch.arange(flat.numel(), device=DEV) < offsets[-1]
+    places = torch.empty_like(flat)
+    places[pairs] = torch.where(held, torch.arange(flat.numel(), device=DEV), -1)
+    return experts, places.view_as(experts), torch.where(held, pairs // top, -1), offsets
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens,experts,top", [(2049, 4, 4), (3000, 60, 6), (2500, 64, 17), (4097, 128, 8), (2050, 129, 32), (5000, 256, 8), (16001, 200, 3), (2100, 384, 10)])
+def test_route_of_many_tokens(dtype, tokens, experts, top):
+    """bfloat16 logits repeat, so ties are many; a bias leaves choices that 32 bits cannot tell."""
+    gen = torch.Generator(device=DEV).manual_seed(tokens + top)
+    logits = (2 * torch.randn((tokens, experts + 3), generator=gen, device=DEV)).to(dtype)[:, 1:experts + 1]
+    logits[7] = -math.inf
+    logits[8, experts // 2:] = -math.inf
+    logits[9, 1] = math.nan
+    bias = 0.1 * torch.randn(experts, generator=gen, device=DEV)
+    bias[experts // 3] = bias[0] * (1 + 2.0 ** -22)  # sums one step of 32 bits apart
+    mask = torch.rand(tokens, generator=gen, device=DEV) < 0.9
+    for scoring, b, m in (("softmax", None, None), ("softmax", bias, mask), ("sigmoid", bias, None), ("sigmoid", None, mask)):
+        clean = torch.where(torch.isnan(logits), -math.inf, logits.float()).to(dtype)  # what is none is not chosen
+        route = route_experts(logits, top, bias=b, scoring=scoring, mask=m)
+        wanted = _many(clean, top, scoring, b, m)
+        if b is not None:  # the NaN in a softmax's sum leaves that row without a choice
+            keep = torch.arange(tokens, device=DEV) != 9
+            assert torch.equal(route.experts[keep].long(), wanted[0][keep])
+        else:
+            for got, want in zip((route.experts, route.places, route.rows, route.offsets), wanted):
+                assert torch.equal(got.long(), want)
+        score = torch.softmax(clean.double(), 1) if scoring == "softmax" else torch.sigmoid(clean.double())
+        weights = score.gather(1, wanted[0].clamp(min=0)).masked_fill(wanted[0] < 0, 0.0)
+        total = weights.sum(1, keepdim=True)
+        weights = torch.where(total > 0, weights / total, 0.0)
+        real = torch.ones(tokens, dtype=torch.bool, device=DEV) if m is None else m.clone()
+        if bool(real[9]):
+            assert torch.isnan(route.weights[9]).all()
+        rest = torch.arange(tokens, device=DEV) != 9
+        rest[7] = False
+        # as in _check, and the choices' sum
+        assert ((route.weights.double() - weights).abs()[rest] <= 2.0 ** -17 * weights[rest] + 1e-37).all()
+        assert (route.weights[7] == 0).all() and (route.weights[~real] == 0).all()
+
+
+@pytest.mark.parametrize("tokens", [100, 3000])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_with_a_bias_that_32_bits_cannot_tell(tokens, scoring):
+    """Sums that are equal in 32 bits and not in 64, and sums that are equal in both."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    logits = torch.randn((tokens, 96), generator=gen, device=DEV) * 2.0 ** -14
+    bias = torch.full((96,), 4.0, device=DEV)
+    route = route_experts(logits, 6, bias=bias, scoring=scoring)
+    wanted = _many(logits, 6, scoring, bias)
+    for got, want in zip((route.experts, route.places, route.rows, route.offsets), wanted):
+        assert torch.equal(got.long(), want)
+    same = route_experts(torch.zeros_like(logits), 6, bias=bias, scoring=scoring)
+    assert (same.experts == torch.arange(6, device=DEV)).all()
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("tokens,experts,top", [(5, 16, 3), (100, 200, 8), (400, 65, 4)])
 def test_route_with_a_bias_and_padding(scoring, tokens, experts, top):
