@@ -32,6 +32,25 @@ struct TiledGroupedArgs : TiledGemmArgs {
     int count, a_rows, experts;
 };
 
+// Tiles of the tiled kernel on groups: the four largest of the dense shapes, and 128 x 128 in five halves of stages, 80 KB, on eight waves that load for themselves, so
+// that two workgroups share a compute unit and one multiplies while the other starts or ends.  A group has few tiles and often a short k: start and end are a third
+// of the time there (333 tokens on 4 of 60 experts of 2816 x 2048: 128 x 128 79.9 -> 73.8 us, with four waves 75.4; 512 on 8 of 128 of 2048 x 768 77.5 -> 59.1;
+// 1024 on 6 of 64 of 2048 x 1408 66.9 -> 58.7).  64 x 128 in the same way gains up to 5 % more where groups have some twenty rows and loses as much above: left out.
+// X(index, TM, TN, WM, WN, NST, WGS) as in HFRK_TILED_SHAPES
+#define HFRK_GROUP_SHAPES(X) \
+    X(0, 4, 2, 2, 4, 5, 1)   \
+    X(1, 2, 2, 4, 2, 3, 1)   \
+    X(2, 2, 2, 2, 2, 5, 1)   \
+    X(3, 2, 1, 2, 2, 3, 2)
+#define HFRK_GROUP_PAIRED(X) X(4, 2, 1, 2, 4, 5, 2)
+
+#define HFRK_GROUP_ROW(I, TM, TN, WM, WN, NST, WGS) {32 * TM * WM, 32 * TN * WN, NST, WGS, tiled_half_stages(TM, WM * WN), 64 * (WM * WN + tiled_loader_waves(TM))},
+#define HFRK_GROUP_PAIR(I, TM, TN, WM, WN, NST, WGS) {32 * TM * WM, 32 * TN * WN, NST, WGS, true, 64 * WM * WN},
+constexpr TiledShape kGroupedShapes[] = {HFRK_GROUP_SHAPES(HFRK_GROUP_ROW) HFRK_GROUP_PAIRED(HFRK_GROUP_PAIR)};
+#undef HFRK_GROUP_PAIR
+#undef HFRK_GROUP_ROW
+constexpr int kGroupedShapeCount = sizeof(kGroupedShapes) / sizeof(kGroupedShapes[0]);
+
 constexpr int kMaxExperts = 512;
 constexpr int kOutsideBuffer = 0x7ffffff0;  // beyond the range of every buffer made here
 

@@ -53,17 +53,6 @@ constexpr bool tiled_half_stages(int tm, int waves) { return tm * waves >= 32; }
 // Waves of a workgroup that only load, beside the WM x WN that multiply (tiled_gemm_kernel.h).
 constexpr int tiled_loader_waves(int tm) { return tm < 4 ? 4 : 0; }
 
-// Groups (grouped_gemm.hip): the four largest shapes, and 128 x 128 in five halves of stages, 80 KB, whose waves load for themselves, so that two workgroups share
-// a compute unit and one multiplies while the other starts or ends.  A group has few tiles and often a short k: start and end are a third of the time
-// there (333 rows of 60 experts, 4 each, 2816 x 2048 fp8: 128 x 128 84.4 -> 76.9 us; 512 tokens, 8 of 128, 2048 x 768 83.9 -> 63.5; 8 x 28672 x 4096 with 250 tokens
-// each 323 -> 310).
-#define HFRK_TILED_GROUPED(X) \
-    X(0, 4, 2, 2, 4, 5, 1)    \
-    X(1, 2, 2, 4, 2, 3, 1)    \
-    X(2, 2, 2, 2, 2, 5, 1)    \
-    X(3, 2, 1, 2, 2, 3, 2)
-#define HFRK_TILED_PAIRED(X) X(4, 2, 2, 2, 2, 5, 2)
-
 struct TiledShape {
     int bm, bn, stages, per_cu;
     bool halves;
@@ -71,10 +60,6 @@ struct TiledShape {
 };
 #define HFRK_TILED_ROW(I, TM, TN, WM, WN, NST, WGS) {32 * TM * WM, 32 * TN * WN, NST, WGS, tiled_half_stages(TM, WM * WN), 64 * (WM * WN + tiled_loader_waves(TM))},
 constexpr TiledShape kTiledShapes[] = {HFRK_TILED_SHAPES(HFRK_TILED_ROW)};
-#define HFRK_TILED_PAIR(I, TM, TN, WM, WN, NST, WGS) {32 * TM * WM, 32 * TN * WN, NST, WGS, true, 64 * WM * WN},
-constexpr TiledShape kGroupedShapes[] = {HFRK_TILED_GROUPED(HFRK_TILED_ROW) HFRK_TILED_PAIRED(HFRK_TILED_PAIR)};
-constexpr int kGroupedShapeCount = sizeof(kGroupedShapes) / sizeof(kGroupedShapes[0]);
-#undef HFRK_TILED_PAIR
 #undef HFRK_TILED_ROW
 #define HFRK_TILED_SAME(I, TM, TN, WM, WN, NST, WGS) \
     static_assert(kTiledShapes[I].bm == 32 * TM * WM && kTiledShapes[I].bn == 32 * TN * WN && kTiledShapes[I].stages == NST && kTiledShapes[I].per_cu == WGS);

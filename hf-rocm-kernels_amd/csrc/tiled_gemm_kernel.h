@@ -501,11 +501,11 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
         auto fetch = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int r = 0; r < PASSES; ++r) {
-                int row = row0 + i * 32 + r * RPI + lane / LPR;
+                int at = (row0 + i * 32 + r * RPI + lane / LPR) * a.sa_stride * 4;
                 if constexpr (GROUPED) {
-                    if (gathers) row = from[i * PASSES + r] < 0 ? kOutside / 4 : from[i * PASSES + r];
+                    if (gathers) at = from[i * PASSES + r] < 0 ? kOutside : from[i * PASSES + r] * a.sa_stride * 4;
                 }
-                sa[i & 1][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsa, row * a.sa_stride * 4, 0, 0));
+                sa[i & 1][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsa, at, 0, 0));
                 add[i & 1][r] = __builtin_amdgcn_raw_buffer_load_b128(rbase, (int)(base_off + (uint32_t)(i * PASSES + r) * base_step), 0, 0);
             }
         };
@@ -547,11 +547,12 @@ __global__ void __launch_bounds__(64 * (WM * WN + LW), WGS * (WM * WN + LW) / 4)
                     int row = m;
                     if constexpr (GROUPED) {
                         if (m >= m0 + rows_a || n >= a.n) continue;
-                        if (gathers) row = max(row_of_number(m - m0, row_number(m - m0)), 0);  // (no row: a sum of zero, times some scale)
+                        if (gathers) row = row_of_number(m - m0, row_number(m - m0));
                     } else {
                         if (m >= a.m || n >= a.n) continue;
                     }
-                    float x = stage[r * RS + c] * (a.scale_a[(long)row * a.sa_stride] * (scales_b ? scales_b[(long)n * a.sb_stride] : 1.0f));
+                    float x = 0.f;  // (of a row that A does not have)
+                    if (!GROUPED || row >= 0) x = stage[r * RS + c] * (a.scale_a[(long)row * a.sa_stride] * (scales_b ? scales_b[(long)n * a.sb_stride] : 1.0f));
                     if (a.base) x += load16<DT>(static_cast<const uint16_t*>(a.base)[(long)m * a.base_stride + n]);
                     static_cast<uint16_t*>(a.D)[(long)m * a.n + n] = (uint16_t)pack_pair<DT>(x, 0.f);
                 }
@@ -606,11 +607,11 @@ static int launch_tiled_groups(const TiledGroupedArgs& args, int shape, long gri
     switch (shape) {
 #define HFRK_TILED_CASE(I, TM, TN, WM, WN, NST, WGS) \
     case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, false, tiled_loader_waves(TM), INT8, true>(args, tiled_lds_bytes(kGroupedShapes[I]), stream, grid);
-        HFRK_TILED_GROUPED(HFRK_TILED_CASE)
+        HFRK_GROUP_SHAPES(HFRK_TILED_CASE)
 #undef HFRK_TILED_CASE
 #define HFRK_TILED_CASE(I, TM, TN, WM, WN, NST, WGS) \
     case I: return launch_tiled_shape<TM, TN, WM, WN, NST, WGS, false, 0, INT8, true, true>(args, tiled_lds_bytes(kGroupedShapes[I]), stream, grid);
-        HFRK_TILED_PAIRED(HFRK_TILED_CASE)
+        HFRK_GROUP_PAIRED(HFRK_TILED_CASE)
 #undef HFRK_TILED_CASE
     }
     return HFRK_INVALID_CONFIG;

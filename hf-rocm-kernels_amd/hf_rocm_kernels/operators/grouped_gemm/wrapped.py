@@ -69,7 +69,7 @@ def grouped_gemm(
         - offsets: (experts + 1,) int32, not decreasing, as `route_experts` gives them.  They stay on the device: no call waits for them, and a captured call
           may be replayed with others
         - rows: (count,) int32 or None: the row of a for each row of the result (`route_experts`' rows: a first projection picks the tokens' rows).  A
-          number that is no row of a gives zeros
+          number that is no row of a counts as a row of zeros
         - output: a (count, n) tensor to write to, or None for a new one of out_dtype (bfloat16 or float16)
     Outputs:
         - (count, n); rows in front of offsets[0] and behind the last group's are not written.  Inference only: the result carries no gradient

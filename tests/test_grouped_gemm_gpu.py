@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import hf_rocm_kernels
+from hf_rocm_kernels import _capi
 from hf_rocm_kernels import grouped_gemm, int8_gemm, quantize_int8, swiglu_dynamic
 from hf_rocm_kernels.layers import Int8Linear, apply_int8_linear, convert_linear_layers
 from hf_rocm_kernels.operators.grouped_gemm import reference_grouped_gemm
@@ -145,6 +146,27 @@ def test_grouped_row_numbers_that_are_no_rows_give_zeros(size):
         good = ((rows[here] >= 0) & (rows[here] < 9)).nonzero().flatten()
         ae, se = a.view(torch.uint8)[index[here][good]].view(FP8), sa[index[here][good]]
         _close(out[here][good], exact[here][good], _magnitude(ae, w[e], se, sb[e]), 128, FP8, cut=_cut(ae, w[e], se, sb[e]))
+
+
+@pytest.mark.parametrize("n", [32, 31])
+@pytest.mark.parametrize("size", [4, 130])
+def test_grouped_scales_of_other_rows_do_not_reach_rows_that_are_none(size, n):
+    """The first row's scale is infinite: rows that pick no row of `a` are zero, those that pick another one are that row's."""
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    a, w = _codes(gen, (9, 128), INT8), _codes(gen, (2, n, 128), INT8)
+    rows = torch.randint(1, 9, (2 * size,), generator=gen, device=DEV, dtype=torch.int32)
+    none = [0, 2, size, 2 * size - 1]
+    rows[none] = torch.tensor([-1, 9, -2 ** 31, 1 << 29], dtype=torch.int32, device=DEV)
+    offsets = torch.tensor([0, size, 2 * size], dtype=torch.int32, device=DEV)
+    sa = _scales(gen, 9)
+    sa[0] = float("inf")
+    out = grouped_gemm(a, w.transpose(1, 2), sa, None, offsets, rows=rows)
+    assert (out[none] == 0).all() and out.isfinite().all()
+    for e, here in enumerate((slice(0, size), slice(size, 2 * size))):
+        good = ((rows[here] > 0) & (rows[here] < 9)).nonzero().flatten()
+        picked = rows[here][good].long()
+        exact = reference_int8_gemm(a[picked], w[e].t(), sa[picked])
+        _close(out[here][good], exact, _magnitude(a[picked], w[e], sa[picked], None), 128, INT8)
 
 
 @pytest.mark.parametrize("offsets", [[0, 50, 20, 60], [-5, 10, 10, 999], [60, 0, 0, 60], [2 ** 31 - 1, -2 ** 31, 30, 60]])
@@ -302,6 +324,40 @@ def test_grouped_on_another_stream_and_in_a_graph(size):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, grouped_gemm(a, w.transpose(1, 2), sa, sb, offsets, rows=rows))
+
+
+def test_int8_gemm_on_two_streams_and_in_two_graphs():
+    """k in parts: every call has partial sums and counters of its own, so calls at once, and two graphs replayed at once, do not meet."""
+    gen = torch.Generator(device=DEV).manual_seed(15)
+    (m, n, k), streams = (65, 256, 16384), [torch.cuda.Stream() for _ in range(2)]
+    assert _capi.load().hfrk_int8_gemm_workspace_bytes(m, n, k) > 0
+    a, w = [_codes(gen, (m, k), INT8) for _ in streams], [_codes(gen, (n, k), INT8) for _ in streams]
+    sa = [_scales(gen, m) for _ in streams]
+    want = [int8_gemm(x, y.t(), s) for x, y, s in zip(a, w, sa)]
+    torch.cuda.synchronize()
+    at_once = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                at_once[i].append(int8_gemm(a[i], w[i].t(), sa[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in at_once[i])
+    outs, graphs = [torch.empty_like(x) for x in want], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            int8_gemm(a[i], w[i].t(), sa[i], output=outs[i])
+    for turn in range(4):
+        for i in range(2):
+            a[i].copy_(_codes(gen, (m, k), INT8))
+            outs[i].fill_(7.0)
+        want = [int8_gemm(x, y.t(), s) for x, y, s in zip(a, w, sa)]
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want)), turn
 
 
 def test_grouped_rows_past_2_31_bytes():
