@@ -29,7 +29,7 @@ HIP_SOURCES = ["hfrk_common.hip", "skinny_gemm.hip", "skinny_gemm_plan.hip", "sk
                "dynamic_quant.hip", "tiled_gemm.hip", "tiled_gemm_rowmajor.hip", "tiled_gemm_packed.hip", "pack_weight.hip", "plan_table_file.hip",
                "rotary.hip", "tree_attention.hip", "tree_attention_d64.hip", "tree_attention_d128.hip", "tree_attention_d256.hip",
                "tree_attention_shared_d64.hip", "tree_attention_shared_d128.hip", "tree_attention_shared_d256.hip",
-               "grouped_gemm.hip", "tiled_int8.hip", "tiled_grouped_fp8.hip", "tiled_grouped_int8.hip", "experts.hip"]
+               "grouped_gemm.hip", "skinny_gemm_rows_int8.hip", "tiled_int8.hip", "tiled_grouped_fp8.hip", "tiled_grouped_int8.hip", "experts.hip"]
 PROBE_SOURCE = os.path.join(HERE, "bench_probes", "probe.hip")
 PROBE_LIB = os.path.join(PKG, "benchmarks", "libhfrk_bench_probes.so")
 LIB_NAME = "libhfrk_gfx950.so"

@@ -12,6 +12,8 @@
 #include <math.h>
 
 #include "grouped_gemm.h"
+#include "skinny_gemm_args.h"
+#include "skinny_gemm_plan.h"
 
 namespace hfrk {
 
@@ -186,7 +188,7 @@ static int launch_rows(GroupedArgs a, hipStream_t stream) {
 // are many, in four tiles a wave; a wave asks for one tile's chunk at a time, and it is the six waves of a SIMD that keep memory busy: with all four tiles'
 // chunks requested together and two sets of registers 100 tokens on 6 of 160 experts of 3008 x 5120 take 471 us instead of 376 (5.9 TB/s), 32 on 2 of 8 of 28672 x
 // 4096 177 and 164.  Fewer columns spread a call over the compute units: one token on 2 of 8 experts of 4096 x 14336 28.9 -> 18.8 us with 32 columns (128 and
-// 256 workgroups), on 6 of 64 of 2816 x 2048 12.2 -> 10.1 with 48, one row of 4096 x 14336 int8 29.2 -> 12.9 with 16; where the rounds do not get fewer they cost (32
+// 256 workgroups), on 6 of 64 of 2816 x 2048 12.2 -> 10.1 with 48, one row of 4096 x 14336 int8 29.2 -> 12.9 with 16 (such a weight now goes to int8_in_bands); where the rounds do not get fewer they cost (32
 // tokens on 2 of 8 of 4096 x 14336 85 -> 113 with 16 columns).  Up to eight chunks of k leave eight waves one each: four waves take k then, and the others other
 // columns (4 tokens on 8 of 128 of 2048 x 768 15.8 -> 12.0 with 128 columns, one token 7.5 -> 6.5 with 64 of them).
 struct FewRows {
@@ -295,7 +297,7 @@ static int launch_grouped(const GroupedArgs& a, hipStream_t stream) {
     return launch_few_rows<INT8>(a, few_rows_kernel(a.n, a.k, fmaxf(active, 1.f), a.count / fmaxf(active, 1.f)), stream);
 }
 
-// One int8 weight: up to 16 rows the rows kernel, up to 32 the one with the smaller predicted time (32 x 4096 x 4096 9.1 us, on tiles 11.4; 32 x 28672 x 4096 41.9 and
+// One int8 weight that has no bands (below): up to 16 rows the rows kernel, up to 32 the one with the smaller predicted time (of weights that bands take now: 32 x 4096 x 4096 9.1 us, on tiles 11.4; 32 x 28672 x 4096 41.9 and
 // 31.8), more the tiled one, k in parts where that is worth clearing their counters (a launch of 2 us) and the caller gave memory for them.
 constexpr int kDenseFewRows = 16;
 
@@ -324,8 +326,45 @@ __global__ void __launch_bounds__(256) clear_counters_kernel(int* counters, int 
     for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) counters[i] = 0;
 }
 
+// Up to 16 rows, and on weights above 8 MiB up to 32, a weight whose rows deal out evenly goes to the kernel of the skinny GEMM that gives every workgroup a band of
+// rows (skinny_gemm_rows_impl.h, under the plan that fp8 codes have), against the kernels below, us: 6144 x 4096 at 1 / 4 / 16 / 17 / 32 rows 6.1 / 6.2 / 7.2 / 8.1 / 9.3
+// and 7.9 / 8.0 / 9.1 / 11.3 / 12.0, 28672 x 4096 20.6 / 20.7 / 21.4 / 22.4 / 25.4 and 24.3 / 25.7 / 27.6 / 30.7 / 31.4, 4096 x 14336 12.0 / 11.2 / 12.7 / 15.3 / 18.0 and
+// 15.3 / 13.0 / 17.4 / 18.3 / 18.4, 2048 x 2048 3.6 / 3.6 / 4.0 / 5.7 / 6.2 and 4.1 / 4.3 / 4.7 / 4.8 / 4.8, 14336 x 512 at 17 rows 6.2 and 5.7.
+constexpr int kBandRows = 32;
+constexpr long kBandFromBytes = 8L << 20;  // above kDenseFewRows rows
+
+static bool int8_in_bands(const GroupedArgs& a, hfrk_gemm_plan* p) {
+    if (a.count > kBandRows || (a.count > kDenseFewRows && (long)a.n * a.k <= kBandFromBytes)) return false;
+    if ((a.base && a.base_stride != 0 && a.base_stride != a.n) || (a.n % 4 == 0 && !a.vec)) return false;
+    return ((long)a.n + 128) * a.b_stride + a.k < (1L << 31) && make_rows_plan(a.count, a.n, a.k, p) == HFRK_SUCCESS;
+}
+
+static int launch_int8_bands(const GroupedArgs& a, const hfrk_gemm_plan& p, hipStream_t stream) {
+    GemmArgs g{};
+    g.A = a.A;
+    g.B = a.B;
+    g.D = a.D;
+    g.base = a.base;
+    g.base_stride = a.base_stride;
+    g.scale_a = a.scale_a;
+    g.scale_b = a.scale_b;
+    g.sa_stride = a.sa_stride;
+    g.sb_stride = a.sb_stride;
+    g.m = a.count;
+    g.n = a.n;
+    g.k = a.k;
+    g.b_stride = a.b_stride;
+    g.d_dtype = a.d_dtype;
+    g.grid = p.grid;
+    g.slabs = p.slabs;
+    set_rows_geometry(&g, p, false);
+    return launch_rows_int8_kernel(g, p.ch, p.wk, p.lds_bytes, stream);
+}
+
 static int launch_int8(const GroupedArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!tiled_size_ok(a.count, a.n, a.k)) return HFRK_BAD_SHAPE;
+    hfrk_gemm_plan bands{};
+    if (int8_in_bands(a, &bands)) return launch_int8_bands(a, bands, stream);
     hfrk_tiled_plan p{};
     FewRows few;
     bool tiles = int8_on_tiles(a.count, a.n, a.k, workspace != nullptr, &p, &few);

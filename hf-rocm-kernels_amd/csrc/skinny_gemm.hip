@@ -686,6 +686,27 @@ struct GemmNeeds {
     bool taken;  // whether these arguments take any of it
     size_t given_bytes() const { return ws_bytes || counters ? kGivenCounters * sizeof(int) + ws_bytes : 0; }
 };
+// How the row-split kernel deals out its 4-row units (plan kind -2): the bands' heights, their tiles and where in k they start.
+void set_rows_geometry(GemmArgs* args, const hfrk_gemm_plan& p, bool swiglu) {
+    const int per_tile = swiglu ? 4 : 4 * p.wk;  // units a tile can hold (SwiGLU: 16 output columns, their gate and their up rows)
+    args->rows_q = p.panels / p.grid;
+    args->rows_r = p.panels % p.grid;
+    auto geometry = [&](int units, int* tiles, int* base, int* extra) {
+        *tiles = (units + per_tile - 1) / per_tile;
+        *base = *tiles ? units / *tiles : 0;
+        *extra = *tiles ? units % *tiles : 0;
+    };
+    geometry(args->rows_q + 1, &args->tiles_a, &args->base_a, &args->extra_a);
+    geometry(args->rows_q, &args->tiles_b, &args->base_b, &args->extra_b);
+    args->kc_magic = (uint32_t)(((1ULL << 32) + (uint64_t)p.slabs - 1) / (uint64_t)p.slabs);
+    // chunks per wave in the band height most workgroups have
+    const int tiles = 2 * args->rows_r > p.grid ? args->tiles_a : args->tiles_b;
+    const long run8 = (long)tiles * p.slabs;  // eight waves' worth
+    const bool same_offset = run8 % 8 == 0 && (run8 / 8) % 16 == 0;
+    const bool shared_lines = p.ch >= 3 && p.panels >= 4 * p.grid;  // (bands of 2-3 units lose 3 %: 2304 x 16384)
+    args->k_rotate = (args->b_stride % 4096 == 0 && (same_offset || shared_lines)) ? 1 : 0;
+}
+
 static int gemm_launch(const void* A, const void* B, void* D, const void* base, const float* scale_a, int sa_stride,
                        const float* scale_b, int sb_stride, const float* out_scale, int m, int n, int k, int b_stride,
                        int d_dtype, int epilogue, const hfrk_gemm_plan* user_plan, hipStream_t stream, bool packed = false,
@@ -861,25 +882,7 @@ static int gemm_launch(const void* A, const void* B, void* D, const void* base, 
     args.ws_bytes = (uint32_t)ws_bytes;
     args.counters = st.counters;
     if (p.wn == -2) {
-        const int per_tile = swiglu ? 4 : 4 * p.wk;  // units a tile can hold (SwiGLU: 16 output columns, their gate and their up rows)
-        args.rows_q = p.panels / p.grid;
-        args.rows_r = p.panels % p.grid;
-        auto geometry = [&](int units, int* tiles, int* base, int* extra) {
-            *tiles = (units + per_tile - 1) / per_tile;
-            *base = *tiles ? units / *tiles : 0;
-            *extra = *tiles ? units % *tiles : 0;
-        };
-        geometry(args.rows_q + 1, &args.tiles_a, &args.base_a, &args.extra_a);
-        geometry(args.rows_q, &args.tiles_b, &args.base_b, &args.extra_b);
-        args.kc_magic = (uint32_t)(((1ULL << 32) + (uint64_t)p.slabs - 1) / (uint64_t)p.slabs);
-        {
-            // chunks per wave in the band height most workgroups have
-            const int tiles = 2 * args.rows_r > p.grid ? args.tiles_a : args.tiles_b;
-            const long run8 = (long)tiles * p.slabs;  // eight waves' worth
-            const bool same_offset = run8 % 8 == 0 && (run8 / 8) % 16 == 0;
-            const bool shared_lines = p.ch >= 3 && p.panels >= 4 * p.grid;  // (bands of 2-3 units lose 3 %: 2304 x 16384)
-            args.k_rotate = (b_stride % 4096 == 0 && (same_offset || shared_lines)) ? 1 : 0;
-        }
+        set_rows_geometry(&args, p, swiglu);
         if (rms) {
             args.rms_input = static_cast<const uint16_t*>(rms->input);
             args.rms_residual = static_cast<const uint16_t*>(rms->residual);

@@ -95,6 +95,10 @@ constexpr bool stream_variant_exists(int act_loads, int row_tiles, bool swiglu =
 // rms: the RMSNorm prologue (args.rms_*): up to 8 rows (act_loads <= 2), k = 4096 or 8192, row_tiles 1 (plain epilogue) or 2 (swiglu);
 // lds_bytes is then rows_rms_lds_bytes(act_loads, row_tiles, k)
 int launch_rows_kernel(const GemmArgs& args, int act_loads, int row_tiles, bool swiglu, bool rms, int lds_bytes, hipStream_t stream);
+// int8 codes: no SwiGLU epilogue, no prologue (skinny_gemm_rows_int8.hip)
+int launch_rows_int8_kernel(const GemmArgs& args, int act_loads, int row_tiles, int lds_bytes, hipStream_t stream);
+// the bands of a plan of kind -2 (b_stride is set); args.grid and args.slabs are the plan's
+void set_rows_geometry(GemmArgs* args, const hfrk_gemm_plan& p, bool swiglu);
 constexpr int kRowsRmsMaxM = 8;
 constexpr int kRowsRmsRedBytes = 8 * kGemmWaves * 4;  // per-row, per-wave partial sums of squares
 constexpr int rows_rms_lds_bytes(int act_loads, int row_tiles, int k) {

@@ -62,8 +62,10 @@ namespace hfrk {
 //                (tile * k/256 + kc) * 4096, already in matrix-core operand order): four 1 KB-contiguous loads per tile
 //                whose registers are the operands, no pass through LDS for the weights.  Chunk sequence, runs per wave,
 //                operands and order of every sum are those of kRowsTiles: the two give the same bits.
+// INT8: codes are int8 and the sums int32 (v_mfma_i32_16x16x64_i8 on either half of a lane's 32 bytes: which bytes of k a lane has does not matter as long as both
+// operands agree), kept in the same registers as bits and made floats in front of the epilogue.
 enum { kRowsUnits = 0, kRowsTiles = 1, kRowsPacked = 2 };
-template <int MA, int RT, bool SWIGLU, bool RMS, int LAYOUT, bool BASE_ROW>
+template <int MA, int RT, bool SWIGLU, bool RMS, int LAYOUT, bool BASE_ROW, bool INT8 = false>
 __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_rows_kernel(const GemmArgs a) {
     constexpr bool TILED = LAYOUT != kRowsUnits, PACKED = LAYOUT == kRowsPacked;
     static_assert(!(TILED && RMS), "the RMSNorm prologue exists for row-major weights dealt out in 4-row units");
@@ -271,7 +273,16 @@ __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_rows_kernel(const Ge
     for (int h = 0; h < 2; ++h) rd_off[h] = li * 256 + ((((8 * h + 2 * lg) ^ li) & 15) << 4);
 
     auto prefetch = [&](int row0, int units, bool wanted) __attribute__((always_inline)) { return epi.prefetch(row0, units, wanted); };
-    auto epilogue = [&](int row0, int units, const v4f (&acc)[MT * RT], const Pre& pre) __attribute__((always_inline)) { epi.store(row0, units, acc, pre); };
+    auto epilogue = [&](int row0, int units, const v4f (&acc)[MT * RT], const Pre& pre) __attribute__((always_inline)) {
+        if constexpr (INT8) {
+            v4f sums[MT * RT];
+#pragma unroll
+            for (int u = 0; u < MT * RT; ++u) sums[u] = __builtin_convertvector(__builtin_bit_cast(v4i, acc[u]), v4f);
+            epi.store(row0, units, sums, pre);
+        } else {
+            epi.store(row0, units, acc, pre);
+        }
+    };
 
     // ---- what the end of the kernel will do, decided now ----------------------------------------------------------------
     // A run that starts inside a tile (kb0 != 0) hands the partial sum of that tile over; a wave without chunks hands over
@@ -371,8 +382,17 @@ __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_rows_kernel(const Ge
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int u = 0; u < MT * RT; ++u)
-                acc[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wop[h][u % RT], aop[h][u / RT], acc[u], 0, 0, 0, 0, 0, 0);
+            for (int u = 0; u < MT * RT; ++u) {
+                const v8i &w = wop[h][u % RT], &x = aop[h][u / RT];
+                if constexpr (INT8) {
+                    v4i c = __builtin_bit_cast(v4i, acc[u]);
+                    c = __builtin_amdgcn_mfma_i32_16x16x64_i8(v4i{w[0], w[1], w[2], w[3]}, v4i{x[0], x[1], x[2], x[3]}, c, 0, 0, 0);
+                    c = __builtin_amdgcn_mfma_i32_16x16x64_i8(v4i{w[4], w[5], w[6], w[7]}, v4i{x[4], x[5], x[6], x[7]}, c, 0, 0, 0);
+                    acc[u] = __builtin_bit_cast(v4f, c);
+                } else {
+                    acc[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[u], 0, 0, 0, 0, 0, 0);
+                }
+            }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if constexpr (RMS) {
@@ -416,18 +436,23 @@ __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_rows_kernel(const Ge
 #pragma unroll
         for (int j = 1; j < kGemmWaves; ++j) {
             const float f = (addmask >> j) & 1u ? 1.0f : 0.0f;
+            const int mask = (addmask >> j) & 1u ? -1 : 0;
 #pragma unroll
             for (int u = 0; u < RT; ++u)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) acc[mt * RT + u][v] = __builtin_fmaf(other[j][u][v], f, acc[mt * RT + u][v]);
+                for (int v = 0; v < 4; ++v) {
+                    v4f& sum = acc[mt * RT + u];
+                    if constexpr (INT8) sum[v] = __int_as_float(__float_as_int(sum[v]) + (__float_as_int(other[j][u][v]) & mask));
+                    else sum[v] = __builtin_fmaf(other[j][u][v], f, sum[v]);
+                }
         }
     }
     epilogue(row0_l, units_l, acc, pre_l);
 }
 
-template <int MA, int RT, bool SWIGLU, bool RMS, int LAYOUT, bool BASE_ROW>
+template <int MA, int RT, bool SWIGLU, bool RMS, int LAYOUT, bool BASE_ROW, bool INT8>
 static int launch_rows_instance(const GemmArgs& args, int lds_bytes, hipStream_t stream) {
-    auto kern = skinny_gemm_rows_kernel<MA, RT, SWIGLU, RMS, LAYOUT, BASE_ROW>;
+    auto kern = skinny_gemm_rows_kernel<MA, RT, SWIGLU, RMS, LAYOUT, BASE_ROW, INT8>;
     static bool attr_done[kMaxDevices] = {};
     int dev = 0;
     HFRK_HIP_TRY(hipGetDevice(&dev));
@@ -440,12 +465,12 @@ static int launch_rows_instance(const GemmArgs& args, int lds_bytes, hipStream_t
     return HFRK_SUCCESS;
 }
 
-template <int MA, int RT, bool SWIGLU, bool RMS, int LAYOUT = kRowsUnits>
+template <int MA, int RT, bool SWIGLU, bool RMS, int LAYOUT = kRowsUnits, bool INT8 = false>
 static int launch_rows_one(const GemmArgs& args, int lds_bytes, hipStream_t stream) {
     if constexpr (!SWIGLU && !RMS) {
-        if (args.base && args.base_stride == 0) return launch_rows_instance<MA, RT, SWIGLU, RMS, LAYOUT, true>(args, lds_bytes, stream);
+        if (args.base && args.base_stride == 0) return launch_rows_instance<MA, RT, SWIGLU, RMS, LAYOUT, true, INT8>(args, lds_bytes, stream);
     }
-    return launch_rows_instance<MA, RT, SWIGLU, RMS, LAYOUT, false>(args, lds_bytes, stream);
+    return launch_rows_instance<MA, RT, SWIGLU, RMS, LAYOUT, false, INT8>(args, lds_bytes, stream);
 }
 
 }  // namespace hfrk

@@ -24,3 +24,13 @@ def test_loads_read_no_scalar_that_a_vector_instruction_has_just_written(source,
 def test_registers_are_enough(source, tmp_path):
     sizes = [int(x) for x in re.findall(r"\.private_segment_fixed_size: (\d+)", "".join(_assembly(source, tmp_path)))]
     assert sizes and max(sizes) == 0, sizes
+
+
+def test_row_split_kernel_on_int8_codes_keeps_its_registers(tmp_path):
+    """As on fp8 codes: the loop of the 32-row instances fills all 256, at most one pair of registers lives in scratch; the scales are asked for with the first chunk."""
+    sizes = [int(x) for x in re.findall(r"\.private_segment_fixed_size: (\d+)", "".join(_assembly("skinny_gemm_rows_int8.hip", tmp_path)))]
+    assert len(sizes) == 20 and max(sizes) <= 8
+    for name, body in _instances("skinny_gemm_rows_int8.hip", "skinny_gemm_rows_kernel", tmp_path).items():
+        first = next(i for i, x in enumerate(body) if x.startswith("buffer_load_dwordx4") and " nt" in x)
+        scale = next(i for i, x in enumerate(body) if x.startswith("global_load_dword "))
+        assert 0 < scale - first < 60, (name, scale - first)

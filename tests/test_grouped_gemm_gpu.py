@@ -194,6 +194,40 @@ def test_int8_gemm(m, n, k, base):
     assert int8_gemm(a, w.t(), sa, sb, base=add, output=into) is into and torch.equal(into, out)
 
 
+@pytest.mark.parametrize("m", [1, 3, 4, 5, 8, 9, 13, 16, 17, 20, 24, 25, 32])
+@pytest.mark.parametrize("n,k,base", [(1024, 512, None), (1030, 768, "row"), (1027, 1280, "full"), (2304, 4096, "full"), (6148, 512, "row"), (5120, 8192, None), (9218, 1024, "row")])
+def test_int8_gemm_on_bands_of_rows(m, n, k, base):
+    gen = torch.Generator(device=DEV).manual_seed(m + n)
+    dtype = torch.bfloat16 if (m + n) % 2 else torch.float16
+    a, wide = _codes(gen, (m, k), INT8), _codes(gen, (n, k + 32), INT8)
+    w = wide[:, :k] if m % 2 else wide[:, :k].contiguous()  # rows further apart than they are long
+    sa, sb = _scales(gen, m) if m != 4 else _scales(gen, 1), _scales(gen, n) if m != 8 else None
+    add = {None: None, "row": torch.randn(n, generator=gen, device=DEV).to(dtype), "full": torch.randn((m, n), generator=gen, device=DEV).to(dtype)}[base]
+    out = int8_gemm(a, w.t(), sa, sb, base=add, out_dtype=dtype)
+    exact = reference_int8_gemm(a, w.t(), sa, sb, add)
+    _close(out, exact, _magnitude(a, w, sa, sb), k, INT8, add)
+    assert torch.equal(int8_gemm(a, w.t(), sa, sb, base=add, out_dtype=dtype), out)
+    if base == "full":
+        assert int8_gemm(a, w.t(), sa, sb, base=add, output=add) is add and torch.equal(add, out)
+
+
+@pytest.mark.parametrize("m", [3, 16, 32])
+def test_int8_gemm_on_bands_largest_sums(m):
+    """Sums above 2^24 that several waves make together stay exact up to the rounding of the result: 2^14 * 130816 and one less, over k in eight parts."""
+    k, n = 130816, 1024
+    a = torch.full((m, k), -128, dtype=torch.int8, device=DEV)
+    w = torch.full((n, k), -128, dtype=torch.int8, device=DEV)
+    w[1] = 127
+    w[2, ::2] = 127
+    w[3, -256:] = 1
+    one = torch.ones(1, device=DEV) * 2.0 ** -20
+    out = int8_gemm(a, w.t(), one, out_dtype=torch.float16)
+    exact = reference_int8_gemm(a[:1], w[:8].t(), one)
+    bound = exact.abs() * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25  # the sum made a float, times one scale, rounded to fp16
+    assert ((out[:, :8].double() - exact).abs() <= bound).all()
+    assert (out == out[:1]).all() and (out[:, 4:] == out[:, 4:5]).all()
+
+
 def test_int8_gemm_largest_sums_and_shared_addend():
     """Every product 2^14 over the longest k: the sum is 2^14 * 131056, just below 2^31."""
     k = 131056
