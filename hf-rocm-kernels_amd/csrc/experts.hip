@@ -256,7 +256,7 @@ __device__ __forceinline__ T row_reduce(T v, OP op) {  // over the 16 lanes of a
 }
 
 // Four tokens a wave, 16 lanes each: expert 16 j + lane in register j, sorted within the lane by key and, of equal keys, number.  Many tokens are bound by
-// the instructions of a choice, most of which are the same for one token and for four: 16000 tokens on 8 of 256 experts 15.2 -> 11.0 us, with a bias 21.0 -> 19.1 (of
+// the instructions of a choice, most of which are the same for one token and for four: 16000 tokens on 8 of 256 experts 15.2 -> 10.5 us, with a bias 21.0 -> 18.9 (of
 // which the tokens that are done again are the end), 4096 on 6 of 64 4.5 -> 3.9.  A single token waits longer for it.  Tokens whose choice 32 bits leave open are done again, a wave each.
 template <int EPL, bool BIAS>
 __global__ void __launch_bounds__(256) choose_many_kernel(const RouteArgs a, int experts) {
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(256) choose_many_kernel(const RouteArgs a, int
 // The pairs in the experts' order: each of up to 128 workgroups has a run of pairs.  Each counts its run's pairs of every expert, and in a second launch adds the
 // runs' counts: those in front of its own and all, which say where its pairs begin; then it deals its run out, 1024 pairs at a time, a wave finding the lanes of
 // the same expert by the bits of its number.  (A workgroup an expert, each going through all pairs twice, took 50 us of 128000 pairs and 256 experts, every
-// workgroup counting all pairs in LDS 21; the two launches take 8.)
+// workgroup counting all pairs in LDS 21; the two launches take 4.2 and 6.5, each a few ways to memory one after the other.)
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortGroups = 128;
 
 __global__ void __launch_bounds__(kSortThreads) count_pairs_kernel(const RouteArgs a, int experts, int run) {
@@ -420,11 +420,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_pairs_kernel(const RouteArg
         const int shares = kSortThreads / experts, share = tid / experts, e = tid - share * experts;  // threads that share an expert's runs
         int front = 0, behind = 0;
         if (share < shares) {
-#pragma unroll 8
-            for (int r = share; r < (int)gridDim.x; r += shares) {
-                const int n = a.counts[r * experts + e];
-                if (r < (int)blockIdx.x) front += n;
-                else behind += n;
+            // through a buffer, so that the runs behind the last read zero: without a rest of single loads, each a way to memory (of 125 runs' counts 8.7 -> 6.5 us)
+            const __amdgpu_buffer_rsrc_t counts = make_rsrc(a.counts, gridDim.x * (uint32_t)experts * 4u);
+            for (int r0 = share; r0 < (int)gridDim.x; r0 += 16 * shares) {
+                int n[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) n[j] = __builtin_amdgcn_raw_buffer_load_b32(counts, ((r0 + j * shares) * experts + e) * 4, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const bool in_front = r0 + j * shares < (int)blockIdx.x;
+                    front += in_front ? n[j] : 0;
+                    behind += in_front ? 0 : n[j];
+                }
             }
             atomicAdd(&before[e], front);
             atomicAdd(&all[e], behind);
