@@ -1173,16 +1173,15 @@ std::tuple<at::Tensor, at::Tensor> swiglu_dynamic_int8_new(const at::Tensor& gat
 }
 
 // D = (base ? base : 0) + scale_a x scale_b x A.B on int8 codes: A [m, k], B [k, n] with unit stride along k, base [n] or [m, n].
-const char* int8_operands(const at::Tensor& A, const at::Tensor& B, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
-                          const std::optional<at::Tensor>& scale_b, at::ScalarType dtype) {
-    if (A.dim() != 2 || !A.is_contiguous() || A.scalar_type() != at::kChar) return "A must be a contiguous [m, k] int8 tensor";
-    const int64_t m = A.size(0), k = A.size(1);
-    if (B.dim() != 2 || B.scalar_type() != at::kChar || B.size(0) != k || (k > 1 && B.stride(0) != 1)) return "B must be [k, n] int8 with unit stride along k";
-    const int64_t n = B.size(1);
-    if (m >= (int64_t(1) << 31) || n >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || (n > 1 && (B.stride(1) < k || B.stride(1) >= (int64_t(1) << 31))))
+// What a product of m rows of k columns on A's device needs of its weight (along_k: the dimension of B that k is), addend, scales and result.
+const char* int8_product(const at::Tensor& A, int64_t m, int64_t k, const at::Tensor& B, int along_k, const std::optional<at::Tensor>& base,
+                         const std::optional<at::Tensor>& scale_b, at::ScalarType dtype) {
+    if (B.dim() != 2 || B.scalar_type() != at::kChar || B.size(along_k) != k || (k > 1 && B.stride(along_k) != 1))
+        return "B must be [k, n] int8 with unit stride along k";
+    const int64_t n = B.size(1 - along_k), stride = B.stride(1 - along_k);
+    if (m >= (int64_t(1) << 31) || n >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || (n > 1 && (stride < k || stride >= (int64_t(1) << 31))))
         return "A, B or B's rows are larger than the kernel's limits";
     if (!is_16bit(dtype)) return "the result must be float16 or bfloat16";
-    if (!float_vector(scale_a, m, A)) return "scale_a must be float32 on A's device with 1 or m elements";
     if (scale_b.has_value() && !float_vector(*scale_b, n, A)) return "scale_b must be float32 on A's device with 1 or n elements";
     if (base.has_value() && !(base->is_contiguous() && base->scalar_type() == dtype && base->device() == A.device() &&
                               ((base->dim() == 1 && base->size(0) == n) || (base->dim() == 2 && base->size(0) == m && base->size(1) == n))))
@@ -1191,17 +1190,24 @@ const char* int8_operands(const at::Tensor& A, const at::Tensor& B, const std::o
     return nullptr;
 }
 
-int run_int8_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tensor& D, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
-                  const std::optional<at::Tensor>& scale_b) {
-    const int m = (int)A.size(0), n = (int)B.size(1), k = (int)A.size(1);
+const char* int8_operands(const at::Tensor& A, const at::Tensor& B, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
+                          const std::optional<at::Tensor>& scale_b, at::ScalarType dtype) {
+    if (A.dim() != 2 || !A.is_contiguous() || A.scalar_type() != at::kChar) return "A must be a contiguous [m, k] int8 tensor";
+    const char* const why = int8_product(A, A.size(0), A.size(1), B, 0, base, scale_b, dtype);
+    if (why) return why;
+    return float_vector(scale_a, A.size(0), A) ? nullptr : "scale_a must be float32 on A's device with 1 or m elements";
+}
+
+// (`on`: a tensor on the device of all; along_k as in int8_product)
+int run_int8_gemm(const at::Tensor& on, const void* A, const float* scale_a, int sa_stride, const at::Tensor& B, int along_k, int m, void* D, int dtype,
+                  const std::optional<at::Tensor>& base, const std::optional<at::Tensor>& scale_b) {
+    const int n = (int)B.size(1 - along_k), k = (int)B.size(along_k);
     // (memory of the call's own: streams and graphs share none)
     const size_t bytes = hfrk_int8_gemm_workspace_bytes(m, n, k);
-    const at::Tensor workspace = bytes ? at::empty({(int64_t)bytes}, A.options().dtype(at::kByte)) : at::Tensor();
-    return hfrk_int8_gemm(A.data_ptr(), B.data_ptr(), D.data_ptr(), base.has_value() ? base->data_ptr() : nullptr,
-                          base.has_value() && base->dim() == 2 ? n : 0, scale_a.data_ptr<float>(), scale_a.numel() == 1 ? 0 : 1,
+    const at::Tensor workspace = bytes ? at::empty({(int64_t)bytes}, on.options().dtype(at::kByte)) : at::Tensor();
+    return hfrk_int8_gemm(A, B.data_ptr(), D, base.has_value() ? base->data_ptr() : nullptr, base.has_value() && base->dim() == 2 ? n : 0, scale_a, sa_stride,
                           scale_b.has_value() ? scale_b->data_ptr<float>() : nullptr, scale_b.has_value() && scale_b->numel() != 1 ? 1 : 0, m, n, k,
-                          n > 1 ? (int)B.stride(1) : k, D.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, bytes ? workspace.data_ptr() : nullptr, bytes,
-                          current_stream(A));
+                          n > 1 ? (int)B.stride(1 - along_k) : k, dtype, bytes ? workspace.data_ptr() : nullptr, bytes, current_stream(on));
 }
 
 void int8_gemm(const at::Tensor& A, const at::Tensor& B, at::Tensor& D, const std::optional<at::Tensor>& base, const at::Tensor& scale_a,
@@ -1214,7 +1220,9 @@ void int8_gemm(const at::Tensor& A, const at::Tensor& B, at::Tensor& D, const st
     TORCH_CHECK(!meets(D, base) || (base->data_ptr() == D.data_ptr() && base->dim() == 2), "D may be base but not share part of it");
     if (A.size(0) == 0) return;
     DeviceScope scope(A);
-    raise_on(run_int8_gemm(A, B, D, base, scale_a, scale_b), "int8_gemm");
+    raise_on(run_int8_gemm(A, A.data_ptr(), scale_a.data_ptr<float>(), scale_a.numel() == 1 ? 0 : 1, B, 0, (int)A.size(0), D.data_ptr(),
+                           D.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, base, scale_b),
+             "int8_gemm");
 }
 
 // As fp8_linear: input [..., k] 16-bit (quantised here, with input_scale or per row) or int8 with its scale(s); weight [n, k] int8.
@@ -1237,25 +1245,34 @@ at::Tensor int8_linear(const at::Tensor& input, const at::Tensor& weight, const 
         if (bias->dim() != 1) return {};
         base = bias;
     }
+    if (quantised && !float_vector(*input_scale, m, input)) return {};
+    if (int8_product(input, m, k, weight, 1, base, weight_scale, dtype)) return {};
     DeviceScope scope(input);
-    at::Tensor codes, scales;
-    if (quantised) {
-        codes = input.dim() == 2 ? input : input.view({m, k});
-        scales = *input_scale;
-    } else {
-        codes = at::empty({m, k}, input.options().dtype(at::kChar));
-        scales = input_scale.has_value() ? *input_scale : at::empty({m}, input.options().dtype(at::kFloat));
-    }
-    const at::Tensor B = weight.t();
-    if (int8_operands(codes, B, base, scales, weight_scale, dtype)) return {};
     at::DimVector sizes(input.sizes());
     sizes.back() = n;
     at::Tensor out = at::empty(sizes, input.options().dtype(dtype));
-    if (!quantised && hfrk_quantize_int8(input.data_ptr(), input_scale.has_value() ? scales.data_ptr<float>() : nullptr, codes.data_ptr(),
-                                         input_scale.has_value() ? nullptr : scales.data_ptr<float>(), (int)m, (int)k,
-                                         input.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16, current_stream(input)) != HFRK_SUCCESS)
-        return {};
-    return run_int8_gemm(codes, B, out, base, scales, weight_scale) == HFRK_SUCCESS ? out : at::Tensor();
+    const int code = dtype == at::kBFloat16 ? HFRK_BF16 : HFRK_F16;
+    const uint8_t* codes = static_cast<const uint8_t*>(input.data_ptr());
+    const float* scales = input_scale.has_value() ? input_scale->data_ptr<float>() : nullptr;
+    int scale_stride = 0;
+    at::Tensor quantised_rows;  // codes, and the rows' scales behind them
+    if (quantised) {
+        scale_stride = input_scale->numel() == 1 ? 0 : 1;
+    } else {
+        const int64_t bytes = (m * k + 15) / 16 * 16;
+        quantised_rows = at::empty({bytes + (scales ? 0 : 4 * m)}, input.options().dtype(at::kByte));
+        uint8_t* const out_codes = static_cast<uint8_t*>(quantised_rows.data_ptr());
+        float* const out_scales = scales ? nullptr : reinterpret_cast<float*>(out_codes + bytes);
+        if (hfrk_quantize_int8(input.data_ptr(), scales, out_codes, out_scales, (int)m, (int)k, input.scalar_type() == at::kBFloat16 ? HFRK_BF16 : HFRK_F16,
+                               current_stream(input)) != HFRK_SUCCESS)
+            return {};
+        codes = out_codes;
+        if (!scales) {
+            scales = out_scales;
+            scale_stride = m == 1 ? 0 : 1;
+        }
+    }
+    return run_int8_gemm(input, codes, scales, scale_stride, weight, 1, (int)m, out.data_ptr(), code, base, weight_scale) == HFRK_SUCCESS ? out : at::Tensor();
 }
 
 // a [a_rows, k], b [experts, k, n] with unit stride along k, offsets [experts + 1], rows [count] or none, output [count, n].

@@ -326,6 +326,31 @@ def test_int8_linear_forms():
     assert torch.equal(loaded(x.half()), q(x.half()))
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("n,k", [(1024, 512), (1030, 768), (6144, 4096), (2304, 8192), (1028, 14336), (1024, 16384), (1024, 16640), (16384, 8192)])
+def test_int8_linear_of_few_rows_is_the_two_calls(m, n, k):
+    """The bits of quantize_int8 and int8_gemm, for every form of scale and addend, with rows of zeros, of large values, and of NaN."""
+    gen = torch.Generator(device=DEV).manual_seed(m + n)
+    w, sw = _codes(gen, (n, k), INT8), _scales(gen, n)
+    for dtype in (torch.bfloat16, torch.float16):
+        x = torch.randn((m, k), generator=gen, device=DEV).to(dtype)
+        x[-1, ::3] *= 100
+        bias, residual = torch.randn(n, generator=gen, device=DEV).to(dtype), torch.randn((m, n), generator=gen, device=DEV).to(dtype)
+        codes, scales = quantize_int8(x)
+        for weight_scale, add in ((sw, None), (sw[:1], bias), (None, residual), (sw, residual)):
+            got = apply_int8_linear(x, w, weight_scale, bias=add if add is bias else None, residual=add if add is residual else None)
+            assert torch.equal(got, int8_gemm(codes, w.t(), scales, weight_scale, base=add, out_dtype=dtype))
+        static = torch.tensor([0.02], device=DEV)
+        fixed, _ = quantize_int8(x, static)
+        assert torch.equal(apply_int8_linear(x, w, sw, static), int8_gemm(fixed, w.t(), static, sw, out_dtype=dtype))
+        x[0] = 0
+        got = apply_int8_linear(x, w, sw, bias=bias)
+        assert torch.equal(got[0], bias)
+        x[m - 1, k - 1] = float("nan") if dtype == torch.bfloat16 else float("inf")
+        got = apply_int8_linear(x, w, sw)
+        assert got[m - 1].isnan().all() and (m == 1 or got[:m - 1].isfinite().all())
+
+
 def test_int8_linear_without_rows_and_with_more_scales_than_rows():
     w, s = torch.ones((24, 64), dtype=INT8, device=DEV), torch.ones(24, device=DEV)
     assert apply_int8_linear(torch.empty((0, 64), dtype=torch.bfloat16, device=DEV), w, s).shape == (0, 24)
