@@ -21,7 +21,7 @@ def expert_mlp_combined_ops(
     factor: float = 1.0,
     mask: Optional[Tensor] = None,
 ) -> Tensor:
-    """Decoder MLP sub-block of experts, six or seven launches on one stream: the normalised hidden states quantised per token, the router's choices, each expert's
+    """Decoder MLP sub-block of experts, six or eight launches on one stream: the normalised hidden states quantised per token, the router's choices, each expert's
     gate and up projection on its tokens, SwiGLU quantised per row, the down projections, and the weighted sum per token.
 
     - hidden: (tokens, hidden) 16-bit, as the layer's norm gives it; logits: (tokens, experts), the router's
