@@ -286,3 +286,57 @@ def test_mlp_of_experts(codes, tokens, experts, top, hidden, inter):
         torch.cuda.synchronize()
         assert torch.equal(out, call())
     check(out)
+
+
+@pytest.mark.parametrize("codes", [FP8, INT8])
+def test_traced_mlp_of_experts_equals_the_eager_one(codes):
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    experts, hidden, inter = 6, 128, 64
+
+    def weight(n, k):
+        w = torch.randint(-120, 121, (experts, n, k), generator=gen, device=DEV, dtype=torch.int8)
+        return (w if codes == INT8 else (w.float() / 64).to(FP8)), torch.rand((experts, n), generator=gen, device=DEV) / 64
+
+    (gate_up, gate_up_scale), (down, down_scale) = weight(2 * inter, hidden), weight(hidden, inter)
+    bias = torch.rand(experts, generator=gen, device=DEV)
+
+    def block(x, logits):
+        return expert_mlp_combined_ops(x, logits, 3, gate_up, gate_up_scale, down, down_scale, residual=x, bias=bias, scoring="sigmoid")
+
+    traced = torch.compile(block, backend="aot_eager", fullgraph=True)
+    for tokens in (1, 9, 9, 80):
+        x, logits = torch.randn((tokens, hidden), generator=gen, device=DEV).bfloat16(), torch.randn((tokens, experts), generator=gen, device=DEV)
+        assert torch.equal(traced(x, logits), block(x, logits)), tokens
+
+
+def test_two_blocks_at_once_do_not_meet():
+    """Two captured blocks replayed side by side, each with its own workspaces, and eager calls between them."""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    experts, hidden, inter, tokens, top = 64, 256, 128, 300, 4
+    gate_up = torch.randint(-127, 128, (experts, 2 * inter, hidden), generator=gen, device=DEV, dtype=torch.int8)
+    down = torch.randint(-127, 128, (experts, hidden, inter), generator=gen, device=DEV, dtype=torch.int8)
+    s1, s2 = torch.rand((experts, 2 * inter), generator=gen, device=DEV) / 512, torch.rand((experts, hidden), generator=gen, device=DEV) / 512
+    x = [torch.randn((tokens, hidden), generator=gen, device=DEV).half() for _ in range(2)]
+    logits = [torch.randn((tokens, experts), generator=gen, device=DEV) for _ in range(2)]
+
+    def call(i):
+        return expert_mlp_combined_ops(x[i], logits[i], top, gate_up, s1, down, s2)
+
+    call(0)
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i in range(2):
+        with torch.cuda.graph(graphs[i]):
+            outs.append(call(i))
+    for _ in range(5):
+        for i in range(2):
+            x[i].copy_(torch.randn((tokens, hidden), generator=gen, device=DEV))
+            logits[i].copy_(torch.randn((tokens, experts), generator=gen, device=DEV))
+        want = [call(i) for i in range(2)]
+        torch.cuda.synchronize()
+        eager = []
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+                eager.append(call(1 - i))
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i]) and torch.equal(eager[i], want[1 - i]) for i in range(2))

@@ -472,3 +472,12 @@ def test_gradients_are_not_recorded_and_no_tensor_is_changed():
     w, s = _codes(gen, (16, 64), INT8), _scales(gen, 16)
     y = apply_int8_linear(x, w, s)
     assert not y.requires_grad and hf_rocm_kernels.quantize_int8(x)[0].dtype == INT8
+
+
+def test_traced_int8_linear_equals_the_eager_layer():
+    torch.manual_seed(1)
+    layer = Int8Linear.from_float(torch.nn.Linear(1024, 1536, bias=True).to(torch.bfloat16).cuda())
+    traced = torch.compile(layer, backend="aot_eager", fullgraph=True)
+    for rows in (1, 8, 8, 70):
+        x = torch.randn(rows, 1024, device=DEV).to(torch.bfloat16)
+        assert torch.equal(traced(x), layer(x)), rows
