@@ -497,7 +497,7 @@ int hfrk_int8_gemm(const void* A, const void* B, void* D, const void* base, int 
  * Products of rows grouped by expert:
  *   output[i, c] = scale_a[r] * scale_b[e, c] * sum_k a[r, k] * b[e, c, k]      for offsets[e] <= i < offsets[e + 1],  r = rows ? rows[i] : i
  *   a        [a_rows, k] codes of `type`: HFRK_FP8_E4M3FN (sums in fp32) or HFRK_INT8 (sums in int32)
- *   rows     [count] int32 or NULL.  A number that is no row of a gives a row of zeros
+ *   rows     [count] int32 or NULL.  A number that is no row of a counts as a row of zeros
  *   b        [experts, n, k] codes, experts expert_stride bytes apart, rows b_stride bytes
  *   scale_a  fp32 [a_rows] (stride 1) or one (0);  scale_b fp32, element (e, c) at e * scale_b_expert_stride + c * scale_b_stride (stride 1, or 0: one an
  *            expert), or NULL: 1
