@@ -188,7 +188,7 @@ static int launch_rows(GroupedArgs a, hipStream_t stream) {
 // are many, in four tiles a wave; a wave asks for one tile's chunk at a time, and it is the six waves of a SIMD that keep memory busy: with all four tiles'
 // chunks requested together and two sets of registers 100 tokens on 6 of 160 experts of 3008 x 5120 take 471 us instead of 376 (5.9 TB/s), 32 on 2 of 8 of 28672 x
 // 4096 177 and 164.  Fewer columns spread a call over the compute units: one token on 2 of 8 experts of 4096 x 14336 28.9 -> 18.8 us with 32 columns (128 and
-// 256 workgroups), on 6 of 64 of 2816 x 2048 12.2 -> 10.1 with 48, one row of 4096 x 14336 int8 29.2 -> 12.9 with 16 (such a weight now goes to int8_in_bands); where the rounds do not get fewer they cost (32
+// 256 workgroups), on 6 of 64 of 2816 x 2048 12.2 -> 10.1 with 48, one row of 4096 x 14336 int8 29.2 -> 12.9 with 16 (such a weight now goes to int8_skinny); where the rounds do not get fewer they cost (32
 // tokens on 2 of 8 of 4096 x 14336 85 -> 113 with 16 columns).  Up to eight chunks of k leave eight waves one each: four waves take k then, and the others other
 // columns (4 tokens on 8 of 128 of 2048 x 768 15.8 -> 12.0 with 128 columns, one token 7.5 -> 6.5 with 64 of them).
 struct FewRows {
@@ -297,7 +297,7 @@ static int launch_grouped(const GroupedArgs& a, hipStream_t stream) {
     return launch_few_rows<INT8>(a, few_rows_kernel(a.n, a.k, fmaxf(active, 1.f), a.count / fmaxf(active, 1.f)), stream);
 }
 
-// One int8 weight that has no bands (below): up to 16 rows the rows kernel, up to 32 the one with the smaller predicted time (of weights that bands take now: 32 x 4096 x 4096 9.1 us, on tiles 11.4; 32 x 28672 x 4096 41.9 and
+// One int8 weight that the skinny GEMM's kernels (below) do not take: up to 16 rows the rows kernel, up to 32 the one with the smaller predicted time (of weights that bands take now: 32 x 4096 x 4096 9.1 us, on tiles 11.4; 32 x 28672 x 4096 41.9 and
 // 31.8), more the tiled one, k in parts where that is worth clearing their counters (a launch of 2 us) and the caller gave memory for them.
 constexpr int kDenseFewRows = 16;
 
@@ -328,18 +328,36 @@ __global__ void __launch_bounds__(256) clear_counters_kernel(int* counters, int 
 
 // Up to 16 rows, and on weights above 8 MiB up to 32, a weight whose rows deal out evenly goes to the kernel of the skinny GEMM that gives every workgroup a band of
 // rows (skinny_gemm_rows_impl.h, under the plan that fp8 codes have), against the kernels below, us: 6144 x 4096 at 1 / 4 / 16 / 17 / 32 rows 6.1 / 6.2 / 7.2 / 8.1 / 9.3
-// and 7.9 / 8.0 / 9.1 / 11.3 / 12.0, 28672 x 4096 20.6 / 20.7 / 21.4 / 22.4 / 25.4 and 24.3 / 25.7 / 27.6 / 30.7 / 31.4, 4096 x 14336 12.0 / 11.2 / 12.7 / 15.3 / 18.0 and
-// 15.3 / 13.0 / 17.4 / 18.3 / 18.4, 2048 x 2048 3.6 / 3.6 / 4.0 / 5.7 / 6.2 and 4.1 / 4.3 / 4.7 / 4.8 / 4.8, 14336 x 512 at 17 rows 6.2 and 5.7.
+// and 7.9 / 8.0 / 9.1 / 11.3 / 12.0, 28672 x 4096 20.6 / 20.7 / 21.4 / 22.4 / 25.4 and 24.3 / 25.7 / 27.6 / 30.7 / 31.4, 4096 x 14336 at 1 / 4 / 16 / 17 rows 12.0 / 11.2 / 12.7 / 15.3 and
+// 15.3 / 13.0 / 17.4 / 18.3, 2048 x 2048 3.6 / 3.6 / 4.0 / 5.7 / 6.2 and 4.1 / 4.3 / 4.7 / 4.8 / 4.8, 14336 x 512 at 17 rows 6.2 and 5.7.
 constexpr int kBandRows = 32;
 constexpr long kBandFromBytes = 8L << 20;  // above kDenseFewRows rows
+constexpr int kBandRowsLongK = 24, kBandLongK = 8192;  // (4096 x 14336 at 32 rows: 18.0 to 20.6 us by what lies in the caches, on tiles 18.4 to 18.9)
 
 static bool int8_in_bands(const GroupedArgs& a, hfrk_gemm_plan* p) {
-    if (a.count > kBandRows || (a.count > kDenseFewRows && (long)a.n * a.k <= kBandFromBytes)) return false;
+    if (a.count > kBandRows || (a.count > kDenseFewRows && (long)a.n * a.k <= kBandFromBytes) || (a.count > kBandRowsLongK && a.k > kBandLongK)) return false;
     if ((a.base && a.base_stride != 0 && a.base_stride != a.n) || (a.n % 4 == 0 && !a.vec)) return false;
     return ((long)a.n + 128) * a.b_stride + a.k < (1L << 31) && make_rows_plan(a.count, a.n, a.k, p) == HFRK_SUCCESS;
 }
 
-static int launch_int8_bands(const GroupedArgs& a, const hfrk_gemm_plan& p, hipStream_t stream) {
+// From 17 rows to 64 with k = 2048 or 4096: the kernel whose waves split k between them and keep their rows in registers (skinny_gemm_ksplit.hip), against bands (up
+// to 32 rows) or tiles, at 32 / 48 / 64 rows, us: 4096 x 4096 7.0 / 7.7 / 8.5 and 8.1 / 12.0 / 12.2, 28672 x 4096 22.9 / 24.5 / 26.3 and 25.5 / 32.7 / 34.0, 2048 x 2048
+// 4.2 / 4.7 / 5.3 and 4.8 / 6.8 / 6.9; the loss is 14336 x 2048 at 33, 9.7 and 9.3.
+static bool int8_in_window(const GroupedArgs& a, hfrk_gemm_plan* p) {
+    if (a.count <= kDenseFewRows || a.count > HFRK_GEMM_MAX_M || (a.n % 4 == 0 && !a.vec)) return false;
+    return ((long)a.n + 128) * a.b_stride + a.k < (1L << 31) && make_ksplit_plan(a.count, a.n, a.k, p) == HFRK_SUCCESS && p->slabs == 1;
+}
+
+// Both where they exist: bands where the 16-row tiles of the other leave a fifth of the compute units' rounds empty (at 24 rows 6144 x 4096, 1.5 rounds, 8.7 and 9.1
+// us, 5120 x 4096, 1.25, 8.0 and 8.8; the other way round 10240 x 4096, 2.5, 12.3 and 11.7).
+static bool int8_skinny(const GroupedArgs& a, hfrk_gemm_plan* p) {
+    const long tiles = ((long)a.n + 15) / 16, rounds = (tiles + kNumCU - 1) / kNumCU;
+    if (tiles > kNumCU && 4 * rounds * kNumCU >= 5 * tiles && int8_in_bands(a, p)) return true;
+    return int8_in_window(a, p) || int8_in_bands(a, p);
+}
+
+// Under a plan of either kind.
+static int launch_int8_skinny(const GroupedArgs& a, const hfrk_gemm_plan& p, hipStream_t stream) {
     GemmArgs g{};
     g.A = a.A;
     g.B = a.B;
@@ -357,14 +375,21 @@ static int launch_int8_bands(const GroupedArgs& a, const hfrk_gemm_plan& p, hipS
     g.d_dtype = a.d_dtype;
     g.grid = p.grid;
     g.slabs = p.slabs;
+    if (p.wn == -1) {
+        g.panels = p.panels;
+        g.units = p.panels * p.slabs;
+        g.chunks_q = g.units / p.grid;
+        g.chunks_r = g.units % p.grid;
+        return launch_ksplit_int8_kernel(g, p.m_tiles, p.wk * 256, p.lds_bytes, stream);
+    }
     set_rows_geometry(&g, p, false);
     return launch_rows_int8_kernel(g, p.ch, p.wk, p.lds_bytes, stream);
 }
 
 static int launch_int8(const GroupedArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!tiled_size_ok(a.count, a.n, a.k)) return HFRK_BAD_SHAPE;
-    hfrk_gemm_plan bands{};
-    if (int8_in_bands(a, &bands)) return launch_int8_bands(a, bands, stream);
+    hfrk_gemm_plan skinny{};
+    if (int8_skinny(a, &skinny)) return launch_int8_skinny(a, skinny, stream);
     hfrk_tiled_plan p{};
     FewRows few;
     bool tiles = int8_on_tiles(a.count, a.n, a.k, workspace != nullptr, &p, &few);
@@ -437,8 +462,16 @@ int hfrk_grouped_gemm(const hfrk_grouped_args* args, void* stream) {
 size_t hfrk_int8_gemm_workspace_bytes(int m, int n, int k) {
     using namespace hfrk;
     hfrk_tiled_plan p{};
+    hfrk_gemm_plan skinny{};
     FewRows few;
-    return tiled_size_ok(m, n, k) && int8_on_tiles(m, n, k, true, &p, &few) ? int8_workspace_bytes(p, m, n) : 0;
+    if (!tiled_size_ok(m, n, k)) return 0;
+    GroupedArgs a{};  // a call on side by side rows
+    a.count = m;
+    a.n = n;
+    a.k = a.b_stride = k;
+    a.vec = 1;
+    if (int8_skinny(a, &skinny)) return 0;
+    return int8_on_tiles(m, n, k, true, &p, &few) ? int8_workspace_bytes(p, m, n) : 0;
 }
 
 int hfrk_int8_gemm(const void* A, const void* B, void* D, const void* base, int base_stride, const float* scale_a, int sa_stride, const float* scale_b,

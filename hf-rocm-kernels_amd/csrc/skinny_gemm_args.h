@@ -119,6 +119,8 @@ constexpr bool rows_variant_exists(int act_loads, int row_tiles) {
 // swiglu: gate rows [0, n/2), up rows [n/2, n); one window must cover K (wave_k = k / 8 = 256 or 512); panels counts the tiles of
 // 16 output columns (n / 32), D is fp8 [m, n/2]
 int launch_ksplit_kernel(const GemmArgs& args, int m_tiles, int wave_k, bool swiglu, int lds_bytes, hipStream_t stream);
+// int8 codes on a row-major weight, 17..64 rows, k = 8 * wave_k = 2048 or 4096 in one window: no workspace
+int launch_ksplit_int8_kernel(const GemmArgs& args, int m_tiles, int wave_k, int lds_bytes, hipStream_t stream);
 constexpr bool ksplit_variant_exists(int m_tiles, int wave_k) {
     return m_tiles >= 1 && (((wave_k == 256 || wave_k == 512) && m_tiles <= 4) || (wave_k == 1024 && m_tiles <= 2));
 }

@@ -31,9 +31,11 @@ namespace hfrk {
 // waves 0..MT-1 keep in registers, then the up tile t + n/32, after which they store
 // e4m3fn(silu(gate) * up / out_scale) into D [m, n/2] instead of the two 16-bit projections -- the SwiGLU kernel of
 // csrc/op_src/swiglu/swiglu_vectorized.cu:27-97 as the GEMM's epilogue, here for 17..64 rows.
-template <int MT, int KW, bool PACKED, bool SWIGLU>
+// INT8: codes are int8 and the sums int32, in the same registers as bits until the epilogue; row-major weights, one window.
+template <int MT, int KW, bool PACKED, bool SWIGLU, bool INT8 = false>
 __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_ksplit_kernel(const GemmArgs a) {
     constexpr uint32_t kOutOfRange = 0x80000000u;
+    static_assert(!INT8 || (!PACKED && !SWIGLU), "int8 codes: row-major weights, plain epilogue");
     constexpr int PASSES = SWIGLU ? 2 : 1;
     constexpr int kCoherent = 17;     // sc0 | sc1
     constexpr int KCH = KW / 256;     // 256-byte column chunks of a wave's weight piece
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_ksplit_kernel(const 
                 for (int t = 0; t < 4; ++t) *reinterpret_cast<v4i*>(tw + c * kTileBytes + wr_off[t]) = wq[c][t];
         }
         if constexpr (kDeferred) {
-            if (S > 1 && wv < MT && stored_tile >= 0) count_arrival();
+            if (!INT8 && S > 1 && wv < MT && stored_tile >= 0) count_arrival();
         }
         const bool more = i + 1 < PASSES * count;
         bool new_window = false;
@@ -307,8 +309,17 @@ __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_ksplit_kernel(const 
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                    acc[mt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wop[h], areg[mt][2 * c + h], acc[mt], 0, 0, 0, 0, 0, 0);
+                for (int mt = 0; mt < MT; ++mt) {
+                    const v8i &w = wop[h], &x = areg[mt][2 * c + h];
+                    if constexpr (INT8) {  // (either half of a lane's 32 bytes: both operands agree on them)
+                        v4i sums = __builtin_bit_cast(v4i, acc[mt]);
+                        sums = __builtin_amdgcn_mfma_i32_16x16x64_i8(v4i{w[0], w[1], w[2], w[3]}, v4i{x[0], x[1], x[2], x[3]}, sums, 0, 0, 0);
+                        sums = __builtin_amdgcn_mfma_i32_16x16x64_i8(v4i{w[4], w[5], w[6], w[7]}, v4i{x[4], x[5], x[6], x[7]}, sums, 0, 0, 0);
+                        acc[mt] = __builtin_bit_cast(v4f, sums);
+                    } else {
+                        acc[mt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[mt], 0, 0, 0, 0, 0, 0);
+                    }
+                }
             if constexpr (PACKED) {
                 if (more) issue_chunk(c, 0u);
             }
@@ -328,9 +339,16 @@ __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_ksplit_kernel(const 
 #pragma unroll
             for (int w = 0; w < kGemmWaves; ++w) part[w] = rb[(w * MT + wv) * 64 + lane];
             v4f sum = part[0];
+            if constexpr (INT8) {
+                v4i whole = __builtin_bit_cast(v4i, part[0]);
 #pragma unroll
-            for (int w = 1; w < kGemmWaves; ++w) sum += part[w];
-            if (S > 1) {
+                for (int w = 1; w < kGemmWaves; ++w) whole += __builtin_bit_cast(v4i, part[w]);
+                sum = __builtin_convertvector(whole, v4f);
+            } else {
+#pragma unroll
+                for (int w = 1; w < kGemmWaves; ++w) sum += part[w];
+            }
+            if (!INT8 && S > 1) {
                 if constexpr (kDeferred) {
                     if (counted_tile >= 0) settle();  // the unit before this one
                 }
@@ -359,16 +377,16 @@ __global__ void __launch_bounds__(kGemmThreads) skinny_gemm_ksplit_kernel(const 
         }
     }
     if constexpr (kDeferred) {
-        if (S > 1 && wv < MT) {  // the last unit's share
+        if (!INT8 && S > 1 && wv < MT) {  // the last unit's share
             if (stored_tile >= 0) count_arrival();
             if (counted_tile >= 0) settle();
         }
     }
 }
 
-template <int MT, int KW, bool PACKED, bool SWIGLU>
+template <int MT, int KW, bool PACKED, bool SWIGLU, bool INT8 = false>
 static int launch_ksplit_packing(const GemmArgs& args, int lds_bytes, hipStream_t stream) {
-    auto kern = skinny_gemm_ksplit_kernel<MT, KW, PACKED, SWIGLU>;
+    auto kern = skinny_gemm_ksplit_kernel<MT, KW, PACKED, SWIGLU, INT8>;
     static bool attr_done[64] = {};
     int dev = 0;
     HFRK_HIP_TRY(hipGetDevice(&dev));
@@ -407,6 +425,21 @@ int launch_ksplit_kernel(const GemmArgs& args, int m_tiles, int wave_k, bool swi
     }
     switch (m_tiles) {
         HFRK_KSPLIT_CASE(1)
+        HFRK_KSPLIT_CASE(2)
+        HFRK_KSPLIT_CASE(3)
+        HFRK_KSPLIT_CASE(4)
+    }
+#undef HFRK_KSPLIT_CASE
+    return HFRK_INVALID_CONFIG;
+}
+
+int launch_ksplit_int8_kernel(const GemmArgs& args, int m_tiles, int wave_k, int lds_bytes, hipStream_t stream) {
+    if (lds_bytes != ksplit_lds_bytes(m_tiles, wave_k) || args.slabs != 1 || args.packed) return HFRK_INVALID_CONFIG;
+#define HFRK_KSPLIT_CASE(MT_)                                                                                          \
+    case MT_:                                                                                                          \
+        return wave_k == 256   ? launch_ksplit_packing<MT_, 256, false, false, true>(args, lds_bytes, stream)          \
+               : wave_k == 512 ? launch_ksplit_packing<MT_, 512, false, false, true>(args, lds_bytes, stream) : HFRK_INVALID_CONFIG;
+    switch (m_tiles) {
         HFRK_KSPLIT_CASE(2)
         HFRK_KSPLIT_CASE(3)
         HFRK_KSPLIT_CASE(4)

@@ -34,3 +34,8 @@ def test_row_split_kernel_on_int8_codes_keeps_its_registers(tmp_path):
         first = next(i for i, x in enumerate(body) if x.startswith("buffer_load_dwordx4") and " nt" in x)
         scale = next(i for i, x in enumerate(body) if x.startswith("global_load_dword "))
         assert 0 < scale - first < 60, (name, scale - first)
+
+
+def test_kernel_that_splits_k_keeps_its_registers(tmp_path):
+    sizes = [int(x) for x in re.findall(r"\.private_segment_fixed_size: (\d+)", "".join(_assembly("skinny_gemm_ksplit.hip", tmp_path)))]
+    assert len(sizes) == 42 and max(sizes) == 0

@@ -211,6 +211,26 @@ def test_int8_gemm_on_bands_of_rows(m, n, k, base):
         assert int8_gemm(a, w.t(), sa, sb, base=add, output=add) is add and torch.equal(add, out)
 
 
+@pytest.mark.parametrize("m", [17, 24, 32, 33, 47, 48, 49, 64])
+@pytest.mark.parametrize("n,k,base", [(8, 2048, None), (1000, 4096, "row"), (1027, 2048, "full"), (4104, 4096, "full"), (6144, 4096, None), (9218, 2048, "row")])
+def test_int8_gemm_with_rows_in_registers(m, n, k, base):
+    gen = torch.Generator(device=DEV).manual_seed(m + n)
+    dtype = torch.bfloat16 if (m + n) % 2 else torch.float16
+    a, wide = _codes(gen, (m, k), INT8), _codes(gen, (n, k + 48), INT8)
+    w = wide[:, :k] if m % 2 else wide[:, :k].contiguous()
+    a[0], w[0] = -128, -128  # a sum of 2^14 k: not a float's
+    a[0, 0] = 127
+    sa, sb = _scales(gen, m) if m != 48 else _scales(gen, 1), _scales(gen, n) if m != 32 else None
+    sa = sa * (1.0 if m != 32 else 2.0 ** -10)  # (within float16)
+    add = {None: None, "row": torch.randn(n, generator=gen, device=DEV).to(dtype), "full": torch.randn((m, n), generator=gen, device=DEV).to(dtype)}[base]
+    out = int8_gemm(a, w.t(), sa, sb, base=add, out_dtype=dtype)
+    exact = reference_int8_gemm(a, w.t(), sa, sb, add)
+    _close(out, exact, _magnitude(a, w, sa, sb), k, INT8, add)
+    assert torch.equal(int8_gemm(a, w.t(), sa, sb, base=add, out_dtype=dtype), out)
+    if base == "full":
+        assert int8_gemm(a, w.t(), sa, sb, base=add, output=add) is add and torch.equal(add, out)
+
+
 @pytest.mark.parametrize("m", [3, 16, 32])
 def test_int8_gemm_on_bands_largest_sums(m):
     """Sums above 2^24 that several waves make together stay exact up to the rounding of the result: 2^14 * 130816 and one less, over k in eight parts."""
