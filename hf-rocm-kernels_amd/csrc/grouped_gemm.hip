@@ -7,7 +7,7 @@
 // read a run of KW * 128 bytes of each weight row at a time.  Operands go from memory to registers (lane l of a 16 x 16 tile holds pieces l / 16 and
 // l / 16 + 4 of row l % 16: which bytes of k a lane has does not matter as long as both operands agree), one tile's chunk ahead of the one that is
 // multiplied; the sums of the waves along k meet in LDS, in wave order.  Bound by memory: 5.8 TB/s on 940 MB of weights.  More rows a group go to the tiled
-// kernel (tiled_gemm_kernel.h).
+// kernel (tiled_gemm_kernel.h).  One int8 weight goes, by rows and k, to the skinny GEMM's kernels, to this one, or to the tiled one (launch_int8).
 #include <limits.h>
 #include <math.h>
 
