@@ -340,3 +340,20 @@ def test_two_blocks_at_once_do_not_meet():
                 eager.append(call(1 - i))
         torch.cuda.synchronize()
         assert all(torch.equal(outs[i], want[i]) and torch.equal(eager[i], want[1 - i]) for i in range(2))
+
+
+def test_route_and_combine_of_the_most_tokens():
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    tokens = 1 << 24
+    logits = torch.randn((tokens, 3), generator=gen, device=DEV)
+    route = route_experts(logits, 1)
+    best = logits.argmax(1)
+    assert torch.equal(route.experts[:, 0].long(), best) and (route.weights == 1.0).all()
+    order = torch.sort(best, stable=True).indices
+    assert torch.equal(route.rows.long(), order) and torch.equal(route.places[order, 0].long(), torch.arange(tokens, device=DEV))
+    assert route.offsets.tolist() == [0, *torch.bincount(best, minlength=3).cumsum(0).tolist()]
+    tokens -= 1
+    y = torch.randn((1000, 8), generator=gen, device=DEV).bfloat16()
+    places = torch.randint(-1, 1000, (tokens, 1), generator=gen, device=DEV, dtype=torch.int32)
+    out = combine_experts(y, torch.full((tokens, 1), 0.5, device=DEV), places)
+    assert torch.equal(out, torch.where(places < 0, 0.0, y[places[:, 0].clamp(min=0).long()] * 0.5).bfloat16())

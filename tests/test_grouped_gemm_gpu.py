@@ -501,3 +501,14 @@ def test_traced_int8_linear_equals_the_eager_layer():
     for rows in (1, 8, 8, 70):
         x = torch.randn(rows, 1024, device=DEV).to(torch.bfloat16)
         assert torch.equal(traced(x), layer(x)), rows
+
+
+def test_quantize_int8_of_more_rows_than_one_launch_has():
+    """2^26 + 5 rows of a wave each: more threads than the runtime counts."""
+    rows = (1 << 26) + 5
+    x = torch.full((rows, 8), 127.0, dtype=torch.bfloat16, device=DEV)
+    x[-7:] = torch.arange(7, device=DEV, dtype=torch.float32).bfloat16()[:, None]
+    codes, scales = quantize_int8(x)
+    assert (codes[:-7] == 127).all() and (scales[:-7] == 1.0).all()
+    want, want_scales = reference_quantize_int8(x[-7:])
+    assert torch.equal(codes[-7:], want) and torch.equal(scales[-7:], want_scales)
