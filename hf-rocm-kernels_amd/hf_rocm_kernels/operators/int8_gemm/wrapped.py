@@ -63,10 +63,11 @@ def int8_gemm(
     Where few tiles have a long k a call takes a workspace from torch's allocator (64 MiB at most).  Inference only: the result carries no gradient.
     """
     if output is None and a.dim() == 2 and b.dim() == 2 and runs_now(a) and a.dtype == torch.int8:
-        out = _int8_linear(a, b.t(), scale_b, scale_a, None if base is None or base.dim() != 1 else base, base if base is not None and base.dim() == 2 else None,
-                           out_dtype)
-        if out is not None:  # one native operator; None: what is wrong, say the checks
-            return out
+        row = base is not None and base.shape == b.shape[1:]
+        if base is None or row or base.shape == (a.size(0), b.size(1)):  # (a linear's residual may have any shape of m * n elements, and its bias be none)
+            out = _int8_linear(a, b.t(), scale_b, scale_a, base if row else None, None if row else base, out_dtype)
+            if out is not None:  # one native operator; None: what is wrong, say the checks
+                return out
     if output is None:
         output = torch.empty(size=(a.size(0), b.size(1)), dtype=out_dtype, device=a.device)
     int8_gemm_checks(a, b, scale_a, scale_b, base, output)
