@@ -12,7 +12,6 @@
 // One workgroup per row; the row's y values stay in registers between the amax reduction and the quantisation, so
 // the input is read once.  Needs 16-byte aligned rows (cols % 8 == 0) and cols <= 32768.
 #include <cfloat>
-#include <climits>
 
 #include "hfrk_internal.h"
 
@@ -249,31 +248,20 @@ extern "C" int hfrk_residual_rms_dynamic(const void* input, void* residual, cons
     const uint16_t* w = static_cast<const uint16_t*>(weight);
     uint8_t* out = static_cast<uint8_t*>(output);
     uint16_t* nb = static_cast<uint16_t*>(next_buffer);
-#define HFRK_DYN_RMS(DT_, IT_)                                                                                       \
-    hipLaunchKernelGGL((residual_rms_dynamic_kernel<DT_, IT_>), dim3(rows), dim3(threads), 0, s, in, res, w, out,     \
-                       scales, nb, epsilon, cols, buffer_cols)
-    if (io_dtype == HFRK_F16) {
-        if (iters == 1) HFRK_DYN_RMS(HFRK_F16, 1); else if (iters == 2) HFRK_DYN_RMS(HFRK_F16, 2); else HFRK_DYN_RMS(HFRK_F16, 4);
-    } else {
-        if (iters == 1) HFRK_DYN_RMS(HFRK_BF16, 1); else if (iters == 2) HFRK_DYN_RMS(HFRK_BF16, 2); else HFRK_DYN_RMS(HFRK_BF16, 4);
-    }
+#define HFRK_DYN_RMS(DT_, IT_)                                                                                                                 \
+    hipLaunchKernelGGL((residual_rms_dynamic_kernel<DT_, IT_>), dim3(count), dim3(threads), 0, s, in + first * cols, res + first * cols, w,     \
+                       out + first * cols, scales + first, nb ? nb + first * buffer_cols : nb, epsilon, cols, buffer_cols)
+    return launches_of_rows(rows, threads, [&](long first, unsigned count) {
+        if (io_dtype == HFRK_F16) {
+            if (iters == 1) HFRK_DYN_RMS(HFRK_F16, 1); else if (iters == 2) HFRK_DYN_RMS(HFRK_F16, 2); else HFRK_DYN_RMS(HFRK_F16, 4);
+        } else {
+            if (iters == 1) HFRK_DYN_RMS(HFRK_BF16, 1); else if (iters == 2) HFRK_DYN_RMS(HFRK_BF16, 2); else HFRK_DYN_RMS(HFRK_BF16, 4);
+        }
+    });
 #undef HFRK_DYN_RMS
-    HFRK_HIP_TRY(hipGetLastError());
-    return HFRK_SUCCESS;
 }
 
 namespace hfrk {
-
-// A workgroup a row, in launches of less than 2^32 threads: the runtime counts them in 32 bits and would run the rest of a larger one, without an error.
-template <typename LAUNCH>
-static int dyn_launches(int rows, int threads, LAUNCH launch) {
-    const long most = UINT_MAX / threads;
-    for (long first = 0; first < rows; first += most) {
-        launch(first, (unsigned)(rows - first < most ? rows - first : most));
-        HFRK_HIP_TRY(hipGetLastError());
-    }
-    return HFRK_SUCCESS;
-}
 
 template <int OUT>
 static int run_swiglu_dynamic(const void* gate_up, void* output, float* scales, void* next_buffer, int rows, int cols, int buffer_cols, int io_dtype,
@@ -293,7 +281,7 @@ static int run_swiglu_dynamic(const void* gate_up, void* output, float* scales, 
 #define HFRK_DYN_SWIGLU(DT_, IT_)                                                                                                          \
     hipLaunchKernelGGL((swiglu_dynamic_kernel<DT_, IT_, OUT>), dim3(count), dim3(threads), 0, s, in + first * 2 * cols, out + first * cols, \
                        scales + first, nb ? nb + first * buffer_cols : nb, cols, buffer_cols)
-    return dyn_launches(rows, threads, [&](long first, unsigned count) {
+    return launches_of_rows(rows, threads, [&](long first, unsigned count) {
         if (io_dtype == HFRK_F16) {
             if (iters == 1) HFRK_DYN_SWIGLU(HFRK_F16, 1); else if (iters == 2) HFRK_DYN_SWIGLU(HFRK_F16, 2); else HFRK_DYN_SWIGLU(HFRK_F16, 4);
         } else {
@@ -318,7 +306,7 @@ static int run_quantize(const void* input, const float* static_scale, void* outp
 #define HFRK_QUANT(DT_, IT_)                                                                                                                 \
     hipLaunchKernelGGL((quantize_rows_kernel<DT_, IT_, OUT>), dim3(count), dim3(threads), 0, s, in + first * cols, static_scale, out + first * cols, \
                        scales ? scales + first : scales, cols)
-    return dyn_launches(rows, threads, [&](long first, unsigned count) {
+    return launches_of_rows(rows, threads, [&](long first, unsigned count) {
         if (io_dtype == HFRK_F16) {
             if (iters == 1) HFRK_QUANT(HFRK_F16, 1); else if (iters == 2) HFRK_QUANT(HFRK_F16, 2); else HFRK_QUANT(HFRK_F16, 4);
         } else {

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
+#include <limits.h>
 #include <stdint.h>
 
 #include "hfrk_gfx950.h"
@@ -31,6 +32,17 @@ void set_last_hip_error(hipError_t e);
             return HFRK_HIP_ERROR;              \
         }                                       \
     } while (0)
+
+// A workgroup a row, in launches of less than 2^32 threads: the runtime counts them in 32 bits and would run the rest of a larger one, without an error.
+template <typename LAUNCH>
+inline int launches_of_rows(int rows, int threads, LAUNCH launch) {
+    const long most = UINT_MAX / threads;
+    for (long first = 0; first < rows; first += most) {
+        launch(first, (unsigned)(rows - first < most ? rows - first : most));
+        HFRK_HIP_TRY(hipGetLastError());
+    }
+    return HFRK_SUCCESS;
+}
 
 // ---- 16-bit <-> fp32, by dtype tag -------------------------------------------------------------------------
 // bf16: upper half of an fp32; conversion to bf16 rounds to nearest even (NaN kept quiet), by v_cvt_pk_bf16_f32.  Written out with
