@@ -176,41 +176,42 @@ static int launch_rms(const void* input, void* residual, const void* weight, con
     uint16_t* res = static_cast<uint16_t*>(residual);
     const uint16_t* w = static_cast<const uint16_t*>(weight);
     uint16_t* nb = static_cast<uint16_t*>(next_buffer);
+    uint8_t* const out = static_cast<uint8_t*>(output);
+    const long out_row = (long)cols * (FP8_OUT ? 1 : 2);  // bytes
     // 16-byte path: aligned rows (cols % 8 == 0 keeps every row aligned) and an aligned output row
     const bool out_ok = FP8_OUT ? ((reinterpret_cast<uintptr_t>(output) & 7) == 0) : aligned16(output);
-    bool vec = !force_scalar && (cols % 8 == 0) && aligned16(input) && aligned16(residual) && aligned16(weight) && out_ok;
+    const bool vec = !force_scalar && (cols % 8 == 0) && aligned16(input) && aligned16(residual) && aligned16(weight) && out_ok;
     int threads = num_threads;
     if (vec) {
         const int nvec = cols / 8;
         if (threads == 0) threads = rms_threads(nvec);
         const int iters = (nvec + threads - 1) / threads;
-        if (iters > 4) vec = false;  // would not fit the register cache: fall through to the strided kernel
-        else {
-#define HFRK_RMS_LAUNCH(IT, ONCE)                                                                                          \
-    hipLaunchKernelGGL((residual_rms_vec_kernel<DT, FP8_OUT, IT, ONCE>), dim3(rows), dim3(threads), 0, stream, in, res, w, \
-                       scale_tensor, output, nb, epsilon, cols, buffer_cols)
+        if (iters <= 4) {  // (more would not fit the register cache: the strided kernel)
+#define HFRK_RMS_LAUNCH(IT, ONCE)                                                                                                                           \
+    hipLaunchKernelGGL((residual_rms_vec_kernel<DT, FP8_OUT, IT, ONCE>), dim3(count), dim3(threads), 0, stream, in + first * cols, res + first * cols, w,     \
+                       scale_tensor, out + first * out_row, nb ? nb + first * buffer_cols : nb, epsilon, cols, buffer_cols)
 #define HFRK_RMS_ITERS(ONCE)                         \
     do {                                             \
         if (iters <= 1) HFRK_RMS_LAUNCH(1, ONCE);    \
         else if (iters == 2) HFRK_RMS_LAUNCH(2, ONCE); \
         else HFRK_RMS_LAUNCH(4, ONCE);               \
     } while (0)
-            if ((long)rows * cols >= kReadOnceFrom) HFRK_RMS_ITERS(true);
-            else HFRK_RMS_ITERS(false);
+            return launches_of_rows(rows, threads, [&](long first, unsigned count) {
+                if ((long)rows * cols >= kReadOnceFrom) HFRK_RMS_ITERS(true);
+                else HFRK_RMS_ITERS(false);
+            });
 #undef HFRK_RMS_ITERS
 #undef HFRK_RMS_LAUNCH
         }
     }
-    if (!vec) {
-        if (threads == 0) {
-            threads = ((cols + 63) / 64) * 64;
-            if (threads > kRmsMaxThreads) threads = kRmsMaxThreads;
-        }
-        hipLaunchKernelGGL((residual_rms_scalar_kernel<DT, FP8_OUT>), dim3(rows), dim3(threads), 0, stream, in, res, w,
-                           scale_tensor, output, nb, epsilon, cols, buffer_cols);
+    if (threads == 0) {
+        threads = ((cols + 63) / 64) * 64;
+        if (threads > kRmsMaxThreads) threads = kRmsMaxThreads;
     }
-    HFRK_HIP_TRY(hipGetLastError());
-    return HFRK_SUCCESS;
+    return launches_of_rows(rows, threads, [&](long first, unsigned count) {
+        hipLaunchKernelGGL((residual_rms_scalar_kernel<DT, FP8_OUT>), dim3(count), dim3(threads), 0, stream, in + first * cols, res + first * cols, w,
+                           scale_tensor, out + first * out_row, nb ? nb + first * buffer_cols : nb, epsilon, cols, buffer_cols);
+    });
 }
 
 bool residual_rms_into_takes(const void* input, const void* residual_in, const void* residual, const void* input_copy, const void* weight, const void* output,

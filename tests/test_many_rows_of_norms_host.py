@@ -9,7 +9,7 @@ import pytest
 from test_workspace_host import _PRELUDE, _STAND_IN, _STRUCT, _fields
 
 _KEEP = """
-static uint64_t kept[64][6], kept_groups[64];
+static uint64_t kept[256][6], kept_groups[256];
 uint64_t stand_in_pointer(int launch, int i) { return kept[launch][i]; }
 uint64_t stand_in_groups_of(int launch) { return kept_groups[launch]; }
 int hipLaunchKernel("""
@@ -19,6 +19,12 @@ _X, _RES, _W, _OUT, _S, _NEXT = ("%d << 48" % i for i in range(1, 7))
 _CALLS = {
     "residual_rms_dynamic": (f"lib.hfrk_residual_rms_dynamic({_X}, {_RES}, {_W}, 1e-5, {_OUT}, {_S}, {_NEXT}, rows, cols, 24, _capi.BF16, 1)",
                              f"(({_X}, 2 * cols), ({_RES}, 2 * cols), ({_W}, 0), ({_OUT}, cols), ({_S}, 4), ({_NEXT}, 48))"),
+    "residual_rms_fp8": (f"lib.hfrk_residual_rms({_X}, {_RES}, {_W}, {_S}, 1e-5, {_OUT}, {_NEXT}, rows, cols, 24, _capi.F16, _capi.FP8_E4M3FN, 0, 0, 1)",
+                         f"(({_X}, 2 * cols), ({_RES}, 2 * cols), ({_W}, 0), ({_S}, 0), ({_OUT}, cols), ({_NEXT}, 48))"),
+    "residual_rms_16_bit": (f"lib.hfrk_residual_rms({_X}, {_RES}, {_W}, None, 1e-5, {_OUT}, {_NEXT}, rows, cols, 24, _capi.BF16, _capi.BF16, 256, 0, 1)",
+                            f"(({_X}, 2 * cols), ({_RES}, 2 * cols), ({_W}, 0), (0, 0), ({_OUT}, 2 * cols), ({_NEXT}, 48))"),
+    "residual_rms_by_elements": (f"lib.hfrk_residual_rms({_X}, {_RES}, {_W}, {_S}, 1e-5, {_OUT}, {_NEXT}, rows, cols, 24, _capi.BF16, _capi.BF16, 0, 1, 1)",
+                                 f"(({_X}, 2 * cols), ({_RES}, 2 * cols), ({_W}, 0), ({_S}, 0), ({_OUT}, 2 * cols), ({_NEXT}, 48))"),
 }
 
 
@@ -27,7 +33,7 @@ def stand_in(tmp_path_factory):
     directory = tmp_path_factory.mktemp("stand_in")
     source, library = os.path.join(directory, "stand_in.c"), os.path.join(directory, "libstand_in.so")
     text = (_STAND_IN % _STRUCT).replace("int hipLaunchKernel(", _KEEP, 1)
-    text = text.replace("    ++launches;", "    if (launches < 64) {\n        kept_groups[launches] = grid;\n"
+    text = text.replace("    ++launches;", "    if (launches < 256) {\n        kept_groups[launches] = grid;\n"
                         "        for (int i = 0; i < 6; ++i) kept[launches][i] = *(uint64_t*)args[i];\n    }\n    ++launches;", 1)
     with open(source, "w") as f:
         f.write(text)
