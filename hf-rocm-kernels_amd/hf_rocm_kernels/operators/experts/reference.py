@@ -27,7 +27,7 @@ def reference_route_experts(
         if renormalize and float(weights[t].sum()) != 0.0:
             weights[t] /= weights[t].sum()
         weights[t] *= factor
-        if bool(torch.isnan(x).any()):
+        if bool(torch.isnan(x).any() or torch.isnan(score).any()):
             weights[t] = math.nan
     flat = experts.reshape(-1).tolist()
     pairs = sorted((i for i in range(len(flat)) if flat[i] >= 0), key=lambda i: flat[i])  # (stable)

@@ -65,7 +65,7 @@ def route_experts(
         - mask: (tokens,) bool or uint8: tokens that are 0 are padding and go nowhere
     Outputs:
         - an `ExpertRoute`.  An expert whose logit (or sum with the bias) is minus infinity or NaN is never chosen; where too few are left the expert is -1
-          and the weight 0.  A NaN among a token's logits makes its weights NaN
+          and the weight 0.  A NaN among a token's logits, or with "softmax" a plus infinity, makes its weights NaN
     Equal calls give equal bits.  Inference only: the weights carry no gradient.
     """
     if scoring in _SCORINGS and runs_now(logits):
