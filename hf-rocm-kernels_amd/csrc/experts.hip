@@ -128,9 +128,6 @@ __device__ __forceinline__ bool choose_largest(uint32_t (&hi)[EPL], uint32_t (&l
 // reciprocal and the product by 3 * 2^-24: below 2^-19 (1 + |v|).
 __device__ __forceinline__ float margin_of(const RouteArgs& a) { return a.sigmoid ? 0x1p-21f : 0x1p-18f; }
 
-// The largest logit of a token that has weights: beside plus infinity a softmax's scores are all NaN, a sigmoid's is 1.
-__device__ __forceinline__ float largest_logit(const RouteArgs& a) { return a.sigmoid ? INFINITY : FLT_MAX; }
-
 // One wave, one token; lane l has the experts EPL l ... in registers.  Choice i's expert (-1: there is none) and weight come back in lane i; what a weight needs is
 // computed for the choices only.  With a bias the choice is made in 32 bits first and is what 64 give where its values lie far enough apart; the few tokens of
 // which they do not are done again.  16000 tokens on 8 of 256 experts, choosing in 64 bits at once: 28 us, with this 20.6.
@@ -161,12 +158,11 @@ __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, 
         x[j] = first + j < experts ? x[j] : -INFINITY;
         bias[j] = BIAS ? a.bias[min(first + j, experts - 1)] : 0.f;
     }
-    bool none = false;  // a logit is NaN, or scores are
-    const float limit = largest_logit(a);
+    bool none = false;  // a logit is NaN
     float most = x[0];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-        none |= !(x[j] <= limit);
+        none |= x[j] != x[j];
         most = fmaxf(most, x[j]);
     }
     none = __ballot(none) != 0;
@@ -181,6 +177,7 @@ __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, 
             part += e[j];
         }
         sum = wave_sum(part);
+        none |= sum != sum;  // (a plus infinity makes every score NaN; a sigmoid's is 1)
     }
     uint32_t hi[EPL], lo[EPL];
     int id[EPL];
@@ -204,7 +201,8 @@ __device__ __forceinline__ void choose_experts(const RouteArgs& a, int experts, 
         double wide[EPL], whole = 0.0;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
-            wide[j] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[j])) : exp((double)x[j] - (double)most);
+            const double y = exp(a.sigmoid ? -(double)x[j] : (double)x[j] - (double)most);  // (one exponential for both: two took the last registers of route_few_kernel)
+            wide[j] = a.sigmoid ? 1.0 / (1.0 + y) : y;
             whole += wide[j];
         }
         if (!a.sigmoid) whole = wave_sum_wide(whole);
@@ -289,12 +287,11 @@ __global__ void __launch_bounds__(256) choose_many_kernel(const RouteArgs a, int
         }
     }
     bool none = false;
-    const float limit = largest_logit(a);
     float most = -INFINITY;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
         x[j] = j * 16 + in_row < experts ? x[j] : -INFINITY;
-        none |= !(x[j] <= limit);
+        none |= x[j] != x[j];
         most = fmaxf(most, x[j]);
     }
     none = row_reduce(none ? 1u : 0u, above) != 0u && real;
@@ -309,6 +306,7 @@ __global__ void __launch_bounds__(256) choose_many_kernel(const RouteArgs a, int
             part += e[j];
         }
         sum = row_reduce(part, add);
+        none |= sum != sum && real;  // (a plus infinity makes every score NaN; a sigmoid's is 1)
     }
     uint32_t hi[EPL], lo[EPL];  // the key, and the inverse of the expert's number: as one integer the larger is chosen first
     const float each = __builtin_amdgcn_rcpf(sum);
