@@ -24,8 +24,9 @@ def reference_route_experts(
         order = sorted((e for e in range(num_experts) if key[e] > -math.inf), key=lambda e: (-float(key[e]), e))[:top_k]
         for j, e in enumerate(order):
             experts[t, j], weights[t, j] = e, score[e]
-        if renormalize and float(weights[t].sum()) != 0.0:
-            weights[t] /= weights[t].sum()
+        if renormalize and order:  # (by logarithms, which scores below 64 bits' range have too)
+            logarithm = torch.nn.functional.logsigmoid(x) if scoring == "sigmoid" else torch.log_softmax(x, 0)
+            weights[t, :len(order)] = torch.softmax(logarithm[order], 0)
         weights[t] *= factor
         if bool(torch.isnan(x).any() or torch.isnan(score).any()):
             weights[t] = math.nan

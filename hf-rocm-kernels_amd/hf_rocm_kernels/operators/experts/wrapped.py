@@ -60,7 +60,7 @@ def route_experts(
         - bias: (num_experts,) float32 that is added to the scores for the choice, not to the weights; None: the largest logits are chosen.  Of equals the lowest
           index comes first.  Scores and bias are added and compared in 64 bits
         - scoring: "softmax" over a token's logits, or "sigmoid" of each
-        - renormalize: divide a token's weights by their sum (where that is not zero)
+        - renormalize: divide a token's weights by their sum.  It is taken of the scores as they are, those below fp32's range among them
         - factor: what the weights are multiplied by at the end
         - mask: (tokens,) bool or uint8: tokens that are 0 are padding and go nowhere
     Outputs:

@@ -526,8 +526,8 @@ int hfrk_grouped_gemm(const hfrk_grouped_args* args, void* stream);
  *   s        softmax of a row (sigmoid != 0: of each value 1 / (1 + e^-x)), fp32
  *   experts  [tokens, top] int32: the choices, largest logit first or, with bias (fp32 [num_experts]), largest s + bias (made and compared in 64 bits); of
  *            equals the lowest index first.  An expert whose logit (or s + bias) is minus infinity or NaN is never chosen: -1 where none is left
- *   weights  [tokens, top] fp32: factor * s of the choice, with renormalize divided by the sum of the row's choices (where that is not 0); 0 for -1.  A
- *            NaN among a row's logits makes its weights NaN, and so does a plus infinity where s is a softmax
+ *   weights  [tokens, top] fp32: factor * s of the choice, with renormalize divided by the sum of the row's choices (also where those are below fp32's range); 0 for
+ *            -1.  A NaN among a row's logits makes its weights NaN, and so does a plus infinity where s is a softmax
  *   mask     [tokens] bytes or NULL: a token whose byte is 0 is padding: experts -1, weights 0
  *   offsets  [num_experts + 1] int32: expert e has the pairs offsets[e] .. offsets[e+1]; offsets[0] = 0
  *   rows     [tokens * top] int32: the token of each pair, in the experts' order and within an expert in the tokens'; -1 behind the last pair
