@@ -200,7 +200,17 @@ __global__ void __launch_bounds__(kDynMaxThreads) quantize_rows_kernel(
         }
     }
     if (static_scale) {
-        dyn_store_row<ITERS, OUT>(y, static_scale[0], 1.0f / static_scale[0], rout);
+        float scale = static_scale[0];
+        if constexpr (OUT == HFRK_INT8) {
+            if (scale < FLT_MIN) {  // its reciprocal may be infinite, and 0 times that is no number: the same quotients, both sides larger
+                scale *= 0x1p64f;
+#pragma unroll
+                for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) y[it][v] *= 0x1p64f;
+            }
+        }
+        dyn_store_row<ITERS, OUT>(y, scale, 1.0f / scale, rout);
         return;
     }
     amax = block_max(amax, red_max);
