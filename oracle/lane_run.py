@@ -40,19 +40,20 @@ def _text(name):
     return re.sub(r"extern __shared__ float (\w+)\[\];", r"float* const \1 = reinterpret_cast<float*>(lanes::dynamic_memory);", text)
 
 
-def build() -> str:
-    """Compiles the sources, unless that has been done for these very ones; the library's path."""
+def build(prefix="lanes", headers=_HEADERS, sources=_SOURCES, own=("lanes.cpp",)) -> str:
+    """Compiles kernels' sources and those beside this file, unless that has been done for these very ones; the library's path."""
     clang = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "clang++")
-    texts = {name: _text(name) for name in _HEADERS + _SOURCES}
-    with open(os.path.join(_LANES, "lanes.cpp")) as f:
-        texts["lanes.cpp"] = f.read()
+    texts = {name: _text(name) for name in headers + sources}
+    for name in own:
+        with open(os.path.join(_LANES, name)) as f:
+            texts[name] = f.read()
     digest = hashlib.sha256()
     for name in sorted(texts):
         digest.update(texts[name].encode())
     for path in (os.path.join(_LANES, "hip", "hip_runtime.h"), os.path.join(_ROOT, "include", "hfrk_gfx950.h")):
         with open(path, "rb") as f:
             digest.update(f.read())
-    lib = os.path.join(_BUILD, f"lanes_{digest.hexdigest()[:16]}.so")
+    lib = os.path.join(_BUILD, f"{prefix}_{digest.hexdigest()[:16]}.so")
     if os.path.exists(lib):
         return lib
     os.makedirs(_BUILD, exist_ok=True)
@@ -70,13 +71,13 @@ def build() -> str:
             assert done.returncode == 0, done.stdout
             return out
         with ThreadPoolExecutor(8) as pool:
-            objects = list(pool.map(compiled, _SOURCES + ("lanes.cpp",)))
+            objects = list(pool.map(compiled, sources + own))
         subprocess.run([clang, "-shared", "-o", os.path.join(work, "all.so"), *objects], check=True)
         os.replace(os.path.join(work, "all.so"), lib)
     finally:
         shutil.rmtree(work)
     for name in os.listdir(_BUILD):  # of earlier sources
-        if name.startswith("lanes_") and name.endswith(".so") and os.path.join(_BUILD, name) != lib:
+        if name.startswith(prefix + "_") and name.endswith(".so") and os.path.join(_BUILD, name) != lib:
             os.remove(os.path.join(_BUILD, name))
     return lib
 

@@ -1,5 +1,5 @@
-// Stands in for the HIP headers when a kernel's source is compiled for the CPU: the names and the gfx950 builtins that the kernels of attention and of the
-// append use.  Every lane runs by itself until it meets a builtin that looks at other lanes of its wave, where it waits for them (lanes.cpp).
+// Stands in for the HIP headers when a kernel's source is compiled for the CPU: the names and the gfx950 builtins that the kernels of attention, of the
+// append, of the router and of groups of few rows use.  Every lane runs by itself until it meets a builtin that looks at other lanes of its wave, where it waits for them (lanes.cpp).
 // Test infrastructure only.
 #pragma once
 
@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <functional>
+#include <utility>
 
 #define __global__
 #define __device__
@@ -61,6 +62,10 @@ inline TO bits(FROM from) {
     memcpy(&to, &from, sizeof to);
     return to;
 }
+inline int __float_as_int(float f) { return bits<int>(f); }
+inline float __int_as_float(int i) { return bits<float>(i); }
+inline long long __double_as_longlong(double d) { return bits<long long>(d); }
+inline int atomicAdd(int* at, int by) { return std::exchange(*at, *at + by); }  // (one lane runs at a time)
 inline float __uint_as_float(uint32_t u) { return bits<float>(u); }
 inline uint32_t __float_as_uint(float f) { return bits<uint32_t>(f); }
 inline uint32_t __umulhi(uint32_t a, uint32_t b) { return (uint64_t)a * b >> 32; }
@@ -194,20 +199,89 @@ inline float __shfl_xor(float v, int by) {
     const lanes::Seen s = lanes::meet_wave({{__float_as_uint(v)}});
     return __uint_as_float(s.of[s.lane ^ by].w[0]);
 }
+inline double __shfl_xor(double v, int by) {
+    const uint64_t mine = bits<uint64_t>(v);
+    const lanes::Seen s = lanes::meet_wave({{(unsigned)mine, (unsigned)(mine >> 32)}});
+    const uint32_t* const w = s.of[s.lane ^ by].w;
+    return bits<double>((uint64_t)w[1] << 32 | w[0]);
+}
 #define __syncthreads lanes::meet_block
 
-// Resources of bounded loads, which these kernels do not use: declared for the shared header's sake.
+// Bounded loads and stores: 4-byte words (or what is smaller) behind the range are zero, or dropped.
 namespace lanes {
-struct Resource {};
-inline uint4 no_load(Resource, int, int, int) { __builtin_trap(); }
+struct Resource {
+    char* base;
+    uint32_t size;
+};
+inline Resource resource(void* base, short, int size, int) { return {(char*)base, (uint32_t)size}; }
+template <typename T>
+inline T bounded_load(Resource r, int offset, int scalar, int) {
+    T v;
+    for (size_t i = 0; i < sizeof v; i += sizeof v < 4 ? sizeof v : 4) {
+        const size_t bytes = sizeof v < 4 ? sizeof v : 4;
+        const uint64_t at = (uint64_t)(uint32_t)offset + (uint32_t)scalar + i;
+        if (at + bytes <= r.size) memcpy((char*)&v + i, r.base + at, bytes);
+        else memset((char*)&v + i, 0, bytes);
+    }
+    return v;
+}
 template <typename V>
-inline void no_store(V, Resource, int, int, int) { __builtin_trap(); }
+inline void bounded_store(V v, Resource r, int offset, int scalar, int) {
+    for (size_t i = 0; i < sizeof v; i += 4) {
+        const uint64_t at = (uint64_t)(uint32_t)offset + (uint32_t)scalar + i;
+        if (at + 4 <= r.size) memcpy(r.base + at, (char*)&v + i, 4);
+    }
+}
+
+// The 8-bit instructions: rows of A and columns of B are lane % 16, a lane's bytes of k those from its share's begin on; C as in product().
+typedef int Ints4 __attribute__((ext_vector_type(4)));
+template <typename A, typename C, typename WIDEN>
+inline C product_of_bytes(A a, A b, C c, WIDEN widen) {
+    constexpr int kWords = sizeof a / 4;
+    Words mine;
+    uint32_t rows[4][4][kWords];
+    memcpy(mine.w, &a, sizeof a);
+    {
+        const Seen s = meet_wave(mine);
+        for (int v = 0; v < 4; ++v)
+            for (int g = 0; g < 4; ++g) memcpy(rows[v][g], s.of[16 * g + 4 * (s.lane / 16) + v].w, sizeof a);
+    }
+    memcpy(mine.w, &b, sizeof b);
+    const Seen s = meet_wave(mine);
+    for (int v = 0; v < 4; ++v) {
+        auto sum = widen(0) * 0;
+        for (int g = 0; g < 4; ++g) {
+            uint8_t x[sizeof a], y[sizeof a];
+            memcpy(x, rows[v][g], sizeof a);
+            memcpy(y, s.of[16 * g + s.lane % 16].w, sizeof a);
+            for (size_t k = 0; k < sizeof a; ++k) sum += widen(x[k]) * widen(y[k]);
+        }
+        c[v] += sum;
+    }
+    return c;
+}
+template <typename A>
+inline Ints4 product_int8(A a, A b, Ints4 c, int, int, int) {
+    return product_of_bytes(a, b, c, [](uint8_t x) { return (int)(int8_t)x; });
+}
+template <typename A, typename C>
+inline C product_fp8(A a, A b, C c, int, int, int, int, int, int) {
+    return product_of_bytes(a, b, c, [](uint8_t x) { return (double)from_e4m3(x); });
+}
+inline unsigned bits_in_front(uint64_t mask, unsigned more) { return more + __builtin_popcountll(mask & ((1ull << thread.x % 64) - 1)); }
 }  // namespace lanes
 #define __amdgpu_buffer_rsrc_t lanes::Resource
-#define __builtin_amdgcn_make_buffer_rsrc(...) lanes::Resource()
-#define __builtin_amdgcn_raw_buffer_load_b128 lanes::no_load
-#define __builtin_amdgcn_raw_buffer_store_b128 lanes::no_store
-#define __builtin_amdgcn_raw_buffer_store_b64 lanes::no_store
+#define __builtin_amdgcn_make_buffer_rsrc lanes::resource
+#define __builtin_amdgcn_raw_buffer_load_b16 lanes::bounded_load<uint16_t>
+#define __builtin_amdgcn_raw_buffer_load_b32 lanes::bounded_load<uint32_t>
+#define __builtin_amdgcn_raw_buffer_load_b128 lanes::bounded_load<lanes::Ints4>
+#define __builtin_amdgcn_raw_buffer_store_b128 lanes::bounded_store
+#define __builtin_amdgcn_raw_buffer_store_b64 lanes::bounded_store
+#define __builtin_amdgcn_mfma_i32_16x16x64_i8 lanes::product_int8
+#define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4 lanes::product_fp8
+#define __builtin_amdgcn_mbcnt_lo(mask, more) lanes::bits_in_front((uint32_t)(mask), more)
+#define __builtin_amdgcn_mbcnt_hi(mask, more) lanes::bits_in_front((uint64_t)(mask) << 32, more)
+#define __builtin_amdgcn_sched_barrier(...)
 
 #define __builtin_amdgcn_exp2f exp2f
 #define __builtin_amdgcn_rcpf(x) (1.f / (x))
