@@ -3,7 +3,7 @@
 // codes of float8_e4m3fn (sums in fp32) or int8 (sums in int32: exact up to k = 131071, then one conversion), scales applied to the whole sum, one
 // rounding to 16 bits.  No counterpart in the reference, whose GEMM has one fp8 weight.
 //
-// grouped_rows_kernel: a workgroup takes 16 MT rows of a group; each of its waves takes 16 RT columns and every KW-th 128-byte chunk of k, so that KW waves
+// grouped_rows_kernel: a workgroup takes 16 rows of a group; each of its waves takes 16 RT columns and every KW-th 128-byte chunk of k, so that KW waves
 // read a run of KW * 128 bytes of each weight row at a time.  Operands go from memory to registers (lane l of a 16 x 16 tile holds pieces l / 16 and
 // l / 16 + 4 of row l % 16: which bytes of k a lane has does not matter as long as both operands agree), one tile's chunk ahead of the one that is
 // multiplied; the sums of the waves along k meet in LDS, in wave order.  Bound by memory: 5.8 TB/s on 940 MB of weights.  More rows a group go to the tiled
@@ -18,6 +18,7 @@
 namespace hfrk {
 
 constexpr int kRowsChunk = 128;  // bytes of k that a wave takes at a time
+constexpr int kRowsTile = 16;    // rows of a workgroup
 
 template <int DT>
 __device__ __forceinline__ uint32_t two_to_16bit(float lo, float hi) {
@@ -25,11 +26,11 @@ __device__ __forceinline__ uint32_t two_to_16bit(float lo, float hi) {
 }
 
 // KW waves split k, CW of them the columns.
-template <bool INT8, int MT, int RT, int KW, int CW>
+template <bool INT8, int RT, int KW, int CW>
 __global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_rows_kernel(const GroupedArgs a) {
-    constexpr int WAVES = KW * CW, TILES = CW * MT * RT;  // matrix tiles of 16 x 16 of the workgroup
+    constexpr int WAVES = KW * CW, TILES = CW * RT;        // matrix tiles of 16 x 16 of the workgroup
     constexpr int EACH = (TILES + WAVES - 1) / WAVES;     // tiles whose sums a wave finishes
-    constexpr int BM = 16 * MT, BN = 16 * RT * CW;
+    constexpr int BM = kRowsTile, BN = 16 * RT * CW;
     __shared__ v4i sums[KW][TILES][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = wave % KW, cw = wave / KW;
 
@@ -42,9 +43,7 @@ __global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_row
     const __amdgpu_buffer_rsrc_t rnumbers = make_rsrc(a.rows + row0, a.rows ? (uint32_t)rows * 4u : 0u);
     auto number_of = [&](int r) __attribute__((always_inline)) { return a.rows ? __builtin_amdgcn_raw_buffer_load_b32(rnumbers, r * 4, 0, 0) : row0 + r; };
     auto row_of = [&](int r, int number) __attribute__((always_inline)) { return r < rows && (uint32_t)number < (uint32_t)a.a_rows ? number : -1; };
-    int number[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) number[i] = number_of(i * 16 + (lane & 15));
+    const int number = number_of(lane & 15);
 
     // gathered rows lie anywhere in A (below 2 GB); others behind the tile's first
     const long a_from = a.rows ? 0 : row0;
@@ -52,20 +51,18 @@ __global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_row
     const __amdgpu_buffer_rsrc_t rb =
         make_rsrc(a.B + t.expert * a.expert_stride + (long)n0 * a.b_stride, (uint32_t)(cols - 1) * (uint32_t)a.b_stride + (uint32_t)a.k);
     const int piece = (lane >> 4) * 16;
-    uint32_t va[MT], vb[RT];
+    uint32_t va, vb[RT];
 #pragma unroll
     for (int j = 0; j < RT; ++j) vb[j] = (uint32_t)((cw * RT + j) * 16 + (lane & 15)) * (uint32_t)a.b_stride + piece;
 
     typedef float acc_f __attribute__((ext_vector_type(4)));
     using Acc = std::conditional_t<INT8, v4i, acc_f>;
-    Acc acc[MT][RT];
+    Acc acc[RT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+    for (int j = 0; j < RT; ++j) acc[j] = Acc{0, 0, 0, 0};
 
     // registers of the tile that is multiplied and of the next one: a tile's own, or with one tile those of every other chunk
-    v4i fa[2][MT][2], fb[RT == 1 ? 2 : RT][2];
+    v4i fa[2][2], fb[RT == 1 ? 2 : RT][2];
     auto get_b = [&](int set, int j, int c) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -75,35 +72,27 @@ __global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_row
     };
     auto get_a = [&](int set, int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int by = c * kRowsChunk + h * 64;
-                fa[set][i][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, by + piece < a.k ? va[i] + (uint32_t)by : (uint32_t)kOutsideBuffer, 0, 0);
-            }
+        for (int h = 0; h < 2; ++h) {
+            const int by = c * kRowsChunk + h * 64;
+            fa[set][h] = __builtin_amdgcn_raw_buffer_load_b128(ra, by + piece < a.k ? va + (uint32_t)by : (uint32_t)kOutsideBuffer, 0, 0);
+        }
     };
     auto multiply = [&](int set, int j) __attribute__((always_inline)) {
         const v4i(&b)[2] = fb[RT == 1 ? set : j];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            if constexpr (INT8) {
-                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[0], fa[set][i][0], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[1], fa[set][i][1], acc[i][j], 0, 0, 0);
-            } else {
-                auto join = [](v4i lo, v4i hi) __attribute__((always_inline)) { return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}; };
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(b[0], b[1]), join(fa[set][i][0], fa[set][i][1]), acc[i][j], 0, 0, 0, 0, 0, 0);
-            }
+        if constexpr (INT8) {
+            acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[0], fa[set][0], acc[j], 0, 0, 0);
+            acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[1], fa[set][1], acc[j], 0, 0, 0);
+        } else {
+            auto join = [](v4i lo, v4i hi) __attribute__((always_inline)) { return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}; };
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(b[0], b[1]), join(fa[set][0], fa[set][1]), acc[j], 0, 0, 0, 0, 0, 0);
         }
     };
 
     // The weight is requested in front of the rows, whose numbers are still on their way.
     const int chunks = (a.k + kRowsChunk - 1) / kRowsChunk;
     get_b(0, 0, kw);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int r = row_of(i * 16 + (lane & 15), number[i]);
-        va[i] = r >= 0 ? (uint32_t)((r - a_from) * a.k + piece) : (uint32_t)kOutsideBuffer;
-    }
+    const int mine = row_of(lane & 15, number);
+    va = mine >= 0 ? (uint32_t)((mine - a_from) * a.k + piece) : (uint32_t)kOutsideBuffer;
     get_a(0, kw);
     for (int c = kw; c < chunks; c += 2 * KW) {
 #pragma unroll
@@ -119,19 +108,15 @@ __global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_row
         }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j) sums[kw][cw * MT * RT + i * RT + j][lane] = __builtin_bit_cast(v4i, acc[i][j]);
-    // what the epilogue needs of this thread's values: tile e of the workgroup is wave e / (MT RT)'s tile e % (MT RT)
-    int e_m[EACH], e_n[EACH];
-    float sa[EACH], sb[EACH][4];
+    for (int j = 0; j < RT; ++j) sums[kw][cw * RT + j][lane] = __builtin_bit_cast(v4i, acc[j]);
+    // what the epilogue needs of this thread's values: tile e of the workgroup is columns 16 e and on
+    const int e_m = lane & 15, from = row_of(e_m, number_of(e_m));
+    const float sa = from >= 0 ? a.scale_a[(long)from * a.sa_stride] : 0.f;
+    int e_n[EACH];
+    float sb[EACH][4];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-        const int tile = wave + e * WAVES, of = tile % (MT * RT);
-        e_m[e] = of / RT * 16 + (lane & 15);
-        e_n[e] = (tile / (MT * RT) * RT + of % RT) * 16 + (lane >> 4) * 4;
-        const int r = row_of(e_m[e], number_of(e_m[e]));
-        sa[e] = r >= 0 ? a.scale_a[(long)r * a.sa_stride] : 0.f;
+        e_n[e] = (wave + e * WAVES) * 16 + (lane >> 4) * 4;
 #pragma unroll
         for (int v = 0; v < 4; ++v)
             sb[e][v] = a.scale_b ? a.scale_b[t.expert * a.sb_expert_stride + (long)min(n0 + e_n[e] + v, a.n - 1) * a.sb_stride] : 1.0f;
@@ -140,18 +125,18 @@ __global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_row
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         const int tile = wave + e * WAVES;
-        if (tile >= TILES || e_m[e] >= rows || e_n[e] >= cols) continue;
+        if (tile >= TILES || e_m >= rows || e_n[e] >= cols) continue;
         Acc total = Acc{0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < KW; ++w) total += __builtin_bit_cast(Acc, sums[w][tile][lane]);
-        const long at = (long)(row0 + e_m[e]) * a.n + n0 + e_n[e], base_at = (long)(row0 + e_m[e]) * a.base_stride + n0 + e_n[e];
+        const long at = (long)(row0 + e_m) * a.n + n0 + e_n[e], base_at = (long)(row0 + e_m) * a.base_stride + n0 + e_n[e];
         uint16_t* const d = static_cast<uint16_t*>(a.D) + at;
         const uint16_t* const base = a.base ? static_cast<const uint16_t*>(a.base) + base_at : nullptr;
         auto finish = [&](auto dt) __attribute__((always_inline)) {
             constexpr int DT = decltype(dt)::value;
             float x[4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) x[v] = (float)total[v] * (sa[e] * sb[e][v]);
+            for (int v = 0; v < 4; ++v) x[v] = (float)total[v] * (sa * sb[e][v]);
             if (a.vec) {
                 if (base) {
                     const uint2 b = *reinterpret_cast<const uint2*>(base);
@@ -172,13 +157,13 @@ __global__ void __launch_bounds__(64 * KW * CW, KW * CW > 8 ? 8 : 6) grouped_row
     }
 }
 
-template <bool INT8, int MT, int RT, int KW, int CW>
+template <bool INT8, int RT, int KW, int CW>
 static int launch_rows(GroupedArgs a, hipStream_t stream) {
     constexpr int BN = 16 * RT * CW, THREADS = 64 * KW * CW;
     a.tiles_n = (a.n + BN - 1) / BN;
-    const long tiles = (a.offsets ? grouped_tiles_bound(a.count, a.experts, 16 * MT) : ((long)a.count + 16 * MT - 1) / (16 * MT)) * a.tiles_n;
+    const long tiles = (a.offsets ? grouped_tiles_bound(a.count, a.experts, kRowsTile) : ((long)a.count + kRowsTile - 1) / kRowsTile) * a.tiles_n;
     if (tiles * THREADS > (long)UINT_MAX) return HFRK_BAD_SHAPE;
-    hipLaunchKernelGGL((grouped_rows_kernel<INT8, MT, RT, KW, CW>), dim3((unsigned)tiles), dim3(THREADS), 0, stream, a);
+    hipLaunchKernelGGL((grouped_rows_kernel<INT8, RT, KW, CW>), dim3((unsigned)tiles), dim3(THREADS), 0, stream, a);
     HFRK_HIP_TRY(hipGetLastError());
     return HFRK_SUCCESS;
 }
@@ -211,12 +196,12 @@ static FewRows few_rows_kernel(int n, int k, float active, float rows) {
 
 template <bool INT8>
 static int launch_few_rows(const GroupedArgs& a, const FewRows& f, hipStream_t stream) {
-    if (f.waves_k == 4) return f.cols == 128 ? launch_rows<INT8, 1, 4, 4, 2>(a, stream) : launch_rows<INT8, 1, 2, 4, 2>(a, stream);
+    if (f.waves_k == 4) return f.cols == 128 ? launch_rows<INT8, 4, 4, 2>(a, stream) : launch_rows<INT8, 2, 4, 2>(a, stream);
     switch (f.cols) {
-        case 64: return launch_rows<INT8, 1, 4, 8, 1>(a, stream);
-        case 48: return launch_rows<INT8, 1, 3, 8, 1>(a, stream);
-        case 32: return launch_rows<INT8, 1, 2, 8, 1>(a, stream);
-        default: return launch_rows<INT8, 1, 1, 8, 1>(a, stream);
+        case 64: return launch_rows<INT8, 4, 8, 1>(a, stream);
+        case 48: return launch_rows<INT8, 3, 8, 1>(a, stream);
+        case 32: return launch_rows<INT8, 2, 8, 1>(a, stream);
+        default: return launch_rows<INT8, 1, 8, 1>(a, stream);
     }
 }
 
