@@ -1,9 +1,10 @@
-// Per-token (per-row) dynamic FP8 quantisation fused into the two element-wise kernels of the decoder block, and on
+// Per-token (per-row) dynamic FP8 (and int8) quantisation fused into the two element-wise kernels of the decoder block, and on
 // its own for activations that come from elsewhere (attention output -> o_proj):
 //   residual_rms_dynamic:  residual <- input + residual;  y = rmsnorm(residual) * weight
 //   swiglu_dynamic:        y = silu(gate) * up
 //   quantize_fp8:          y = x   (also with one static scale: the reference's fp8_quantize, utils/fp8.py:6-29, on device)
-// (the last two also to int8: scale[row] = max(amax / 127, FLT_MIN), output = rint(y / scale[row])) and in both:            scale[row] = max(amax_row |y| / 448, FLT_MIN);  output = e4m3fn(y / scale[row])
+// and in all three:        scale[row] = max(amax_row |y| / 448, FLT_MIN);  output = e4m3fn(y / scale[row])
+// The last two also to int8: scale[row] = max(amax_row |y| / 127, FLT_MIN);  output = rint(y / scale[row]), ties to even.
 // The per-row scales feed the GEMM's per-token scale_a directly, so no activation scale has to be calibrated ahead
 // of time.  The reference only has the static-scale forms (one scale_tensor for the whole tensor:
 // operators/residual_rms/wrapped.py:94-95, operators/swiglu/wrapped.py:49-84); these kernels have no counterpart

@@ -2,10 +2,10 @@
 // No counterpart in the reference, whose MLP is dense.
 //
 // route_experts.  s[t, :] = softmax or sigmoid of the logits, in fp32.  A token goes to the `top` experts with the largest logit (scores are in the same
-// order) or, with a bias, the largest s + bias; those sums lie close together, so they are made and compared in 64 bits.  Of equals the
-// lowest index comes first.  weights[t, j] = factor * s of the j-th choice, divided by the choices' sum where that is asked for.  Then the (token, choice)
+// order) or, with a bias, the largest s + bias; those sums lie close together, so the choice is the one that 64 bits make (choose_experts).  Of equals the
+// lowest index comes first.  weights[t, j] = factor * s of the j-th choice, divided by the choices' sum where that is asked for (score_of).  Then the (token, choice)
 // pairs are put in the experts' order, a token in front of a later one: rows[i] is the token of pair i, places[t, j] is where pair (t, j) went, and
-// offsets[e] is where expert e begins: a counting sort, without atomics, so that equal calls give equal bits.
+// offsets[e] is where expert e begins: a counting sort, without atomics on memory (those in LDS add integers), so that equal calls give equal bits.
 //
 // combine_experts.  out[t] = (base ? base[t] : 0) + sum_j weights[t, j] * y[places[t, j]], in fp32, in the choices' order.
 #include <cfloat>

@@ -58,7 +58,7 @@ def route_experts(
         - logits: (tokens, num_experts) bfloat16, float16 or float32, unit stride along the experts; up to 512 experts
         - top_k: experts per token, up to 32
         - bias: (num_experts,) float32 that is added to the scores for the choice, not to the weights; None: the largest logits are chosen.  Of equals the lowest
-          index comes first.  Scores and bias are added and compared in 64 bits
+          index comes first.  The choice is the one that sums in 64 bits give
         - scoring: "softmax" over a token's logits, or "sigmoid" of each
         - renormalize: divide a token's weights by their sum.  It is taken of the scores as they are, those below fp32's range among them
         - factor: what the weights are multiplied by at the end

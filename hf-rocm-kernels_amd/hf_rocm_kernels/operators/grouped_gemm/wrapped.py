@@ -61,7 +61,8 @@ def grouped_gemm(
     out_dtype: torch.dtype = torch.bfloat16,
 ) -> Tensor:
     """Products of rows grouped by expert: row i of the result, offsets[e] <= i < offsets[e + 1], is scale_a[r] * scale_b[e] * (a[r] @ b[e]) with
-    r = rows[i], or i without rows.  Sums in fp32 (float8_e4m3fn) or exact (int8), scales in fp32, one rounding.
+    r = rows[i], or i without rows.  int8 sums are exact; float8_e4m3fn sums are the matrix cores' (a run of eight products is aligned to its largest and loses
+    what is below 2^-13 of that, runs are added in fp32), as in every fp8 product here.  Scales in fp32, one rounding.
     Args:
         - a: a (rows, k) float8_e4m3fn or int8 tensor in row-major format, k a multiple of 16 (int8: up to 131056)
         - b: (experts, k, n) of a's dtype with unit stride along k (the `.transpose(1, 2)` of an (experts, n, k) weight); experts up to 512
@@ -69,7 +70,7 @@ def grouped_gemm(
         - offsets: (experts + 1,) int32, not decreasing, as `route_experts` gives them.  They stay on the device: no call waits for them, and a captured call
           may be replayed with others
         - rows: (count,) int32 or None: the row of a for each row of the result (`route_experts`' rows: a first projection picks the tokens' rows).  A
-          number that is no row of a counts as a row of zeros
+          number that is no row of a counts as a row of zeros (under a scale_b that is infinite or NaN the result there is zero or NaN)
         - output: a (count, n) tensor to write to, or None for a new one of out_dtype (bfloat16 or float16)
     Outputs:
         - (count, n); rows in front of offsets[0] and behind the last group's are not written.  Inference only: the result carries no gradient
