@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kDynMaxThreads) quantize_rows_kernel(
     if (static_scale) {
         float scale = static_scale[0];
         if constexpr (OUT == HFRK_INT8) {
-            if (scale < FLT_MIN) {  // its reciprocal may be infinite, and 0 times that is no number: the same quotients, both sides larger
+            if (fabsf(scale) < FLT_MIN) {  // its reciprocal may be infinite, and 0 times that is no number: the same quotients, both sides larger
                 scale *= 0x1p64f;
 #pragma unroll
                 for (int it = 0; it < ITERS; ++it)

@@ -26,3 +26,13 @@ def test_small_static_scales(dtype, scale):
     # half a step, and what the quotient's rounding to fp32 moves it by
     assert ((codes.double() - quotient).abs() <= 0.5 + 2.0 ** -23 * 127).all()
     assert (codes[x == 0] == 0).all()
+
+
+@pytest.mark.parametrize("scale", [-0.02, -1e20, -3e-39])
+def test_scales_below_zero_turn_the_codes(scale):
+    """No scale that a checkpoint has; its quotients have codes all the same."""
+    x = torch.tensor([[1.0, -2.0, 0.0, 1e20, -3e22, 3e-39, -2e-37, 0.5]], device=DEV, dtype=torch.bfloat16)
+    static = torch.tensor([scale], device=DEV)
+    codes, _ = quantize_int8(x, static)
+    quotient = (x.double() / static.double()).clamp(-127, 127)
+    assert ((codes.double() - quotient).abs() <= 0.5 + 2.0 ** -23 * 127).all()
